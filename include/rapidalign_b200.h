@@ -438,6 +438,53 @@ RA_API int ra_pdl_backward(const ra_pdl_cloud *src, const ra_pdl_cloud *tgt, int
                            int32_t D, const double *grad_loss, float *grad_src, float *grad_tgt,
                            void *workspace, size_t workspace_bytes, ra_stream_t stream);
 
+/* ---- linear cross entropy ------------------------------------------------ */
+/* Softmax cross entropy of rows x_i [rows, dim] against a table w_v [vocab,
+ * dim] without the logits in memory: z_iv = scale x_i.w_v, or
+ * softcap tanh(scale x_i.w_v / softcap) where softcap > 0;
+ * lse_i = log sum_v exp(z_iv); loss_i = lse_i - z_i,target_i, 0 for rows whose
+ * target is ignore_index, NaN for a target outside the table (never read).
+ *
+ * x and w: `dtype` (both), row strides ld_x, ld_w in elements; for the 16-bit
+ * types the strides are multiples of 8 and the addresses of 16 bytes.
+ * target: int64 [rows].  loss: float [rows] (RA_REDUCE_NONE) or [1] (sum, or
+ * mean over the rows with a label); lse: float [rows].  `state` (256-byte
+ * aligned, ra_ce_state_bytes) keeps what the backward needs; `workspace`
+ * (256-byte aligned, ra_ce_workspace_bytes for the pass) is scratch.
+ * `status`: an int the device can write (pinned host or device memory), to
+ * which a bounded wait that expires adds bit 0; the outputs are then invalid.
+ * Nothing is allocated and the host never waits, so the calls can be captured. */
+enum ra_dtype { RA_F32 = 0, RA_BF16 = 1, RA_F16 = 2 };
+enum ra_reduction { RA_REDUCE_NONE = 0, RA_REDUCE_SUM = 1, RA_REDUCE_MEAN = 2 };
+typedef struct ra_ce_desc {
+  int64_t rows;
+  int64_t vocab;
+  int64_t ld_x;
+  int64_t ld_w;
+  int64_t ignore_index;
+  int32_t dim;
+  int32_t dtype;
+  int32_t reduction;
+  float scale;
+  float softcap;
+  int32_t reserved;
+  int32_t *status;
+} ra_ce_desc;
+
+RA_API size_t ra_ce_state_bytes(const ra_ce_desc *desc);
+RA_API size_t ra_ce_workspace_bytes(const ra_ce_desc *desc, int backward_pass);
+RA_API int ra_ce_forward(const ra_ce_desc *desc, const void *x, const void *w,
+                         const int64_t *target, float *loss, float *lse, void *state,
+                         size_t state_bytes, void *workspace, size_t workspace_bytes,
+                         ra_stream_t stream);
+/* Gradients for upstream g_loss (as loss; NULL = zero) and g_lse ([rows];
+ * NULL = zero) into dx [rows, dim] and dw [vocab, dim] (contiguous, `dtype`,
+ * 16-byte aligned; either may be NULL).  Reads the state its forward left. */
+RA_API int ra_ce_backward(const ra_ce_desc *desc, const void *x, const void *w,
+                          const int64_t *target, const float *g_loss, const float *g_lse,
+                          void *dx, void *dw, void *state, size_t state_bytes, void *workspace,
+                          size_t workspace_bytes, ra_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

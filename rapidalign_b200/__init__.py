@@ -4,6 +4,7 @@ differentiable segmented_kde_loss)."""
 from .kde import (batch_ptrs, kde_mmd_loss, kde_mmd_loss_bands, kde_mmd_loss_dense,
                   pyg_batch_kde_mmd_loss, pyg_kde_mmd_loss)
 from .algorithms import pairwise_distance_loss
+from .cross_entropy import linear_cross_entropy
 from .autograd_kde import SegmentedKDELossFunction, segmented_kde_loss
 
 __all__ = [
@@ -15,5 +16,6 @@ __all__ = [
     "batch_ptrs",
     "segmented_kde_loss",
     "pairwise_distance_loss",
+    "linear_cross_entropy",
     "SegmentedKDELossFunction",
 ]

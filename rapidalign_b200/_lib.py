@@ -76,6 +76,29 @@ class RaKdeDesc(ctypes.Structure):
     ]
 
 
+RA_F32, RA_BF16, RA_F16 = 0, 1, 2
+DTYPES = {torch.float32: RA_F32, torch.bfloat16: RA_BF16, torch.float16: RA_F16}
+
+RA_REDUCE_NONE, RA_REDUCE_SUM, RA_REDUCE_MEAN = 0, 1, 2
+
+
+class RaCeDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("ld_x", ctypes.c_int64),
+        ("ld_w", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 class RaPdlCloud(ctypes.Structure):
     _fields_ = [
         ("points", ctypes.c_void_p),
@@ -171,6 +194,12 @@ SIGNATURES = {
                                       _I64, _I32, _V, _V, _SZ, _V]),
     "ra_pdl_backward": (ctypes.c_int, [ctypes.POINTER(RaPdlCloud), ctypes.POINTER(RaPdlCloud),
                                        _I64, _I32, _V, _V, _V, _V, _SZ, _V]),
+    "ra_ce_state_bytes": (_SZ, [ctypes.POINTER(RaCeDesc)]),
+    "ra_ce_workspace_bytes": (_SZ, [ctypes.POINTER(RaCeDesc), ctypes.c_int]),
+    "ra_ce_forward": (ctypes.c_int, [ctypes.POINTER(RaCeDesc), _V, _V, _V, _V, _V, _V, _SZ, _V,
+                                     _SZ, _V]),
+    "ra_ce_backward": (ctypes.c_int, [ctypes.POINTER(RaCeDesc), _V, _V, _V, _V, _V, _V, _V, _V,
+                                      _SZ, _V, _SZ, _V]),
     "ra_kernel_launch_count": (ctypes.c_ulonglong, []),
     "ra_probe_fp32_peak": (ctypes.c_int, [_V, _I64, ctypes.c_int, ctypes.POINTER(_D), _V]),
 }
@@ -227,6 +256,28 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     buf = torch.empty(max(int(nbytes), 1) + 256, dtype=torch.uint8, device=device)
     off = (-buf.data_ptr()) % 256
     return buf[off:off + max(int(nbytes), 1)]
+
+
+_STATUS: Optional[torch.Tensor] = None
+
+
+def status_word() -> int:
+    """Address of the process's status word: a page-locked int that kernels
+    with bounded waits write when one expires.  Reading it costs the host
+    nothing, so it is checked at the next call (`check_status`)."""
+    global _STATUS
+    if _STATUS is None:
+        with _lock:
+            if _STATUS is None:
+                _STATUS = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+    return _STATUS.data_ptr()
+
+
+def check_status(what: str) -> None:
+    """Raise if a bounded wait of an earlier call expired (and forget it)."""
+    if _STATUS is not None and ctypes.c_int32.from_address(_STATUS.data_ptr()).value:
+        _STATUS.zero_()
+        check(RA_ERR_DEVICE_TIMEOUT, what + " (an earlier call)")
 
 
 def launch_count() -> int:

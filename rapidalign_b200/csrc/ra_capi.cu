@@ -18,6 +18,7 @@
 #include "ra_common.cuh"
 #include "ra_epilogue.cuh"
 #include "ra_exact.cuh"
+#include "ra_host.h"
 #include "ra_pdl.cuh"
 #include "ra_plan.cuh"
 #include "ra_prep.cuh"
@@ -26,11 +27,13 @@
 #include "ra_tiles3.cuh"
 #include "ra_tilesg.cuh"
 
+namespace ra {
+std::atomic<unsigned long long> g_launches{0};
+}
+
 namespace {
 
 using namespace ra;
-
-std::atomic<unsigned long long> g_launches{0};
 
 constexpr int kPrepThreads = 256;
 constexpr int kEpiThreads = 256;

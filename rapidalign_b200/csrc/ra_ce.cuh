@@ -1,0 +1,427 @@
+// ra_ce.cuh -- softmax cross entropy of rows x_i against a table of vectors
+// w_v (a large vocabulary), without the logits in memory.
+//
+//   z_iv = s x_i.w_v            or  c tanh(s x_i.w_v / c)   (soft cap c)
+//   lse_i = log sum_v e^z_iv    loss_i = lse_i - z_{i,t_i}
+//   dz_iv = (gl_i + ge_i) e^(z_iv - lse_i) - gl_i [v = t_i]
+//   du_iv = dz_iv (1 - (z_iv / c)^2)
+//   dx_i = s sum_v du_iv w_v    dw_v = s sum_i du_iv x_i
+// with gl, ge the upstream gradients of loss and lse.
+//
+// Forward: one product (ra_gemm16.cuh) whose epilogue keeps a running maximum
+// and sum of exponentials of each row over its 128 columns; `ce_rows_kernel`
+// joins the column tiles.  All in base 2: t = z log2 e, 2^(t - m).
+// Backward: the vocabulary in pieces; per piece the logits again, du in 16
+// bits (with the rows' coefficients, so both products read it as it is), then
+// dx += du W and dw = du^T X.  Sums over pieces and K slices have one writer
+// each and a fixed order: no atomics, bitwise repeatable.
+// du is rounded to the operands' 16-bit type (half a step, 2^-9 or 2^-12
+// relative, independent from element to element, so sums of many keep less);
+// for fp32 inputs du, x and w are fp16 pairs hi + lo (22 bits).
+#pragma once
+
+#include "ra_gemm16.cuh"
+#include "ra_host.h"
+
+namespace ra {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
+
+// header of the state buffer
+struct CeHead {
+  unsigned amax_x, amax_w;  // bits of the largest finite |x|, |w| (fp32 inputs)
+  unsigned amax_g;          // of the upstream coefficients (backward)
+  unsigned ticket;          // blocks of ce_rows_kernel done
+  long long count;          // rows with a label
+};
+
+// Power of two that brings a largest magnitude into [2^13, 2^14): with twice
+// that (du) still below the fp16 maximum 65504.
+__device__ __forceinline__ int ce_exp(unsigned amax_bits) {
+  if (amax_bits == 0) return 0;
+  int e;
+  frexpf(__uint_as_float(amax_bits), &e);  // amax = f 2^e, f in [1/2, 1)
+  e = 14 - e;
+  return e > 100 ? 100 : (e < -100 ? -100 : e);
+}
+__device__ __forceinline__ float ce_pow2(int e) { return ldexpf(1.f, e); }
+
+__device__ __forceinline__ unsigned finite_bits(float v) {
+  const unsigned b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// largest finite |a| of a [rows, cols] fp32 matrix into *word
+__global__ void __launch_bounds__(256) ce_amax_kernel(const float *a, int64_t rows, int cols,
+                                                      int64_t ld, unsigned *word) {
+  unsigned best = 0;
+  const int64_t n = rows * cols;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / cols;
+    const unsigned b = finite_bits(a[r * ld + (i - r * cols)]);
+    best = b > best ? b : best;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned b = __shfl_xor_sync(kFull, best, o);
+    best = b > best ? b : best;
+  }
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(word, best);  // a maximum: any order
+}
+
+// a 2^e = hi + lo in fp16, rows padded to ldp with zeros
+__global__ void __launch_bounds__(256) ce_split_kernel(const float *a, int64_t rows, int cols,
+                                                       int64_t ld, int ldp, const unsigned *word,
+                                                       __half *hi, __half *lo) {
+  const float sc = ce_pow2(ce_exp(*word));
+  const int64_t n = rows * ldp;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / ldp;
+    const int c = (int)(i - r * ldp);
+    const float v = c < cols ? a[r * ld + c] * sc : 0.f;
+    const __half h = __float2half_rn(v);
+    hi[i] = h;
+    lo[i] = __float2half_rn(v - __half2float(h));
+  }
+}
+
+// z = s acc or c tanh(s acc / c), in units of log 2
+struct CeLogit {
+  float scale, cap;
+  const CeHead *head;  // split scales; null for 16-bit inputs
+  __device__ __forceinline__ float factor() const {
+    const float f = head ? ce_pow2(-ce_exp(head->amax_x) - ce_exp(head->amax_w)) : 1.f;
+    return cap > 0.f ? scale * f / cap : scale * f * kLog2e;
+  }
+  // acc times factor() -> t; `th` is tanh where capped
+  __device__ __forceinline__ float logit2(float u, float &th) const {
+    if (cap > 0.f) {
+      th = tanhf(u);
+      return th * (cap * kLog2e);
+    }
+    th = 0.f;
+    return u;
+  }
+};
+
+// Forward epilogue: maximum and sum of 2^(t - m) over the thread's columns.
+struct CeEpiLse {
+  CeLogit lg;
+  int64_t rows, vocab;
+  const int64_t *target;
+  float2 *part;  // [2 n_tiles][ld]
+  int64_t ld;
+  float *zt;  // [rows] t at the label
+  int TN;
+  __device__ __forceinline__ void operator()(const GmUnit &w, int row, int col, uint32_t taddr) const {
+    const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
+    const float f = lg.factor();
+    const int64_t tg = r < rows ? target[r] : -1;
+    float m = -INFINITY, s = 0.f;
+    for (int c = 0; c < TN / 2; c += 32) {
+      float v[32];
+      tmem_ld32(taddr + c, v);
+      const int64_t left = vocab - (c0 + c);
+      float th;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = lg.logit2(v[j] * f, th);
+      if (left < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j >= left) v[j] = -INFINITY;
+      }
+      const int64_t at = tg - (c0 + c);
+      if (at >= 0 && at < 32 && at < left) {
+        float z = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z = j == (int)at ? v[j] : z;
+        zt[r] = z;
+      }
+      float mx = v[0];
+#pragma unroll
+      for (int j = 1; j < 32; ++j) mx = fmaxf(mx, v[j]);
+      const float mn = fmaxf(m, mx);
+      if (mn > -INFINITY || mx != mx) {
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          a += ex2(v[j] - mn);
+          b += ex2(v[j + 1] - mn);
+        }
+        s = s * (m > -INFINITY ? ex2(m - mn) : 0.f) + (a + b);
+        m = mn;
+      }
+    }
+    part[((int64_t)w.n * 2 + (col ? 1 : 0)) * ld + r] = make_float2(m, s);
+  }
+};
+
+// Joins the column tiles of 32 rows of a pass over rows [r0, r0 + pass_rows); losses, lse, the rows' (m, sum) for the
+// backward, and the sum or mean of the losses (block sums in fp64, added in
+// block order by the block that finishes last).
+__global__ void __launch_bounds__(1024) ce_rows_kernel(const float2 *part, int64_t ld, int parts,
+                                                       int64_t r0, int64_t pass_rows,
+                                                       int64_t rows, int64_t vocab,
+                                                       const int64_t *target, int64_t ignore,
+                                                       const float *zt, int reduction,
+                                                       float *loss, float *lse, float2 *stats,
+                                                       CeHead *head, double2 *blocks) {
+  __shared__ float2 sh[32][33];
+  __shared__ double red[32 * 2];
+  __shared__ bool last;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t in_pass = blockIdx.x * (int64_t)32 + tx, r = r0 + in_pass;
+  const unsigned all_blocks = (unsigned)ceil_div(rows, (int64_t)32);
+  float m = -INFINITY, s = 0.f;
+  if (in_pass < pass_rows) {
+    for (int p = ty; p < parts; p += 32) {
+      const float2 v = part[p * ld + in_pass];
+      const float mn = fmaxf(m, v.x);
+      if (mn > -INFINITY || v.y != v.y) {
+        s = (m > -INFINITY ? s * ex2(m - mn) : 0.f) + v.y * (v.x > -INFINITY ? ex2(v.x - mn) : 1.f);
+        m = mn;
+      }
+    }
+  }
+  sh[ty][tx] = make_float2(m, s);
+  __syncthreads();
+  if (ty == 0) {
+    double row_loss = 0.0;
+    long long labelled = 0;
+    if (in_pass < pass_rows) {
+      float M = -INFINITY;
+      for (int k = 0; k < 32; ++k) M = fmaxf(M, sh[k][tx].x);
+      float S = 0.f;
+      for (int k = 0; k < 32; ++k) {
+        const float2 v = sh[k][tx];
+        S += v.x > -INFINITY ? v.y * ex2(v.x - M) : v.y;
+      }
+      const double l = (double)M * kLn2 + log((double)S);
+      const int64_t t = target[r];
+      if (t != ignore) {
+        labelled = 1;
+        // a label outside the table is never read: its loss is NaN
+        row_loss = t >= 0 && t < vocab ? l - (double)zt[r] * kLn2 : (double)NAN;
+      }
+      lse[r] = (float)l;
+      stats[r] = make_float2(M, S);
+      if (reduction == RA_REDUCE_NONE) loss[r] = (float)row_loss;
+    }
+    if (reduction != RA_REDUCE_NONE) {
+      const double sum = warp_sum(row_loss);
+      const double cnt = warp_sum((double)labelled);
+      if (tx == 0) {
+        blocks[r0 / 32 + blockIdx.x] = make_double2(sum, cnt);
+        __threadfence();
+        last = atomicAdd(&head->ticket, 1u) == all_blocks - 1;
+      }
+    }
+  }
+  if (reduction == RA_REDUCE_NONE) return;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double acc[2] = {0.0, 0.0};
+  for (int64_t b = threadIdx.x; b < all_blocks; b += 1024) {
+    const double2 v = __ldcg(blocks + b);
+    acc[0] += v.x;
+    acc[1] += v.y;
+  }
+  block_sum_n<2>(acc, red);
+  if (threadIdx.x == 0) {
+    *loss = (float)(reduction == RA_REDUCE_MEAN ? acc[0] / acc[1] : acc[0]);
+    head->count = (long long)acc[1];
+  }
+}
+
+// Per row (gl + ge, gl) of the backward; 0 for a row without a label, NaN
+// for a label outside the table (as its loss).
+__global__ void __launch_bounds__(256) ce_coef_kernel(const int64_t *target, int64_t rows,
+                                                      int64_t vocab, int64_t ignore, int reduction,
+                                                      const float *g_loss, const float *g_lse,
+                                                      CeHead *head, float2 *coef) {
+  unsigned best = 0;
+  for (int64_t r = blockIdx.x * (int64_t)256 + threadIdx.x; r < rows;
+       r += (int64_t)gridDim.x * 256) {
+    const int64_t t = target[r];
+    float gl = 0.f;
+    if (g_loss != nullptr && t != ignore) {
+      gl = g_loss[reduction == RA_REDUCE_NONE ? r : 0];
+      if (reduction == RA_REDUCE_MEAN) gl = (float)((double)gl / (double)head->count);
+      if (t < 0 || t >= vocab) gl = NAN;
+    }
+    const float c = gl + (g_lse != nullptr ? g_lse[r] : 0.f);
+    coef[r] = make_float2(c, gl);
+    const unsigned a = finite_bits(c), b = finite_bits(gl);
+    best = a > best ? a : best;
+    best = b > best ? b : best;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned b = __shfl_xor_sync(kFull, best, o);
+    best = b > best ? b : best;
+  }
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(&head->amax_g, best);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Backward epilogue: du of one piece of the vocabulary, in 16 bits.
+template <bool BF16, bool SPLIT>
+struct CeEpiGrad {
+  CeLogit lg;
+  int64_t rows, vocab, v0;  // v0: the piece's first column
+  const int64_t *target;
+  const float2 *stats, *coef;
+  const CeHead *head;
+  uint16_t *hi, *lo;  // [128 m_tiles, ldg]
+  int64_t ldg;
+  int TN;
+  __device__ __forceinline__ void operator()(const GmUnit &w, int row, int col, uint32_t taddr) const {
+    const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
+    const float f = lg.factor();
+    float2 cf = make_float2(0.f, 0.f), st = make_float2(0.f, 1.f);
+    int64_t tg = -1;
+    if (r < rows) {
+      cf = coef[r];
+      st = stats[r];
+      tg = target[r] - v0;
+    }
+    const bool off = cf.x == 0.f && cf.y == 0.f;
+    if (!BF16) {
+      const float g = ce_pow2(ce_exp(head->amax_g));
+      cf.x *= g;
+      cf.y *= g;
+    }
+    const float pc = cf.x / st.y;
+    uint16_t *ph = hi + r * ldg + c0;
+    uint16_t *pl = SPLIT ? lo + r * ldg + c0 : nullptr;
+    for (int c = 0; c < TN / 2; c += 32) {
+      float v[32];
+      tmem_ld32(taddr + c, v);
+      const int64_t at = tg - (c0 + c);
+      const bool hit = at >= 0 && at < 32;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        float th;
+        const float t = lg.logit2(v[j] * f, th);
+        float g = ex2(t - st.x) * pc;
+        if (hit && j == (int)at) g -= cf.y;
+        if (lg.cap > 0.f) g *= 1.f - th * th;
+        v[j] = off ? 0.f : g;
+      }
+      uint32_t h[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        h[j] = BF16 ? pack_bf16(v[2 * j], v[2 * j + 1]) : pack_f16(v[2 * j], v[2 * j + 1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        reinterpret_cast<uint4 *>(ph + c)[j] =
+            make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+      if (SPLIT) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+          h[j] = pack_f16(v[2 * j] - b.x, v[2 * j + 1] - b.y);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          reinterpret_cast<uint4 *>(pl + c)[j] =
+              make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void store_as(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_as(__half *p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_as(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+
+// what undoes the scales of a product: s 2^-(exponents)
+struct CeAlpha {
+  float scale;
+  const unsigned *a, *b;  // amax words, or null
+  __device__ __forceinline__ float value() const {
+    return scale * ce_pow2(-(a ? ce_exp(*a) : 0) - (b ? ce_exp(*b) : 0));
+  }
+};
+
+// Gradient epilogue: the finished product, or one K slice's sum over the
+// pieces (`add`: later pieces).
+template <class T>
+struct CeEpiOut {
+  CeAlpha alpha;
+  int64_t rows, cols;
+  T *out;       // [rows, cols], or null
+  float *part;  // [slices][rows, cols]
+  int add, TN;
+  __device__ __forceinline__ void operator()(const GmUnit &w, int row, int col, uint32_t taddr) const {
+    const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
+    const float al = out ? alpha.value() : 1.f;
+    float *pp = part + ((int64_t)w.slice * rows + r) * cols + c0;
+    T *po = out + r * cols + c0;
+    const bool wide = (cols & 3) == 0;  // 16-byte aligned fp32 rows
+    for (int c = 0; c < TN / 2; c += 32) {
+      float v[32];
+      tmem_ld32(taddr + c, v);
+      const int64_t left = cols - (c0 + c);
+      if (r >= rows || left <= 0) continue;
+      if (out != nullptr) {
+        if (left >= 32 && (cols & 7) == 0) {
+          if (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              reinterpret_cast<float4 *>(po + c)[j] = make_float4(
+                  v[4 * j] * al, v[4 * j + 1] * al, v[4 * j + 2] * al, v[4 * j + 3] * al);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              alignas(16) T t[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) store_as(t + k, v[8 * j + k] * al);
+              reinterpret_cast<uint4 *>(po + c)[j] = *reinterpret_cast<const uint4 *>(t);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < left) store_as(po + c + j, v[j] * al);
+        }
+      } else if (wide && left >= 32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float4 *q = reinterpret_cast<float4 *>(pp + c) + j;
+          float4 o = add ? *q : make_float4(0.f, 0.f, 0.f, 0.f);
+          *q = make_float4(o.x + v[4 * j], o.y + v[4 * j + 1], o.z + v[4 * j + 2],
+                           o.w + v[4 * j + 3]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < left) pp[c + j] = v[j] + (add ? pp[c + j] : 0.f);
+      }
+    }
+  }
+};
+
+// out = alpha (sum of the K slices, in order)
+template <class T>
+__global__ void __launch_bounds__(256) ce_join_kernel(const float *part, int slices, int64_t n,
+                                                      CeAlpha alpha, T *out) {
+  const float al = alpha.value();
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float v = 0.f;
+    for (int s = 0; s < slices; ++s) v += part[s * n + i];
+    store_as(out + i, v * al);
+  }
+}
+
+}  // namespace ra

@@ -1,0 +1,273 @@
+// ra_gemm16.cuh -- persistent tensor-core matrix product with a fused
+// epilogue: the three products of the linear cross entropy (ra_ce.cuh).
+//
+//   D[m, n] = sum_k A[m, k] B[n, k]      16-bit operands, fp32 accumulators
+//
+// Either operand may lie K-major (rows of K in memory) or MN-major (rows of
+// M or N), so that G W and G^T X need no transposed copies.  Operands come
+// as tensor maps with 128-byte swizzle; elements outside a map read as zero,
+// so no edge of M, N or K is special before the epilogue.
+//
+// fp32 inputs come as two fp16 halves (a = hi + lo, 22 significant bits, one
+// power-of-two scale per tensor) and three products hi hi + hi lo + lo hi,
+// which are three passes over K into the same accumulators.
+//
+// Roles (320 threads, one CTA per SM, persistent over (tile, K slice) units):
+//   warps 0-7  epilogue: warp w reads TMEM lanes 32 (w % 4).. and half w / 4
+//              of the tile's columns
+//   warp 8     lane 0 copies operand tiles into the shared-memory ring
+//   warp 9     lane 0 issues the MMAs
+// Two accumulators in TMEM: the epilogue of one unit runs under the MMAs of
+// the next.  Every wait is bounded; on expiry the CTA records the timeout,
+// drains its copies, frees its TMEM and returns.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ra_common.cuh"
+#include "ra_tcprim.cuh"
+
+namespace ra {
+
+constexpr int kGmM = 128, kGmK = 64, kGmStages = 4;
+constexpr int kGmThreads = 320, kGmEpiWarps = 8;
+constexpr int kGmABytes = kGmM * kGmK * 2;
+
+__host__ __device__ constexpr int gm_stage_bytes(int TN) { return kGmABytes + TN * kGmK * 2; }
+__host__ __device__ constexpr size_t gm_smem_bytes(int TN) {
+  return 1024 + (size_t)kGmStages * gm_stage_bytes(TN) + 256;
+}
+
+// The units of one launch: tiles of 128 x TN, each cut into `slices` of K.
+// m runs fastest where the B operand is the large one (m_fast), so that
+// concurrent CTAs share a B tile.
+struct GmShape {
+  int m_tiles, n_tiles, k_steps, slices, products;
+  int m_fast;
+  unsigned spin_limit;
+  int *status;
+};
+
+struct GmMaps {
+  CUtensorMap a_hi, a_lo, b_hi, b_lo;
+};
+
+__host__ __device__ constexpr uint32_t gm_idesc(int N, bool bf16, bool a_mn, bool b_mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) |
+         (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kGmM >> 4) << 24);
+}
+// 128-byte swizzled operand tiles.  K-major: rows of 64 k (128 bytes), eight
+// rows an atom, atoms 1024 bytes apart.  MN-major: chunks of 64 m (or n),
+// each 64 k rows of 128 bytes; 8-k groups 1024 bytes apart, chunks 8192.
+__device__ __forceinline__ uint64_t gm_desc(uint32_t saddr, bool mn) {
+  const uint64_t lbo = mn ? 8192u >> 4 : 1u, sbo = 1024u >> 4;
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (lbo << 16) | (sbo << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+__device__ __forceinline__ void gm_mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                       uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(mbar)
+      : "memory");
+}
+
+struct GmUnit {
+  int m, n, slice, k0, k1;
+};
+__device__ __forceinline__ GmUnit gm_unit(const GmShape &s, int u) {
+  GmUnit r;
+  r.slice = u % s.slices;
+  const int t = u / s.slices;
+  if (s.m_fast) {
+    r.m = t % s.m_tiles;
+    r.n = t / s.m_tiles;
+  } else {
+    r.n = t % s.n_tiles;
+    r.m = t / s.n_tiles;
+  }
+  r.k0 = (int)((int64_t)s.k_steps * r.slice / s.slices);
+  r.k1 = (int)((int64_t)s.k_steps * (r.slice + 1) / s.slices);
+  return r;
+}
+
+// Epi: operator()(unit, row in tile, first column in tile, TMEM address of
+// the thread's lane at that column, columns) for one thread's row and its
+// half of the tile's columns.
+template <int TN, bool BF16, bool A_MN, bool B_MN, class Epi>
+__global__ void __launch_bounds__(kGmThreads, 1)
+    gemm16_kernel(const __grid_constant__ GmMaps maps, const GmShape s,
+                  const __grid_constant__ Epi epi) {
+  extern __shared__ uint8_t gm_raw[];
+  const uint32_t raw = smem_u32(gm_raw);
+  const uint32_t base = (raw + 1023) & ~1023u;
+  constexpr int kStage = gm_stage_bytes(TN);
+  constexpr int kTmemCols = 2 * TN;
+  const uint32_t bars = base + kGmStages * kStage;
+  // full[4] empty[4] accfull[2] accempty[2], then the TMEM address and abort flag
+  const uint32_t full = bars, empty = bars + 8 * kGmStages, accfull = bars + 16 * kGmStages,
+                 accempty = accfull + 16, tmem_slot = accempty + 16;
+  volatile int *abort_flag = (volatile int *)(gm_raw + (tmem_slot + 4 - raw));
+  volatile uint32_t *tmem_addr = (volatile uint32_t *)(gm_raw + (tmem_slot - raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = s.m_tiles * s.n_tiles * s.slices;
+
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tmem_slot),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kGmStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(accfull + 8 * i, 1);
+      mbar_init(accempty + 8 * i, kGmEpiWarps);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_addr;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      int issued = 0;  // operand tiles issued; tile i sits in stage i % kGmStages
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        const GmUnit w = gm_unit(s, u);
+        for (int p = 0; ok && p < s.products; ++p) {
+          const CUtensorMap *ma = p == 2 ? &maps.a_lo : &maps.a_hi;
+          const CUtensorMap *mb = p == 1 ? &maps.b_lo : &maps.b_hi;
+          for (int k = w.k0; k < w.k1; ++k, ++issued) {
+            const int st = issued % kGmStages;
+            if (issued >= kGmStages &&
+                !ws_wait(empty + 8 * st, ((issued / kGmStages) - 1) & 1, abort_flag,
+                         s.spin_limit)) {
+              ok = false;
+              break;
+            }
+            const uint32_t a = base + st * kStage, b = a + kGmABytes, bar = full + 8 * st;
+            mbar_expect_tx(bar, kStage);
+            if (A_MN) {
+#pragma unroll
+              for (int c = 0; c < kGmM / 64; ++c)
+                tma_2d(a + c * 8192, ma, w.m * kGmM + c * 64, k * kGmK, bar);
+            } else {
+              tma_2d(a, ma, k * kGmK, w.m * kGmM, bar);
+            }
+            if (B_MN) {
+#pragma unroll
+              for (int c = 0; c < TN / 64; ++c)
+                tma_2d(b + c * 8192, mb, w.n * TN + c * 64, k * kGmK, bar);
+            } else {
+              tma_2d(b, mb, k * kGmK, w.n * TN, bar);
+            }
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      // a CTA does not leave while copies into its shared memory are in flight
+      const int first = issued > kGmStages ? issued - kGmStages : 0;
+      for (int i = first; i < issued; ++i)
+        if (!mbar_wait(full + 8 * (i % kGmStages), (i / kGmStages) & 1, s.spin_limit)) ok = false;
+      if (!ok) atomicOr(s.status, 1);
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = gm_idesc(TN, BF16, A_MN, B_MN);
+      int used = 0, t = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++t) {
+        const GmUnit w = gm_unit(s, u);
+        const int buf = t & 1;
+        if (t >= 2 && !ws_wait(accempty + 8 * buf, ((t >> 1) - 1) & 1, abort_flag, s.spin_limit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * TN;
+        const int steps = s.products * (w.k1 - w.k0);
+        for (int i = 0; i < steps; ++i, ++used) {
+          const int st = used % kGmStages;
+          if (!ws_wait(full + 8 * st, (used / kGmStages) & 1, abort_flag, s.spin_limit)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = base + st * kStage, b = a + kGmABytes;
+          const uint64_t da = gm_desc(a, A_MN), db = gm_desc(b, B_MN);
+#pragma unroll
+          for (int kk = 0; kk < kGmK / 16; ++kk) {
+            // 16 k: 32 bytes along a K-major row, two 8-k groups MN-major
+            gm_mma(acc, da + (uint64_t)(kk * (A_MN ? 2048 : 32) >> 4),
+                   db + (uint64_t)(kk * (B_MN ? 2048 : 32) >> 4), idesc, i > 0 || kk > 0);
+          }
+          tc_commit(empty + 8 * st);
+        }
+        if (ok) tc_commit(accfull + 8 * buf);
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        atomicOr(s.status, 1);
+      }
+    }
+  } else {
+    const int half = warp >> 2;
+    const int row = 32 * (warp & 3) + lane;
+    int t = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++t) {
+      const GmUnit w = gm_unit(s, u);
+      const int buf = t & 1;
+      const bool got = ws_wait(accfull + 8 * buf, (t >> 1) & 1, abort_flag, s.spin_limit);
+      if (!__all_sync(kFull, got)) {
+        *abort_flag = 1;
+        if (lane == 0) atomicOr(s.status, 1);
+        break;
+      }
+      tc_fence_after();
+      epi(w, row, half * (TN / 2),
+          tmem + buf * TN + half * (TN / 2) + ((uint32_t)(32 * (warp & 3)) << 16));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(accempty + 8 * buf);
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (*abort_flag && warp == 9 && lane == 0) {
+    // products in flight still write TMEM and read shared memory: one more
+    // commit completes after all of them
+    const uint32_t bar = accempty;  // no role uses it any more
+    asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+    mbar_init(bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc_commit(bar);
+    mbar_wait(bar, 0, s.spin_limit);
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols));
+  }
+}
+
+}  // namespace ra
