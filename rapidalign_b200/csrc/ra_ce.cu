@@ -50,8 +50,10 @@ CeState ce_state(const ra_ce_desc *d) {
 }
 
 // Width of the tiles over n columns: 256 unless half of a last tile or of
-// the last wave of CTAs would idle.
-int tile_width(int64_t m_tiles, int64_t n, int sms) {
+// the last wave of CTAs would idle.  Logits of pairs take 128: their rounds
+// and the epilogue's arithmetic share the registers (256 spills 5 KB).
+int tile_width(int64_t m_tiles, int64_t n, int sms, bool pair_logits = false) {
+  if (pair_logits) return 128;
   auto waves = [&](int tn) {
     const int64_t t = m_tiles * ceil_div(n, (int64_t)tn);
     return (double)(ceil_div(t, (int64_t)sms) * tn);
@@ -69,7 +71,7 @@ int k_slices(int64_t tiles, int64_t steps, int sms) {
 }
 
 struct CePlan {
-  int sms, products, elem;
+  int sms, elem;
   int64_t mt;             // 128-row tiles of x
   int tn_z, parts;        // forward
   int64_t piece, ldg;     // vocabulary piece (columns of du)
@@ -85,11 +87,10 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   CePlan p{};
   p.sms = sms;
   const bool split = d->dtype == RA_F32;
-  p.products = split ? 3 : 1;
   p.elem = split ? 4 : 2;
   p.mt = ceil_div(d->rows, (int64_t)kGmM);
   const int64_t pass = std::min<int64_t>(d->rows, kCeRowsPerPass);
-  p.tn_z = tile_width(ceil_div(pass, (int64_t)kGmM), d->vocab, sms);
+  p.tn_z = tile_width(ceil_div(pass, (int64_t)kGmM), d->vocab, sms, split);
   p.parts = 2 * (int)ceil_div(d->vocab, (int64_t)p.tn_z);
   size_t o = 0;
   p.f_part = o;
@@ -131,10 +132,10 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   return p;
 }
 
-template <int TN, bool BF16, bool A_MN, bool B_MN, class Epi>
+template <int TN, bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
 int launch_gemm(const GmMaps &maps, const GmShape &s, const Epi &epi, int sms, cudaStream_t st) {
   const size_t smem = gm_smem_bytes(TN);
-  auto k = gemm16_kernel<TN, BF16, A_MN, B_MN, Epi>;
+  auto k = gemm16_kernel<TN, BF16, PAIRS, A_MN, B_MN, Epi>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
     return RA_ERR_CUDA;
@@ -144,15 +145,11 @@ int launch_gemm(const GmMaps &maps, const GmShape &s, const Epi &epi, int sms, c
   return launched();
 }
 
-template <bool A_MN, bool B_MN, class Epi>
-int launch_gemm(bool bf16, int tn, const GmMaps &maps, const GmShape &s, Epi epi, int sms,
+template <bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
+int launch_gemm(int tn, const GmMaps &maps, const GmShape &s, const Epi &epi, int sms,
                 cudaStream_t st) {
-  epi.TN = tn;
-  if (tn == 256)
-    return bf16 ? launch_gemm<256, true, A_MN, B_MN>(maps, s, epi, sms, st)
-                : launch_gemm<256, false, A_MN, B_MN>(maps, s, epi, sms, st);
-  return bf16 ? launch_gemm<128, true, A_MN, B_MN>(maps, s, epi, sms, st)
-              : launch_gemm<128, false, A_MN, B_MN>(maps, s, epi, sms, st);
+  return tn == 256 ? launch_gemm<256, BF16, PAIRS, A_MN, B_MN>(maps, s, epi, sms, st)
+                   : launch_gemm<128, BF16, PAIRS, A_MN, B_MN>(maps, s, epi, sms, st);
 }
 
 struct Operands {  // 16-bit x and w, or their halves
@@ -190,7 +187,7 @@ CeLogit logit_of(const ra_ce_desc *d, const CeHead *head) {
 
 GmShape shape_of(const ra_ce_desc *d, const CePlan &p, int64_t mt, int64_t nt, int64_t k, int slices,
                  int m_fast) {
-  return {(int)mt, (int)nt, (int)ceil_div(k, (int64_t)kGmK), slices, p.products, m_fast,
+  return {(int)mt, (int)nt, (int)ceil_div(k, (int64_t)kGmK), slices, m_fast,
           kTcSpinLimit, d->status};
 }
 
@@ -203,22 +200,23 @@ int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int
   float *px = (float *)(ws + p.b_px), *pw = (float *)(ws + p.b_pw);
   const int dim = d->dim;
   const int64_t nt = ceil_div((int64_t)dim, (int64_t)p.tn_d);
-  const unsigned *ag = BF16 ? nullptr : &head->amax_g;
-  const CeAlpha al_x{d->scale, ag, SPLIT ? &head->amax_w : nullptr};
-  const CeAlpha al_w{d->scale, ag, SPLIT ? &head->amax_x : nullptr};
+  const float undo = d->scale / kCeGradScale<BF16>;
+  const CeAlpha al_x{undo, &head->amax_g, SPLIT ? &head->amax_w : nullptr};
+  const CeAlpha al_w{undo, &head->amax_g, SPLIT ? &head->amax_x : nullptr};
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, cols = std::min<int64_t>(p.piece, d->vocab - v0);
     GmMaps m;
-    const int tn = tile_width(p.mt, cols, p.sms);
+    const int tn = tile_width(p.mt, cols, p.sms, SPLIT);
     if (!logit_maps(&m, BF16, op, dim, 0, d->rows, v0, cols, tn)) return RA_ERR_INVALID_ARGUMENT;
     CeEpiGrad<BF16, SPLIT> eg{logit_of(d, head), d->rows, d->vocab, v0, target,
                               (const float2 *)(state + sl.stats), (const float2 *)(ws + p.b_coef),
-                              head, gh, gl, p.ldg, 0};
+                              head, gh, gl, p.ldg};
     int rc;
     const GmShape sz = shape_of(d, p, p.mt, ceil_div(cols, (int64_t)tn), dim, 1, 1);
-    eg.TN = tn;
-    rc = tn == 256 ? launch_gemm<256, BF16, false, false>(m, sz, eg, p.sms, st)
-                   : launch_gemm<128, BF16, false, false>(m, sz, eg, p.sms, st);
+    if constexpr (SPLIT)
+      rc = launch_gemm<128, BF16, true, false, false>(m, sz, eg, p.sms, st);
+    else
+      rc = launch_gemm<BF16, false, false, false>(tn, m, sz, eg, p.sms, st);
     if (rc) return rc;
     if (dx != nullptr) {
       if (!map16(&m.a_hi, BF16, gh, d->rows, cols, p.ldg, kGmM) ||
@@ -227,10 +225,9 @@ int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int
           !map16(&m.b_lo, BF16, op.wl + v0 * op.ldw, cols, dim, op.ldw, kGmK))
         return RA_ERR_INVALID_ARGUMENT;
       const int slices = std::min<int>(p.sx, (int)ceil_div(cols, (int64_t)kGmK));
-      CeEpiOut<T> eo{al_x, d->rows, dim, p.direct_x ? dx : nullptr, px, i > 0, p.tn_d};
+      CeEpiOut<T> eo{al_x, d->rows, dim, p.direct_x ? dx : nullptr, px, i > 0};
       const GmShape s = shape_of(d, p, p.mt, nt, cols, slices, 0);
-      rc = p.tn_d == 256 ? launch_gemm<256, BF16, false, true>(m, s, eo, p.sms, st)
-                         : launch_gemm<128, BF16, false, true>(m, s, eo, p.sms, st);
+      rc = launch_gemm<BF16, SPLIT, false, true>(p.tn_d, m, s, eo, p.sms, st);
       if (rc) return rc;
     }
     if (dw != nullptr) {
@@ -239,10 +236,9 @@ int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int
           !map16(&m.b_hi, BF16, op.xh, d->rows, dim, op.ldx, kGmK) ||
           !map16(&m.b_lo, BF16, op.xl, d->rows, dim, op.ldx, kGmK))
         return RA_ERR_INVALID_ARGUMENT;
-      CeEpiOut<T> eo{al_w, cols, dim, p.direct_w ? dw + v0 * dim : nullptr, pw, 0, p.tn_d};
+      CeEpiOut<T> eo{al_w, cols, dim, p.direct_w ? dw + v0 * dim : nullptr, pw, 0};
       const GmShape s = shape_of(d, p, ceil_div(cols, (int64_t)kGmM), nt, d->rows, p.sw, 0);
-      rc = p.tn_d == 256 ? launch_gemm<256, BF16, true, true>(m, s, eo, p.sms, st)
-                         : launch_gemm<128, BF16, true, true>(m, s, eo, p.sms, st);
+      rc = launch_gemm<BF16, SPLIT, true, true>(p.tn_d, m, s, eo, p.sms, st);
       if (rc) return rc;
       if (!p.direct_w) {
         ce_join_kernel<T><<<grid_for(cols * dim, p.sms), 256, 0, st>>>(pw, p.sw, cols * dim, al_w,
@@ -321,10 +317,13 @@ int ra_ce_forward(const ra_ce_desc *d, const void *x, const void *w, const int64
     GmMaps m;
     if (!logit_maps(&m, bf16, op, d->dim, r0, rows, 0, d->vocab, p.tn_z))
       return RA_ERR_INVALID_ARGUMENT;
-    CeEpiLse e{logit_of(d, head), rows, d->vocab, target + r0, part, mt * kGmM, zt + r0, 0};
+    CeEpiLse e{logit_of(d, head), rows, d->vocab, target + r0, part, mt * kGmM, zt + r0};
     const GmShape s =
         shape_of(d, p, mt, ceil_div(d->vocab, (int64_t)p.tn_z), d->dim, 1, 1);
-    if ((rc = launch_gemm<false, false>(bf16, p.tn_z, m, s, e, p.sms, st))) return rc;
+    rc = d->dtype == RA_F32 ? launch_gemm<128, false, true, false, false>(m, s, e, p.sms, st)
+         : bf16             ? launch_gemm<true, false, false, false>(p.tn_z, m, s, e, p.sms, st)
+                            : launch_gemm<false, false, false, false>(p.tn_z, m, s, e, p.sms, st);
+    if (rc) return rc;
     ce_rows_kernel<<<(unsigned)ceil_div(rows, (int64_t)32), 1024, 0, st>>>(
         part, mt * kGmM, p.parts, r0, rows, d->rows, d->vocab, target, d->ignore_index, zt,
         d->reduction, loss, lse, (float2 *)(sb + sl.stats), head, (double2 *)(ws + p.f_blocks));

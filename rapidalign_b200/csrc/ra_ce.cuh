@@ -15,9 +15,13 @@
 // bits (with the rows' coefficients, so both products read it as it is), then
 // dx += du W and dw = du^T X.  Sums over pieces and K slices have one writer
 // each and a fixed order: no atomics, bitwise repeatable.
-// du is rounded to the operands' 16-bit type (half a step, 2^-9 or 2^-12
-// relative, independent from element to element, so sums of many keep less);
-// for fp32 inputs du, x and w are fp16 pairs hi + lo (22 bits).
+// du is rounded to the operands' 16-bit type (half a step, 2^-8 or 2^-11 of an
+// element).  It is held divided by the largest coefficient: a mean's rows then
+// have coefficient 1, and the label's element, which outweighs the others, is
+// near -1 and exact, where 1 / count would round alike in every row (bf16
+// gradients off by 3.9e-3 instead of 2e-3).  In fp16 2^13 more keeps small
+// elements normal.  For fp32 inputs du, x and w are fp16 pairs hi + lo (22
+// bits).
 #pragma once
 
 #include "ra_gemm16.cuh"
@@ -31,13 +35,13 @@ constexpr double kLn2 = 0.6931471805599453;
 // header of the state buffer
 struct CeHead {
   unsigned amax_x, amax_w;  // bits of the largest finite |x|, |w| (fp32 inputs)
-  unsigned amax_g;          // of the upstream coefficients (backward)
+  unsigned amax_g;          // bits of the largest finite coefficient (backward)
   unsigned ticket;          // blocks of ce_rows_kernel done
   long long count;          // rows with a label
 };
 
-// Power of two that brings a largest magnitude into [2^13, 2^14): with twice
-// that (du) still below the fp16 maximum 65504.
+// Power of two that brings a largest magnitude into [2^13, 2^14), below the
+// fp16 maximum 65504.
 __device__ __forceinline__ int ce_exp(unsigned amax_bits) {
   if (amax_bits == 0) return 0;
   int e;
@@ -113,15 +117,16 @@ struct CeEpiLse {
   float2 *part;  // [2 n_tiles][ld]
   int64_t ld;
   float *zt;  // [rows] t at the label
-  int TN;
-  __device__ __forceinline__ void operator()(const GmUnit &w, int row, int col, uint32_t taddr) const {
+  template <int TN, class Src>
+  __device__ __forceinline__ void run(const GmUnit &w, int row, int col, const Src &src) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
     const float f = lg.factor();
     const int64_t tg = r < rows ? target[r] : -1;
     float m = -INFINITY, s = 0.f;
+#pragma unroll Src::unroll
     for (int c = 0; c < TN / 2; c += 32) {
       float v[32];
-      tmem_ld32(taddr + c, v);
+      src.get(c, v);
       const int64_t left = vocab - (c0 + c);
       float th;
 #pragma unroll
@@ -274,6 +279,9 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+template <bool BF16>
+constexpr float kCeGradScale = BF16 ? 1.f : 8192.f;  // |du| < 2 times this
+
 // Backward epilogue: du of one piece of the vocabulary, in 16 bits.
 template <bool BF16, bool SPLIT>
 struct CeEpiGrad {
@@ -284,8 +292,8 @@ struct CeEpiGrad {
   const CeHead *head;
   uint16_t *hi, *lo;  // [128 m_tiles, ldg]
   int64_t ldg;
-  int TN;
-  __device__ __forceinline__ void operator()(const GmUnit &w, int row, int col, uint32_t taddr) const {
+  template <int TN, class Src>
+  __device__ __forceinline__ void run(const GmUnit &w, int row, int col, const Src &src) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
     const float f = lg.factor();
     float2 cf = make_float2(0.f, 0.f), st = make_float2(0.f, 1.f);
@@ -296,17 +304,16 @@ struct CeEpiGrad {
       tg = target[r] - v0;
     }
     const bool off = cf.x == 0.f && cf.y == 0.f;
-    if (!BF16) {
-      const float g = ce_pow2(ce_exp(head->amax_g));
-      cf.x *= g;
-      cf.y *= g;
-    }
+    const float top = __uint_as_float(head->amax_g);
+    cf.x = cf.x / top * kCeGradScale<BF16>;
+    cf.y = cf.y / top * kCeGradScale<BF16>;
     const float pc = cf.x / st.y;
     uint16_t *ph = hi + r * ldg + c0;
     uint16_t *pl = SPLIT ? lo + r * ldg + c0 : nullptr;
+#pragma unroll Src::unroll
     for (int c = 0; c < TN / 2; c += 32) {
       float v[32];
-      tmem_ld32(taddr + c, v);
+      src.get(c, v);
       const int64_t at = tg - (c0 + c);
       const bool hit = at >= 0 && at < 32;
 #pragma unroll
@@ -345,12 +352,13 @@ __device__ __forceinline__ void store_as(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store_as(__half *p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_as(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
-// what undoes the scales of a product: s 2^-(exponents)
+// what undoes the scales of a product: s top / kCeGradScale 2^-exponent
 struct CeAlpha {
   float scale;
-  const unsigned *a, *b;  // amax words, or null
+  const unsigned *top;    // the largest coefficient
+  const unsigned *other;  // amax word of the other operand, or null
   __device__ __forceinline__ float value() const {
-    return scale * ce_pow2(-(a ? ce_exp(*a) : 0) - (b ? ce_exp(*b) : 0));
+    return scale * __uint_as_float(*top) * ce_pow2(other ? -ce_exp(*other) : 0);
   }
 };
 
@@ -362,16 +370,18 @@ struct CeEpiOut {
   int64_t rows, cols;
   T *out;       // [rows, cols], or null
   float *part;  // [slices][rows, cols]
-  int add, TN;
-  __device__ __forceinline__ void operator()(const GmUnit &w, int row, int col, uint32_t taddr) const {
+  int add;
+  template <int TN, class Src>
+  __device__ __forceinline__ void run(const GmUnit &w, int row, int col, const Src &src) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
     const float al = out ? alpha.value() : 1.f;
     float *pp = part + ((int64_t)w.slice * rows + r) * cols + c0;
     T *po = out + r * cols + c0;
     const bool wide = (cols & 3) == 0;  // 16-byte aligned fp32 rows
+#pragma unroll Src::unroll
     for (int c = 0; c < TN / 2; c += 32) {
       float v[32];
-      tmem_ld32(taddr + c, v);
+      src.get(c, v);
       const int64_t left = cols - (c0 + c);
       if (r >= rows || left <= 0) continue;
       if (out != nullptr) {

@@ -9,8 +9,13 @@
 // so no edge of M, N or K is special before the epilogue.
 //
 // fp32 inputs come as two fp16 halves (a = hi + lo, 22 significant bits, one
-// power-of-two scale per tensor) and three products hi hi + hi lo + lo hi,
-// which are three passes over K into the same accumulators.
+// power-of-two scale per tensor) and three products lo hi + hi lo + hi hi,
+// which are three passes over K into the same accumulators, the small ones
+// first.  The tensor core drops the bits below an accumulator's last one
+// instead of rounding them: over a long K the loss adds up (2.5e-5 of dw at
+// K = 65537 in one chain, where fp32 sums keep 1e-6).  So a unit of pairs is
+// cut into rounds of kGmRound k steps; each round starts a fresh accumulator
+// and the epilogue adds the rounds in registers, rounding to nearest.
 //
 // Roles (320 threads, one CTA per SM, persistent over (tile, K slice) units):
 //   warps 0-7  epilogue: warp w reads TMEM lanes 32 (w % 4).. and half w / 4
@@ -34,6 +39,7 @@ namespace ra {
 constexpr int kGmM = 128, kGmK = 64, kGmStages = 4;
 constexpr int kGmThreads = 320, kGmEpiWarps = 8;
 constexpr int kGmABytes = kGmM * kGmK * 2;
+constexpr int kGmRound = 4;  // k steps (of 64) of a round of pairs
 
 __host__ __device__ constexpr int gm_stage_bytes(int TN) { return kGmABytes + TN * kGmK * 2; }
 __host__ __device__ constexpr size_t gm_smem_bytes(int TN) {
@@ -44,7 +50,7 @@ __host__ __device__ constexpr size_t gm_smem_bytes(int TN) {
 // m runs fastest where the B operand is the large one (m_fast), so that
 // concurrent CTAs share a B tile.
 struct GmShape {
-  int m_tiles, n_tiles, k_steps, slices, products;
+  int m_tiles, n_tiles, k_steps, slices;
   int m_fast;
   unsigned spin_limit;
   int *status;
@@ -103,10 +109,27 @@ __device__ __forceinline__ GmUnit gm_unit(const GmShape &s, int u) {
   return r;
 }
 
-// Epi: operator()(unit, row in tile, first column in tile, TMEM address of
-// the thread's lane at that column, columns) for one thread's row and its
-// half of the tile's columns.
-template <int TN, bool BF16, bool A_MN, bool B_MN, class Epi>
+// The thread's row of a finished tile, 32 columns at a time: straight from
+// TMEM, or from the registers that joined the rounds.
+struct GmFromTmem {
+  uint32_t taddr;
+  static constexpr int unroll = 1;
+  __device__ __forceinline__ void get(int c, float (&v)[32]) const { tmem_ld32(taddr + c, v); }
+};
+template <int NC>
+struct GmFromRegs {
+  const float (&acc)[NC];
+  static constexpr int unroll = NC / 32;
+  __device__ __forceinline__ void get(int c, float (&v)[32]) const {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = acc[c + j];
+  }
+};
+
+// Epi: run<TN>(unit, row in tile, first column in tile, source) for one
+// thread's row and its half of the tile's columns.  PAIRS: three products, in
+// rounds; else one product and one round.
+template <int TN, bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
 __global__ void __launch_bounds__(kGmThreads, 1)
     gemm16_kernel(const __grid_constant__ GmMaps maps, const GmShape s,
                   const __grid_constant__ Epi epi) {
@@ -115,6 +138,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
   const uint32_t base = (raw + 1023) & ~1023u;
   constexpr int kStage = gm_stage_bytes(TN);
   constexpr int kTmemCols = 2 * TN;
+  constexpr int kProducts = PAIRS ? 3 : 1;
+  constexpr int kRound = PAIRS ? kGmRound : 1 << 30;
   const uint32_t bars = base + kGmStages * kStage;
   // full[4] empty[4] accfull[2] accempty[2], then the TMEM address and abort flag
   const uint32_t full = bars, empty = bars + 8 * kGmStages, accfull = bars + 16 * kGmStages,
@@ -153,10 +178,12 @@ __global__ void __launch_bounds__(kGmThreads, 1)
       bool ok = true;
       for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
         const GmUnit w = gm_unit(s, u);
-        for (int p = 0; ok && p < s.products; ++p) {
-          const CUtensorMap *ma = p == 2 ? &maps.a_lo : &maps.a_hi;
-          const CUtensorMap *mb = p == 1 ? &maps.b_lo : &maps.b_hi;
-          for (int k = w.k0; k < w.k1; ++k, ++issued) {
+        for (int k0 = w.k0; ok && k0 < w.k1; k0 += kRound)
+        for (int p = 0; ok && p < kProducts; ++p) {
+          const CUtensorMap *ma = PAIRS && p == 0 ? &maps.a_lo : &maps.a_hi;
+          const CUtensorMap *mb = PAIRS && p == 1 ? &maps.b_lo : &maps.b_hi;
+          const int k1 = min(k0 + kRound, w.k1);
+          for (int k = k0; k < k1; ++k, ++issued) {
             const int st = issued % kGmStages;
             if (issued >= kGmStages &&
                 !ws_wait(empty + 8 * st, ((issued / kGmStages) - 1) & 1, abort_flag,
@@ -195,34 +222,37 @@ __global__ void __launch_bounds__(kGmThreads, 1)
       constexpr uint32_t idesc = gm_idesc(TN, BF16, A_MN, B_MN);
       int used = 0, t = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++t) {
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
         const GmUnit w = gm_unit(s, u);
-        const int buf = t & 1;
-        if (t >= 2 && !ws_wait(accempty + 8 * buf, ((t >> 1) - 1) & 1, abort_flag, s.spin_limit)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t acc = tmem + buf * TN;
-        const int steps = s.products * (w.k1 - w.k0);
-        for (int i = 0; i < steps; ++i, ++used) {
-          const int st = used % kGmStages;
-          if (!ws_wait(full + 8 * st, (used / kGmStages) & 1, abort_flag, s.spin_limit)) {
+        for (int k0 = w.k0; ok && k0 < w.k1; k0 += kRound, ++t) {
+          const int buf = t & 1;
+          if (t >= 2 &&
+              !ws_wait(accempty + 8 * buf, ((t >> 1) - 1) & 1, abort_flag, s.spin_limit)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a = base + st * kStage, b = a + kGmABytes;
-          const uint64_t da = gm_desc(a, A_MN), db = gm_desc(b, B_MN);
+          const uint32_t acc = tmem + buf * TN;
+          const int steps = kProducts * (min(k0 + kRound, w.k1) - k0);
+          for (int i = 0; i < steps; ++i, ++used) {
+            const int st = used % kGmStages;
+            if (!ws_wait(full + 8 * st, (used / kGmStages) & 1, abort_flag, s.spin_limit)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a = base + st * kStage, b = a + kGmABytes;
+            const uint64_t da = gm_desc(a, A_MN), db = gm_desc(b, B_MN);
 #pragma unroll
-          for (int kk = 0; kk < kGmK / 16; ++kk) {
-            // 16 k: 32 bytes along a K-major row, two 8-k groups MN-major
-            gm_mma(acc, da + (uint64_t)(kk * (A_MN ? 2048 : 32) >> 4),
-                   db + (uint64_t)(kk * (B_MN ? 2048 : 32) >> 4), idesc, i > 0 || kk > 0);
+            for (int kk = 0; kk < kGmK / 16; ++kk) {
+              // 16 k: 32 bytes along a K-major row, two 8-k groups MN-major
+              gm_mma(acc, da + (uint64_t)(kk * (A_MN ? 2048 : 32) >> 4),
+                     db + (uint64_t)(kk * (B_MN ? 2048 : 32) >> 4), idesc, i > 0 || kk > 0);
+            }
+            tc_commit(empty + 8 * st);
           }
-          tc_commit(empty + 8 * st);
+          if (ok) tc_commit(accfull + 8 * buf);
         }
-        if (ok) tc_commit(accfull + 8 * buf);
       }
       if (!ok) {
         *abort_flag = 1;
@@ -232,22 +262,49 @@ __global__ void __launch_bounds__(kGmThreads, 1)
   } else {
     const int half = warp >> 2;
     const int row = 32 * (warp & 3) + lane;
+    const uint32_t lane_addr =
+        tmem + half * (TN / 2) + ((uint32_t)(32 * (warp & 3)) << 16);
     int t = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++t) {
-      const GmUnit w = gm_unit(s, u);
-      const int buf = t & 1;
-      const bool got = ws_wait(accfull + 8 * buf, (t >> 1) & 1, abort_flag, s.spin_limit);
+    // waits for round t's accumulator; false (for the whole warp) on expiry
+    auto ready = [&]() {
+      const bool got = ws_wait(accfull + 8 * (t & 1), (t >> 1) & 1, abort_flag, s.spin_limit);
       if (!__all_sync(kFull, got)) {
         *abort_flag = 1;
         if (lane == 0) atomicOr(s.status, 1);
-        break;
+        return false;
       }
       tc_fence_after();
-      epi(w, row, half * (TN / 2),
-          tmem + buf * TN + half * (TN / 2) + ((uint32_t)(32 * (warp & 3)) << 16));
+      return true;
+    };
+    auto release = [&]() {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(accempty + 8 * buf);
+      if (lane == 0) mbar_arrive(accempty + 8 * (t & 1));
+      ++t;
+    };
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      const GmUnit w = gm_unit(s, u);
+      if constexpr (PAIRS) {
+        float acc[TN / 2];
+        for (int k0 = w.k0; k0 < w.k1; k0 += kRound) {
+          if (!(ok = ready())) break;
+          const uint32_t from = lane_addr + (t & 1) * TN;
+#pragma unroll
+          for (int c = 0; c < TN / 2; c += 32) {
+            float v[32];
+            tmem_ld32(from + c, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[c + j] = k0 == w.k0 ? v[j] : acc[c + j] + v[j];
+          }
+          release();
+        }
+        if (ok) epi.template run<TN>(w, row, half * (TN / 2), GmFromRegs<TN / 2>{acc});
+      } else {
+        if (!(ok = ready())) break;
+        epi.template run<TN>(w, row, half * (TN / 2), GmFromTmem{lane_addr + (t & 1) * TN});
+        release();
+      }
     }
   }
   __syncwarp();
