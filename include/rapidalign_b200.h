@@ -485,6 +485,60 @@ RA_API int ra_ce_backward(const ra_ce_desc *desc, const void *x, const void *w,
                           void *dx, void *dw, void *state, size_t state_bytes, void *workspace,
                           size_t workspace_bytes, ra_stream_t stream);
 
+/* ---- kernel attention ----------------------------------------------------- */
+/* Attention of the queries of each graph over the keys of the same graph
+ * (ragged: rows ptr[g] .. ptr[g + 1] - 1 are graph g's):
+ *   s_ij = u or softcap tanh(u / softcap), u = scale q_i.k_j,
+ *          minus |p_i - p_j|^2 / (2 sigma_h^2) where pos_dim > 0
+ *   out_i = sum_j softmax_j(s_ij) v_j; 0 for a query without keys.
+ *
+ * q [num_q][heads][dim], k and v [num_k][kv_heads][dim]: `dtype`, unit stride
+ * along dim, the other strides in elements (0 allowed); heads is a multiple of
+ * kv_heads.  q_ptr, k_ptr: device int64 [graphs + 1], checked by the caller
+ * (0 first, num last, no decrease).  q_tiles, k_tiles: device int32
+ * [tiles][2], (graph, n) for every 128 rows of every graph's queries and keys,
+ * in the order they are to be taken.  max_q, max_k: the longest graph's rows.
+ * With both offsets NULL (padded clouds) every graph has max_q queries and
+ * max_k keys, and the tile counts are those of that.
+ * q_pos, k_pos: float [num][pos_dim], pos_dim 1 to 3; sigma: float [heads].
+ * q_mask, k_mask: uint8 [num] or NULL; a masked query gives 0, masked keys (and
+ * what their rows hold) take no part.  `status` as in ra_ce_desc.
+ * out: [num_q][heads][dim]; for a backward also out32 (the same, unrounded;
+ * NULL for RA_F32) and stats (float [heads][num_q][2]).  Nothing is allocated
+ * and the host never waits. */
+typedef struct ra_attn_desc {
+  int64_t graphs, num_q, num_k;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int64_t q_tiles, k_tiles, max_q, max_k;
+  int32_t heads, kv_heads, dim, pos_dim;
+  int32_t dtype;
+  float scale, softcap;
+  int32_t reserved;
+  int32_t *status;
+} ra_attn_desc;
+typedef struct ra_attn_inputs {
+  const void *q, *k, *v;
+  const int64_t *q_ptr, *k_ptr;
+  const int32_t *q_tiles, *k_tiles;
+  const float *q_pos, *k_pos, *sigma;
+  const uint8_t *q_mask, *k_mask;
+} ra_attn_inputs;
+/* Any of them may be NULL; contiguous, laid out as the inputs they belong to. */
+typedef struct ra_attn_grads {
+  void *dq, *dk, *dv;
+  float *dq_pos, *dk_pos, *dsigma;
+} ra_attn_grads;
+
+RA_API size_t ra_attn_workspace_bytes(const ra_attn_desc *desc, int backward_pass);
+RA_API int ra_attn_forward(const ra_attn_desc *desc, const ra_attn_inputs *in, void *out,
+                           float *out32, float *stats, void *workspace, size_t workspace_bytes,
+                           ra_stream_t stream);
+/* dout: contiguous, as out. */
+RA_API int ra_attn_backward(const ra_attn_desc *desc, const ra_attn_inputs *in, const void *dout,
+                            const void *out, const float *out32, const float *stats,
+                            const ra_attn_grads *grads, void *workspace, size_t workspace_bytes,
+                            ra_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

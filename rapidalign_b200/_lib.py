@@ -99,6 +99,26 @@ class RaCeDesc(ctypes.Structure):
     ]
 
 
+class RaAttnDesc(ctypes.Structure):
+    _fields_ = (
+        [(n, ctypes.c_int64) for n in ("graphs", "num_q", "num_k", "q_row", "q_head", "k_row",
+                                       "k_head", "v_row", "v_head", "q_tiles", "k_tiles",
+                                       "max_q", "max_k")] +
+        [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "pos_dim", "dtype")] +
+        [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("reserved", ctypes.c_int32),
+         ("status", ctypes.c_void_p)])
+
+
+class RaAttnInputs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_ptr", "k_ptr", "q_tiles",
+                                               "k_tiles", "q_pos", "k_pos", "sigma", "q_mask",
+                                               "k_mask")]
+
+
+class RaAttnGrads(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "dq_pos", "dk_pos", "dsigma")]
+
+
 class RaPdlCloud(ctypes.Structure):
     _fields_ = [
         ("points", ctypes.c_void_p),
@@ -200,6 +220,12 @@ SIGNATURES = {
                                      _SZ, _V]),
     "ra_ce_backward": (ctypes.c_int, [ctypes.POINTER(RaCeDesc), _V, _V, _V, _V, _V, _V, _V, _V,
                                       _SZ, _V, _SZ, _V]),
+    "ra_attn_workspace_bytes": (_SZ, [ctypes.POINTER(RaAttnDesc), ctypes.c_int]),
+    "ra_attn_forward": (ctypes.c_int, [ctypes.POINTER(RaAttnDesc), ctypes.POINTER(RaAttnInputs),
+                                       _V, _V, _V, _V, _SZ, _V]),
+    "ra_attn_backward": (ctypes.c_int, [ctypes.POINTER(RaAttnDesc), ctypes.POINTER(RaAttnInputs),
+                                        _V, _V, _V, _V, ctypes.POINTER(RaAttnGrads), _V, _SZ,
+                                        _V]),
     "ra_kernel_launch_count": (ctypes.c_ulonglong, []),
     "ra_probe_fp32_peak": (ctypes.c_int, [_V, _I64, ctypes.c_int, ctypes.POINTER(_D), _V]),
 }

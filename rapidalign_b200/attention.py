@@ -1,0 +1,322 @@
+"""Kernel attention over ragged batches of graphs and padded clouds.
+
+Attention of the points (nodes) of each graph over the points of the same
+graph, with an optional Gaussian kernel of the points' distances: the score
+of query i and key j in head h is
+
+    softcap * tanh(u / softcap) or u,  u = scale * q_i . k_j,
+    minus |p_i - p_j|^2 / (2 sigma_h^2)
+
+so with q = k = 0 the weights are the kernel terms that ``kde_mmd_loss`` adds
+up, normalised per point.  ``pyg_kernel_attention`` takes ragged batches (ptr
+offsets or sorted batch vectors, as ``pyg_kde_mmd_loss``),
+``kernel_attention_dense`` padded clouds with masks (as
+``kde_mmd_loss_dense``).  Both are differentiable in q, k, v, the positions and
+sigma.  Inputs must be CUDA tensors: there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .kde import _ensure_ptr, _read_back
+
+Tensor = torch.Tensor
+
+__all__ = ["AttentionSegments", "attention_segments", "kernel_attention_dense",
+           "pyg_kernel_attention"]
+
+_TILE = 128  # rows of a work item
+_MAX_DIM = 256
+
+
+@dataclass(frozen=True)
+class AttentionSegments:
+    """The graphs of a ragged batch as the attention kernels take them: made
+    (and checked) once per batch by ``attention_segments``, used by any number
+    of calls.  Holds its own copy of the offsets."""
+    q_ptr: Tensor
+    k_ptr: Tensor
+    q_tiles: Tensor
+    k_tiles: Tensor
+    graphs: int
+    num_q: int
+    num_k: int
+    max_q: int
+    max_k: int
+
+
+def _tiles(lengths: Tensor, cost: Tensor, total: int) -> Tensor:
+    """(graph, tile) of every 128 rows, the graphs with the most work first."""
+    dev = lengths.device
+    if total == 0:
+        return torch.zeros((0, 2), dtype=torch.int32, device=dev)
+    order = torch.argsort(cost, descending=True, stable=True)
+    each = (lengths[order] + _TILE - 1) // _TILE
+    graph = torch.repeat_interleave(order, each, output_size=total)
+    first = torch.repeat_interleave(each.cumsum(0) - each, each, output_size=total)
+    tile = torch.arange(total, device=dev) - first
+    return torch.stack([graph, tile], 1).to(torch.int32).contiguous()
+
+
+def attention_segments(q_ptr: Optional[Tensor] = None, k_ptr: Optional[Tensor] = None, *,
+                       q_batch: Optional[Tensor] = None,
+                       k_batch: Optional[Tensor] = None) -> AttentionSegments:
+    """Checks the graphs' offsets (one host synchronisation) and lays out the
+    work.  Queries and keys come as ptr offsets (graphs + 1) or sorted batch
+    vectors; without keys' the keys are the queries' rows (self-attention)."""
+    if q_ptr is None and q_batch is None:
+        raise ValueError("either ptr or batch must be provided")
+    device = _lib.require_cuda(q_ptr if q_ptr is not None else q_batch)
+    qp = _ensure_ptr(q_ptr, q_batch, 0 if q_batch is None else q_batch.numel(), device)[0].clone()
+    if k_ptr is None and k_batch is None:
+        kp = qp
+    else:
+        kp = _ensure_ptr(k_ptr, k_batch, 0 if k_batch is None else k_batch.numel(),
+                         device)[0].clone()
+    if qp.numel() != kp.numel():
+        raise ValueError("query and key batches must have the same length")
+    graphs = qp.numel() - 1
+    nq, nk = qp[1:] - qp[:-1], kp[1:] - kp[:-1]
+    zero = torch.zeros((), dtype=torch.long, device=device)
+
+    def facts(p, n):
+        if graphs == 0:
+            return [p[0], p[0], zero, zero, zero]
+        return [p[0], p[-1], n.min(), n.max(), ((n + _TILE - 1) // _TILE).sum()]
+
+    info = _read_back(torch.stack(facts(qp, nq) + facts(kp, nk)))
+    for first, _, least, _, _ in (info[:5], info[5:]):
+        if first != 0:
+            raise ValueError("ptr must start at 0")
+        if least < 0:
+            raise ValueError("ptr offsets must match node stacks")
+    return AttentionSegments(qp, kp, _tiles(nq, nk, info[4]), _tiles(nk, nq, info[9]), graphs,
+                             info[1], info[6], info[3], info[8])
+
+
+class _KernelAttention(torch.autograd.Function):
+    """(q, k, v, q_pos, k_pos, sigma) -> out; q, k, v as (rows, heads, dim)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap,
+                need_grad):
+        lib = _lib.load()
+        dev = q.device
+        d = _lib.RaAttnDesc()
+        (d.graphs, d.num_q, d.num_k, d.max_q, d.max_k) = shape[:5]
+        q_ptr, k_ptr, q_tiles, k_tiles = shape[5:]
+        d.q_row, d.q_head = q.stride(0), q.stride(1)
+        d.k_row, d.k_head = k.stride(0), k.stride(1)
+        d.v_row, d.v_head = v.stride(0), v.stride(1)
+        if q_ptr is None:
+            d.q_tiles = d.graphs * -(-d.max_q // _TILE)
+            d.k_tiles = d.graphs * -(-d.max_k // _TILE)
+        else:
+            d.q_tiles, d.k_tiles = q_tiles.shape[0], k_tiles.shape[0]
+        d.heads, d.dim, d.kv_heads = q.shape[1], q.shape[2], k.shape[1]
+        d.pos_dim = 0 if q_pos is None else q_pos.shape[1]
+        d.dtype, d.scale, d.softcap = _lib.DTYPES[q.dtype], scale, softcap
+        d.status = _lib.status_word()
+        inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in (q, k, v, q_ptr, k_ptr, q_tiles, k_tiles,
+                                                        q_pos, k_pos, sigma, q_mask, k_mask)])
+        with torch.cuda.device(dev):
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            out32 = stats = None
+            if need_grad:
+                # unrounded outputs: the backward's do.o would carry the
+                # rounding of 16 bits into every score's gradient
+                if q.dtype != torch.float32:
+                    out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
+                stats = torch.empty((d.heads, d.num_q, 2), dtype=torch.float32, device=dev)
+            ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 0), dev)
+            rc = lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), out.data_ptr(),
+                                     _lib.ptr(out32), _lib.ptr(stats), ws.data_ptr(), ws.numel(),
+                                     _lib.stream_handle(dev))
+        _lib.check(rc, "kernel attention")
+        if need_grad:
+            ctx.desc, ctx.layout = d, (q_ptr, k_ptr, q_tiles, k_tiles)
+            ctx.save_for_backward(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask,
+                                  out if out32 is None else out32, stats)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        lib = _lib.load()
+        q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, out32, stats = ctx.saved_tensors
+        d, dev = ctx.desc, q.device
+        inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in (q, k, v, *ctx.layout, q_pos, k_pos, sigma,
+                                                        q_mask, k_mask)])
+        g = g.contiguous()
+        need = ctx.needs_input_grad
+        with torch.cuda.device(dev):
+            grads = [torch.empty(t.shape, dtype=t.dtype, device=dev)
+                     if t is not None and need[i] else None
+                     for i, t in enumerate((q, k, v, q_pos, k_pos, sigma))]
+            gr = _lib.RaAttnGrads(*[_lib.ptr(t) for t in grads])
+            ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 1), dev)
+            rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), g.data_ptr(), None,
+                                      out32.data_ptr(), stats.data_ptr(), ctypes.byref(gr),
+                                      ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+        _lib.check(rc, "kernel attention backward")
+        return (*grads, None, None, None, None, None, None)
+
+
+def _checked(q, k, v, ndim, shape_text):
+    if q.ndim != ndim or k.ndim != ndim or v.ndim != ndim:
+        raise ValueError(f"q, k and v must have shape {shape_text}")
+    if k.shape != v.shape or q.shape[-1] != k.shape[-1]:
+        raise ValueError("k and v must have the same shape, and q the same head dimension")
+    if q.dtype not in _lib.DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share dtype float32, bfloat16 or float16")
+    heads, kv_heads, dim = q.shape[-2], k.shape[-2], q.shape[-1]
+    if heads < 1 or kv_heads < 1 or heads > 4096 or heads % kv_heads:
+        raise ValueError("the heads of q must be a multiple of those of k and v")
+    if not 1 <= dim <= _MAX_DIM:
+        raise ValueError(f"head dimension must be between 1 and {_MAX_DIM}")
+    if not (k.device == q.device and v.device == q.device):
+        raise ValueError("q, k and v must be on the same device")
+
+
+def _positions(q_pos, k_pos, sigma, num_q, num_k, heads, device):
+    """float32 positions (rows, c) and sigma (heads,), or three Nones."""
+    if q_pos is None:
+        if k_pos is not None or sigma is not None:
+            raise ValueError("positions of queries and sigma go together")
+        return None, None, None
+    if sigma is None:
+        raise ValueError("positions need a sigma")
+    if k_pos is None:
+        k_pos = q_pos
+    if q_pos.ndim != 2 or k_pos.ndim != 2 or q_pos.shape[1] != k_pos.shape[1] or \
+            not 1 <= q_pos.shape[1] <= 3:
+        raise ValueError("positions must have 1 to 3 coordinates, the same for queries and keys")
+    if q_pos.shape[0] != num_q or k_pos.shape[0] != num_k:
+        raise ValueError("positions length must equal number of rows")
+    if not isinstance(sigma, Tensor):
+        if not sigma > 0:
+            raise ValueError("sigma must be positive")
+        sigma = torch.full((heads,), float(sigma), dtype=torch.float32, device=device)
+    elif sigma.numel() != 1 and sigma.shape != (heads,):
+        raise ValueError("sigma must be a scalar or one value per head")
+    if q_pos.device != device or k_pos.device != device:
+        raise ValueError("positions must be on the device of q")
+    sigma = sigma.to(device=device, dtype=torch.float32).reshape(-1).expand(heads)
+    return (q_pos.to(torch.float32).contiguous(), k_pos.to(torch.float32).contiguous(),
+            sigma.contiguous())
+
+
+def _factors(scale, softcap, dim):
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    softcap = float(softcap)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not (softcap >= 0.0 and math.isfinite(softcap)):
+        raise ValueError("softcap must be finite and not negative")
+    return scale, softcap
+
+
+def _mask(mask, shape, device):
+    if mask is None:
+        return None
+    if tuple(mask.shape) != tuple(shape):
+        raise ValueError(f"masks must have shape {tuple(shape)}")
+    return mask.to(device=device, dtype=torch.bool).reshape(-1).to(torch.uint8).contiguous()
+
+
+def _unit_rows(t: Tensor) -> Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _run(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap):
+    _lib.check_status("kernel attention")
+    need = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, q_pos, k_pos, sigma))
+    return _KernelAttention.apply(_unit_rows(q), _unit_rows(k), _unit_rows(v), q_pos, k_pos, sigma,
+                                  q_mask, k_mask, shape, scale, softcap, need)
+
+
+def pyg_kernel_attention(q: Tensor, k: Tensor, v: Tensor, *, q_ptr: Optional[Tensor] = None,
+                         k_ptr: Optional[Tensor] = None, q_batch: Optional[Tensor] = None,
+                         k_batch: Optional[Tensor] = None,
+                         segments: Optional[AttentionSegments] = None,
+                         q_pos: Optional[Tensor] = None, k_pos: Optional[Tensor] = None,
+                         sigma=None, q_mask: Optional[Tensor] = None,
+                         k_mask: Optional[Tensor] = None, scale: Optional[float] = None,
+                         softcap: float = 0.0) -> Tensor:
+    """Attention inside each graph of a ragged batch.
+
+    Args:
+        q: (Nq, H, D), float32, bfloat16 or float16, D up to 256.
+        k, v: (Nk, H', D) of the same dtype; H is a multiple of H', and heads
+            h of q use head h // (H / H') of k and v.
+        q_ptr, k_ptr / q_batch, k_batch: the graphs, as ptr offsets or sorted
+            batch vectors; without the keys', keys are the queries' rows.
+            Checked with one host synchronisation.
+        segments: instead of those, ``attention_segments(...)`` of the batch:
+            no call with it waits for the device (and it can be captured).
+        q_pos, k_pos: (Nq, c), (Nk, c) positions, c = 1 to 3, with ``sigma``, a
+            number or a tensor () or (H,): the Gaussian kernel's bandwidth.
+            k_pos defaults to q_pos.  A number is checked; a tensor's zeros
+            give NaN.
+        q_mask, k_mask: (Nq,), (Nk,) booleans: masked keys take no part
+            (whatever their rows hold), masked queries give 0.
+        scale: factor of the products, 1 / sqrt(D) by default.
+        softcap: where positive, products are capped by softcap * tanh.
+
+    Returns:
+        (Nq, H, D) in q's dtype; 0 for a query without keys.  Differentiable
+        in q, k, v, the positions and sigma (bitwise repeatable).
+    """
+    _checked(q, k, v, 3, "(N, heads, dim)")
+    scale, softcap = _factors(scale, softcap, q.shape[2])
+    device = _lib.require_cuda(q, k, v)
+    if segments is None:
+        segments = attention_segments(q_ptr, k_ptr, q_batch=q_batch, k_batch=k_batch)
+    elif any(t is not None for t in (q_ptr, k_ptr, q_batch, k_batch)):
+        raise ValueError("give either segments or ptr and batch")
+    if segments.num_q != q.shape[0] or segments.num_k != k.shape[0]:
+        raise ValueError("ptr[-1] must equal number of nodes")
+    if segments.q_ptr.device != device:
+        raise ValueError("segments must be on the device of q")
+    pos = _positions(q_pos, k_pos, sigma, q.shape[0], k.shape[0], q.shape[1], device)
+    shape = (segments.graphs, segments.num_q, segments.num_k, segments.max_q, segments.max_k,
+             segments.q_ptr, segments.k_ptr, segments.q_tiles, segments.k_tiles)
+    return _run(q, k, v, *pos, _mask(q_mask, q.shape[:1], device),
+                _mask(k_mask, k.shape[:1], device), shape, scale, softcap)
+
+
+def kernel_attention_dense(q: Tensor, k: Tensor, v: Tensor, mask_q: Optional[Tensor] = None,
+                           mask_k: Optional[Tensor] = None, *, q_pos: Optional[Tensor] = None,
+                           k_pos: Optional[Tensor] = None, sigma=None,
+                           scale: Optional[float] = None, softcap: float = 0.0) -> Tensor:
+    """``pyg_kernel_attention`` on padded clouds: q (B, N, H, D), k and v
+    (B, M, H', D), masks (B, N) and (B, M) of any pattern (None: all valid),
+    positions (B, N, c) and (B, M, c).  Returns (B, N, H, D); masked queries
+    and clouds without valid keys give 0, and what masked rows hold (NaN too)
+    reaches no result and no gradient."""
+    _checked(q, k, v, 4, "(B, N, heads, dim)")
+    B, N, H, D = q.shape
+    M = k.shape[1]
+    if k.shape[0] != B:
+        raise ValueError("q, k and v must have the same number of clouds")
+    scale, softcap = _factors(scale, softcap, D)
+    device = _lib.require_cuda(q, k, v)
+    for p, n in ((q_pos, N), (k_pos, M)):
+        if p is not None and (p.ndim != 3 or tuple(p.shape[:2]) != (B, n)):
+            raise ValueError("positions must have shape (B, N, c)")
+    if k_pos is None and q_pos is not None and N != M:
+        raise ValueError("positions length must equal number of rows")
+    flat = [None if p is None else p.reshape(-1, p.shape[2]) for p in (q_pos, k_pos)]
+    pos = _positions(flat[0], flat[1], sigma, B * N, B * M, H, device)
+    shape = (B, B * N, B * M, N if B else 0, M if B else 0, None, None, None, None)
+    out = _run(q.reshape(B * N, H, D), k.reshape(B * M, k.shape[2], D),
+               v.reshape(B * M, k.shape[2], D), *pos, _mask(mask_q, (B, N), device),
+               _mask(mask_k, (B, M), device), shape, scale, softcap)
+    return out.reshape(B, N, H, D)

@@ -16,7 +16,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "librapidalign_b200.so")
-SOURCES = [os.path.join(CSRC, f) for f in ("ra_capi.cu", "ra_ce.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("ra_capi.cu", "ra_ce.cu", "ra_attn.cu")]
 OBJ_DIR = os.path.join(HERE, "_build")
 HEADERS = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))] + [
     os.path.join(HERE, os.pardir, "include", "rapidalign_b200.h")]
