@@ -529,15 +529,19 @@ typedef struct ra_attn_grads {
   float *dq_pos, *dk_pos, *dsigma;
 } ra_attn_grads;
 
+/* `state` (256-byte aligned, ra_attn_state_bytes) keeps what the backward
+ * needs, `workspace` (256-byte aligned, ra_attn_workspace_bytes for the pass)
+ * is scratch.  out, out32, dout, dq, dk and dv are 16-byte aligned. */
+RA_API size_t ra_attn_state_bytes(const ra_attn_desc *desc);
 RA_API size_t ra_attn_workspace_bytes(const ra_attn_desc *desc, int backward_pass);
 RA_API int ra_attn_forward(const ra_attn_desc *desc, const ra_attn_inputs *in, void *out,
-                           float *out32, float *stats, void *workspace, size_t workspace_bytes,
-                           ra_stream_t stream);
+                           float *out32, float *stats, void *state, size_t state_bytes,
+                           void *workspace, size_t workspace_bytes, ra_stream_t stream);
 /* dout: contiguous, as out. */
 RA_API int ra_attn_backward(const ra_attn_desc *desc, const ra_attn_inputs *in, const void *dout,
                             const void *out, const float *out32, const float *stats,
-                            const ra_attn_grads *grads, void *workspace, size_t workspace_bytes,
-                            ra_stream_t stream);
+                            const ra_attn_grads *grads, void *state, size_t state_bytes,
+                            void *workspace, size_t workspace_bytes, ra_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -220,12 +220,13 @@ SIGNATURES = {
                                      _SZ, _V]),
     "ra_ce_backward": (ctypes.c_int, [ctypes.POINTER(RaCeDesc), _V, _V, _V, _V, _V, _V, _V, _V,
                                       _SZ, _V, _SZ, _V]),
+    "ra_attn_state_bytes": (_SZ, [ctypes.POINTER(RaAttnDesc)]),
     "ra_attn_workspace_bytes": (_SZ, [ctypes.POINTER(RaAttnDesc), ctypes.c_int]),
     "ra_attn_forward": (ctypes.c_int, [ctypes.POINTER(RaAttnDesc), ctypes.POINTER(RaAttnInputs),
-                                       _V, _V, _V, _V, _SZ, _V]),
+                                       _V, _V, _V, _V, _SZ, _V, _SZ, _V]),
     "ra_attn_backward": (ctypes.c_int, [ctypes.POINTER(RaAttnDesc), ctypes.POINTER(RaAttnInputs),
-                                        _V, _V, _V, _V, ctypes.POINTER(RaAttnGrads), _V, _SZ,
-                                        _V]),
+                                        _V, _V, _V, _V, ctypes.POINTER(RaAttnGrads), _V, _SZ, _V,
+                                        _SZ, _V]),
     "ra_kernel_launch_count": (ctypes.c_ulonglong, []),
     "ra_probe_fp32_peak": (ctypes.c_int, [_V, _I64, ctypes.c_int, ctypes.POINTER(_D), _V]),
 }

@@ -134,13 +134,15 @@ class _KernelAttention(torch.autograd.Function):
                 if q.dtype != torch.float32:
                     out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
                 stats = torch.empty((d.heads, d.num_q, 2), dtype=torch.float32, device=dev)
+            state = _lib.workspace(lib.ra_attn_state_bytes(ctypes.byref(d)), dev)
             ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 0), dev)
             rc = lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), out.data_ptr(),
-                                     _lib.ptr(out32), _lib.ptr(stats), ws.data_ptr(), ws.numel(),
+                                     _lib.ptr(out32), _lib.ptr(stats), state.data_ptr(),
+                                     state.numel(), ws.data_ptr(), ws.numel(),
                                      _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention")
         if need_grad:
-            ctx.desc, ctx.layout = d, (q_ptr, k_ptr, q_tiles, k_tiles)
+            ctx.desc, ctx.state, ctx.layout = d, state, (q_ptr, k_ptr, q_tiles, k_tiles)
             ctx.save_for_backward(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask,
                                   out if out32 is None else out32, stats)
         return out
@@ -154,6 +156,8 @@ class _KernelAttention(torch.autograd.Function):
         inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in (q, k, v, *ctx.layout, q_pos, k_pos, sigma,
                                                         q_mask, k_mask)])
         g = g.contiguous()
+        if g.data_ptr() % 16:
+            g = g.clone()
         need = ctx.needs_input_grad
         with torch.cuda.device(dev):
             grads = [torch.empty(t.shape, dtype=t.dtype, device=dev)
@@ -163,7 +167,7 @@ class _KernelAttention(torch.autograd.Function):
             ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 1), dev)
             rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), g.data_ptr(), None,
                                       out32.data_ptr(), stats.data_ptr(), ctypes.byref(gr),
-                                      ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+                                      ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention backward")
         return (*grads, None, None, None, None, None, None)
 
@@ -231,7 +235,13 @@ def _mask(mask, shape, device):
 
 
 def _unit_rows(t: Tensor) -> Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """Unit stride along the head dimension, and 16-byte aligned rows for the
+    16-bit tensor-core kernels (widths that are multiples of 8)."""
+    unit = t.stride(-1) == 1 or t.shape[-1] == 1
+    if unit and t.dtype != torch.float32 and t.shape[-1] % 8 == 0:
+        unit = t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
+        return t if unit else t.clone(memory_format=torch.contiguous_format)
+    return t if unit else t.contiguous()
 
 
 def _run(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap):

@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "ra_attn.cuh"
+#include "ra_attn_tc.cuh"
 #include "ra_host.h"
 
 namespace {
@@ -60,8 +61,64 @@ AttnArgs args_of(const ra_attn_desc *d, const ra_attn_inputs *in) {
   return a;
 }
 
+// Head widths the tensor-core kernels take (ra_attn_tc.cuh); other widths and
+// 16-bit operands that are not 16-byte aligned go to the warp-per-row kernels.
+bool use_tc(const ra_attn_desc *d) { return d->dim <= 128 && d->dim % 8 == 0; }
+bool operands_aligned(const ra_attn_desc *d, const ra_attn_inputs *in) {
+  if (d->dtype == RA_F32) return true;
+  const int64_t s = d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head;
+  return (s & 7) == 0 && (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v) & 15) == 0;
+}
+
+// The state a backward needs: bounds, and the halves of fp32 inputs.
+struct AttnState {
+  size_t qh, ql, kh, kl, vh, vl, total;
+};
+AttnState state_layout(const ra_attn_desc *d) {
+  AttnState s{};
+  size_t o = 256;
+  if (d->dtype == RA_F32 && use_tc(d)) {
+    const size_t q = align256(2 * (size_t)d->num_q * d->heads * d->dim);
+    const size_t k = align256(2 * (size_t)d->num_k * d->kv_heads * d->dim);
+    s.qh = o, s.ql = o + q, o += 2 * q;
+    s.kh = o, s.kl = o + k, o += 2 * k;
+    s.vh = o, s.vl = o + k, o += 2 * k;
+  }
+  s.total = o;
+  return s;
+}
+
+// Key ranges of a row tile: as many as fill the SMs twice, each at least four
+// key tiles of the longest graph.
+int key_splits(const ra_attn_desc *d, int sms) {
+  const int64_t ctas = d->q_tiles * d->heads;
+  if (ctas < 1 || ctas >= 2 * sms) return 1;
+  int64_t s = 2 * sms / ctas;
+  s = std::min<int64_t>(s, ceil_div(d->max_k, (int64_t)64) / 4);
+  return s < 1 ? 1 : (int)s;
+}
+
+struct AttnFwd {
+  int splits;
+  size_t part_o, part_s, total;
+};
+AttnFwd fwd_layout(const ra_attn_desc *d, int sms) {
+  AttnFwd f{};
+  f.splits = use_tc(d) ? key_splits(d, sms) : 1;
+  size_t o = 0;
+  if (f.splits > 1) {
+    const size_t rows = (size_t)f.splits * d->num_q * d->heads;
+    f.part_o = o;
+    o += align256(4 * rows * d->dim);
+    f.part_s = o;
+    o += align256(8 * rows);
+  }
+  f.total = o;
+  return f;
+}
+
 struct AttnBwd {
-  size_t delta, pos_q, pos_k, total;
+  size_t delta, pos_q, pos_k, gh, gl, total;
 };
 AttnBwd bwd_layout(const ra_attn_desc *d) {
   AttnBwd b{};
@@ -72,6 +129,10 @@ AttnBwd bwd_layout(const ra_attn_desc *d) {
   if (d->pos_dim) o += align256(sizeof(float4) * (size_t)d->num_q * d->heads);
   b.pos_k = o;
   if (d->pos_dim) o += align256(sizeof(float4) * (size_t)d->num_k * d->kv_heads);
+  if (d->dtype == RA_F32 && use_tc(d)) {
+    const size_t g = align256(2 * (size_t)d->num_q * d->heads * d->dim);
+    b.gh = o, b.gl = o + g, o += 2 * g;
+  }
   b.total = o;
   return b;
 }
@@ -79,32 +140,168 @@ AttnBwd bwd_layout(const ra_attn_desc *d) {
 unsigned grid_rows(int64_t n, int per) { return (unsigned)ceil_div(n, (int64_t)per); }
 
 template <class T>
-int forward(const AttnArgs &a, cudaStream_t st) {
-  attn_row_fwd_kernel<T>
-      <<<grid_rows(a.num_q * a.heads, kAttnWarps), 32 * kAttnWarps, 0, st>>>(a);
+int bounds(const AttnPrep &p, unsigned *words, int sms, cudaStream_t st) {
+  int64_t rows = 1;
+  for (int t = 0; t < p.count; ++t) rows = std::max(rows, p.rows[t] * p.heads[t]);
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, (int64_t)8), sms * 8), p.count);
+  attn_bounds_kernel<T><<<grid, 256, 0, st>>>(p, words);
+  return launched();
+}
+int halves(const AttnPrep &p, const unsigned *words, int sms, cudaStream_t st) {
+  int64_t n = 1;
+  for (int t = 0; t < p.count; ++t) n = std::max(n, p.rows[t] * p.heads[t] * p.dim);
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, (int64_t)256), sms * 16), p.count);
+  attn_halves_kernel<<<grid, 256, 0, st>>>(p, words);
+  return launched();
+}
+void add(AttnPrep &p, const void *x, int64_t rows, int heads, int64_t row, int64_t head,
+         const uint8_t *mask, int word, void *hi, void *lo) {
+  const int t = p.count++;
+  p.x[t] = x, p.rows[t] = rows, p.heads[t] = heads, p.row[t] = row, p.head[t] = head;
+  p.mask[t] = mask, p.word[t] = word, p.hi[t] = (uint16_t *)hi, p.lo[t] = (uint16_t *)lo;
+}
+
+// 16-bit operands of q, k, v: as given, or the halves in the state
+void operands(const ra_attn_desc *d, const ra_attn_inputs *in, char *state, AttnTcArgs *x) {
+  x->words = (const unsigned *)state;
+  if (d->dtype != RA_F32) {
+    const uint16_t *q = (const uint16_t *)in->q, *k = (const uint16_t *)in->k,
+                   *v = (const uint16_t *)in->v;
+    x->q = {q, q, d->q_row, d->q_head};
+    x->k = {k, k, d->k_row, d->k_head};
+    x->v = {v, v, d->v_row, d->v_head};
+    return;
+  }
+  const AttnState s = state_layout(d);
+  const int64_t qr = (int64_t)d->heads * d->dim, kr = (int64_t)d->kv_heads * d->dim;
+  auto at = [&](size_t o) { return (const uint16_t *)(state + o); };
+  x->q = {at(s.qh), at(s.ql), qr, d->dim};
+  x->k = {at(s.kh), at(s.kl), kr, d->dim};
+  x->v = {at(s.vh), at(s.vl), kr, d->dim};
+}
+
+template <class K>
+int launch(K kernel, int64_t grid, int threads, int smem, const AttnArgs &a, const AttnTcArgs &x,
+           cudaStream_t st) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+      cudaSuccess)
+    return RA_ERR_CUDA;
+  if (grid > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
+  if (grid < 1) return RA_OK;
+  kernel<<<(unsigned)grid, threads, smem, st>>>(a, x);
   return launched();
 }
 
-template <class T>
-int backward(AttnArgs a, const ra_attn_grads *gr, char *ws, cudaStream_t st) {
+template <class Kind, int DP>
+int tc_forward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
+  return launch(attn_tc_fwd_kernel<Kind, DP>, a.n_q_tiles * a.heads * x.splits, 128,
+                FwdCfg<Kind, DP>::smem, a, x, st);
+}
+template <class Kind, int DP>
+int tc_backward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
+  int rc = RA_OK;
+  if (a.dq || a.pos_q)
+    rc = launch(attn_tc_dq_kernel<Kind, DP>, a.n_q_tiles * a.heads, DqCfg<Kind, DP>::NT,
+                DqCfg<Kind, DP>::smem, a, x, st);
+  if (!rc && (a.dk || a.dv || a.pos_k))
+    rc = launch(attn_tc_dkv_kernel<Kind, DP>, a.n_k_tiles * a.kv_heads, DkvCfg<Kind, DP>::NT,
+                DkvCfg<Kind, DP>::smem, a, x, st);
+  return rc;
+}
+
+template <class Kind>
+int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, char *state,
+            char *ws, cudaStream_t st) {
+  using T = typename Kind::T;
+  if (!use_tc(d) || !operands_aligned(d, in)) {
+    attn_row_fwd_kernel<T>
+        <<<grid_rows(a.num_q * a.heads, kAttnWarps), 32 * kAttnWarps, 0, st>>>(a);
+    return launched();
+  }
+  const int sms = sm_count();
+  int rc;
+  AttnTcArgs x{};
+  operands(d, in, state, &x);
+  if (Kind::pair) {
+    const AttnState s = state_layout(d);
+    if (cudaMemsetAsync(state, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
+    AttnPrep p{};
+    p.dim = d->dim;
+    add(p, in->q, d->num_q, d->heads, d->q_row, d->q_head, in->q_mask, kWq, state + s.qh,
+        state + s.ql);
+    add(p, in->k, d->num_k, d->kv_heads, d->k_row, d->k_head, in->k_mask, kWk, state + s.kh,
+        state + s.kl);
+    add(p, in->v, d->num_k, d->kv_heads, d->v_row, d->v_head, in->k_mask, kWv, state + s.vh,
+        state + s.vl);
+    if ((rc = bounds<float>(p, (unsigned *)state, sms, st))) return rc;
+    if ((rc = halves(p, (const unsigned *)state, sms, st))) return rc;
+  }
+  const AttnFwd f = fwd_layout(d, sms);
+  x.splits = f.splits;
+  x.part_o = (float *)(ws + f.part_o), x.part_s = (float2 *)(ws + f.part_s);
+  x.pair_p = a.out32 != nullptr;
+  rc = d->dim <= 32   ? tc_forward<Kind, 32>(a, x, st)
+       : d->dim <= 64 ? tc_forward<Kind, 64>(a, x, st)
+                      : tc_forward<Kind, 128>(a, x, st);
+  if (rc || f.splits == 1) return rc;
+  const int64_t rows = a.num_q * a.heads;
+  attn_join_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(rows, (int64_t)8), sms * 16), 256, 0,
+                        st>>>(a, f.splits, x.part_o, x.part_s);
+  return launched();
+}
+
+template <class Kind>
+int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const ra_attn_grads *gr,
+             char *state, char *ws, cudaStream_t st) {
+  using T = typename Kind::T;
   int rc;
   const int sms = sm_count();
+  const AttnBwd b = bwd_layout(d);
+  const bool tc = use_tc(d) && operands_aligned(d, in);
   if (a.num_q > 0) {
     const unsigned grid =
         (unsigned)std::min<int64_t>(ceil_div(a.num_q * a.heads, (int64_t)8), (int64_t)sms * 16);
     attn_delta_kernel<T><<<grid, 256, 0, st>>>((const T *)a.dout, (const T *)a.out, a.out32,
                                                a.num_q, a.heads, a.dim, (float *)a.delta);
     if ((rc = launched())) return rc;
-    if (a.dq || a.pos_q) {
+  }
+  if (tc) {
+    AttnTcArgs x{};
+    operands(d, in, state, &x);
+    const uint16_t *g = (const uint16_t *)a.dout;
+    const int64_t qr = (int64_t)d->heads * d->dim;
+    x.go = {g, g, qr, d->dim};
+    unsigned *words = (unsigned *)state;
+    if (!Kind::bf16) {
+      AttnPrep p{};
+      p.dim = d->dim;
+      add(p, a.dout, d->num_q, d->heads, qr, d->dim, in->q_mask, kWdo, ws + b.gh, ws + b.gl);
+      if (Kind::pair) {
+        if (cudaMemsetAsync(words + kWdo, 0, 8, st) != cudaSuccess) return RA_ERR_CUDA;
+        x.go = {(const uint16_t *)(ws + b.gh), (const uint16_t *)(ws + b.gl), qr, d->dim};
+      } else {
+        if (cudaMemsetAsync(words, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
+        add(p, in->v, d->num_k, d->kv_heads, d->v_row, d->v_head, in->k_mask, kWv, nullptr,
+            nullptr);
+      }
+      if ((rc = bounds<T>(p, words, sms, st))) return rc;
+      if (Kind::pair && (rc = halves(p, words, sms, st))) return rc;
+    }
+    rc = d->dim <= 32   ? tc_backward<Kind, 32>(a, x, st)
+         : d->dim <= 64 ? tc_backward<Kind, 64>(a, x, st)
+                        : tc_backward<Kind, 128>(a, x, st);
+    if (rc) return rc;
+  } else {
+    if (a.num_q > 0 && (a.dq || a.pos_q)) {
       attn_row_dq_kernel<T>
           <<<grid_rows(a.num_q * a.heads, kAttnWarps), 32 * kAttnWarps, 0, st>>>(a);
       if ((rc = launched())) return rc;
     }
-  }
-  if (a.num_k > 0 && (a.dk || a.dv || a.pos_k)) {
-    attn_row_dkv_kernel<T>
-        <<<grid_rows(a.num_k * a.kv_heads, kAttnWarps), 32 * kAttnWarps, 0, st>>>(a);
-    if ((rc = launched())) return rc;
+    if (a.num_k > 0 && (a.dk || a.dv || a.pos_k)) {
+      attn_row_dkv_kernel<T>
+          <<<grid_rows(a.num_k * a.kv_heads, kAttnWarps), 32 * kAttnWarps, 0, st>>>(a);
+      if ((rc = launched())) return rc;
+    }
   }
   if (gr->dq_pos && a.num_q > 0) {
     attn_pos_kernel<<<(unsigned)std::min<int64_t>(ceil_div(a.num_q, (int64_t)256), sms * 8), 256, 0,
@@ -131,38 +328,46 @@ extern "C" {
 
 size_t ra_attn_workspace_bytes(const ra_attn_desc *d, int backward_pass) {
   if (!attn_ok(d)) return 0;
-  return std::max<size_t>(256, backward_pass ? bwd_layout(d).total : 0);
+  return std::max<size_t>(256, backward_pass ? bwd_layout(d).total : fwd_layout(d, sm_count()).total);
 }
 
+size_t ra_attn_state_bytes(const ra_attn_desc *d) { return attn_ok(d) ? state_layout(d).total : 0; }
+
 int ra_attn_forward(const ra_attn_desc *d, const ra_attn_inputs *in, void *out, float *out32,
-                    float *stats, void *workspace, size_t workspace_bytes, ra_stream_t stream) {
+                    float *stats, void *state, size_t state_bytes, void *workspace,
+                    size_t workspace_bytes, ra_stream_t stream) {
   if (!attn_ok(d) || !inputs_ok(d, in)) return RA_ERR_INVALID_ARGUMENT;
   if (d->num_q == 0) return RA_OK;
-  if (out == nullptr) return RA_ERR_INVALID_ARGUMENT;
+  if (out == nullptr || (((uintptr_t)out | (uintptr_t)out32) & 15)) return RA_ERR_INVALID_ARGUMENT;
   if (workspace == nullptr || !aligned256(workspace) ||
-      workspace_bytes < ra_attn_workspace_bytes(d, 0))
+      workspace_bytes < ra_attn_workspace_bytes(d, 0) || state == nullptr || !aligned256(state) ||
+      state_bytes < state_layout(d).total)
     return RA_ERR_WORKSPACE;
   AttnArgs a = args_of(d, in);
   a.out = out, a.out32 = out32, a.stats = (float2 *)stats;
   cudaStream_t st = (cudaStream_t)stream;
-  if (d->dtype == RA_F32) return forward<float>(a, st);
-  if (d->dtype == RA_BF16) return forward<__nv_bfloat16>(a, st);
-  return forward<__half>(a, st);
+  char *sb = (char *)state, *ws = (char *)workspace;
+  if (d->dtype == RA_F32) return forward<KindF32>(d, in, a, sb, ws, st);
+  if (d->dtype == RA_BF16) return forward<KindBf16>(d, in, a, sb, ws, st);
+  return forward<KindF16>(d, in, a, sb, ws, st);
 }
 
 int ra_attn_backward(const ra_attn_desc *d, const ra_attn_inputs *in, const void *dout,
                      const void *out, const float *out32, const float *stats,
-                     const ra_attn_grads *grads, void *workspace, size_t workspace_bytes,
-                     ra_stream_t stream) {
+                     const ra_attn_grads *grads, void *state, size_t state_bytes, void *workspace,
+                     size_t workspace_bytes, ra_stream_t stream) {
   if (!attn_ok(d) || !inputs_ok(d, in) || grads == nullptr) return RA_ERR_INVALID_ARGUMENT;
   if (d->num_q > 0 && (dout == nullptr || stats == nullptr || (out == nullptr && out32 == nullptr)))
     return RA_ERR_INVALID_ARGUMENT;
   if (d->pos_dim == 0 && (grads->dq_pos || grads->dk_pos || grads->dsigma))
     return RA_ERR_INVALID_ARGUMENT;
   const AttnBwd b = bwd_layout(d);
-  if (workspace == nullptr || !aligned256(workspace) || workspace_bytes < b.total)
+  if (workspace == nullptr || !aligned256(workspace) || workspace_bytes < b.total ||
+      state == nullptr || !aligned256(state) || state_bytes < state_layout(d).total)
     return RA_ERR_WORKSPACE;
-  char *ws = (char *)workspace;
+  if ((((uintptr_t)grads->dq | (uintptr_t)grads->dk | (uintptr_t)grads->dv | (uintptr_t)dout) & 15))
+    return RA_ERR_INVALID_ARGUMENT;
+  char *sb = (char *)state, *ws = (char *)workspace;
   AttnArgs a = args_of(d, in);
   a.out = const_cast<void *>(out), a.out32 = const_cast<float *>(out32);
   a.stats = (float2 *)stats, a.dout = dout, a.delta = (float *)(ws + b.delta);
@@ -170,9 +375,9 @@ int ra_attn_backward(const ra_attn_desc *d, const ra_attn_inputs *in, const void
   if (grads->dq_pos || grads->dsigma) a.pos_q = (float4 *)(ws + b.pos_q);
   if (grads->dk_pos) a.pos_k = (float4 *)(ws + b.pos_k);
   cudaStream_t st = (cudaStream_t)stream;
-  if (d->dtype == RA_F32) return backward<float>(a, grads, ws, st);
-  if (d->dtype == RA_BF16) return backward<__nv_bfloat16>(a, grads, ws, st);
-  return backward<__half>(a, grads, ws, st);
+  if (d->dtype == RA_F32) return backward<KindF32>(d, in, a, grads, sb, ws, st);
+  if (d->dtype == RA_BF16) return backward<KindBf16>(d, in, a, grads, sb, ws, st);
+  return backward<KindF16>(d, in, a, grads, sb, ws, st);
 }
 
 }  // extern "C"

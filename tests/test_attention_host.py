@@ -116,7 +116,7 @@ def test_c_refuses(lib, bad):
     base = 1 << 20
     inp = _lib.RaAttnInputs(*[base] * 12)
     rc = lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), base, base, base, base, 1 << 30,
-                             None)
+                             base, 1 << 30, None)
     assert rc == _lib.RA_ERR_INVALID_ARGUMENT
 
 
@@ -127,7 +127,7 @@ def test_c_refuses_missing_inputs(lib, missing):
     inp = _lib.RaAttnInputs(*[base] * 12)
     setattr(inp, missing, None)
     rc = lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), base, base, base, base, 1 << 30,
-                             None)
+                             base, 1 << 30, None)
     assert rc == _lib.RA_ERR_INVALID_ARGUMENT
 
 
@@ -135,17 +135,23 @@ def test_c_refuses_buffers(lib):
     base = 1 << 20
     d = desc()
     inp = _lib.RaAttnInputs(*[base] * 12)
-    assert lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), base, base, base, base + 8,
-                               1 << 30, None) == _lib.RA_ERR_WORKSPACE
+    big = 1 << 30
+    for state, n_state, ws, n_ws in ((base + 8, big, base, big), (base, 16, base, big),
+                                     (base, big, base + 8, big), (base, big, base, 16)):
+        assert lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), base, base, base, state,
+                                   n_state, ws, n_ws, None) == _lib.RA_ERR_WORKSPACE
+    assert lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), base + 2, base, base, base,
+                               big, base, big, None) == _lib.RA_ERR_INVALID_ARGUMENT
     gr = _lib.RaAttnGrads(*[base] * 6)
     assert lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), base, None, base, base,
-                                ctypes.byref(gr), base, 256, None) == _lib.RA_ERR_WORKSPACE
+                                ctypes.byref(gr), base, big, base, 256,
+                                None) == _lib.RA_ERR_WORKSPACE
     d.pos_dim = 0
     assert lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), base, None, base, base,
-                                ctypes.byref(gr), base, 1 << 30,
+                                ctypes.byref(gr), base, big, base, big,
                                 None) == _lib.RA_ERR_INVALID_ARGUMENT
     # padded clouds: the counts have to fit
     inp = _lib.RaAttnInputs(*[base] * 12)
     inp.q_ptr = inp.k_ptr = None
     assert lib.ra_attn_forward(ctypes.byref(desc()), ctypes.byref(inp), base, base, base, base,
-                               1 << 30, None) == _lib.RA_ERR_INVALID_ARGUMENT
+                               big, base, big, None) == _lib.RA_ERR_INVALID_ARGUMENT

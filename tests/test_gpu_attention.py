@@ -10,8 +10,11 @@ E = 2^-23 for each fp32 addition, n terms in a sum:
   D_i    sum |do| (out's bound with P as a pair, 2^-16, in u's place)
   dS     P (rel P (|dP| + |D|) + err dP + err D); times q or k also u |dS|
   dq dk  the same with dS (1 - tanh^2); dv as out
-An fp16 operand below its normal range is off by 2^-25 of its scale: P is held
-up to 2^7 or more, dS up to 2^13 of the bound max |do| max |v| or more.
+An fp16 number below its normal range has an absolute half step of 2^-25, and a
+pair's low half reaches there too: P is held up to 2^7 or more; dS at 2^13 or
+more for 2 max |do| max |v|, so dS is off by 2^-37 of max |do| max |v|; and each
+fp32 tensor's pairs at 2^13 or more for its largest element, so their elements
+are off by 2^-38 of it.
 Positions and sigma get dS as it is, in fp32.
 """
 import math
@@ -64,9 +67,12 @@ def exact(d, nq, nk, scale, cap, q_mask=None, k_mask=None):
     keep_q = torch.ones(sum(nq), dtype=torch.bool, device="cuda") if q_mask is None else q_mask
     keep_k = torch.ones(sum(nk), dtype=torch.bool, device="cuda") if k_mask is None else k_mask
     small_ds = 0.0
+    # of an element of q, k, v, do held as a pair
+    s_el = {x: (2.0 ** -38 * float(w[x][keep].abs().max()) if pair and keep.any() else 0.0)
+            for x, keep in (("q", keep_q), ("k", keep_k), ("v", keep_k), ("g", keep_q))}
     if dtype != torch.bfloat16 and keep_q.any() and keep_k.any():
         small_ds = float(w["g"][keep_q].norm(dim=-1).max() * w["v"][keep_k].norm(dim=-1).max()) \
-            * 2.0 ** (-38)
+            * 2.0 ** -37 * 1.01  # 2^-25 at 2^13 for 2 max |do| max |v| (and 1.001 for its sums)
     a0 = c0 = 0
     for n, m in zip(nq, nk):
         I = torch.nonzero(keep_q[a0:a0 + n])[:, 0] + a0
@@ -79,6 +85,8 @@ def exact(d, nq, nk, scale, cap, q_mask=None, k_mask=None):
         go = w["g"][I].transpose(0, 1)
         U = scale * q @ k.transpose(1, 2)
         ez = abs(scale) * ((D + 4) * E + pair) * (q.abs() @ k.abs().transpose(1, 2))
+        ez = ez + abs(scale) * (s_el["q"] * k.abs().sum(-1)[:, None]
+                                + s_el["k"] * q.abs().sum(-1)[:, :, None])
         S = cap * torch.tanh(U / cap) if cap else U
         ez = ez + 8 * E * (S.abs() + cap)
         slope = 1 - (S / cap) ** 2 if cap else torch.ones_like(S)
@@ -97,12 +105,14 @@ def exact(d, nq, nk, scale, cap, q_mask=None, k_mask=None):
         smallp = 0.0 if dtype == torch.bfloat16 else 2.0 ** -31 * (2.0 ** -8 if pair else 1)
         nj, ni = J.numel(), I.numel()
         o = P @ v
-        bo = lambda r: (P * (r + rp + (nj + 4) * E) + smallp * peak) @ v.abs()  # noqa: E731
+        bo = lambda r: (P * (r + rp + (nj + 4) * E) + smallp * peak) @ v.abs() \
+            + s_el["v"]  # noqa: E731
         out[I] = o.transpose(0, 1)
         b_out[I] = (bo(up) + u * o.abs()).transpose(0, 1)
         dP = go @ v.transpose(1, 2)
         Di = (go * o).sum(-1, keepdim=True)
         edp = ((D + 4) * E + pair) * (go.abs() @ v.abs().transpose(1, 2))
+        edp = edp + s_el["g"] * v.abs().sum(-1)[:, None] + s_el["v"] * go.abs().sum(-1)[:, :, None]
         eD = (go.abs() * (bo(fine) + (D + 4) * E * o.abs())).sum(-1, keepdim=True)
         dS = P * (dP - Di)
         eS = P * (rp * (dP.abs() + Di.abs()) + edp + eD + 4 * E * (dP - Di).abs())
@@ -121,11 +131,14 @@ def exact(d, nq, nk, scale, cap, q_mask=None, k_mask=None):
         eU = eS * slope + dS.abs() * eslope + up * dU.abs() + small_ds + 4 * E * dU.abs()
         gr["q"][I] = (scale * dU @ k).transpose(0, 1)
         b["q"][I] = (abs(scale) * (eU + ((nj + 4) * E + pair) * dU.abs()) @ k.abs()).transpose(0, 1)
+        b["q"][I] += abs(scale) * s_el["k"] * dU.abs().sum(-1).T[..., None]
         dk = scale * dU.transpose(1, 2) @ q
         n_all = ni * (heads // kv)
         bk = abs(scale) * (eU + ((n_all + 4) * E + pair) * dU.abs()).transpose(1, 2) @ q.abs()
         dv = P.transpose(1, 2) @ go
         bv = (P * (up + rp + (n_all + 4) * E + pair) + 2.0 ** -36).transpose(1, 2) @ go.abs()
+        bk = bk + abs(scale) * s_el["q"] * dU.abs().sum(1)[..., None]
+        bv = bv + s_el["g"] * P.sum(1)[..., None]
         for name, t, e in (("k", dk, bk), ("v", dv, bv)):
             fold = lambda x: x.reshape(kv, heads // kv, *x.shape[1:]).sum(1).transpose(0, 1)  # noqa: E731
             gr[name][J] = fold(t)
