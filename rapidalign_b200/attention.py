@@ -165,8 +165,10 @@ class _KernelAttention(torch.autograd.Function):
                      for i, t in enumerate((q, k, v, q_pos, k_pos, sigma))]
             gr = _lib.RaAttnGrads(*[_lib.ptr(t) for t in grads])
             ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 1), dev)
-            rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), g.data_ptr(), None,
-                                      out32.data_ptr(), stats.data_ptr(), ctypes.byref(gr),
+            f32 = q.dtype == torch.float32
+            rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), g.data_ptr(),
+                                      out32.data_ptr() if f32 else None,
+                                      None if f32 else out32.data_ptr(), stats.data_ptr(), ctypes.byref(gr),
                                       ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention backward")
         return (*grads, None, None, None, None, None, None)

@@ -143,14 +143,15 @@ template <class T>
 int bounds(const AttnPrep &p, unsigned *words, int sms, cudaStream_t st) {
   int64_t rows = 1;
   for (int t = 0; t < p.count; ++t) rows = std::max(rows, p.rows[t] * p.heads[t]);
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, (int64_t)8), sms * 8), p.count);
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows * (p.dim / 8), (int64_t)1024), sms * 8),
+                  p.count);
   attn_bounds_kernel<T><<<grid, 256, 0, st>>>(p, words);
   return launched();
 }
 int halves(const AttnPrep &p, const unsigned *words, int sms, cudaStream_t st) {
   int64_t n = 1;
   for (int t = 0; t < p.count; ++t) n = std::max(n, p.rows[t] * p.heads[t] * p.dim);
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, (int64_t)256), sms * 16), p.count);
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, (int64_t)4096), sms * 16), p.count);
   attn_halves_kernel<<<grid, 256, 0, st>>>(p, words);
   return launched();
 }
@@ -186,6 +187,9 @@ int launch(K kernel, int64_t grid, int threads, int smem, const AttnArgs &a, con
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess)
     return RA_ERR_CUDA;
+  // as much shared memory as there is: the CTAs of an SM hide each other's waits
+  cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                       cudaSharedmemCarveoutMaxShared);
   if (grid > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
   if (grid < 1) return RA_OK;
   kernel<<<(unsigned)grid, threads, smem, st>>>(a, x);
@@ -200,7 +204,7 @@ int tc_forward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
 template <class Kind, int DP>
 int tc_backward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
   int rc = RA_OK;
-  if (a.dq || a.pos_q)
+  if (a.dq || a.pos_q || a.dk)  // dk reads the D that this kernel puts right
     rc = launch(attn_tc_dq_kernel<Kind, DP>, a.n_q_tiles * a.heads, DqCfg<Kind, DP>::NT,
                 DqCfg<Kind, DP>::smem, a, x, st);
   if (!rc && (a.dk || a.dv || a.pos_k))
@@ -259,10 +263,20 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
   const AttnBwd b = bwd_layout(d);
   const bool tc = use_tc(d) && operands_aligned(d, in);
   if (a.num_q > 0) {
-    const unsigned grid =
-        (unsigned)std::min<int64_t>(ceil_div(a.num_q * a.heads, (int64_t)8), (int64_t)sms * 16);
-    attn_delta_kernel<T><<<grid, 256, 0, st>>>((const T *)a.dout, (const T *)a.out, a.out32,
-                                               a.num_q, a.heads, a.dim, (float *)a.delta);
+    const float *o32 = Kind::pair ? (const float *)a.out : a.out32;
+    if (tc) {
+      int lanes = 1;
+      while (lanes * 8 < a.dim) lanes <<= 1;
+      const unsigned grid = (unsigned)std::min<int64_t>(
+          ceil_div(a.num_q * a.heads * lanes, (int64_t)512), (int64_t)sms * 16);
+      attn_delta8_kernel<T><<<grid, 256, 0, st>>>((const T *)a.dout, o32, a.num_q, a.heads, a.dim,
+                                                  lanes, a.delta);
+    } else {
+      const unsigned grid =
+          (unsigned)std::min<int64_t>(ceil_div(a.num_q * a.heads, (int64_t)8), (int64_t)sms * 16);
+      attn_delta_kernel<T><<<grid, 256, 0, st>>>((const T *)a.dout, o32, a.num_q, a.heads, a.dim,
+                                                 a.delta);
+    }
     if ((rc = launched())) return rc;
   }
   if (tc) {
@@ -357,7 +371,7 @@ int ra_attn_backward(const ra_attn_desc *d, const ra_attn_inputs *in, const void
                      const ra_attn_grads *grads, void *state, size_t state_bytes, void *workspace,
                      size_t workspace_bytes, ra_stream_t stream) {
   if (!attn_ok(d) || !inputs_ok(d, in) || grads == nullptr) return RA_ERR_INVALID_ARGUMENT;
-  if (d->num_q > 0 && (dout == nullptr || stats == nullptr || (out == nullptr && out32 == nullptr)))
+  if (d->num_q > 0 && (dout == nullptr || stats == nullptr || (d->dtype == RA_F32 ? out : out32) == nullptr))
     return RA_ERR_INVALID_ARGUMENT;
   if (d->pos_dim == 0 && (grads->dq_pos || grads->dk_pos || grads->dsigma))
     return RA_ERR_INVALID_ARGUMENT;
@@ -372,7 +386,7 @@ int ra_attn_backward(const ra_attn_desc *d, const ra_attn_inputs *in, const void
   a.out = const_cast<void *>(out), a.out32 = const_cast<float *>(out32);
   a.stats = (float2 *)stats, a.dout = dout, a.delta = (float *)(ws + b.delta);
   a.dq = grads->dq, a.dk = grads->dk, a.dv = grads->dv;
-  if (grads->dq_pos || grads->dsigma) a.pos_q = (float4 *)(ws + b.pos_q);
+  if (grads->dq_pos || grads->dk_pos || grads->dsigma) a.pos_q = (float4 *)(ws + b.pos_q);
   if (grads->dk_pos) a.pos_k = (float4 *)(ws + b.pos_k);
   cudaStream_t st = (cudaStream_t)stream;
   if (d->dtype == RA_F32) return backward<KindF32>(d, in, a, grads, sb, ws, st);

@@ -70,7 +70,7 @@ struct AttnArgs {
   float2 *stats;    // [heads][num_q]
   // backward
   const void *dout;         // [num_q][heads][dim]
-  const float *delta;       // [heads][num_q]
+  float *delta;             // [heads][num_q]
   void *dq, *dk, *dv;       // contiguous
   float4 *pos_q, *pos_k;    // [heads][num_q], [kv_heads][num_k]; or null
   int *status;
@@ -136,15 +136,14 @@ struct AttnScore {
 
 // D_i = do_i . o_i, one warp a row and head
 template <class T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const T *dout, const T *out,
-                                                         const float *out32, int64_t num_q,
-                                                         int heads, int dim, float *delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(const T *dout, const float *out32,
+                                                         int64_t num_q, int heads, int dim,
+                                                         float *delta) {
   const int lane = threadIdx.x & 31;
   const int64_t n = num_q * heads;
   for (int64_t r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < n; r += gridDim.x * 8LL) {
     float s = 0.f;
-    for (int d = lane; d < dim; d += 32)
-      s = fmaf(to_f(dout[r * dim + d]), out32 ? out32[r * dim + d] : to_f(out[r * dim + d]), s);
+    for (int d = lane; d < dim; d += 32) s = fmaf(to_f(dout[r * dim + d]), out32[r * dim + d], s);
     s = warp_sum(s);
     if (lane == 0) delta[(r % heads) * num_q + r / heads] = s;
   }

@@ -9,12 +9,12 @@
 //                              dV += P^T dO, dK += dU^T Q
 // The two backward kernels each make S and dP (7 products instead of 5), so
 // every result has one writer: no atomics, bitwise repeatable.
-// What bounds them is not the tensor core (S and P V take 2 x 64 cycles a
-// 128 x 64 tile at DP = 64) but the elementwise part: about 12 fp32 operations
-// and an EX2 a score with positions, 800 issue slots of each SM quarter a tile.
-// So the flow within a CTA is simple -- all threads wait for the products, work
-// on the scores, one thread issues the next products -- and two to four CTAs on
-// an SM hide each other's waits.
+// What bounds them is not the tensor core (S and P V take 2 x 128 cycles a
+// 128 x 64 tile at DP = 64) but the elementwise part: 10 fp32 operations and an
+// EX2 a score with positions, about 700 issue slots of each SM quarter a tile
+// in the packed two-lane forms.  So the flow within a CTA is simple -- all
+// threads wait for the products, work on the scores, one thread issues the next
+// products -- and two to four CTAs on an SM hide each other's waits.
 //
 // Tiles lie in shared memory in the canonical no-swizzle layout, 16-byte chunk
 // (d / 8, row) at (d / 8 * rows + row) * 16: read K-major (S, dP) and MN-major
@@ -23,21 +23,27 @@
 // reaches no product.
 //
 // fp32 inputs are fp16 pairs (hi + lo, one power of two per tensor), three
-// products for one.  P of 16-bit inputs is a pair too where the output is kept
-// unrounded for a backward (D_i = do.o must be as exact as dP); dU is one
-// 16-bit number for 16-bit inputs (half a step, independent between elements).
+// products for one; the two small ones have an accumulator of their own where
+// TMEM has room (the tensor core drops the bits below an accumulator's last one
+// at each step: a third of the steps on the large sums, a third of the loss).
+// P of 16-bit inputs is a pair too where the output is kept unrounded for a
+// backward (D_i = do.o wants it); dU is one 16-bit number for 16-bit inputs (half
+// a step, independent between elements).  The dq kernel also sums dS: the sum
+// is what D_i was off by, since each row's P add up to 1, and it puts D_i right
+// for the positions and for the dk, dv kernel.
 // In fp16 P is held 2^7 up, and dU in units of the power of two that keeps
-// 2 max |do| max |v| >= |dU| / slope below 2^14.
+// 2 dim max |do| max |v| >= |dU| / slope below 2^14.
 #pragma once
+
+#include <new>
 
 #include "ra_attn.cuh"
 #include "ra_tcprim.cuh"
 
 namespace ra {
 
-// words of the bounds (bits of non-negative floats): largest finite element
-// and row norm of each tensor
-enum AttnWord { kWq = 0, kWk = 2, kWv = 4, kWdo = 6, kWords = 8 };
+// words of the bounds: bits of the largest finite magnitude of each tensor
+enum AttnWord { kWq = 0, kWk = 1, kWv = 2, kWdo = 3 };
 
 struct AttnOp {  // 16-bit operand, or its halves
   const uint16_t *hi, *lo;
@@ -77,11 +83,11 @@ template <class Kind>
 __device__ __forceinline__ int elem_exp(const AttnTcArgs &X, int w) {
   return Kind::pair ? attn_exp(__uint_as_float(X.words[w])) : 0;
 }
-// of dU: 2 |do| |v| bounds |dP - D|
+// of dU: 2 dim max |do| max |v| bounds |dP - D|
 template <class Kind>
-__device__ __forceinline__ int du_exp(const AttnTcArgs &X) {
+__device__ __forceinline__ int du_exp(const AttnTcArgs &X, int dim) {
   if (Kind::bf16) return 0;
-  return attn_exp(2.f * __uint_as_float(X.words[kWdo + 1]) * __uint_as_float(X.words[kWv + 1]));
+  return attn_exp(2.f * dim * __uint_as_float(X.words[kWdo]) * __uint_as_float(X.words[kWv]));
 }
 
 // no-swizzle descriptor of a tile of `rows` rows
@@ -161,19 +167,22 @@ __device__ __forceinline__ void products_rows(uint32_t d, uint32_t a, uint32_t b
 }
 // D[128, DP] (+)= W[128, KT] X[KT, DP]: W in TMEM (per 32 columns of the
 // scores 16 columns of hi, 16 of lo), X a streamed tile read MN-major
-template <class Kind, int KT, int DP>
+// SMALL: the small products of pairs go to the accumulator behind D
+template <class Kind, int KT, int DP, bool SMALL>
 __device__ __forceinline__ void products_weighted(uint32_t d, uint32_t w, uint32_t x, bool w_pair,
-                                                  uint32_t acc) {
+                                                  bool more) {
   constexpr uint32_t idesc = attn_idesc(DP, Kind::bf16, true);
   const int first = Kind::pair || w_pair ? 0 : 2;
+  uint32_t acc = more;
 #pragma unroll
   for (int p = 0; p < 3; ++p) {  // lo hi, hi lo (pairs of x only), hi hi
     if (p < first || (p == 1 && !Kind::pair)) continue;
     const uint64_t dx = tile_desc_mn(x + (Kind::pair && p == 1 ? tile_bytes<KT, DP> : 0), KT);
+    if (SMALL && p == 2) acc = more;
 #pragma unroll
     for (int k = 0; k < KT / 16; ++k) {
-      mma_ts(d, w + (k >> 1) * 32 + (k & 1) * 8 + (p == 0 ? 16 : 0), dx + (uint64_t)(k * 256 >> 4),
-             idesc, acc);
+      mma_ts(SMALL && p < 2 ? d + DP : d, w + (k >> 1) * 32 + (k & 1) * 8 + (p == 0 ? 16 : 0),
+             dx + (uint64_t)(k * 256 >> 4), idesc, acc);
       acc = 1;
     }
   }
@@ -224,17 +233,73 @@ __device__ __forceinline__ float tanh_kind(float u) {
   return fabsf(u) < 0.1f ? small : big;
 }
 
-// raw products of 32 scores -> base-2 scores before the distances; th: tanh
-// where capped
-template <class Kind>
-__device__ __forceinline__ void scores32(float (&v)[32], float su, float capl) {
-  if (capl > 0.f) {
+// Positions of a streamed tile in shared memory: x, y, z of its rows.
+template <int R>
+struct TilePos {
+  float c[3][R];
+};
+__device__ __forceinline__ f2_t two(float v) { return pk(v, v); }
+struct RowPos {  // -p of this thread's row, twice
+  f2_t x, y, z;
+  __device__ __forceinline__ void set(const AttnPos &p) {
+    x = two(-p.x), y = two(-p.y), z = two(-p.z);
+  }
+};
+// p_c - p_row and its square for columns c .. c + 3
+struct Diff4 {
+  f2_t x[2], y[2], z[2], r2[2];
+  template <int R>
+  __device__ __forceinline__ Diff4(const TilePos<R> &t, int c, const RowPos &p) {
+    const ulonglong2 tx = *reinterpret_cast<const ulonglong2 *>(t.c[0] + c);
+    const ulonglong2 ty = *reinterpret_cast<const ulonglong2 *>(t.c[1] + c);
+    const ulonglong2 tz = *reinterpret_cast<const ulonglong2 *>(t.c[2] + c);
+    x[0] = add2(tx.x, p.x), x[1] = add2(tx.y, p.x);
+    y[0] = add2(ty.x, p.y), y[1] = add2(ty.y, p.y);
+    z[0] = add2(tz.x, p.z), z[1] = add2(tz.y, p.z);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = capl * tanh_kind<Kind>(v[j] * su);
+    for (int k = 0; k < 2; ++k) r2[k] = fma2(z[k], z[k], fma2(y[k], y[k], mul2(x[k], x[k])));
+  }
+};
+
+// raw products of 32 scores -> base-2 scores
+template <class Kind, int R>
+__device__ __forceinline__ void scores32(const float (&v)[32], f2_t (&t)[16], const AttnScore &sc,
+                                         bool pos, const TilePos<R> &tp, int c0,
+                                         const RowPos &rp) {
+  const f2_t su = two(sc.su);
+  if (sc.capl > 0.f) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      t[j] = pk(sc.capl * tanh_kind<Kind>(v[2 * j] * sc.su),
+                sc.capl * tanh_kind<Kind>(v[2 * j + 1] * sc.su));
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= su;
+    for (int j = 0; j < 16; ++j) t[j] = mul2(pk(v[2 * j], v[2 * j + 1]), su);
   }
+  if (pos) {
+    const f2_t nw = two(-sc.w);
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const Diff4 d(tp, c0 + j, rp);
+      t[j / 2] = fma2(nw, d.r2[0], t[j / 2]);
+      t[j / 2 + 1] = fma2(nw, d.r2[1], t[j / 2 + 1]);
+    }
+  }
+}
+
+// One past the last row of [0, n) that the mask leaves, for the whole CTA:
+// padded tails cost nothing.  `slot`: an int in shared memory.
+__device__ __forceinline__ int64_t masked_extent(const uint8_t *mask, int64_t n, int nt,
+                                                 unsigned long long *slot) {
+  if (mask == nullptr) return n;
+  if (threadIdx.x == 0) *slot = 0;
+  __syncthreads();
+  int64_t last = 0;
+  for (int64_t i = threadIdx.x; i < n; i += nt)
+    if (mask[i]) last = i + 1;
+  if (last) atomicMax(slot, (unsigned long long)last);
+  __syncthreads();
+  return (int64_t)*slot;
 }
 
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
@@ -255,13 +320,19 @@ __host__ __device__ constexpr int tmem_round(int c) {
 }
 
 // dim of a row's fp32 values (from TMEM, times f) to T and to fp32
-template <class T, int DP>
+template <class T, int DP, bool SMALL>
 __device__ __forceinline__ void write_row(uint32_t taddr, float f, bool on, bool zero, int dim,
                                           T *out, float *out32) {
 #pragma unroll 1
   for (int c = 0; c < DP; c += 32) {
     float v[32];
     tmem_ld32(taddr + c, v);
+    if (SMALL) {
+      float u[32];
+      tmem_ld32(taddr + DP + c, u);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += u[j];
+    }
     if (!on || c >= dim) continue;
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = zero ? 0.f : v[j] * f;
@@ -301,47 +372,109 @@ struct AttnPrep {
   int dim, count;
 };
 
-// largest finite element and row norm of each tensor; one warp a row and head
+// (row, head, chunk of 8) of the e-th chunk
+struct PrepAt {
+  int64_t i;
+  int h, c;
+  __device__ __forceinline__ PrepAt(int64_t e, int heads, int dim8, bool small) {
+    if (small) {
+      const unsigned u = (unsigned)e, r = u / dim8;
+      c = u - r * dim8;
+      i = r / heads;
+      h = r - (unsigned)i * heads;
+    } else {
+      const int64_t r = e / dim8;
+      c = (int)(e - r * dim8);
+      i = r / heads;
+      h = (int)(r - i * heads);
+    }
+  }
+};
+template <class T>
+__device__ __forceinline__ void load8(const T *x, bool wide, float (&v)[8]) {
+  if (wide) {
+    alignas(16) T t[8];
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+      reinterpret_cast<uint4 *>(t)[k] = reinterpret_cast<const uint4 *>(x)[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = to_f(t[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = to_f(x[k]);
+  }
+}
+template <class T>
+__device__ __forceinline__ bool rows_wide(const AttnPrep &p, int t) {
+  constexpr int e = 16 / sizeof(T);
+  return ((uintptr_t)p.x[t] & 15) == 0 && p.row[t] % e == 0 && p.head[t] % e == 0;
+}
+
+// largest finite magnitude of each tensor
 template <class T>
 __global__ void __launch_bounds__(256) attn_bounds_kernel(const AttnPrep p, unsigned *words) {
-  const int t = blockIdx.y, lane = threadIdx.x & 31;
-  const int64_t n = p.rows[t] * p.heads[t];
-  float top = 0.f, norm = 0.f;
-  for (int64_t r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < n; r += gridDim.x * 8LL) {
-    const int64_t i = r / p.heads[t];
-    if (p.mask[t] != nullptr && p.mask[t][i] == 0) continue;
-    const T *x = (const T *)p.x[t] + i * p.row[t] + (r % p.heads[t]) * p.head[t];
-    float m = 0.f, s = 0.f;
-    for (int d = lane; d < p.dim; d += 32) {
-      const float v = to_f(x[d]);
-      if (fabsf(v) < INFINITY) m = fmaxf(m, fabsf(v));
-      s = fmaf(v, v, s);
-    }
-    s = warp_sum(s);
-    top = fmaxf(top, m);
-    if (s < INFINITY) norm = fmaxf(norm, s);
+  const int t = blockIdx.y, dim8 = p.dim >> 3;
+  const int64_t n = p.rows[t] * p.heads[t] * dim8;
+  const bool small = n < ((int64_t)1 << 31), wide = rows_wide<T>(p, t);
+  float top = 0.f;
+  for (int64_t e = blockIdx.x * 256LL + threadIdx.x; e < n; e += gridDim.x * 256LL) {
+    const PrepAt at(e, p.heads[t], dim8, small);
+    if (p.mask[t] != nullptr && p.mask[t][at.i] == 0) continue;
+    float v[8];
+    load8((const T *)p.x[t] + at.i * p.row[t] + at.h * p.head[t] + at.c * 8, wide, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (fabsf(v[k]) < INFINITY) top = fmaxf(top, fabsf(v[k]));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-  if (lane == 0) {  // maxima of bits: any order
-    if (top > 0.f) atomicMax(words + p.word[t], __float_as_uint(top));
-    norm = sqrtf(norm) * 1.001f;
-    if (norm > 0.f) atomicMax(words + p.word[t] + 1, __float_as_uint(norm));
+  // maxima of bits: any order
+  if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(words + p.word[t], __float_as_uint(top));
+}
+
+// x 2^e = hi + lo in fp16
+__global__ void __launch_bounds__(256) attn_halves_kernel(const AttnPrep p, const unsigned *words) {
+  const int t = blockIdx.y, dim8 = p.dim >> 3;
+  const float sc = ldexpf(1.f, attn_exp(__uint_as_float(words[p.word[t]])));
+  const int64_t n = p.rows[t] * p.heads[t] * dim8;
+  const bool small = n < ((int64_t)1 << 31), wide = rows_wide<float>(p, t);
+  for (int64_t e = blockIdx.x * 256LL + threadIdx.x; e < n; e += gridDim.x * 256LL) {
+    const PrepAt at(e, p.heads[t], dim8, small);
+    float v[8];
+    load8((const float *)p.x[t] + at.i * p.row[t] + at.h * p.head[t] + at.c * 8, wide, v);
+    alignas(16) __half hi[8];
+    alignas(16) __half lo[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float y = v[k] * sc;
+      hi[k] = __float2half_rn(y);
+      lo[k] = __float2half_rn(y - __half2float(hi[k]));
+    }
+    reinterpret_cast<uint4 *>(p.hi[t])[e] = *reinterpret_cast<const uint4 *>(hi);
+    reinterpret_cast<uint4 *>(p.lo[t])[e] = *reinterpret_cast<const uint4 *>(lo);
   }
 }
 
-__global__ void __launch_bounds__(256) attn_halves_kernel(const AttnPrep p, const unsigned *words) {
-  const int t = blockIdx.y;
-  const float sc = ldexpf(1.f, attn_exp(__uint_as_float(words[p.word[t]])));
-  const int64_t n = p.rows[t] * p.heads[t] * p.dim;
-  const int64_t per = (int64_t)p.heads[t] * p.dim;
-  for (int64_t e = blockIdx.x * 256LL + threadIdx.x; e < n; e += gridDim.x * 256LL) {
-    const int64_t i = e / per;
-    const int r = (int)(e - i * per), h = r / p.dim, d = r - h * p.dim;
-    const float v = ((const float *)p.x[t])[i * p.row[t] + h * p.head[t] + d] * sc;
-    const __half hi = __float2half_rn(v);
-    p.hi[t][e] = __half_as_ushort(hi);
-    p.lo[t][e] = __half_as_ushort(__float2half_rn(v - __half2float(hi)));
+// D_i = do_i . o_i: 2^k lanes a row and head, 8 elements each
+template <class T>
+__global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const float *out32,
+                                                          int64_t num_q, int heads, int dim,
+                                                          int lanes, float *delta) {
+  const int l = threadIdx.x % lanes;
+  const int64_t n = num_q * heads, step = gridDim.x * 256LL / lanes;
+  // all lanes of a warp go round together: the shuffles need them
+  for (int64_t r0 = (blockIdx.x * 256LL + (threadIdx.x & ~31)) / lanes; r0 < n; r0 += step) {
+    const int64_t r = r0 + (threadIdx.x & 31) / lanes;
+    float s = 0.f;
+    if (r < n && l * 8 < dim) {
+      float a[8], b[8];
+      load8(dout + r * dim + l * 8, true, a);
+      load8(out32 + r * dim + l * 8, true, b);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fmaf(a[k], b[k], s);
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+    if (r < n && l == 0) delta[(r % heads) * num_q + r / heads] = s;
   }
 }
 
@@ -352,21 +485,23 @@ struct FwdCfg {
   static constexpr int KT = Kind::pair && DP == 128 ? 32 : 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
-  static constexpr int TMEM = tmem_round(KT + DP);
-  static constexpr int pos = Q + 4 * KV;                 // float4 [2][KT]
-  static constexpr int val = pos + 2 * KT * 16;          // unsigned [2][2]
-  static constexpr int bar = val + 16, slot = bar + 8;
+  static constexpr bool SMALL = Kind::pair;
+  static constexpr int TMEM = tmem_round(KT + (SMALL ? 2 : 1) * DP);
+  static constexpr int pos = Q + 4 * KV;                 // TilePos<KT> [2]
+  static constexpr int val = pos + 2 * KT * 12;          // unsigned [2][2]
+  static constexpr int bar = val + 16, slot = bar + 8;   // slot: also the mask's extent
   static constexpr int smem = slot + 8;
+  static constexpr int CTAS = smem <= 56 * 1024 ? 4 : smem <= 113 * 1024 ? 2 : 1;
 };
 
 template <class Kind, int DP>
-__global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, const AttnTcArgs X) {
+__global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kernel(const AttnArgs A, const AttnTcArgs X) {
   using C = FwdCfg<Kind, DP>;
   constexpr int KT = C::KT;
   extern __shared__ __align__(1024) uint8_t sm[];
   const uint32_t base = smem_u32(sm);
   const uint32_t sQ = base, sK = base + C::Q, sV = sK + 2 * C::KV, bar = base + C::bar;
-  float4 *kpos = reinterpret_cast<float4 *>(sm + C::pos);
+  TilePos<KT> *kpos = reinterpret_cast<TilePos<KT> *>(sm + C::pos);
   unsigned *kval = reinterpret_cast<unsigned *>(sm + C::val);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -376,8 +511,13 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
   const int2 tile = A.qs.tile(item / X.splits / A.heads);
   const int64_t i0 = A.qs.begin(tile.x) + 128LL * tile.y, j0 = A.ks.begin(tile.x);
   const int nq = (int)min((int64_t)128, A.qs.end(tile.x) - i0);
-  const int64_t nk = A.ks.end(tile.x) - j0;
-  const int64_t all = (nk + KT - 1) / KT;
+  const int64_t i = i0 + threadIdx.x;
+  const bool row_on = threadIdx.x < nq && (A.q_mask == nullptr || A.q_mask[i] != 0);
+  const int64_t nk =
+      masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, A.ks.end(tile.x) - j0, 128,
+                    reinterpret_cast<unsigned long long *>(sm + C::slot));
+  // no row to work for: no keys to see
+  const int64_t all = __syncthreads_or(row_on) ? (nk + KT - 1) / KT : 0;
   const int64_t t0 = all * split / X.splits, t1 = all * (split + 1) / X.splits;
   const int dim8 = A.dim >> 3;
 
@@ -399,7 +539,7 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
       if (lane == 0) kval[2 * b + warp] = bits;
       AttnPos p{0.f, 0.f, 0.f};
       if (on) p = pos_of(A.k_pos, A.pos_dim, r0 + r);
-      kpos[b * KT + r] = make_float4(p.x, p.y, p.z, 0.f);
+      kpos[b].c[0][r] = p.x, kpos[b].c[1][r] = p.y, kpos[b].c[2][r] = p.z;
     }
   };
   load_tile<Kind, 128, DP, 128>(sQ, X.q, h, i0, nq, dim8, A.q_mask);
@@ -412,13 +552,11 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + C::slot);
   const uint32_t tS = tmem, tO = tmem + KT, lane_off = (uint32_t)(32 * warp) << 16;
 
-  const int64_t i = i0 + threadIdx.x;
-  const bool row_on = threadIdx.x < nq && (A.q_mask == nullptr || A.q_mask[i] != 0);
   AttnScore sc;
   sc.init(A, h);
   sc.su *= ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
-  AttnPos pi{0.f, 0.f, 0.f};
-  if (row_on) pi = pos_of(A.q_pos, A.pos_dim, i);
+  RowPos rp;
+  rp.set(row_on ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
   constexpr float kUp = Kind::bf16 ? 0.f : 7.f;  // P is held 2^kUp up
   const bool p_pair = Kind::pair || X.pair_p;
   float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to
@@ -435,31 +573,26 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) load_keys(t + 1);  // its buffers' products are done
-    float v[KT / 32][32];
-    const unsigned vb[2] = {kval[2 * b], KT > 32 ? kval[2 * b + 1] : 0u};
-#pragma unroll
-    for (int c = 0; c < KT / 32; ++c) {
-      tmem_ld32(tS + lane_off + 32 * c, v[c]);
-      scores32<Kind>(v[c], sc.su, sc.capl);
-      if (A.pos_dim > 0) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float4 p = kpos[b * KT + 32 * c + j];
-          const float dx = pi.x - p.x, dy = pi.y - p.y, dz = pi.z - p.z;
-          v[c][j] = fmaf(-sc.w, fmaf(dz, dz, fmaf(dy, dy, dx * dx)), v[c][j]);
-        }
-      }
-      if (vb[c] != kFull) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (!((vb[c] >> j) & 1)) v[c][j] = -INFINITY;
-      }
-    }
+    f2_t s2[KT / 32][16];
     float mx = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < KT / 32; ++c)
+    for (int c = 0; c < KT / 32; ++c) {
+      float v[32];
+      tmem_ld32(tS + lane_off + 32 * c, v);
+      scores32<Kind>(v, s2[c], sc, A.pos_dim > 0, kpos[b], 32 * c, rp);
+      const unsigned bits = kval[2 * b + c];
+      if (bits != kFull) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[c][j]);
+        for (int j = 0; j < 16; ++j) {
+          float x, y;
+          upk(s2[c][j], x, y);
+          s2[c][j] = pk((bits >> (2 * j)) & 1 ? x : -INFINITY,
+                        (bits >> (2 * j + 1)) & 1 ? y : -INFINITY);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, fmaxf(lo_of(s2[c][j]), hi_of(s2[c][j])));
+    }
     // the reference follows the maximum only where it grew by more than 2^8:
     // sums and O stay relative to one reference, whichever it is
     const bool grow = mx > m + 8.f;  // also from -inf
@@ -469,7 +602,7 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
       l *= f;
       if (t > t0) {
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = 0; c < (C::SMALL ? 2 : 1) * DP; c += 32) {
           float o[32];
           tmem_ld32(tO + lane_off + c, o);
           uint32_t u[32];
@@ -480,20 +613,23 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
       }
       m = mn;
     }
-    const float ref = (m > -INFINITY ? m : 0.f) - kUp;
-    float s0 = 0.f, s1 = 0.f;
+    const f2_t ref = two(kUp - (m > -INFINITY ? m : 0.f));
+    f2_t sum[2] = {0, 0};
 #pragma unroll
     for (int c = 0; c < KT / 32; ++c) {
+      float v[32];
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        v[c][j] = ex2(v[c][j] - ref);
-        v[c][j + 1] = ex2(v[c][j + 1] - ref);
-        s0 += v[c][j];
-        s1 += v[c][j + 1];
+      for (int j = 0; j < 16; ++j) {
+        float x, y;
+        upk(add2(s2[c][j], ref), x, y);
+        v[2 * j] = ex2(x);
+        v[2 * j + 1] = ex2(y);
+        sum[j & 1] = add2(sum[j & 1], pk(v[2 * j], v[2 * j + 1]));
       }
-      put_weights<Kind>(tS + lane_off + 32 * c, v[c], p_pair);
+      put_weights<Kind>(tS + lane_off + 32 * c, v, p_pair);
     }
-    l += s0 + s1;
+    const f2_t both = add2(sum[0], sum[1]);
+    l += lo_of(both) + hi_of(both);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     cp_wait_all();
     fence_async_smem();
@@ -501,7 +637,7 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
     if ((bad = __syncthreads_or(bad))) break;
     if (threadIdx.x == 0) {
       tc_fence_after();
-      products_weighted<Kind, KT, DP>(tO, tS, sV + b * C::KV, p_pair, t > t0);
+      products_weighted<Kind, KT, DP, C::SMALL>(tO, tS, sV + b * C::KV, p_pair, t > t0);
       if (t + 1 < t1) products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
       tc_commit(bar);
     }
@@ -520,14 +656,14 @@ __global__ void __launch_bounds__(128) attn_tc_fwd_kernel(const AttnArgs A, cons
   const bool in = threadIdx.x < nq;
   if (X.splits > 1) {
     float *po = X.part_o + ((split * A.num_q + i) * A.heads + h) * A.dim;
-    write_row<float, DP>(tO + lane_off, unscale, in, empty, A.dim, po, nullptr);
+    write_row<float, DP, C::SMALL>(tO + lane_off, unscale, in, empty, A.dim, po, nullptr);
     if (in)
       X.part_s[((int64_t)split * A.heads + h) * A.num_q + i] =
           make_float2(empty ? -INFINITY : (m > -INFINITY ? m : 0.f) - kUp, empty ? 0.f : l);
   } else {
     const float r = empty ? 0.f : 1.f / l;
     const int64_t at = (i * A.heads + h) * A.dim;
-    write_row<T, DP>(tO + lane_off, unscale * r, in, empty, A.dim, (T *)A.out + at,
+    write_row<T, DP, C::SMALL>(tO + lane_off, unscale * r, in, empty, A.dim, (T *)A.out + at,
                      A.out32 ? A.out32 + at : nullptr);
     if (in && A.stats)
       A.stats[h * A.num_q + i] =
@@ -580,90 +716,134 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs A, int sp
 
 // ---- backward -------------------------------------------------------------------
 
-// The elementwise part of 32 scores of a row, all in one pass so that only the
-// scores and dP are held.  `v` raw products, `dp` raw dP; out: dU in dp (and P
-// in v where the rows are keys).  g: the sums of dS (p_i - p_j) [, dS r^2].
+// The elementwise part of 32 scores of a row, four at a time, all in one pass
+// so that only the scores and dP are held.  `v` raw products, `dp` raw dP; out:
+// dU in dp (and P in v where the rows are keys).
 // CAP, POS, PG: the cap, positions and their gradients are there.
 struct BwdRow {
-  float su, capl, w, dps, up;
-  AttnPos p;
+  AttnScore sc;
+  float dps, up;  // of raw dP; of dU
+  RowPos p;
 };
-template <class Kind, bool CAP, bool POS, bool PG>
-__device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], const BwdRow &R,
+// dq: the row's statistics, and its sums of dS, dS (p_j - p_i), dS r^2 and of
+// P (p_j - p_i), P r^2, each in two lanes
+struct DqSums {
+  f2_t ds = 0, g[4] = {}, q[4] = {};
+};
+template <class Kind, bool CAP, bool POS, bool PG, int R>
+__device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], const BwdRow &B,
                                             float m, float rl, float delta, unsigned bits,
-                                            const float4 *kpos, float (&g)[4]) {
+                                            const TilePos<R> &tp, int c0, DqSums &S) {
   const bool every = bits == kFull;
+  const f2_t su = two(B.sc.su), nm = two(-m), nw = two(-B.sc.w), dps = two(B.dps),
+             nd = two(-delta), r2l = two(rl), up = two(B.up);
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    float t = v[j] * R.su, th = 0.f, r2 = 0.f, dx = 0.f, dy = 0.f, dz = 0.f;
-    if (CAP) {
-      th = tanh_kind<Kind>(t);
-      t = th * R.capl;
+  for (int j = 0; j < 32; j += 4) {
+    Diff4 *d = nullptr;
+    alignas(Diff4) char raw[sizeof(Diff4)];
+    if (POS) d = new (raw) Diff4(tp, c0 + j, B.p);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = j + 2 * k;
+      f2_t t, th;
+      if (CAP) {
+        th = pk(tanh_kind<Kind>(v[e] * B.sc.su), tanh_kind<Kind>(v[e + 1] * B.sc.su));
+        t = fma2(th, two(B.sc.capl), nm);
+      } else {
+        t = fma2(pk(v[e], v[e + 1]), su, nm);
+      }
+      if (POS) t = fma2(nw, d->r2[k], t);
+      float x, y;
+      upk(t, x, y);
+      x = ex2(x), y = ex2(y);
+      if (!every) {
+        x = (bits >> e) & 1 ? x : 0.f;
+        y = (bits >> (e + 1)) & 1 ? y : 0.f;
+      }
+      const f2_t p = mul2(pk(x, y), r2l);
+      f2_t ds = mul2(p, fma2(pk(dp[e], dp[e + 1]), dps, nd));
+      S.ds = add2(S.ds, ds);
+      if (PG) {
+        S.g[0] = fma2(ds, d->x[k], S.g[0]), S.q[0] = fma2(p, d->x[k], S.q[0]);
+        S.g[1] = fma2(ds, d->y[k], S.g[1]), S.q[1] = fma2(p, d->y[k], S.q[1]);
+        S.g[2] = fma2(ds, d->z[k], S.g[2]), S.q[2] = fma2(p, d->z[k], S.q[2]);
+        S.g[3] = fma2(ds, d->r2[k], S.g[3]), S.q[3] = fma2(p, d->r2[k], S.q[3]);
+      }
+      if (CAP) ds = mul2(ds, fma2(mul2(th, two(-1.f)), th, two(1.f)));
+      if (!Kind::bf16) ds = mul2(ds, up);
+      upk(ds, dp[e], dp[e + 1]);
     }
-    if (POS) {
-      const float4 p = kpos[j];
-      dx = R.p.x - p.x, dy = R.p.y - p.y, dz = R.p.z - p.z;
-      r2 = fmaf(dz, dz, fmaf(dy, dy, dx * dx));
-      t = fmaf(-R.w, r2, t);
-    }
-    float ds = ex2(t - m) * rl * fmaf(dp[j], R.dps, -delta);
-    if (!every) ds = (bits >> j) & 1 ? ds : 0.f;
-    if (PG) {
-      g[0] = fmaf(ds, dx, g[0]);
-      g[1] = fmaf(ds, dy, g[1]);
-      g[2] = fmaf(ds, dz, g[2]);
-      g[3] = fmaf(ds, r2, g[3]);
-    }
-    if (CAP) ds *= fmaf(-th, th, 1.f);
-    dp[j] = Kind::bf16 ? ds : ds * R.up;
   }
 }
-template <class Kind, bool CAP, bool POS, bool PG>
-__device__ __forceinline__ void dkv_elements(float (&v)[32], float (&dp)[32], const BwdRow &R,
-                                             float p_up, const float2 *qst, const float4 *qpos,
-                                             float (&g)[4]) {
+// dk, dv: the columns' (queries') statistics in shared memory
+template <int R>
+struct TileStat {
+  float nm[R], rl[R], nd[R];  // -m, 1 / l, -D
+};
+template <class Kind, bool CAP, bool POS, bool PG, int R>
+__device__ __forceinline__ void dkv_elements(float (&v)[32], float (&dp)[32], const BwdRow &B,
+                                             float p_up, const TileStat<R> &st,
+                                             const TilePos<R> &tp, int c0, f2_t (&g)[3]) {
+  const f2_t su = two(B.sc.su), nw = two(-B.sc.w), dps = two(B.dps), up = two(B.up);
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
-    float t = v[c] * R.su, th = 0.f, dx = 0.f, dy = 0.f, dz = 0.f;
-    const float4 p = qpos[c];
-    const float2 st = qst[c];
-    if (CAP) {
-      th = tanh_kind<Kind>(t);
-      t = th * R.capl;
+  for (int j = 0; j < 32; j += 4) {
+    Diff4 *d = nullptr;
+    alignas(Diff4) char raw[sizeof(Diff4)];
+    if (POS) d = new (raw) Diff4(tp, c0 + j, B.p);
+    const ulonglong2 nm = *reinterpret_cast<const ulonglong2 *>(st.nm + c0 + j);
+    const ulonglong2 rl = *reinterpret_cast<const ulonglong2 *>(st.rl + c0 + j);
+    const ulonglong2 nd = *reinterpret_cast<const ulonglong2 *>(st.nd + c0 + j);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = j + 2 * k;
+      f2_t t, th;
+      if (CAP) {
+        th = pk(tanh_kind<Kind>(v[e] * B.sc.su), tanh_kind<Kind>(v[e + 1] * B.sc.su));
+        t = fma2(th, two(B.sc.capl), k ? nm.y : nm.x);
+      } else {
+        t = fma2(pk(v[e], v[e + 1]), su, k ? nm.y : nm.x);
+      }
+      if (POS) t = fma2(nw, d->r2[k], t);
+      float x, y;
+      upk(t, x, y);
+      f2_t p = mul2(pk(ex2(x), ex2(y)), k ? rl.y : rl.x);
+      f2_t ds = mul2(p, fma2(pk(dp[e], dp[e + 1]), dps, k ? nd.y : nd.x));
+      if (PG) {
+        g[0] = fma2(ds, d->x[k], g[0]);
+        g[1] = fma2(ds, d->y[k], g[1]);
+        g[2] = fma2(ds, d->z[k], g[2]);
+      }
+      if (CAP) ds = mul2(ds, fma2(mul2(th, two(-1.f)), th, two(1.f)));
+      if (!Kind::bf16) {
+        ds = mul2(ds, up);
+        p = mul2(p, two(p_up));
+      }
+      upk(ds, dp[e], dp[e + 1]);
+      upk(p, v[e], v[e + 1]);
     }
-    if (POS) {
-      dx = p.x - R.p.x, dy = p.y - R.p.y, dz = p.z - R.p.z;
-      t = fmaf(-R.w, fmaf(dz, dz, fmaf(dy, dy, dx * dx)), t);
-    }
-    const float pr = ex2(t - st.x) * st.y;
-    float ds = pr * fmaf(dp[c], R.dps, -p.w);
-    if (PG) {
-      g[0] = fmaf(ds, dx, g[0]);
-      g[1] = fmaf(ds, dy, g[1]);
-      g[2] = fmaf(ds, dz, g[2]);
-    }
-    if (CAP) ds *= fmaf(-th, th, 1.f);
-    v[c] = Kind::bf16 ? pr : pr * p_up;
-    dp[c] = Kind::bf16 ? ds : ds * R.up;
   }
 }
+__device__ __forceinline__ float sum_of(f2_t v) { return lo_of(v) + hi_of(v); }
 
 template <class Kind, int DP>
 struct DqCfg {
   static constexpr int KT = Kind::pair && DP == 128 ? 32 : 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
-  static constexpr int STAGES = Kind::pair && DP == 128 ? 1 : 2;
-  static constexpr int TMEM = tmem_round(2 * KT + DP);
+  // two CTAs on an SM are worth more than a second buffer
+  static constexpr int STAGES = 2 * Q + 4 * KV <= 100 * 1024 ? 2 : 1;
+  static constexpr bool SMALL = Kind::pair;
+  static constexpr int TMEM = tmem_round(2 * KT + (SMALL ? 2 : 1) * DP);
   static constexpr int NT = 128 * (KT / 32);
-  static constexpr int pos = 2 * Q + 2 * STAGES * KV;
-  static constexpr int val = pos + 2 * KT * 16;
+  static constexpr int pos = 2 * Q + 2 * STAGES * KV;  // TilePos<KT> [2]
+  static constexpr int val = pos + 2 * KT * 12;
   static constexpr int bar = val + 16, slot = bar + 8;
   static constexpr int smem = slot + 8;
+  static constexpr int CTAS = smem <= 113 * 1024 && TMEM <= 256 ? 2 : 1;
 };
 
 template <class Kind, int DP>
-__global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const AttnArgs A,
+__global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) attn_tc_dq_kernel(const AttnArgs A,
                                                                          const AttnTcArgs X) {
   using C = DqCfg<Kind, DP>;
   constexpr int KT = C::KT, NT = C::NT;
@@ -671,7 +851,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const A
   const uint32_t base = smem_u32(sm);
   const uint32_t sQ = base, sG = base + C::Q, sK = sG + C::Q, sV = sK + C::STAGES * C::KV,
                  bar = base + C::bar;
-  float4 *kpos = reinterpret_cast<float4 *>(sm + C::pos);
+  TilePos<KT> *kpos = reinterpret_cast<TilePos<KT> *>(sm + C::pos);
   unsigned *kval = reinterpret_cast<unsigned *>(sm + C::val);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = warp >> 2, row = threadIdx.x & 127;  // columns 32 part.. of the tile
@@ -681,8 +861,15 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const A
   const int2 tile = A.qs.tile(item / A.heads);
   const int64_t i0 = A.qs.begin(tile.x) + 128LL * tile.y, j0 = A.ks.begin(tile.x);
   const int nq = (int)min((int64_t)128, A.qs.end(tile.x) - i0);
-  const int64_t nk = A.ks.end(tile.x) - j0;
-  const int64_t t1 = (nk + KT - 1) / KT;
+  const int64_t nk =
+      masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, A.ks.end(tile.x) - j0, NT,
+                    reinterpret_cast<unsigned long long *>(sm + C::slot));
+  const int64_t i = i0 + row;
+  const bool in = row < nq;
+  float2 st = make_float2(INFINITY, 0.f);
+  if (in) st = A.stats[h * A.num_q + i];
+  const bool live = st.y != 0.f;  // has keys, and is not masked
+  const int64_t t1 = __syncthreads_or(live) ? (nk + KT - 1) / KT : 0;
   const int dim8 = A.dim >> 3;
 
   if (warp == 0) tmem_alloc<C::TMEM>(base + C::slot);
@@ -703,7 +890,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const A
       if (lane == 0) kval[2 * pb + warp] = bits;
       AttnPos p{0.f, 0.f, 0.f};
       if (on) p = pos_of(A.k_pos, A.pos_dim, r0 + r);
-      kpos[pb * KT + r] = make_float4(p.x, p.y, p.z, 0.f);
+      kpos[pb].c[0][r] = p.x, kpos[pb].c[1][r] = p.y, kpos[pb].c[2][r] = p.z;
     }
   };
   load_tile<Kind, 128, DP, NT>(sQ, X.q, h, i0, nq, dim8, A.q_mask);
@@ -718,21 +905,15 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const A
   const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
   const uint32_t tS = tmem, tP = tmem + KT, tD = tmem + 2 * KT;
 
-  const int64_t i = i0 + row;
-  const bool in = row < nq;
-  float2 st = make_float2(INFINITY, 0.f);
-  if (in) st = A.stats[h * A.num_q + i];
-  const bool live = st.y != 0.f;  // has keys, and is not masked
   const float delta = live ? A.delta[h * A.num_q + i] : 0.f;
-  AttnScore sc;
-  sc.init(A, h);
-  sc.su *= ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
-  const int eu = du_exp<Kind>(X);
-  BwdRow R{sc.su, sc.capl, sc.w,
-           ldexpf(1.f, -elem_exp<Kind>(X, kWdo) - elem_exp<Kind>(X, kWv)), ldexpf(1.f, eu),
-           {0.f, 0.f, 0.f}};
-  if (live) R.p = pos_of(A.q_pos, A.pos_dim, i);
-  float g[4] = {};
+  BwdRow B;
+  B.sc.init(A, h);
+  B.sc.su *= ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
+  const int eu = du_exp<Kind>(X, A.dim);
+  B.dps = ldexpf(1.f, -elem_exp<Kind>(X, kWdo) - elem_exp<Kind>(X, kWv));
+  B.up = ldexpf(1.f, eu);
+  B.p.set(live ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
+  DqSums S;
   const bool pos_grad = A.pos_q != nullptr;
   bool bad = false;
   unsigned phase = 0;
@@ -752,10 +933,9 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const A
     tmem_ld32(tS + lane_off + 32 * part, v);
     tmem_ld32(tP + lane_off + 32 * part, dp);
     const unsigned bits = live ? kval[2 * pb + part] : 0u;
-    const float4 *kp = kpos + pb * KT + 32 * part;
-#define RA_DQ(C, P, G) \
-  dq_elements<Kind, C, P, G>(v, dp, R, st.x, st.y, delta, bits, kp, g)
-    if (R.capl > 0.f) {
+#define RA_DQ(C, P, G)                                                                       \
+  dq_elements<Kind, C, P, G>(v, dp, B, st.x, st.y, delta, bits, kpos[pb], 32 * part, S)
+    if (B.sc.capl > 0.f) {
       if (pos_grad) RA_DQ(true, true, true);
       else if (A.pos_dim > 0) RA_DQ(true, true, false);
       else RA_DQ(true, false, false);
@@ -773,7 +953,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const A
     if ((bad = __syncthreads_or(bad))) break;
     if (threadIdx.x == 0) {
       tc_fence_after();
-      products_weighted<Kind, KT, DP>(tD, tS, sK + b * C::KV, false, t > 0);
+      products_weighted<Kind, KT, DP, C::SMALL>(tD, tS, sK + b * C::KV, false, t > 0);
       if (C::STAGES > 1 && t + 1 < t1) {
         products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
         products_rows<Kind, KT, DP>(tP, sG, sV + (b ^ 1) * C::KV);
@@ -803,19 +983,29 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT) attn_tc_dq_kernel(const A
   if (bad && threadIdx.x == 0) atomicOr(A.status, 1);
   using T = typename Kind::T;
   if (A.dq != nullptr && part == 0)
-    write_row<T, DP>(tD + lane_off, A.scale * ldexpf(1.f, -eu - elem_exp<Kind>(X, kWk)), in,
+    write_row<T, DP, C::SMALL>(tD + lane_off, A.scale * ldexpf(1.f, -eu - elem_exp<Kind>(X, kWk)), in,
                      !live || t1 == 0, A.dim, (T *)A.dq + (i * A.heads + h) * A.dim, nullptr);
-  if (pos_grad) {
-    float4 *sum = reinterpret_cast<float4 *>(sm);  // the tiles are done with
-    if (part > 0) sum[row] = make_float4(g[0], g[1], g[2], g[3]);
-    __syncthreads();
-    if (part == 0 && in) {
-      if (KT > 32) {
-        const float4 o = sum[row];
-        g[0] += o.x, g[1] += o.y, g[2] += o.z, g[3] += o.w;
-      }
+  // both halves of the columns; what the row's dS add up to is D's error
+  float all[9] = {sum_of(S.ds)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) all[1 + k] = sum_of(S.g[k]), all[5 + k] = sum_of(S.q[k]);
+  float *other = reinterpret_cast<float *>(sm);  // [9][128]: the tiles are done with
+  if (part > 0) {
+#pragma unroll
+    for (int k = 0; k < 9; ++k) other[k * 128 + row] = all[k];
+  }
+  __syncthreads();
+  if (part == 0 && in) {
+    if (KT > 32) {
+#pragma unroll
+      for (int k = 0; k < 9; ++k) all[k] += other[k * 128 + row];
+    }
+    if (live) A.delta[h * A.num_q + i] = delta + all[0];
+    if (pos_grad) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) all[1 + k] = live ? fmaf(-all[0], all[5 + k], all[1 + k]) : 0.f;
       const float s = A.sigma[h], w = 1.f / (s * s);
-      A.pos_q[h * A.num_q + i] = make_float4(-w * g[0], -w * g[1], -w * g[2], g[3]);
+      A.pos_q[h * A.num_q + i] = make_float4(w * all[1], w * all[2], w * all[3], all[4]);
     }
   }
   tc_fence_before();
@@ -831,17 +1021,19 @@ struct DkvCfg {
   static constexpr int QT = Kind::pair && DP == 128 ? 32 : 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
   static constexpr int K = HALF * tile_bytes<128, DP>, QG = HALF * tile_bytes<QT, DP>;
-  static constexpr int STAGES = Kind::pair && DP == 128 ? 1 : 2;
-  static constexpr int TMEM = tmem_round(2 * QT + 2 * DP);
+  static constexpr bool SMALL = Kind::pair && DP <= 64;  // at 128 TMEM is full
+  static constexpr int TMEM = tmem_round(2 * QT + (SMALL ? 4 : 2) * DP);
+  static constexpr int STAGES = 2 * K + 4 * QG <= 100 * 1024 || (TMEM == 512 && QT == 64) ? 2 : 1;
   static constexpr int NT = 128 * (QT / 32);
-  static constexpr int pos = 2 * K + 2 * STAGES * QG;  // float4 [2][QT]: x y z delta
-  static constexpr int stt = pos + 2 * QT * 16;        // float2 [2][QT]: m, 1 / l
-  static constexpr int bar = stt + 2 * QT * 8, slot = bar + 8;
+  static constexpr int pos = 2 * K + 2 * STAGES * QG;  // TilePos<QT> [2]
+  static constexpr int stt = pos + 2 * QT * 12;        // TileStat<QT> [2]
+  static constexpr int bar = stt + 2 * QT * 12, slot = bar + 8;
   static constexpr int smem = slot + 8;
+  static constexpr int CTAS = smem <= 113 * 1024 && TMEM <= 256 ? 2 : 1;
 };
 
 template <class Kind, int DP>
-__global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const AttnArgs A,
+__global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) attn_tc_dkv_kernel(const AttnArgs A,
                                                                            const AttnTcArgs X) {
   using C = DkvCfg<Kind, DP>;
   constexpr int QT = C::QT, NT = C::NT;
@@ -849,8 +1041,8 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
   const uint32_t base = smem_u32(sm);
   const uint32_t sK = base, sV = base + C::K, sQ = sV + C::K, sG = sQ + C::STAGES * C::QG,
                  bar = base + C::bar;
-  float4 *qpos = reinterpret_cast<float4 *>(sm + C::pos);
-  float2 *qst = reinterpret_cast<float2 *>(sm + C::stt);
+  TilePos<QT> *qpos = reinterpret_cast<TilePos<QT> *>(sm + C::pos);
+  TileStat<QT> *qst = reinterpret_cast<TileStat<QT> *>(sm + C::stt);
   const int warp = threadIdx.x >> 5;
   const int part = warp >> 2, row = threadIdx.x & 127;
 
@@ -859,8 +1051,14 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
   const int2 tile = A.ks.tile(item / A.kv_heads);
   const int64_t j0 = A.ks.begin(tile.x) + 128LL * tile.y, i0 = A.qs.begin(tile.x);
   const int nk = (int)min((int64_t)128, A.ks.end(tile.x) - j0);
-  const int64_t nq = A.qs.end(tile.x) - i0;
-  const int64_t per = (nq + QT - 1) / QT, t1 = per * group;  // query tiles, head by head
+  const int64_t j = j0 + row;
+  const bool in = row < nk;
+  const bool live = in && (A.k_mask == nullptr || A.k_mask[j] != 0);
+  const int64_t nq =
+      masked_extent(A.q_mask ? A.q_mask + i0 : nullptr, A.qs.end(tile.x) - i0, NT,
+                    reinterpret_cast<unsigned long long *>(sm + C::slot));
+  const int64_t per = (nq + QT - 1) / QT;
+  const int64_t t1 = __syncthreads_or(live) ? per * group : 0;  // query tiles, head by head
   const int dim8 = A.dim >> 3;
 
   if (warp == 0) tmem_alloc<C::TMEM>(base + C::slot);
@@ -885,8 +1083,8 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
         p = pos_of(A.q_pos, A.pos_dim, r0 + r);
         d = A.delta[h * A.num_q + r0 + r];
       }
-      qst[pb * QT + r] = st;
-      qpos[pb * QT + r] = make_float4(p.x, p.y, p.z, d);
+      qst[pb].nm[r] = -st.x, qst[pb].rl[r] = st.y, qst[pb].nd[r] = -d;
+      qpos[pb].c[0][r] = p.x, qpos[pb].c[1][r] = p.y, qpos[pb].c[2][r] = p.z;
     }
   };
   load_tile<Kind, 128, DP, NT>(sK, X.k, hk, j0, nk, dim8, A.k_mask);
@@ -899,19 +1097,17 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + C::slot);
   const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-  const uint32_t tS = tmem, tP = tmem + QT, tDk = tmem + 2 * QT, tDv = tDk + DP;
+  const uint32_t tS = tmem, tP = tmem + QT, tDk = tmem + 2 * QT, tDv = tDk + (C::SMALL ? 2 : 1) * DP;
 
-  const int64_t j = j0 + row;
-  const bool in = row < nk;
-  const bool live = in && (A.k_mask == nullptr || A.k_mask[j] != 0);
   const float us = ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
-  const int eu = du_exp<Kind>(X);
+  const int eu = du_exp<Kind>(X, A.dim);
   constexpr float kUp = Kind::bf16 ? 1.f : 8192.f;  // of P
-  BwdRow R{0.f, 0.f, 0.f, ldexpf(1.f, -elem_exp<Kind>(X, kWdo) - elem_exp<Kind>(X, kWv)),
-           ldexpf(1.f, eu), {0.f, 0.f, 0.f}};
-  if (live) R.p = pos_of(A.k_pos, A.pos_dim, j);
+  BwdRow B;
+  B.dps = ldexpf(1.f, -elem_exp<Kind>(X, kWdo) - elem_exp<Kind>(X, kWv));
+  B.up = ldexpf(1.f, eu);
+  B.p.set(live ? pos_of(A.k_pos, A.pos_dim, j) : AttnPos{0.f, 0.f, 0.f});
   float px = 0.f, py = 0.f, pz = 0.f;  // over all heads, times 1 / sigma^2
-  float g[4] = {};                     // of the current head
+  f2_t g[3] = {};                      // of the current head
   const bool pos_grad = A.pos_k != nullptr;
   bool bad = false;
   unsigned phase = 0;
@@ -925,9 +1121,11 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
   auto close_head = [&]() {
     if (cur >= 0 && pos_grad) {
       const float s = A.sigma[cur], w = 1.f / (s * s);
-      px = fmaf(w, g[0], px), py = fmaf(w, g[1], py), pz = fmaf(w, g[2], pz);
+      px = fmaf(w, sum_of(g[0]), px);
+      py = fmaf(w, sum_of(g[1]), py);
+      pz = fmaf(w, sum_of(g[2]), pz);
     }
-    g[0] = g[1] = g[2] = 0.f;
+    g[0] = g[1] = g[2] = 0;
   };
   for (int64_t t = 0; t < t1; ++t) {
     const int pb = (int)(t & 1), b = C::STAGES == 1 ? 0 : pb;
@@ -935,9 +1133,8 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
     if (h != cur) {
       close_head();
       cur = h;
-      AttnScore sc;
-      sc.init(A, h);
-      R.su = sc.su * us, R.capl = sc.capl, R.w = sc.w;
+      B.sc.init(A, h);
+      B.sc.su *= us;
     }
     bad = !mbar_wait(bar, phase);
     phase ^= 1;
@@ -946,10 +1143,9 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
     tmem_ld32(tP + lane_off + 32 * part, dp);
-    const float4 *qp = qpos + pb * QT + 32 * part;
-    const float2 *qs = qst + pb * QT + 32 * part;
-#define RA_DKV(C, P, G) dkv_elements<Kind, C, P, G>(v, dp, R, kUp, qs, qp, g)
-    if (R.capl > 0.f) {
+#define RA_DKV(C, P, G) \
+  dkv_elements<Kind, C, P, G>(v, dp, B, kUp, qst[pb], qpos[pb], 32 * part, g)
+    if (B.sc.capl > 0.f) {
       if (pos_grad) RA_DKV(true, true, true);
       else if (A.pos_dim > 0) RA_DKV(true, true, false);
       else RA_DKV(true, false, false);
@@ -968,8 +1164,8 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
     if ((bad = __syncthreads_or(bad))) break;
     if (threadIdx.x == 0) {
       tc_fence_after();
-      products_weighted<Kind, QT, DP>(tDv, tS, sG + b * C::QG, false, t > 0);
-      products_weighted<Kind, QT, DP>(tDk, tP, sQ + b * C::QG, false, t > 0);
+      products_weighted<Kind, QT, DP, C::SMALL>(tDv, tS, sG + b * C::QG, false, t > 0);
+      products_weighted<Kind, QT, DP, C::SMALL>(tDk, tP, sQ + b * C::QG, false, t > 0);
       if (C::STAGES > 1 && t + 1 < t1) {
         products_rows<Kind, QT, DP>(tS, sK, sQ + (b ^ 1) * C::QG);
         products_rows<Kind, QT, DP>(tP, sV, sG + (b ^ 1) * C::QG);
@@ -1003,10 +1199,10 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT) attn_tc_dkv_kernel(const
   const bool zero = !live || t1 == 0;
   constexpr int last = QT / 32 - 1;
   if (A.dk != nullptr && part == 0)
-    write_row<T, DP>(tDk + lane_off, A.scale * ldexpf(1.f, -eu - elem_exp<Kind>(X, kWq)), in, zero,
+    write_row<T, DP, C::SMALL>(tDk + lane_off, A.scale * ldexpf(1.f, -eu - elem_exp<Kind>(X, kWq)), in, zero,
                      A.dim, (T *)A.dk + at, nullptr);
   if (A.dv != nullptr && part == last)
-    write_row<T, DP>(tDv + lane_off, ldexpf(1.f, -elem_exp<Kind>(X, kWdo)) / kUp, in, zero, A.dim,
+    write_row<T, DP, C::SMALL>(tDv + lane_off, ldexpf(1.f, -elem_exp<Kind>(X, kWdo)) / kUp, in, zero, A.dim,
                      (T *)A.dv + at, nullptr);
   if (pos_grad) {
     float4 *sum = reinterpret_cast<float4 *>(sm);

@@ -12,9 +12,9 @@ E = 2^-23 for each fp32 addition, n terms in a sum:
   dq dk  the same with dS (1 - tanh^2); dv as out
 An fp16 number below its normal range has an absolute half step of 2^-25, and a
 pair's low half reaches there too: P is held up to 2^7 or more; dS at 2^13 or
-more for 2 max |do| max |v|, so dS is off by 2^-37 of max |do| max |v|; and each
-fp32 tensor's pairs at 2^13 or more for its largest element, so their elements
-are off by 2^-38 of it.
+more for 2 D max |do| max |v| (elements' maxima), so dS is off by 2^-37 of
+D max |do| max |v|; and each fp32 tensor's pairs at 2^13 or more for its largest
+element, so their elements are off by 2^-38 of it.
 Positions and sigma get dS as it is, in fp32.
 """
 import math
@@ -71,8 +71,7 @@ def exact(d, nq, nk, scale, cap, q_mask=None, k_mask=None):
     s_el = {x: (2.0 ** -38 * float(w[x][keep].abs().max()) if pair and keep.any() else 0.0)
             for x, keep in (("q", keep_q), ("k", keep_k), ("v", keep_k), ("g", keep_q))}
     if dtype != torch.bfloat16 and keep_q.any() and keep_k.any():
-        small_ds = float(w["g"][keep_q].norm(dim=-1).max() * w["v"][keep_k].norm(dim=-1).max()) \
-            * 2.0 ** -37 * 1.01  # 2^-25 at 2^13 for 2 max |do| max |v| (and 1.001 for its sums)
+        small_ds = D * float(w["g"][keep_q].abs().max() * w["v"][keep_k].abs().max()) * 2.0 ** -37
     a0 = c0 = 0
     for n, m in zip(nq, nk):
         I = torch.nonzero(keep_q[a0:a0 + n])[:, 0] + a0
@@ -261,9 +260,12 @@ def test_neighbours_do_not_leak(dtype, cuda_device):
                                     sigma=leaves[5])
         return (o, *torch.autograd.grad(o, leaves[:5], x["g"]))
 
-    want = run(d)
     bad = {k: t.clone() for k, t in d.items()}
     rows = slice(53, 253)
+    for x in (d, bad):  # fp16 operands are scaled by their tensor's maximum: in a clean row
+        for k in ("q", "k", "v", "g"):
+            x[k][0, 0, 0] = 8.0
+    want = run(d)
     for k in ("q", "k", "v", "g"):
         bad[k][rows] = math.nan
     got = run(bad)
