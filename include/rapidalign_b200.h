@@ -504,7 +504,7 @@ RA_API int ra_ce_backward(const ra_ce_desc *desc, const void *x, const void *w,
  * q_mask, k_mask: uint8 [num] or NULL; a masked query gives 0, masked keys (and
  * what their rows hold) take no part.  `status` as in ra_ce_desc.
  * out: [num_q][heads][dim]; for a backward also out32 (the same, unrounded;
- * NULL for RA_F32) and stats (float [heads][num_q][2]).  Nothing is allocated
+ * NULL for RA_F32) and stats (float [2][heads][num_q]).  Nothing is allocated
  * and the host never waits. */
 typedef struct ra_attn_desc {
   int64_t graphs, num_q, num_k;

@@ -133,7 +133,7 @@ class _KernelAttention(torch.autograd.Function):
                 # rounding of 16 bits into every score's gradient
                 if q.dtype != torch.float32:
                     out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
-                stats = torch.empty((d.heads, d.num_q, 2), dtype=torch.float32, device=dev)
+                stats = torch.empty((2, d.heads, d.num_q), dtype=torch.float32, device=dev)
             state = _lib.workspace(lib.ra_attn_state_bytes(ctypes.byref(d)), dev)
             ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 0), dev)
             rc = lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), out.data_ptr(),

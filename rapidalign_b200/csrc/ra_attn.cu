@@ -270,12 +270,12 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
       const unsigned grid = (unsigned)std::min<int64_t>(
           ceil_div(a.num_q * a.heads * lanes, (int64_t)512), (int64_t)sms * 16);
       attn_delta8_kernel<T><<<grid, 256, 0, st>>>((const T *)a.dout, o32, a.num_q, a.heads, a.dim,
-                                                  lanes, a.delta);
+                                                  lanes, a.neg_d);
     } else {
       const unsigned grid =
           (unsigned)std::min<int64_t>(ceil_div(a.num_q * a.heads, (int64_t)8), (int64_t)sms * 16);
       attn_delta_kernel<T><<<grid, 256, 0, st>>>((const T *)a.dout, o32, a.num_q, a.heads, a.dim,
-                                                 a.delta);
+                                                 a.neg_d);
     }
     if ((rc = launched())) return rc;
   }
@@ -358,7 +358,8 @@ int ra_attn_forward(const ra_attn_desc *d, const ra_attn_inputs *in, void *out, 
       state_bytes < state_layout(d).total)
     return RA_ERR_WORKSPACE;
   AttnArgs a = args_of(d, in);
-  a.out = out, a.out32 = out32, a.stats = (float2 *)stats;
+  a.out = out, a.out32 = out32;
+  if (stats) a.neg_m = stats, a.rl = stats + d->num_q * d->heads;
   cudaStream_t st = (cudaStream_t)stream;
   char *sb = (char *)state, *ws = (char *)workspace;
   if (d->dtype == RA_F32) return forward<KindF32>(d, in, a, sb, ws, st);
@@ -384,7 +385,8 @@ int ra_attn_backward(const ra_attn_desc *d, const ra_attn_inputs *in, const void
   char *sb = (char *)state, *ws = (char *)workspace;
   AttnArgs a = args_of(d, in);
   a.out = const_cast<void *>(out), a.out32 = const_cast<float *>(out32);
-  a.stats = (float2 *)stats, a.dout = dout, a.delta = (float *)(ws + b.delta);
+  a.neg_m = const_cast<float *>(stats), a.rl = a.neg_m + d->num_q * d->heads;
+  a.dout = dout, a.neg_d = (float *)(ws + b.delta);
   a.dq = grads->dq, a.dk = grads->dk, a.dv = grads->dv;
   if (grads->dq_pos || grads->dk_pos || grads->dsigma) a.pos_q = (float4 *)(ws + b.pos_q);
   if (grads->dk_pos) a.pos_k = (float4 *)(ws + b.pos_k);

@@ -9,8 +9,8 @@
 //   dq_i = sum_j dU k_j,  dk_j = sum_i dU q_i,  dv_j = sum_i P do_i
 //   dp_i = -sum_hj dS (p_i - p_j) / sigma_h^2,  dp_j the same with + over i
 //   dsigma_h = sum_ij dS |p_i - p_j|^2 / sigma_h^3
-// Scores are kept in base 2 (t = s log2 e), statistics per row as (m, 1 / l)
-// with l = sum 2^(t - m); a row without keys has (+inf, 0), so that every P of
+// Scores are kept in base 2 (t = s log2 e), statistics per row as m and 1 / l
+// with l = sum 2^(t - m); a row without keys has +inf and 0, so that every P of
 // it is 0.  All sums are in fp32 or more; one writer per result, no atomics.
 //
 // This file: the parts every variant shares, and the kernels with one warp a
@@ -67,13 +67,21 @@ struct AttnArgs {
   // forward results
   void *out;        // [num_q][heads][dim]
   float *out32;     // the same unrounded, or null
-  float2 *stats;    // [heads][num_q]
+  float *neg_m, *rl;  // [heads][num_q]: -m and 1 / l, or null
   // backward
   const void *dout;         // [num_q][heads][dim]
-  float *delta;             // [heads][num_q]
+  float *neg_d;             // [heads][num_q]: -D
   void *dq, *dk, *dv;       // contiguous
   float4 *pos_q, *pos_k;    // [heads][num_q], [kv_heads][num_k]; or null
   int *status;
+
+  __device__ __forceinline__ float2 stats(int h, int64_t i) const {
+    return make_float2(-neg_m[h * num_q + i], rl[h * num_q + i]);
+  }
+  __device__ __forceinline__ void put_stats(int h, int64_t i, float m, float r) const {
+    neg_m[h * num_q + i] = -m;
+    rl[h * num_q + i] = r;
+  }
 };
 
 template <class T>
@@ -138,14 +146,14 @@ struct AttnScore {
 template <class T>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const T *dout, const float *out32,
                                                          int64_t num_q, int heads, int dim,
-                                                         float *delta) {
+                                                         float *neg_d) {
   const int lane = threadIdx.x & 31;
   const int64_t n = num_q * heads;
   for (int64_t r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < n; r += gridDim.x * 8LL) {
     float s = 0.f;
     for (int d = lane; d < dim; d += 32) s = fmaf(to_f(dout[r * dim + d]), out32[r * dim + d], s);
     s = warp_sum(s);
-    if (lane == 0) delta[(r % heads) * num_q + r / heads] = s;
+    if (lane == 0) neg_d[(r % heads) * num_q + r / heads] = -s;
   }
 }
 
@@ -246,7 +254,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attn_row_fwd_kernel(const Att
       put(out + lane + 32 * c, o);
       if (A.out32) A.out32[item * D + lane + 32 * c] = o;
     }
-  if (lane == 0 && A.stats) A.stats[h * A.num_q + i] = make_float2(any ? m : INFINITY, r);
+  if (lane == 0 && A.neg_m) A.put_stats(h, i, any ? m : INFINITY, r);
 }
 
 template <class T>
@@ -271,8 +279,8 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attn_row_dq_kernel(const Attn
   AttnScore sc;
   sc.init(A, h);
   const AttnPos pi = pos_of(A.q_pos, A.pos_dim, i);
-  const float2 st = A.stats[h * A.num_q + i];
-  const float delta = A.delta[h * A.num_q + i];
+  const float2 st = A.stats(h, i);
+  const float delta = -A.neg_d[h * A.num_q + i];
   const bool live = st.y != 0.f;  // no key, or masked
   float acc[kAttnMaxDim / 32] = {};
   float gx = 0.f, gy = 0.f, gz = 0.f, gs = 0.f;
@@ -349,7 +357,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attn_row_dkv_kernel(const Att
       float p = 0.f, du = 0.f;
       bool on = i < i1;
       if (on) {
-        const float2 st = A.stats[h * A.num_q + i];
+        const float2 st = A.stats(h, i);
         on = st.y != 0.f;
         if (on) {
           float dot = 0.f, dp = 0.f, slope;
@@ -361,7 +369,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attn_row_dkv_kernel(const Att
           const float dx = pi.x - pj.x, dy = pi.y - pj.y, dz = pi.z - pj.z;
           const float t = sc(dot, dx * dx + dy * dy + dz * dz, slope);
           p = ex2(t - st.x) * st.y;
-          const float ds = p * (dp - A.delta[h * A.num_q + i]);
+          const float ds = p * (dp + A.neg_d[h * A.num_q + i]);
           gx = fmaf(ds, dx, gx);
           gy = fmaf(ds, dy, gy);
           gz = fmaf(ds, dz, gz);

@@ -124,21 +124,38 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 template <int ROWS, int DP>
 constexpr int tile_bytes = ROWS * DP * 2;
 
+// A warp copies 16 rows x 2 chunks at a time: whole 32-byte sectors, and no
+// bank conflicts in shared memory.
 template <int ROWS, int DP, int NT>
 __device__ __forceinline__ void load_half(uint32_t dst, const uint16_t *src, int64_t row0, int n,
                                           int64_t stride, int dim8, const uint8_t *mask) {
-  constexpr int kChunks = ROWS * DP / 8;
-#pragma unroll 4
-  for (int c = threadIdx.x; c < kChunks; c += NT) {
-    // 16 rows x 2 chunks a warp: whole 32-byte sectors, no bank conflicts
-    const int rest = c >> 5, row = (rest / (DP / 16)) * 16 + (c & 15),
-              d8 = (rest % (DP / 16)) * 2 + ((c >> 4) & 1);
-    const bool on = row < n && d8 < dim8 && (mask == nullptr || mask[row0 + row] != 0);
-    const uint16_t *from = on ? src + (row0 + row) * stride + d8 * 8 : src;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (d8 * ROWS + row) * 16),
-                 "l"(from), "r"(on ? 16 : 0)
-                 : "memory");
+  constexpr int W = NT / 32, PAIRS = DP / 16;
+  constexpr int SIDE = W >= PAIRS ? W / PAIRS : 1;  // warps beside each other on the rows
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r0 = (W >= PAIRS ? warp / PAIRS : 0) * 16 + (lane & 15);
+  const uint16_t *first = src + row0 * stride;
+#pragma unroll
+  for (int m = 0; m < (PAIRS + W - 1) / W; ++m) {
+    const int d8 = (W >= PAIRS ? warp % PAIRS : warp + m * W) * 2 + (lane >> 4);
+    const uint32_t to = dst + (d8 * ROWS + r0) * 16;
+    const uint16_t *from = first + r0 * stride + d8 * 8;
+    const int rows = d8 < dim8 ? n : 0;
+#pragma unroll
+    for (int k = 0; k < (ROWS / 16 + SIDE - 1) / SIDE; ++k) {
+      const int row = r0 + k * SIDE * 16;
+      if (ROWS / 16 % SIDE != 0 && row >= ROWS) break;
+      const bool on = row < rows && (mask == nullptr || mask[row0 + row] != 0);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * SIDE * 256),
+                   "l"(on ? from + k * SIDE * 16 * stride : src), "r"(on ? 16 : 0)
+                   : "memory");
+    }
   }
+}
+// One number, or zero.
+__device__ __forceinline__ void load_word(const float *dst, const float *src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(on ? 4 : 0)
+               : "memory");
 }
 template <class Kind, int ROWS, int DP, int NT>
 __device__ __forceinline__ void load_tile(uint32_t dst, const AttnOp &op, int head, int64_t row0,
@@ -237,6 +254,14 @@ __device__ __forceinline__ float tanh_kind(float u) {
 template <int R>
 struct TilePos {
   float c[3][R];
+  // row r of the tile is row i of p [num][dim]; zero where it is not `on`
+  __device__ __forceinline__ void load(int r, const float *p, int dim, int64_t i, bool on) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const bool there = on && k < dim;
+      load_word(c[k] + r, there ? p + i * dim + k : p, there);
+    }
+  }
 };
 __device__ __forceinline__ f2_t two(float v) { return pk(v, v); }
 struct RowPos {  // -p of this thread's row, twice
@@ -459,7 +484,7 @@ __global__ void __launch_bounds__(256) attn_halves_kernel(const AttnPrep p, cons
 template <class T>
 __global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const float *out32,
                                                           int64_t num_q, int heads, int dim,
-                                                          int lanes, float *delta) {
+                                                          int lanes, float *neg_d) {
   const int l = threadIdx.x % lanes;
   const int64_t n = num_q * heads, step = gridDim.x * 256LL / lanes;
   // all lanes of a warp go round together: the shuffles need them
@@ -474,7 +499,7 @@ __global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const f
       for (int k = 0; k < 8; ++k) s = fmaf(a[k], b[k], s);
     }
     for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
-    if (r < n && l == 0) delta[(r % heads) * num_q + r / heads] = s;
+    if (r < n && l == 0) neg_d[(r % heads) * num_q + r / heads] = -s;
   }
 }
 
@@ -537,9 +562,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kerne
       const bool on = r < n && (A.k_mask == nullptr || A.k_mask[r0 + r] != 0);
       const unsigned bits = __ballot_sync(kFull, on);
       if (lane == 0) kval[2 * b + warp] = bits;
-      AttnPos p{0.f, 0.f, 0.f};
-      if (on) p = pos_of(A.k_pos, A.pos_dim, r0 + r);
-      kpos[b].c[0][r] = p.x, kpos[b].c[1][r] = p.y, kpos[b].c[2][r] = p.z;
+      if (A.pos_dim > 0) kpos[b].load(r, A.k_pos, A.pos_dim, r0 + r, on);
     }
   };
   load_tile<Kind, 128, DP, 128>(sQ, X.q, h, i0, nq, dim8, A.q_mask);
@@ -665,9 +688,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kerne
     const int64_t at = (i * A.heads + h) * A.dim;
     write_row<T, DP, C::SMALL>(tO + lane_off, unscale * r, in, empty, A.dim, (T *)A.out + at,
                      A.out32 ? A.out32 + at : nullptr);
-    if (in && A.stats)
-      A.stats[h * A.num_q + i] =
-          make_float2(empty ? INFINITY : (m > -INFINITY ? m : 0.f) - kUp, r);
+    if (in && A.neg_m) A.put_stats(h, i, empty ? INFINITY : (m > -INFINITY ? m : 0.f) - kUp, r);
   }
   tc_fence_before();
   __syncthreads();
@@ -710,7 +731,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs A, int sp
         put((T *)A.out + r * A.dim + lane + 32 * c, o);
         if (A.out32) A.out32[r * A.dim + lane + 32 * c] = o;
       }
-    if (lane == 0 && A.stats) A.stats[h * A.num_q + i] = make_float2(any ? m : INFINITY, rl);
+    if (lane == 0 && A.neg_m) A.put_stats(h, i, any ? m : INFINITY, rl);
   }
 }
 
@@ -867,7 +888,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
   const int64_t i = i0 + row;
   const bool in = row < nq;
   float2 st = make_float2(INFINITY, 0.f);
-  if (in) st = A.stats[h * A.num_q + i];
+  if (in) st = A.stats(h, i);
   const bool live = st.y != 0.f;  // has keys, and is not masked
   const int64_t t1 = __syncthreads_or(live) ? (nk + KT - 1) / KT : 0;
   const int dim8 = A.dim >> 3;
@@ -888,9 +909,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
       const bool on = r < n && (A.k_mask == nullptr || A.k_mask[r0 + r] != 0);
       const unsigned bits = __ballot_sync(kFull, on);
       if (lane == 0) kval[2 * pb + warp] = bits;
-      AttnPos p{0.f, 0.f, 0.f};
-      if (on) p = pos_of(A.k_pos, A.pos_dim, r0 + r);
-      kpos[pb].c[0][r] = p.x, kpos[pb].c[1][r] = p.y, kpos[pb].c[2][r] = p.z;
+      if (A.pos_dim > 0) kpos[pb].load(r, A.k_pos, A.pos_dim, r0 + r, on);
     }
   };
   load_tile<Kind, 128, DP, NT>(sQ, X.q, h, i0, nq, dim8, A.q_mask);
@@ -905,7 +924,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
   const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
   const uint32_t tS = tmem, tP = tmem + KT, tD = tmem + 2 * KT;
 
-  const float delta = live ? A.delta[h * A.num_q + i] : 0.f;
+  const float delta = live ? -A.neg_d[h * A.num_q + i] : 0.f;
   BwdRow B;
   B.sc.init(A, h);
   B.sc.su *= ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
@@ -1000,7 +1019,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
 #pragma unroll
       for (int k = 0; k < 9; ++k) all[k] += other[k * 128 + row];
     }
-    if (live) A.delta[h * A.num_q + i] = delta + all[0];
+    A.neg_d[h * A.num_q + i] = live ? -(delta + all[0]) : 0.f;
     if (pos_grad) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) all[1 + k] = live ? fmaf(-all[0], all[5 + k], all[1 + k]) : 0.f;
@@ -1075,16 +1094,13 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) 
     load_tile<Kind, QT, DP, NT>(sG + b * C::QG, X.go, h, r0, n, dim8, A.q_mask);
     if (threadIdx.x < QT) {
       const int r = threadIdx.x;
-      float2 st = make_float2(INFINITY, 0.f);  // P = 0
-      if (r < n) st = A.stats[h * A.num_q + r0 + r];
-      AttnPos p{0.f, 0.f, 0.f};
-      float d = 0.f;
-      if (st.y != 0.f) {
-        p = pos_of(A.q_pos, A.pos_dim, r0 + r);
-        d = A.delta[h * A.num_q + r0 + r];
-      }
-      qst[pb].nm[r] = -st.x, qst[pb].rl[r] = st.y, qst[pb].nd[r] = -d;
-      qpos[pb].c[0][r] = p.x, qpos[pb].c[1][r] = p.y, qpos[pb].c[2][r] = p.z;
+      // rows that are not there: all zero, so P = 2^(score <= 0) 0 = 0
+      const bool on = r < n && (A.q_mask == nullptr || A.q_mask[r0 + r] != 0);
+      const int64_t at = on ? h * A.num_q + r0 + r : 0;
+      load_word(qst[pb].nm + r, A.neg_m + at, on);
+      load_word(qst[pb].rl + r, A.rl + at, on);
+      load_word(qst[pb].nd + r, A.neg_d + at, on);
+      if (A.pos_dim > 0) qpos[pb].load(r, A.q_pos, A.pos_dim, r0 + r, on);
     }
   };
   load_tile<Kind, 128, DP, NT>(sK, X.k, hk, j0, nk, dim8, A.k_mask);
