@@ -496,8 +496,9 @@ RA_API int ra_ce_backward(const ra_ce_desc *desc, const void *x, const void *w,
  * along dim, the other strides in elements (0 allowed); heads is a multiple of
  * kv_heads.  q_ptr, k_ptr: device int64 [graphs + 1], checked by the caller
  * (0 first, num last, no decrease).  q_tiles, k_tiles: device int32
- * [tiles][2], (graph, n) for every 128 rows of every graph's queries and keys,
- * in the order they are to be taken.  max_q, max_k: the longest graph's rows.
+ * [tiles][4], for every 128 rows of every graph's queries (keys) their first
+ * row and their count, then the first row and the count of the graph's keys
+ * (queries), in the order they are to be taken; 16-byte aligned.  max_q, max_k: the longest graph's rows.
  * With both offsets NULL (padded clouds) every graph has max_q queries and
  * max_k keys, and the tile counts are those of that.
  * q_pos, k_pos: float [num][pos_dim], pos_dim 1 to 3; sigma: float [heads].

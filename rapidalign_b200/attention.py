@@ -51,17 +51,22 @@ class AttentionSegments:
     max_k: int
 
 
-def _tiles(lengths: Tensor, cost: Tensor, total: int) -> Tensor:
-    """(graph, tile) of every 128 rows, the graphs with the most work first."""
+def _tiles(first: Tensor, lengths: Tensor, other_first: Tensor, other_lengths: Tensor,
+           total: int) -> Tensor:
+    """Every 128 rows of every graph: their first row and count, then the other
+    side's first row and count; the tiles with the most work first."""
     dev = lengths.device
     if total == 0:
-        return torch.zeros((0, 2), dtype=torch.int32, device=dev)
-    order = torch.argsort(cost, descending=True, stable=True)
-    each = (lengths[order] + _TILE - 1) // _TILE
-    graph = torch.repeat_interleave(order, each, output_size=total)
-    first = torch.repeat_interleave(each.cumsum(0) - each, each, output_size=total)
-    tile = torch.arange(total, device=dev) - first
-    return torch.stack([graph, tile], 1).to(torch.int32).contiguous()
+        return torch.zeros((0, 4), dtype=torch.int32, device=dev)
+    order = torch.argsort(other_lengths, descending=True, stable=True)
+    lengths = lengths[order]
+    each = (lengths + _TILE - 1) // _TILE
+    graph = torch.repeat_interleave(each, output_size=total)  # places in `order`
+    row = (torch.arange(total, device=dev) - (each.cumsum(0) - each)[graph]) * _TILE
+    count = (lengths[graph] - row).clamp(max=_TILE)
+    graph = order[graph]
+    return torch.stack([first[graph] + row, count, other_first[graph], other_lengths[graph]],
+                       1).to(torch.int32).contiguous()
 
 
 def attention_segments(q_ptr: Optional[Tensor] = None, k_ptr: Optional[Tensor] = None, *,
@@ -96,8 +101,11 @@ def attention_segments(q_ptr: Optional[Tensor] = None, k_ptr: Optional[Tensor] =
             raise ValueError("ptr must start at 0")
         if least < 0:
             raise ValueError("ptr offsets must match node stacks")
-    return AttentionSegments(qp, kp, _tiles(nq, nk, info[4]), _tiles(nk, nq, info[9]), graphs,
-                             info[1], info[6], info[3], info[8])
+    if max(info[1], info[6]) > 2 ** 31 - 256:
+        raise ValueError("attention_segments: at most 2^31 - 256 rows")
+    return AttentionSegments(qp, kp, _tiles(qp[:-1], nq, kp[:-1], nk, info[4]),
+                             _tiles(kp[:-1], nk, qp[:-1], nq, info[9]), graphs, info[1], info[6],
+                             info[3], info[8])
 
 
 class _KernelAttention(torch.autograd.Function):
@@ -241,7 +249,8 @@ def _unit_rows(t: Tensor) -> Tensor:
     16-bit tensor-core kernels (widths that are multiples of 8)."""
     unit = t.stride(-1) == 1 or t.shape[-1] == 1
     if unit and t.dtype != torch.float32 and t.shape[-1] % 8 == 0:
-        unit = t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
+        unit = t.data_ptr() % 16 == 0 and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in
+                                              zip(t.stride()[:-1], t.shape[:-1]))
         return t if unit else t.clone(memory_format=torch.contiguous_format)
     return t if unit else t.contiguous()
 

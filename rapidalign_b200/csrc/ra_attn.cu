@@ -4,6 +4,7 @@
 #include "ra_attn.cuh"
 #include "ra_attn_tc.cuh"
 #include "ra_host.h"
+#include "ra_tmap.h"
 
 namespace {
 
@@ -49,8 +50,8 @@ AttnArgs args_of(const ra_attn_desc *d, const ra_attn_inputs *in) {
   a.q_row = d->q_row, a.q_head = d->q_head, a.k_row = d->k_row, a.k_head = d->k_head;
   a.v_row = d->v_row, a.v_head = d->v_head;
   a.q = in->q, a.k = in->k, a.v = in->v;
-  a.qs = {in->q_ptr, (const int2 *)in->q_tiles, d->max_q};
-  a.ks = {in->k_ptr, (const int2 *)in->k_tiles, d->max_k};
+  a.qs = {in->q_ptr, (const int4 *)in->q_tiles, d->max_q};
+  a.ks = {in->k_ptr, (const int4 *)in->k_tiles, d->max_k};
   a.n_q_tiles = d->q_tiles, a.n_k_tiles = d->k_tiles;
   a.q_pos = d->pos_dim ? in->q_pos : nullptr, a.k_pos = d->pos_dim ? in->k_pos : nullptr;
   a.sigma = in->sigma;
@@ -67,7 +68,12 @@ bool use_tc(const ra_attn_desc *d) { return d->dim <= 128 && d->dim % 8 == 0; }
 bool operands_aligned(const ra_attn_desc *d, const ra_attn_inputs *in) {
   if (d->dtype == RA_F32) return true;
   const int64_t s = d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head;
-  return (s & 7) == 0 && (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v) & 15) == 0;
+  // a stride of 0 (broadcast heads or rows) has no tensor map
+  const bool moves = (d->num_q < 2 || d->q_row > 0) && (d->heads < 2 || d->q_head > 0) &&
+                     (d->num_k < 2 || (d->k_row > 0 && d->v_row > 0)) &&
+                     (d->kv_heads < 2 || (d->k_head > 0 && d->v_head > 0));
+  return moves && (s & 7) == 0 &&
+         (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v) & 15) == 0;
 }
 
 // The state a backward needs: bounds, and the halves of fp32 inputs.
@@ -162,23 +168,45 @@ void add(AttnPrep &p, const void *x, int64_t rows, int heads, int64_t row, int64
   p.mask[t] = mask, p.word[t] = word, p.hi[t] = (uint16_t *)hi, p.lo[t] = (uint16_t *)lo;
 }
 
+// Tensor maps [rows][heads][dim] of an operand, or of its halves.
+bool map_heads(CUtensorMap *m, bool bf16, const void *p, int64_t rows, int heads, int dim,
+               int64_t row, int64_t head, int cw, int box_rows) {
+  std::memset(m, 0, sizeof(*m));
+  EncodeTiledFn fn = encode_tiled();
+  if (fn == nullptr) return false;
+  if (rows < 1) return true;  // no tile is ever loaded
+  if (heads < 2) head = dim;  // not used; has to be a valid stride
+  if (rows < 2) row = (int64_t)heads * dim;
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2};
+  const cuuint32_t box[3] = {(cuuint32_t)cw, 1, (cuuint32_t)box_rows};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            cw == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+int padded_dim(const ra_attn_desc *d) { return d->dim <= 32 ? 32 : d->dim <= 64 ? 64 : 128; }
+bool map_operand(const ra_attn_desc *d, AttnMap *m, const void *hi, const void *lo, int64_t rows,
+                 int heads, int64_t row, int64_t head) {
+  const bool bf16 = d->dtype == RA_BF16, pair = d->dtype == RA_F32;
+  const int dp = padded_dim(d), cw = dp == 32 ? 32 : 64, br = pair && dp == 128 ? 32 : 64;
+  return map_heads(&m->hi, bf16, hi, rows, heads, d->dim, row, head, cw, br) &&
+         map_heads(&m->lo, bf16, lo, rows, heads, d->dim, row, head, cw, br);
+}
+
 // 16-bit operands of q, k, v: as given, or the halves in the state
-void operands(const ra_attn_desc *d, const ra_attn_inputs *in, char *state, AttnTcArgs *x) {
+bool operands(const ra_attn_desc *d, const ra_attn_inputs *in, char *state, AttnTcArgs *x) {
   x->words = (const unsigned *)state;
-  if (d->dtype != RA_F32) {
-    const uint16_t *q = (const uint16_t *)in->q, *k = (const uint16_t *)in->k,
-                   *v = (const uint16_t *)in->v;
-    x->q = {q, q, d->q_row, d->q_head};
-    x->k = {k, k, d->k_row, d->k_head};
-    x->v = {v, v, d->v_row, d->v_head};
-    return;
-  }
+  if (d->dtype != RA_F32)
+    return map_operand(d, &x->q, in->q, in->q, d->num_q, d->heads, d->q_row, d->q_head) &&
+           map_operand(d, &x->k, in->k, in->k, d->num_k, d->kv_heads, d->k_row, d->k_head) &&
+           map_operand(d, &x->v, in->v, in->v, d->num_k, d->kv_heads, d->v_row, d->v_head);
   const AttnState s = state_layout(d);
   const int64_t qr = (int64_t)d->heads * d->dim, kr = (int64_t)d->kv_heads * d->dim;
-  auto at = [&](size_t o) { return (const uint16_t *)(state + o); };
-  x->q = {at(s.qh), at(s.ql), qr, d->dim};
-  x->k = {at(s.kh), at(s.kl), kr, d->dim};
-  x->v = {at(s.vh), at(s.vl), kr, d->dim};
+  return map_operand(d, &x->q, state + s.qh, state + s.ql, d->num_q, d->heads, qr, d->dim) &&
+         map_operand(d, &x->k, state + s.kh, state + s.kl, d->num_k, d->kv_heads, kr, d->dim) &&
+         map_operand(d, &x->v, state + s.vh, state + s.vl, d->num_k, d->kv_heads, kr, d->dim);
 }
 
 template <class K>
@@ -225,7 +253,7 @@ int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, 
   const int sms = sm_count();
   int rc;
   AttnTcArgs x{};
-  operands(d, in, state, &x);
+  if (!operands(d, in, state, &x)) return RA_ERR_INVALID_ARGUMENT;
   if (Kind::pair) {
     const AttnState s = state_layout(d);
     if (cudaMemsetAsync(state, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
@@ -281,10 +309,11 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
   }
   if (tc) {
     AttnTcArgs x{};
-    operands(d, in, state, &x);
-    const uint16_t *g = (const uint16_t *)a.dout;
     const int64_t qr = (int64_t)d->heads * d->dim;
-    x.go = {g, g, qr, d->dim};
+    const void *gh = Kind::pair ? ws + b.gh : a.dout, *gl = Kind::pair ? ws + b.gl : a.dout;
+    if (!operands(d, in, state, &x) ||
+        !map_operand(d, &x.go, gh, gl, d->num_q, d->heads, qr, d->dim))
+      return RA_ERR_INVALID_ARGUMENT;
     unsigned *words = (unsigned *)state;
     if (!Kind::bf16) {
       AttnPrep p{};
@@ -292,7 +321,6 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
       add(p, a.dout, d->num_q, d->heads, qr, d->dim, in->q_mask, kWdo, ws + b.gh, ws + b.gl);
       if (Kind::pair) {
         if (cudaMemsetAsync(words + kWdo, 0, 8, st) != cudaSuccess) return RA_ERR_CUDA;
-        x.go = {(const uint16_t *)(ws + b.gh), (const uint16_t *)(ws + b.gl), qr, d->dim};
       } else {
         if (cudaMemsetAsync(words, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
         add(p, in->v, d->num_k, d->kv_heads, d->v_row, d->v_head, in->k_mask, kWv, nullptr,

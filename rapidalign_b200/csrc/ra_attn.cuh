@@ -32,14 +32,15 @@ constexpr float kAttnLog2e = 1.4426950408889634f;
 // list (ragged), or of `per` rows each (padded clouds).
 struct AttnSegs {
   const int64_t *ptr;  // [graphs + 1], or null
-  const int2 *tiles;   // (graph, tile in graph), or null with ptr
+  const int4 *tiles;   // (first row, rows, the other side's first row and rows)
   int64_t per;
   __device__ __forceinline__ int64_t begin(int64_t g) const { return ptr ? ptr[g] : g * per; }
   __device__ __forceinline__ int64_t end(int64_t g) const { return ptr ? ptr[g + 1] : (g + 1) * per; }
-  __device__ __forceinline__ int2 tile(int64_t t) const {
+  __device__ __forceinline__ int4 tile(int64_t t, const AttnSegs &other) const {
     if (ptr) return tiles[t];
-    const int64_t each = (per + 127) >> 7;
-    return make_int2((int)(t / each), (int)(t % each));
+    const int64_t each = (per + 127) >> 7, g = t / each, n = t % each;
+    return make_int4((int)(g * per + 128 * n), (int)min((int64_t)128, per - 128 * n),
+                     (int)(g * other.per), (int)other.per);
   }
   // the graph of row i (skips empty graphs)
   __device__ __forceinline__ int64_t graph_of(int64_t graphs, int64_t i) const {

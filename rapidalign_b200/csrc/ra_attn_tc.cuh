@@ -16,11 +16,13 @@
 // threads wait for the products, work on the scores, one thread issues the next
 // products -- and two to four CTAs on an SM hide each other's waits.
 //
-// Tiles lie in shared memory in the canonical no-swizzle layout, 16-byte chunk
-// (d / 8, row) at (d / 8 * rows + row) * 16: read K-major (S, dP) and MN-major
-// (P V, dU K) from one copy.  cp.async copies 16 bytes a thread and fills rows
-// behind the graph's end and masked rows with zeros, so whatever those hold
-// reaches no product.
+// Tiles come by TMA in boxes of 64 columns (32 at DP = 32) with 128-byte (64)
+// swizzle and are read K-major (S, dP) and MN-major (P V, dU K) from one copy.
+// (Copied by the threads with cp.async 16 bytes each, the issue alone took 2,000
+// to 3,000 cycles a tile.)  A streamed tile's rows behind the graph's end and
+// masked rows are set to zero in shared memory before any product, so whatever
+// those hold reaches none.  What a tile needs of its rows besides (positions,
+// statistics) is loaded into registers an iteration ahead.
 //
 // fp32 inputs are fp16 pairs (hi + lo, one power of two per tensor), three
 // products for one; the two small ones have an accumulator of their own where
@@ -37,6 +39,8 @@
 
 #include <new>
 
+#include <cuda.h>
+
 #include "ra_attn.cuh"
 #include "ra_tcprim.cuh"
 
@@ -45,12 +49,11 @@ namespace ra {
 // words of the bounds: bits of the largest finite magnitude of each tensor
 enum AttnWord { kWq = 0, kWk = 1, kWv = 2, kWdo = 3 };
 
-struct AttnOp {  // 16-bit operand, or its halves
-  const uint16_t *hi, *lo;
-  int64_t row, head;  // element strides
+struct AttnMap {  // 16-bit operand, or its halves
+  CUtensorMap hi, lo;
 };
 struct AttnTcArgs {
-  AttnOp q, k, v, go;
+  AttnMap q, k, v, go;
   const unsigned *words;  // null where nothing is scaled
   int splits;             // forward: key ranges of a row tile
   float *part_o;          // [splits][num_q][heads][dim], unnormalised
@@ -90,12 +93,19 @@ __device__ __forceinline__ int du_exp(const AttnTcArgs &X, int dim) {
   return attn_exp(2.f * dim * __uint_as_float(X.words[kWdo]) * __uint_as_float(X.words[kWv]));
 }
 
-// no-swizzle descriptor of a tile of `rows` rows
-__device__ __forceinline__ uint64_t tile_desc_k(uint32_t s, int rows) {
-  return tc_desc(s, (uint32_t)rows * 16, 128);
+// Swizzled tiles: [chunk of CW columns][row][CW]; eight rows make an atom.
+template <int DP>
+constexpr int kCw = DP >= 64 ? 64 : 32;  // columns of a box
+template <int DP>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t s, uint32_t lbo) {
+  constexpr uint64_t sbo = 8 * kCw<DP> * 2, mode = DP >= 64 ? 2 : 4;
+  return (uint64_t)((s >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((sbo >> 4) << 32) |
+         (1ull << 46) | (mode << 61);
 }
-__device__ __forceinline__ uint64_t tile_desc_mn(uint32_t s, int rows) {
-  return tc_desc(s, 128, (uint32_t)rows * 16);
+// byte offset of 16 columns (K-major) in a tile of ROWS rows
+template <int ROWS, int DP>
+__host__ __device__ constexpr int k_step(int k) {
+  return k * 16 / kCw<DP> * (ROWS * kCw<DP> * 2) + k * 16 % kCw<DP> * 2;
 }
 __host__ __device__ constexpr uint32_t attn_idesc(int N, bool bf16, bool b_mn) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) |
@@ -124,46 +134,40 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 template <int ROWS, int DP>
 constexpr int tile_bytes = ROWS * DP * 2;
 
-// A warp copies 16 rows x 2 chunks at a time: whole 32-byte sectors, and no
-// bank conflicts in shared memory.
-template <int ROWS, int DP, int NT>
-__device__ __forceinline__ void load_half(uint32_t dst, const uint16_t *src, int64_t row0, int n,
-                                          int64_t stride, int dim8, const uint8_t *mask) {
-  constexpr int W = NT / 32, PAIRS = DP / 16;
-  constexpr int SIDE = W >= PAIRS ? W / PAIRS : 1;  // warps beside each other on the rows
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r0 = (W >= PAIRS ? warp / PAIRS : 0) * 16 + (lane & 15);
-  const uint16_t *first = src + row0 * stride;
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int col, int head,
+                                         int row, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(col), "r"(head), "r"(row), "r"(mbar)
+      : "memory");
+}
+// One thread: rows row0 .. of a head into a tile, BR rows a box; the barrier
+// expects tile_bytes (twice for pairs).
+template <class Kind, int ROWS, int DP, int BR>
+__device__ __forceinline__ void load_tile(uint32_t dst, const AttnMap &op, int head, int row0,
+                                          uint32_t mbar) {
 #pragma unroll
-  for (int m = 0; m < (PAIRS + W - 1) / W; ++m) {
-    const int d8 = (W >= PAIRS ? warp % PAIRS : warp + m * W) * 2 + (lane >> 4);
-    const uint32_t to = dst + (d8 * ROWS + r0) * 16;
-    const uint16_t *from = first + r0 * stride + d8 * 8;
-    const int rows = d8 < dim8 ? n : 0;
+  for (int h = 0; h < (Kind::pair ? 2 : 1); ++h)
 #pragma unroll
-    for (int k = 0; k < (ROWS / 16 + SIDE - 1) / SIDE; ++k) {
-      const int row = r0 + k * SIDE * 16;
-      if (ROWS / 16 % SIDE != 0 && row >= ROWS) break;
-      const bool on = row < rows && (mask == nullptr || mask[row0 + row] != 0);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * SIDE * 256),
-                   "l"(on ? from + k * SIDE * 16 * stride : src), "r"(on ? 16 : 0)
-                   : "memory");
+    for (int c = 0; c < DP / kCw<DP>; ++c)
+#pragma unroll
+      for (int r = 0; r < ROWS; r += BR)
+        tma_rows(dst + h * tile_bytes<ROWS, DP> + (c * ROWS + r) * kCw<DP> * 2,
+                 h ? &op.lo : &op.hi, c * kCw<DP>, head, row0 + r, mbar);
+}
+// This thread's row of a streamed tile to zero.
+template <class Kind, int ROWS, int DP>
+__device__ __forceinline__ void zero_row(uint8_t *tile, int row) {
+#pragma unroll 1
+  for (int h = 0; h < (Kind::pair ? 2 : 1); ++h)
+#pragma unroll 1
+    for (int c = 0; c < DP / kCw<DP>; ++c) {
+      uint4 *p = reinterpret_cast<uint4 *>(tile + h * tile_bytes<ROWS, DP> +
+                                           (c * ROWS + row) * kCw<DP> * 2);
+#pragma unroll
+      for (int k = 0; k < kCw<DP> / 8; ++k) p[k] = make_uint4(0, 0, 0, 0);
     }
-  }
-}
-// One number, or zero.
-__device__ __forceinline__ void load_word(const float *dst, const float *src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src),
-               "r"(on ? 4 : 0)
-               : "memory");
-}
-template <class Kind, int ROWS, int DP, int NT>
-__device__ __forceinline__ void load_tile(uint32_t dst, const AttnOp &op, int head, int64_t row0,
-                                          int n, int dim8, const uint8_t *mask) {
-  load_half<ROWS, DP, NT>(dst, op.hi + head * op.head, row0, n, op.row, dim8, mask);
-  if (Kind::pair)
-    load_half<ROWS, DP, NT>(dst + tile_bytes<ROWS, DP>, op.lo + head * op.head, row0, n, op.row,
-                            dim8, mask);
 }
 
 // D (+)= A B^T over the head width: A 128 rows, B N rows, both K-major
@@ -175,11 +179,11 @@ __device__ __forceinline__ void products_rows(uint32_t d, uint32_t a, uint32_t b
   for (int p = 0; p < P; ++p) {  // lo hi, hi lo, hi hi: the small ones first
     const uint32_t ap = a + (Kind::pair && p == 0 ? tile_bytes<128, DP> : 0);
     const uint32_t bp = b + (Kind::pair && p == 1 ? tile_bytes<N, DP> : 0);
-    const uint64_t da = tile_desc_k(ap, 128), db = tile_desc_k(bp, N);
+    const uint64_t da = tile_desc<DP>(ap, 16), db = tile_desc<DP>(bp, 16);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k)
-      mma_ss(d, da + (uint64_t)(k * 2 * 128 * 16 >> 4), db + (uint64_t)(k * 2 * N * 16 >> 4), idesc,
-             p > 0 || k > 0);
+      mma_ss(d, da + (uint64_t)(k_step<128, DP>(k) >> 4), db + (uint64_t)(k_step<N, DP>(k) >> 4),
+             idesc, p > 0 || k > 0);
   }
 }
 // D[128, DP] (+)= W[128, KT] X[KT, DP]: W in TMEM (per 32 columns of the
@@ -194,12 +198,13 @@ __device__ __forceinline__ void products_weighted(uint32_t d, uint32_t w, uint32
 #pragma unroll
   for (int p = 0; p < 3; ++p) {  // lo hi, hi lo (pairs of x only), hi hi
     if (p < first || (p == 1 && !Kind::pair)) continue;
-    const uint64_t dx = tile_desc_mn(x + (Kind::pair && p == 1 ? tile_bytes<KT, DP> : 0), KT);
+    const uint64_t dx = tile_desc<DP>(x + (Kind::pair && p == 1 ? tile_bytes<KT, DP> : 0),
+                                      KT * kCw<DP> * 2);
     if (SMALL && p == 2) acc = more;
 #pragma unroll
     for (int k = 0; k < KT / 16; ++k) {
       mma_ts(SMALL && p < 2 ? d + DP : d, w + (k >> 1) * 32 + (k & 1) * 8 + (p == 0 ? 16 : 0),
-             dx + (uint64_t)(k * 256 >> 4), idesc, acc);
+             dx + (uint64_t)(k * 16 * kCw<DP> * 2 >> 4), idesc, acc);
       acc = 1;
     }
   }
@@ -254,13 +259,8 @@ __device__ __forceinline__ float tanh_kind(float u) {
 template <int R>
 struct TilePos {
   float c[3][R];
-  // row r of the tile is row i of p [num][dim]; zero where it is not `on`
-  __device__ __forceinline__ void load(int r, const float *p, int dim, int64_t i, bool on) {
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const bool there = on && k < dim;
-      load_word(c[k] + r, there ? p + i * dim + k : p, there);
-    }
+  __device__ __forceinline__ void put(int r, const AttnPos &p) {
+    c[0][r] = p.x, c[1][r] = p.y, c[2][r] = p.z;
   }
 };
 __device__ __forceinline__ f2_t two(float v) { return pk(v, v); }
@@ -326,8 +326,6 @@ __device__ __forceinline__ int64_t masked_extent(const uint8_t *mask, int64_t n,
   __syncthreads();
   return (int64_t)*slot;
 }
-
-__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <int COLS>
 __device__ __forceinline__ void tmem_alloc(uint32_t slot) {
@@ -505,27 +503,45 @@ __global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const f
 
 // ---- forward --------------------------------------------------------------------
 
+// rows of a TMA box
+template <class Kind, int DP>
+constexpr int box_rows = Kind::pair && DP == 128 ? 32 : 64;
+
 template <class Kind, int DP>
 struct FwdCfg {
   static constexpr int KT = Kind::pair && DP == 128 ? 32 : 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
+  static constexpr int BR = box_rows<Kind, DP>;
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
   static constexpr bool SMALL = Kind::pair;
   static constexpr int TMEM = tmem_round(KT + (SMALL ? 2 : 1) * DP);
   static constexpr int pos = Q + 4 * KV;                 // TilePos<KT> [2]
   static constexpr int val = pos + 2 * KT * 12;          // unsigned [2][2]
-  static constexpr int bar = val + 16, slot = bar + 8;   // slot: also the mask's extent
-  static constexpr int smem = slot + 8;
+  static constexpr int bar = val + 16, slot = bar + 24;  // slot: also the mask's extent
+  static constexpr int smem = slot + 8 + 1024;           // 1024: the tiles' alignment
   static constexpr int CTAS = smem <= 56 * 1024 ? 4 : smem <= 113 * 1024 ? 2 : 1;
 };
 
+// This thread's row of the next streamed tile, fetched an iteration ahead.
+struct NextRow {
+  AttnPos p;
+  float nm, rl, nd;  // dk, dv: the query's statistics
+  bool on;
+};
+__device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
+  return p + ((1024 - (smem_u32(p) & 1023)) & 1023);
+}
+
 template <class Kind, int DP>
-__global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kernel(const AttnArgs A, const AttnTcArgs X) {
+__global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
+    attn_tc_fwd_kernel(const AttnArgs A, const __grid_constant__ AttnTcArgs X) {
   using C = FwdCfg<Kind, DP>;
   constexpr int KT = C::KT;
-  extern __shared__ __align__(1024) uint8_t sm[];
+  extern __shared__ uint8_t raw_sm[];
+  uint8_t *sm = align1024(raw_sm);
   const uint32_t base = smem_u32(sm);
-  const uint32_t sQ = base, sK = base + C::Q, sV = sK + 2 * C::KV, bar = base + C::bar;
+  const uint32_t sQ = base, sK = base + C::Q, sV = sK + 2 * C::KV, bar = base + C::bar,
+                 full = bar + 8;
   TilePos<KT> *kpos = reinterpret_cast<TilePos<KT> *>(sm + C::pos);
   unsigned *kval = reinterpret_cast<unsigned *>(sm + C::val);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -533,42 +549,61 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kerne
   const int64_t item = blockIdx.x;
   const int split = (int)(item % X.splits);
   const int h = (int)(item / X.splits % A.heads), hk = h / (A.heads / A.kv_heads);
-  const int2 tile = A.qs.tile(item / X.splits / A.heads);
-  const int64_t i0 = A.qs.begin(tile.x) + 128LL * tile.y, j0 = A.ks.begin(tile.x);
-  const int nq = (int)min((int64_t)128, A.qs.end(tile.x) - i0);
-  const int64_t i = i0 + threadIdx.x;
+  const int4 tile = A.qs.tile(item / X.splits / A.heads, A.ks);
+  const int i0 = tile.x, nq = tile.y, j0 = tile.z;
+  const int64_t i = i0 + (int)threadIdx.x;
   const bool row_on = threadIdx.x < nq && (A.q_mask == nullptr || A.q_mask[i] != 0);
-  const int64_t nk =
-      masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, A.ks.end(tile.x) - j0, 128,
-                    reinterpret_cast<unsigned long long *>(sm + C::slot));
+  const int nk = (int)masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, tile.w, 128,
+                                    reinterpret_cast<unsigned long long *>(sm + C::slot));
   // no row to work for: no keys to see
   const int64_t all = __syncthreads_or(row_on) ? (nk + KT - 1) / KT : 0;
-  const int64_t t0 = all * split / X.splits, t1 = all * (split + 1) / X.splits;
-  const int dim8 = A.dim >> 3;
+  const int t0 = (int)(all * split / X.splits), t1 = (int)(all * (split + 1) / X.splits);
 
-  if (warp == 0) tmem_alloc<C::TMEM>(base + C::slot);
+  auto issue = [&](int t, uint32_t more) {
+    const uint32_t fb = full + 8 * (t & 1);
+    mbar_expect_tx(fb, more + 2 * C::KV);
+    load_tile<Kind, KT, DP, C::BR>(sK + (t & 1) * C::KV, X.k, hk, j0 + t * KT, fb);
+    load_tile<Kind, KT, DP, C::BR>(sV + (t & 1) * C::KV, X.v, hk, j0 + t * KT, fb);
+  };
+  NextRow nx;
+  auto fetch = [&](int t) {
+    const int r = threadIdx.x;
+    if (r >= KT) return;
+    const int64_t j = j0 + t * KT + r;
+    nx.on = t * KT + r < nk && (A.k_mask == nullptr || A.k_mask[j] != 0);
+    nx.p = nx.on ? pos_of(A.k_pos, A.pos_dim, j) : AttnPos{0.f, 0.f, 0.f};
+  };
+  auto settle = [&](int t) {  // the tile is there: its rows' marks and positions
+    const int r = threadIdx.x, b = t & 1;
+    if (r < KT) {
+      const unsigned bits = __ballot_sync(kFull, nx.on);
+      if (lane == 0) kval[2 * b + warp] = bits;
+      if (A.pos_dim > 0) kpos[b].put(r, nx.p);
+      if (!nx.on) {
+        zero_row<Kind, KT, DP>(sm + C::Q + b * C::KV, r);
+        zero_row<Kind, KT, DP>(sm + C::Q + (2 + b) * C::KV, r);
+      }
+    }
+    fence_async_smem();
+  };
+  if (warp == 1) tmem_alloc<C::TMEM>(base + C::slot);
   if (threadIdx.x == 0) {
     mbar_init(bar, 1);
+    mbar_init(full, 1);
+    mbar_init(full + 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  auto load_keys = [&](int64_t t) {
-    const int b = (int)(t & 1);
-    const int64_t r0 = j0 + t * KT;
-    const int n = (int)min((int64_t)KT, nk - t * KT);
-    load_tile<Kind, KT, DP, 128>(sK + b * C::KV, X.k, hk, r0, n, dim8, A.k_mask);
-    load_tile<Kind, KT, DP, 128>(sV + b * C::KV, X.v, hk, r0, n, dim8, A.k_mask);
-    if (warp < KT / 32) {
-      const int r = threadIdx.x;
-      const bool on = r < n && (A.k_mask == nullptr || A.k_mask[r0 + r] != 0);
-      const unsigned bits = __ballot_sync(kFull, on);
-      if (lane == 0) kval[2 * b + warp] = bits;
-      if (A.pos_dim > 0) kpos[b].load(r, A.k_pos, A.pos_dim, r0 + r, on);
+    if (t0 < t1) {
+      issue(t0, C::Q);
+      load_tile<Kind, 128, DP, C::BR>(sQ, X.q, h, i0, full + 8 * (t0 & 1));
     }
-  };
-  load_tile<Kind, 128, DP, 128>(sQ, X.q, h, i0, nq, dim8, A.q_mask);
-  if (t0 < t1) load_keys(t0);
-  cp_wait_all();
-  fence_async_smem();
+  }
+  bool bad = false;
+  if (t0 < t1) fetch(t0);
+  __syncthreads();
+  if (t0 < t1) {
+    bad = !mbar_wait(full + 8 * (t0 & 1), 0);
+    settle(t0);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -583,19 +618,21 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kerne
   constexpr float kUp = Kind::bf16 ? 0.f : 7.f;  // P is held 2^kUp up
   const bool p_pair = Kind::pair || X.pair_p;
   float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to
-  bool bad = false;
   unsigned phase = 0;
 
   if (t0 < t1 && threadIdx.x == 0) {
-    products_rows<Kind, KT, DP>(tS, sQ, sK + (int)(t0 & 1) * C::KV);
+    products_rows<Kind, KT, DP>(tS, sQ, sK + (t0 & 1) * C::KV);
     tc_commit(bar);
   }
-  for (int64_t t = t0; t < t1; ++t) {
-    const int b = (int)(t & 1);
-    bad = !mbar_wait(bar, phase);
+  for (int t = t0; t < t1; ++t) {
+    const int b = t & 1;
+    bad |= !mbar_wait(bar, phase);
     phase ^= 1;
     tc_fence_after();
-    if (t + 1 < t1) load_keys(t + 1);  // its buffers' products are done
+    if (t + 1 < t1) {  // the products on its buffers are done
+      if (threadIdx.x == 0) issue(t + 1, 0);
+      fetch(t + 1);
+    }
     f2_t s2[KT / 32][16];
     float mx = -INFINITY;
 #pragma unroll
@@ -654,8 +691,10 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kerne
     const f2_t both = add2(sum[0], sum[1]);
     l += lo_of(both) + hi_of(both);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-    cp_wait_all();
-    fence_async_smem();
+    if (t + 1 < t1) {
+      bad |= !mbar_wait(full + 8 * (b ^ 1), ((t + 1 - t0) >> 1) & 1);
+      settle(t + 1);
+    }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
     if (threadIdx.x == 0) {
@@ -692,7 +731,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS) attn_tc_fwd_kerne
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_free<C::TMEM>(tmem);
   }
@@ -850,6 +889,7 @@ template <class Kind, int DP>
 struct DqCfg {
   static constexpr int KT = Kind::pair && DP == 128 ? 32 : 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
+  static constexpr int BR = box_rows<Kind, DP>;
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
   // two CTAs on an SM are worth more than a second buffer
   static constexpr int STAGES = 2 * Q + 4 * KV <= 100 * 1024 ? 2 : 1;
@@ -858,20 +898,21 @@ struct DqCfg {
   static constexpr int NT = 128 * (KT / 32);
   static constexpr int pos = 2 * Q + 2 * STAGES * KV;  // TilePos<KT> [2]
   static constexpr int val = pos + 2 * KT * 12;
-  static constexpr int bar = val + 16, slot = bar + 8;
-  static constexpr int smem = slot + 8;
+  static constexpr int bar = val + 16, slot = bar + 24;
+  static constexpr int smem = slot + 8 + 1024;
   static constexpr int CTAS = smem <= 113 * 1024 && TMEM <= 256 ? 2 : 1;
 };
 
 template <class Kind, int DP>
-__global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) attn_tc_dq_kernel(const AttnArgs A,
-                                                                         const AttnTcArgs X) {
+__global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
+    attn_tc_dq_kernel(const AttnArgs A, const __grid_constant__ AttnTcArgs X) {
   using C = DqCfg<Kind, DP>;
   constexpr int KT = C::KT, NT = C::NT;
-  extern __shared__ __align__(1024) uint8_t sm[];
+  extern __shared__ uint8_t raw_sm[];
+  uint8_t *sm = align1024(raw_sm);
   const uint32_t base = smem_u32(sm);
   const uint32_t sQ = base, sG = base + C::Q, sK = sG + C::Q, sV = sK + C::STAGES * C::KV,
-                 bar = base + C::bar;
+                 bar = base + C::bar, full = bar + 8;
   TilePos<KT> *kpos = reinterpret_cast<TilePos<KT> *>(sm + C::pos);
   unsigned *kval = reinterpret_cast<unsigned *>(sm + C::val);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -879,44 +920,67 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
 
   const int64_t item = blockIdx.x;
   const int h = (int)(item % A.heads), hk = h / (A.heads / A.kv_heads);
-  const int2 tile = A.qs.tile(item / A.heads);
-  const int64_t i0 = A.qs.begin(tile.x) + 128LL * tile.y, j0 = A.ks.begin(tile.x);
-  const int nq = (int)min((int64_t)128, A.qs.end(tile.x) - i0);
-  const int64_t nk =
-      masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, A.ks.end(tile.x) - j0, NT,
-                    reinterpret_cast<unsigned long long *>(sm + C::slot));
+  const int4 tile = A.qs.tile(item / A.heads, A.ks);
+  const int i0 = tile.x, nq = tile.y, j0 = tile.z;
+  const int nk = (int)masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, tile.w, NT,
+                                    reinterpret_cast<unsigned long long *>(sm + C::slot));
   const int64_t i = i0 + row;
   const bool in = row < nq;
   float2 st = make_float2(INFINITY, 0.f);
   if (in) st = A.stats(h, i);
   const bool live = st.y != 0.f;  // has keys, and is not masked
-  const int64_t t1 = __syncthreads_or(live) ? (nk + KT - 1) / KT : 0;
-  const int dim8 = A.dim >> 3;
+  const int t1 = __syncthreads_or(live) ? (nk + KT - 1) / KT : 0;
 
-  if (warp == 0) tmem_alloc<C::TMEM>(base + C::slot);
+  auto issue = [&](int t, uint32_t more) {
+    const int b = C::STAGES == 1 ? 0 : t & 1;
+    const uint32_t fb = full + 8 * b;
+    mbar_expect_tx(fb, more + 2 * C::KV);
+    load_tile<Kind, KT, DP, C::BR>(sK + b * C::KV, X.k, hk, j0 + t * KT, fb);
+    load_tile<Kind, KT, DP, C::BR>(sV + b * C::KV, X.v, hk, j0 + t * KT, fb);
+  };
+  NextRow nx;
+  auto fetch = [&](int t) {
+    const int r = threadIdx.x;
+    if (r >= KT) return;
+    const int64_t j = j0 + t * KT + r;
+    nx.on = t * KT + r < nk && (A.k_mask == nullptr || A.k_mask[j] != 0);
+    nx.p = nx.on ? pos_of(A.k_pos, A.pos_dim, j) : AttnPos{0.f, 0.f, 0.f};
+  };
+  auto settle = [&](int t) {
+    const int r = threadIdx.x, pb = t & 1, b = C::STAGES == 1 ? 0 : pb;
+    if (r < KT) {
+      const unsigned bits = __ballot_sync(kFull, nx.on);
+      if (lane == 0) kval[2 * pb + warp] = bits;
+      if (A.pos_dim > 0) kpos[pb].put(r, nx.p);
+      if (!nx.on) {
+        zero_row<Kind, KT, DP>(sm + 2 * C::Q + b * C::KV, r);
+        zero_row<Kind, KT, DP>(sm + 2 * C::Q + (C::STAGES + b) * C::KV, r);
+      }
+    }
+    fence_async_smem();
+  };
+  auto landed = [&](int t) {
+    return C::STAGES == 1 ? mbar_wait(full, t & 1) : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1);
+  };
+  if (warp == 1) tmem_alloc<C::TMEM>(base + C::slot);
   if (threadIdx.x == 0) {
     mbar_init(bar, 1);
+    mbar_init(full, 1);
+    mbar_init(full + 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  auto load_keys = [&](int64_t t) {
-    const int b = C::STAGES == 1 ? 0 : (int)(t & 1), pb = (int)(t & 1);
-    const int64_t r0 = j0 + t * KT;
-    const int n = (int)min((int64_t)KT, nk - t * KT);
-    load_tile<Kind, KT, DP, NT>(sK + b * C::KV, X.k, hk, r0, n, dim8, A.k_mask);
-    load_tile<Kind, KT, DP, NT>(sV + b * C::KV, X.v, hk, r0, n, dim8, A.k_mask);
-    if (warp < KT / 32) {
-      const int r = threadIdx.x;
-      const bool on = r < n && (A.k_mask == nullptr || A.k_mask[r0 + r] != 0);
-      const unsigned bits = __ballot_sync(kFull, on);
-      if (lane == 0) kval[2 * pb + warp] = bits;
-      if (A.pos_dim > 0) kpos[pb].load(r, A.k_pos, A.pos_dim, r0 + r, on);
+    if (t1 > 0) {
+      issue(0, 2 * C::Q);
+      load_tile<Kind, 128, DP, C::BR>(sQ, X.q, h, i0, full);
+      load_tile<Kind, 128, DP, C::BR>(sG, X.go, h, i0, full);
     }
-  };
-  load_tile<Kind, 128, DP, NT>(sQ, X.q, h, i0, nq, dim8, A.q_mask);
-  load_tile<Kind, 128, DP, NT>(sG, X.go, h, i0, nq, dim8, A.q_mask);
-  if (t1 > 0) load_keys(0);
-  cp_wait_all();
-  fence_async_smem();
+  }
+  bool bad = false;
+  if (t1 > 0) fetch(0);
+  __syncthreads();
+  if (t1 > 0) {
+    bad = !landed(0);
+    settle(0);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -934,7 +998,6 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
   B.p.set(live ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
   DqSums S;
   const bool pos_grad = A.pos_q != nullptr;
-  bool bad = false;
   unsigned phase = 0;
 
   if (t1 > 0 && threadIdx.x == 0) {
@@ -942,12 +1005,15 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
     products_rows<Kind, KT, DP>(tP, sG, sV);
     tc_commit(bar);
   }
-  for (int64_t t = 0; t < t1; ++t) {
-    const int pb = (int)(t & 1), b = C::STAGES == 1 ? 0 : pb;
-    bad = !mbar_wait(bar, phase);
+  for (int t = 0; t < t1; ++t) {
+    const int pb = t & 1, b = C::STAGES == 1 ? 0 : pb;
+    bad |= !mbar_wait(bar, phase);
     phase ^= 1;
     tc_fence_after();
-    if (C::STAGES > 1 && t + 1 < t1) load_keys(t + 1);
+    if (t + 1 < t1) {
+      if (C::STAGES > 1 && threadIdx.x == 0) issue(t + 1, 0);
+      fetch(t + 1);
+    }
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
     tmem_ld32(tP + lane_off + 32 * part, dp);
@@ -966,8 +1032,10 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
 #undef RA_DQ
     put_weights<Kind>(tS + lane_off + 32 * part, dp, Kind::pair);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-    cp_wait_all();
-    fence_async_smem();
+    if (C::STAGES > 1 && t + 1 < t1) {
+      bad |= !landed(t + 1);
+      settle(t + 1);
+    }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
     if (threadIdx.x == 0) {
@@ -980,11 +1048,11 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
       tc_commit(bar);
     }
     if (C::STAGES == 1 && t + 1 < t1) {  // one buffer: its products first
-      bad = !mbar_wait(bar, phase);
+      bad |= !mbar_wait(bar, phase);
       phase ^= 1;
-      load_keys(t + 1);
-      cp_wait_all();
-      fence_async_smem();
+      if (threadIdx.x == 0) issue(t + 1, 0);
+      bad |= !landed(t + 1);
+      settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
       if (threadIdx.x == 0) {
         tc_fence_after();
@@ -1029,7 +1097,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS) at
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_free<C::TMEM>(tmem);
   }
@@ -1039,6 +1107,7 @@ template <class Kind, int DP>
 struct DkvCfg {
   static constexpr int QT = Kind::pair && DP == 128 ? 32 : 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
+  static constexpr int BR = box_rows<Kind, DP>;
   static constexpr int K = HALF * tile_bytes<128, DP>, QG = HALF * tile_bytes<QT, DP>;
   static constexpr bool SMALL = Kind::pair && DP <= 64;  // at 128 TMEM is full
   static constexpr int TMEM = tmem_round(2 * QT + (SMALL ? 4 : 2) * DP);
@@ -1046,20 +1115,21 @@ struct DkvCfg {
   static constexpr int NT = 128 * (QT / 32);
   static constexpr int pos = 2 * K + 2 * STAGES * QG;  // TilePos<QT> [2]
   static constexpr int stt = pos + 2 * QT * 12;        // TileStat<QT> [2]
-  static constexpr int bar = stt + 2 * QT * 12, slot = bar + 8;
-  static constexpr int smem = slot + 8;
+  static constexpr int bar = stt + 2 * QT * 12, slot = bar + 24;
+  static constexpr int smem = slot + 8 + 1024;
   static constexpr int CTAS = smem <= 113 * 1024 && TMEM <= 256 ? 2 : 1;
 };
 
 template <class Kind, int DP>
-__global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) attn_tc_dkv_kernel(const AttnArgs A,
-                                                                           const AttnTcArgs X) {
+__global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
+    attn_tc_dkv_kernel(const AttnArgs A, const __grid_constant__ AttnTcArgs X) {
   using C = DkvCfg<Kind, DP>;
   constexpr int QT = C::QT, NT = C::NT;
-  extern __shared__ __align__(1024) uint8_t sm[];
+  extern __shared__ uint8_t raw_sm[];
+  uint8_t *sm = align1024(raw_sm);
   const uint32_t base = smem_u32(sm);
   const uint32_t sK = base, sV = base + C::K, sQ = sV + C::K, sG = sQ + C::STAGES * C::QG,
-                 bar = base + C::bar;
+                 bar = base + C::bar, full = bar + 8;
   TilePos<QT> *qpos = reinterpret_cast<TilePos<QT> *>(sm + C::pos);
   TileStat<QT> *qst = reinterpret_cast<TileStat<QT> *>(sm + C::stt);
   const int warp = threadIdx.x >> 5;
@@ -1067,47 +1137,69 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) 
 
   const int64_t item = blockIdx.x;
   const int hk = (int)(item % A.kv_heads), group = A.heads / A.kv_heads;
-  const int2 tile = A.ks.tile(item / A.kv_heads);
-  const int64_t j0 = A.ks.begin(tile.x) + 128LL * tile.y, i0 = A.qs.begin(tile.x);
-  const int nk = (int)min((int64_t)128, A.ks.end(tile.x) - j0);
+  const int4 tile = A.ks.tile(item / A.kv_heads, A.qs);
+  const int j0 = tile.x, nk = tile.y, i0 = tile.z;
   const int64_t j = j0 + row;
   const bool in = row < nk;
   const bool live = in && (A.k_mask == nullptr || A.k_mask[j] != 0);
-  const int64_t nq =
-      masked_extent(A.q_mask ? A.q_mask + i0 : nullptr, A.qs.end(tile.x) - i0, NT,
-                    reinterpret_cast<unsigned long long *>(sm + C::slot));
-  const int64_t per = (nq + QT - 1) / QT;
-  const int64_t t1 = __syncthreads_or(live) ? per * group : 0;  // query tiles, head by head
-  const int dim8 = A.dim >> 3;
+  const int nq = (int)masked_extent(A.q_mask ? A.q_mask + i0 : nullptr, tile.w, NT,
+                                    reinterpret_cast<unsigned long long *>(sm + C::slot));
+  const int per = (nq + QT - 1) / QT;
+  const int t1 = __syncthreads_or(live) ? per * group : 0;  // query tiles, head by head
 
-  if (warp == 0) tmem_alloc<C::TMEM>(base + C::slot);
+  auto issue = [&](int t, uint32_t more) {
+    const int b = C::STAGES == 1 ? 0 : t & 1, h = hk * group + t / per, r0 = i0 + t % per * QT;
+    const uint32_t fb = full + 8 * b;
+    mbar_expect_tx(fb, more + 2 * C::QG);
+    load_tile<Kind, QT, DP, C::BR>(sQ + b * C::QG, X.q, h, r0, fb);
+    load_tile<Kind, QT, DP, C::BR>(sG + b * C::QG, X.go, h, r0, fb);
+  };
+  NextRow nx;
+  auto fetch = [&](int t) {
+    if (threadIdx.x >= QT) return;
+    const int h = hk * group + t / per, r = t % per * QT + threadIdx.x;
+    const int64_t i = i0 + r, at = h * A.num_q + i;
+    nx.on = r < nq && (A.q_mask == nullptr || A.q_mask[i] != 0);
+    // a row that is not there is all zero: P = 2^(score <= 0) 0 = 0
+    nx.nm = nx.on ? A.neg_m[at] : 0.f;
+    nx.rl = nx.on ? A.rl[at] : 0.f;
+    nx.nd = nx.on ? A.neg_d[at] : 0.f;
+    nx.p = nx.on ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f};
+  };
+  auto settle = [&](int t) {
+    const int r = threadIdx.x, pb = t & 1, b = C::STAGES == 1 ? 0 : pb;
+    if (r < QT) {
+      qst[pb].nm[r] = nx.nm, qst[pb].rl[r] = nx.rl, qst[pb].nd[r] = nx.nd;
+      if (A.pos_dim > 0) qpos[pb].put(r, nx.p);
+      if (!nx.on) {
+        zero_row<Kind, QT, DP>(sm + 2 * C::K + b * C::QG, r);
+        zero_row<Kind, QT, DP>(sm + 2 * C::K + (C::STAGES + b) * C::QG, r);
+      }
+    }
+    fence_async_smem();
+  };
+  auto landed = [&](int t) {
+    return C::STAGES == 1 ? mbar_wait(full, t & 1) : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1);
+  };
+  if (warp == 1) tmem_alloc<C::TMEM>(base + C::slot);
   if (threadIdx.x == 0) {
     mbar_init(bar, 1);
+    mbar_init(full, 1);
+    mbar_init(full + 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  auto load_queries = [&](int64_t t) {
-    const int b = C::STAGES == 1 ? 0 : (int)(t & 1), pb = (int)(t & 1);
-    const int h = hk * group + (int)(t / per);
-    const int64_t q0 = (t % per) * QT, r0 = i0 + q0;
-    const int n = (int)min((int64_t)QT, nq - q0);
-    load_tile<Kind, QT, DP, NT>(sQ + b * C::QG, X.q, h, r0, n, dim8, A.q_mask);
-    load_tile<Kind, QT, DP, NT>(sG + b * C::QG, X.go, h, r0, n, dim8, A.q_mask);
-    if (threadIdx.x < QT) {
-      const int r = threadIdx.x;
-      // rows that are not there: all zero, so P = 2^(score <= 0) 0 = 0
-      const bool on = r < n && (A.q_mask == nullptr || A.q_mask[r0 + r] != 0);
-      const int64_t at = on ? h * A.num_q + r0 + r : 0;
-      load_word(qst[pb].nm + r, A.neg_m + at, on);
-      load_word(qst[pb].rl + r, A.rl + at, on);
-      load_word(qst[pb].nd + r, A.neg_d + at, on);
-      if (A.pos_dim > 0) qpos[pb].load(r, A.q_pos, A.pos_dim, r0 + r, on);
+    if (t1 > 0) {
+      issue(0, 2 * C::K);
+      load_tile<Kind, 128, DP, C::BR>(sK, X.k, hk, j0, full);
+      load_tile<Kind, 128, DP, C::BR>(sV, X.v, hk, j0, full);
     }
-  };
-  load_tile<Kind, 128, DP, NT>(sK, X.k, hk, j0, nk, dim8, A.k_mask);
-  load_tile<Kind, 128, DP, NT>(sV, X.v, hk, j0, nk, dim8, A.k_mask);
-  if (t1 > 0) load_queries(0);
-  cp_wait_all();
-  fence_async_smem();
+  }
+  bool bad = false;
+  if (t1 > 0) fetch(0);
+  __syncthreads();
+  if (t1 > 0) {
+    bad = !landed(0);
+    settle(0);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1125,7 +1217,6 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) 
   float px = 0.f, py = 0.f, pz = 0.f;  // over all heads, times 1 / sigma^2
   f2_t g[3] = {};                      // of the current head
   const bool pos_grad = A.pos_k != nullptr;
-  bool bad = false;
   unsigned phase = 0;
   int cur = -1;
 
@@ -1143,19 +1234,22 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) 
     }
     g[0] = g[1] = g[2] = 0;
   };
-  for (int64_t t = 0; t < t1; ++t) {
-    const int pb = (int)(t & 1), b = C::STAGES == 1 ? 0 : pb;
-    const int h = hk * group + (int)(t / per);
+  for (int t = 0; t < t1; ++t) {
+    const int pb = t & 1, b = C::STAGES == 1 ? 0 : pb;
+    const int h = hk * group + t / per;
     if (h != cur) {
       close_head();
       cur = h;
       B.sc.init(A, h);
       B.sc.su *= us;
     }
-    bad = !mbar_wait(bar, phase);
+    bad |= !mbar_wait(bar, phase);
     phase ^= 1;
     tc_fence_after();
-    if (C::STAGES > 1 && t + 1 < t1) load_queries(t + 1);
+    if (t + 1 < t1) {
+      if (C::STAGES > 1 && threadIdx.x == 0) issue(t + 1, 0);
+      fetch(t + 1);
+    }
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
     tmem_ld32(tP + lane_off + 32 * part, dp);
@@ -1174,8 +1268,10 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) 
     put_weights<Kind>(tS + lane_off + 32 * part, v, Kind::pair);
     put_weights<Kind>(tP + lane_off + 32 * part, dp, Kind::pair);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-    cp_wait_all();
-    fence_async_smem();
+    if (C::STAGES > 1 && t + 1 < t1) {
+      bad |= !landed(t + 1);
+      settle(t + 1);
+    }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
     if (threadIdx.x == 0) {
@@ -1189,11 +1285,11 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) 
       tc_commit(bar);
     }
     if (C::STAGES == 1 && t + 1 < t1) {
-      bad = !mbar_wait(bar, phase);
+      bad |= !mbar_wait(bar, phase);
       phase ^= 1;
-      load_queries(t + 1);
-      cp_wait_all();
-      fence_async_smem();
+      if (threadIdx.x == 0) issue(t + 1, 0);
+      bad |= !landed(t + 1);
+      settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
       if (threadIdx.x == 0) {
         tc_fence_after();
@@ -1235,7 +1331,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS) 
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_free<C::TMEM>(tmem);
   }

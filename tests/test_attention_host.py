@@ -71,11 +71,14 @@ def test_tiles():
     """Every 128 rows of every graph once, the costly graphs first."""
     from rapidalign_b200.attention import _tiles
     lengths = torch.tensor([0, 1, 128, 129, 300])
-    cost = torch.tensor([9, 5, 7, 5, 100])
-    got = _tiles(lengths, cost, 7)
+    other = torch.tensor([9, 5, 7, 5, 100])
+    first, ofirst = lengths.cumsum(0) - lengths, other.cumsum(0) - other
+    got = _tiles(first, lengths, ofirst, other, 7)
     assert got.dtype == torch.int32
-    assert got.tolist() == [[4, 0], [4, 1], [4, 2], [2, 0], [1, 0], [3, 0], [3, 1]]
-    assert _tiles(torch.tensor([0, 0]), torch.tensor([1, 2]), 0).shape == (0, 2)
+    assert got.tolist() == [[258, 128, 26, 100], [386, 128, 26, 100], [514, 44, 26, 100],
+                            [1, 128, 14, 7], [0, 1, 9, 5], [129, 128, 21, 5], [257, 1, 21, 5]]
+    empty = _tiles(torch.tensor([0, 0]), torch.tensor([0, 0]), first[:2], other[:2], 0)
+    assert empty.shape == (0, 4)
 
 
 @pytest.fixture(scope="module")
