@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "ra_attn.cuh"
+#include "ra_attn_few.cuh"
 #include "ra_attn_tc.cuh"
 #include "ra_host.h"
 #include "ra_tmap.h"
@@ -104,13 +105,33 @@ int key_splits(const ra_attn_desc *d, int sms) {
   return s < 1 ? 1 : (int)s;
 }
 
+// A few rows a graph: bound by the keys' bytes (ra_attn_few.cuh).
+bool use_few(const ra_attn_desc *d) {
+  return use_tc(d) && d->max_q * (d->heads / d->kv_heads) <= kFewRows;
+}
+// 16-byte loads of eight columns
+bool few_aligned(const ra_attn_desc *d, const ra_attn_inputs *in) {
+  const int64_t s = d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head;
+  return (s & (d->dtype == RA_F32 ? 3 : 7)) == 0 &&
+         (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v) & 15) == 0;
+}
+// Key ranges: as many as fill the SMs once (three CTAs each, two of eight
+// rows), each at least 512 keys.
+int few_splits(const ra_attn_desc *d, int sms) {
+  const int64_t ctas = d->graphs * d->kv_heads;
+  const int64_t fit = sms * (d->max_q * (d->heads / d->kv_heads) > 4 ? 2 : 3);
+  if (ctas < 1 || ctas >= fit) return 1;
+  const int64_t s = std::min<int64_t>(fit / ctas, d->max_k / 512);
+  return s < 1 ? 1 : (int)s;
+}
+
 struct AttnFwd {
   int splits;
   size_t part_o, part_s, total;
 };
 AttnFwd fwd_layout(const ra_attn_desc *d, int sms) {
   AttnFwd f{};
-  f.splits = use_tc(d) ? key_splits(d, sms) : 1;
+  f.splits = use_few(d) ? few_splits(d, sms) : use_tc(d) ? key_splits(d, sms) : 1;
   size_t o = 0;
   if (f.splits > 1) {
     const size_t rows = (size_t)f.splits * d->num_q * d->heads;
@@ -241,6 +262,41 @@ int tc_backward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
   return rc;
 }
 
+template <class T>
+int join(const AttnArgs &a, const AttnFwd &f, char *ws, int sms, cudaStream_t st) {
+  if (f.splits == 1) return RA_OK;
+  const int64_t rows = a.num_q * a.heads;
+  if (rows > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
+  attn_join_kernel<T><<<(unsigned)rows, 256, 0, st>>>(a, f.splits, (float *)(ws + f.part_o),
+                                                      (float2 *)(ws + f.part_s));
+  return launched();
+}
+
+template <class T, int N, int LPK>
+int few_launch(const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
+  const int64_t grid = a.graphs * a.kv_heads * f.splits;
+  if (grid > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
+  attn_few_kernel<T, N, LPK><<<(unsigned)grid, 32 * kFewWarps, 0, st>>>(
+      a, f.splits, (float *)(ws + f.part_o), (float2 *)(ws + f.part_s));
+  return launched();
+}
+template <class T, int N>
+int few_width(const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
+  // a row's scores need lanes of their own: N <= LPK
+  return a.dim <= 32   ? few_launch<T, N, (N > 4 ? 8 : 4)>(a, f, ws, st)
+         : a.dim <= 64 ? few_launch<T, N, 8>(a, f, ws, st)
+                       : few_launch<T, N, 16>(a, f, ws, st);
+}
+template <class T>
+int few_forward(const ra_attn_desc *d, const AttnArgs &a, const AttnFwd &f, char *ws,
+                cudaStream_t st) {
+  const int64_t rows = d->max_q * (d->heads / d->kv_heads);
+  return rows <= 1   ? few_width<T, 1>(a, f, ws, st)
+         : rows <= 2 ? few_width<T, 2>(a, f, ws, st)
+         : rows <= 4 ? few_width<T, 4>(a, f, ws, st)
+                     : few_width<T, 8>(a, f, ws, st);
+}
+
 template <class Kind>
 int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, char *state,
             char *ws, cudaStream_t st) {
@@ -251,7 +307,12 @@ int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, 
     return launched();
   }
   const int sms = sm_count();
+  const AttnFwd f = fwd_layout(d, sms);
   int rc;
+  if (use_few(d) && few_aligned(d, in) && !(Kind::pair && a.neg_m)) {
+    rc = few_forward<T>(d, a, f, ws, st);
+    return rc ? rc : join<T>(a, f, ws, sms, st);
+  }
   AttnTcArgs x{};
   if (!operands(d, in, state, &x)) return RA_ERR_INVALID_ARGUMENT;
   if (Kind::pair) {
@@ -268,18 +329,13 @@ int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, 
     if ((rc = bounds<float>(p, (unsigned *)state, sms, st))) return rc;
     if ((rc = halves(p, (const unsigned *)state, sms, st))) return rc;
   }
-  const AttnFwd f = fwd_layout(d, sms);
   x.splits = f.splits;
   x.part_o = (float *)(ws + f.part_o), x.part_s = (float2 *)(ws + f.part_s);
   x.pair_p = a.out32 != nullptr;
   rc = d->dim <= 32   ? tc_forward<Kind, 32>(a, x, st)
        : d->dim <= 64 ? tc_forward<Kind, 64>(a, x, st)
                       : tc_forward<Kind, 128>(a, x, st);
-  if (rc || f.splits == 1) return rc;
-  const int64_t rows = a.num_q * a.heads;
-  attn_join_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(rows, (int64_t)8), sms * 16), 256, 0,
-                        st>>>(a, f.splits, x.part_o, x.part_s);
-  return launched();
+  return rc ? rc : join<T>(a, f, ws, sms, st);
 }
 
 template <class Kind>

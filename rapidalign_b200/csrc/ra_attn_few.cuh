@@ -1,0 +1,273 @@
+// ra_attn_few.cuh -- forward of kernel attention for a few query rows a graph
+// (one query a graph: pooling, scoring, single new tokens).
+//
+// Bound by the bytes of the keys and values, each read once for all the
+// query heads of a key head.  A CTA takes one graph, key head and range of keys;
+// its N = queries x group rows stay in registers.  LPK lanes share a key, eight
+// columns (16 bytes of a 16-bit type) each, so a warp reads 32 / LPK whole rows
+// an instruction; U keys a lane are in flight at once.  The N U dots of a step
+// are joined over the LPK lanes by halving (each exchange leaves a lane half of
+// its values), so that every lane finishes N U / LPK scores of one row and none
+// is worked on twice; their weights go back by shuffles.  Every lane group
+// keeps the maximum and sums of its own keys, joined at the end over the warp,
+// the CTA (shared memory) and the key ranges (attn_join_kernel).
+// Measured: one query of 8 heads on 2 key heads of 64 against 262144 keys, bf16
+// (134 MB): FEW1; 1024 graphs of 64-512 keys: FEW2.  The tile kernel of
+// ra_attn_tc.cuh, 128 rows for these few, took 272 and 288 us.
+#pragma once
+
+#include "ra_attn.cuh"
+
+namespace ra {
+
+constexpr int kFewRows = 8;    // most rows (queries of a graph x heads a key head)
+constexpr int kFewWarps = 4;
+
+template <class T>
+struct Few8 {  // eight columns of a row, as loaded
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p, bool on) {
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+      u[k] = on ? __ldg(reinterpret_cast<const uint4 *>(p) + k) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void get(f2_t (&f)[4]) const {
+    T t[8];
+    memcpy(t, u, sizeof(t));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = pk(to_f(t[2 * k]), to_f(t[2 * k + 1]));
+  }
+};
+
+// Sums v[0 .. NV) over LPK lanes; lane c is left with v[0 .. max(1, NV / LPK)),
+// the values c NV / LPK ...
+template <int NV, int LPK, int S = LPK / 2, int CNT = NV>
+__device__ __forceinline__ void few_halve(float (&v)[NV], int c) {
+  if constexpr (S >= 1) {
+    if constexpr (CNT > 1) {
+      const bool up = c & S;
+#pragma unroll
+      for (int k = 0; k < CNT / 2; ++k) {
+        const float mine = up ? v[CNT / 2 + k] : v[k], send = up ? v[k] : v[CNT / 2 + k];
+        v[k] = mine + __shfl_xor_sync(kFull, send, S);
+      }
+      few_halve<NV, LPK, S / 2, CNT / 2>(v, c);
+    } else {
+      v[0] += __shfl_xor_sync(kFull, v[0], S);
+      few_halve<NV, LPK, S / 2, 1>(v, c);
+    }
+  }
+}
+
+template <class T, int N>
+constexpr int few_keys = (N == 1 ? 8 : N == 8 ? 2 : 4) / (sizeof(T) == 4 && N < 8 ? 2 : 1);
+
+template <class T, int N, int LPK>
+__global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
+    attn_few_kernel(const AttnArgs A, int splits, float *part_o, float2 *part_s) {
+  constexpr int KPW = 32 / LPK, U = few_keys<T, N>, NV = N * U;
+  constexpr int V = NV >= LPK ? NV / LPK : 1;  // scores a lane finishes, all of one row
+  static_assert(V <= U, "a lane's scores are of one row");
+  __shared__ float sacc[kFewWarps][N][LPK * 8];
+  __shared__ float2 sml[kFewWarps][N];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = lane % LPK, sub = lane / LPK, D = A.dim;
+  // the key heads of a range side by side: their rows are
+  const int hk = (int)(blockIdx.x % A.kv_heads), group = A.heads / A.kv_heads;
+  const int split = (int)(blockIdx.x / A.kv_heads % splits);
+  const int64_t g = blockIdx.x / A.kv_heads / splits;
+  const int64_t i0 = A.qs.begin(g), j0 = A.ks.begin(g), nk = A.ks.end(g) - j0;
+  const int n = (int)min((int64_t)N, (A.qs.end(g) - i0) * group);
+  const int64_t k0 = nk * split / splits, k1 = nk * (split + 1) / splits;
+  const bool cols = c * 8 < D, pos = A.pos_dim > 0, capped = A.cap > 0.f;
+  const float su = capped ? A.scale / A.cap : A.scale * kAttnLog2e, capl = A.cap * kAttnLog2e;
+
+  f2_t q[N][4];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const int64_t i = i0 + r / group;
+    const int h = hk * group + r % group;
+    const bool live = r < n && (A.q_mask == nullptr || A.q_mask[i] != 0);
+    Few8<T> x;
+    x.load((const T *)A.q + (live ? i * A.q_row + h * A.q_head + c * 8 : 0), live && cols);
+    x.get(q[r]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[r][k] = mul2(q[r][k], pk(su, su));
+  }
+  // the scores this lane finishes: row mr, keys u0 .. u0 + V - 1
+  const int first = c * NV / LPK, mr = first / U, u0 = first % U;
+  AttnPos pi{0.f, 0.f, 0.f};
+  float w = 0.f;
+  if (pos && mr < n) {
+    const int64_t i = i0 + mr / group;
+    if (A.q_mask == nullptr || A.q_mask[i] != 0) {
+      pi = pos_of(A.q_pos, A.pos_dim, i);
+      const float s = A.sigma[hk * group + mr % group];
+      w = kAttnLog2e / (2.f * s * s);
+    }
+  }
+  float mm = -INFINITY, ml = 0.f;  // of row mr, this lane group's keys; ml: this lane's part
+  f2_t acc[N][4] = {};
+  // This lane's keys of a step: rows u KPW apart from kp, vp.  Keys of the next
+  // step are loaded once the scores of this one are made, values while they are
+  // being made.
+  constexpr int kStep = kFewWarps * KPW * U;
+  const int64_t start = j0 + k0 + warp * (KPW * U) + sub;
+  const T *kp = (const T *)A.k + hk * A.k_head + c * 8 + start * A.k_row;
+  const T *vp = (const T *)A.v + hk * A.v_head + c * 8 + start * A.v_row;
+  const float *pp = pos ? A.k_pos + (start + u0 * KPW) * A.pos_dim : nullptr;
+  const uint8_t *mp = A.k_mask ? A.k_mask + start : nullptr;
+  int left = (int)(k1 - k0) - warp * (KPW * U) - sub;  // keys from this lane's first on
+  Few8<T> kx[U];
+  AttnPos pj[V];
+  unsigned on = 0;
+  auto fetch = [&]() {
+    on = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool here = u * KPW < left && (mp == nullptr || mp[u * KPW] != 0);
+      on |= (unsigned)here << u;
+      kx[u].load(kp + u * KPW * A.k_row, here && cols);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      pj[e] = AttnPos{0.f, 0.f, 0.f};
+      if (pos && ((on >> (u0 + e)) & 1)) pj[e] = pos_of(pp + e * KPW * A.pos_dim, A.pos_dim, 0);
+    }
+  };
+  int steps = (int)((k1 - k0) - warp * (KPW * U) + kStep - 1) / kStep;  // the warp's
+  if (steps > 0) fetch();
+  for (; steps > 0; --steps) {
+    Few8<T> vx[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) vx[u].load(vp + u * KPW * A.v_row, ((on >> u) & 1) && cols);
+    vp += kStep * A.v_row;
+    float t[NV];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      f2_t x[4];
+      kx[u].get(x);
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        f2_t s = mul2(q[r][0], x[0]);
+#pragma unroll
+        for (int k = 1; k < 4; ++k) s = fma2(q[r][k], x[k], s);
+        t[r * U + u] = lo_of(s) + hi_of(s);
+      }
+    }
+    few_halve<NV, LPK>(t, c);
+    float mx = mm;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float s = t[e];
+      if (capped) s = capl * tanhf(s);
+      if (pos) {
+        const float dx = pi.x - pj[e].x, dy = pi.y - pj[e].y, dz = pi.z - pj[e].z;
+        s = fmaf(-w, fmaf(dz, dz, fmaf(dy, dy, dx * dx)), s);
+      }
+      t[e] = (on >> (u0 + e)) & 1 ? s : -INFINITY;
+      mx = fmaxf(mx, t[e]);
+    }
+    if (steps > 1) {
+      kp += kStep * A.k_row;
+      if (pos) pp += kStep * A.pos_dim;
+      if (mp) mp += kStep;
+      left -= kStep;
+      fetch();
+    }
+    // the row's other lanes: U keys (or, of duplicates, the same)
+#pragma unroll
+    for (int o = 1; o < LPK / N; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
+    const float ref = mx > -INFINITY ? mx : 0.f;
+    if (__any_sync(kFull, mx > mm)) {
+      const float keep = mm > -INFINITY ? ex2(mm - ref) : 0.f;
+      ml *= keep;
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        const float f = __shfl_sync(kFull, keep, sub * LPK + r * U * LPK / NV);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[r][k] = mul2(acc[r][k], pk(f, f));
+      }
+      mm = mx;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      t[e] = ex2(t[e] - ref);
+      ml += t[e];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      f2_t x[4];
+      vx[u].get(x);
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        const int v = r * U + u;
+        const float p = __shfl_sync(kFull, t[v % V], sub * LPK + v * LPK / NV);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[r][k] = fma2(pk(p, p), x[k], acc[r][k]);
+      }
+    }
+  }
+  // each row's maximum and sum to all lanes of the group
+  constexpr int kDup = NV >= LPK ? 1 : LPK / NV;  // lanes that finish the same score
+#pragma unroll
+  for (int o = kDup; o < LPK / N; o <<= 1) ml += __shfl_xor_sync(kFull, ml, o);
+  float m[N], l[N];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    m[r] = __shfl_sync(kFull, mm, sub * LPK + r * U * LPK / NV);
+    l[r] = __shfl_sync(kFull, ml, sub * LPK + r * U * LPK / NV);
+  }
+  // the lane groups of the warp, then the warps, in a fixed order
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    float mx = m[r];
+#pragma unroll
+    for (int o = 16; o >= LPK; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
+    const float f = m[r] > -INFINITY ? ex2(m[r] - mx) : l[r] != l[r] ? 1.f : 0.f;
+    l[r] *= f;
+#pragma unroll
+    for (int o = 16; o >= LPK; o >>= 1) l[r] += __shfl_xor_sync(kFull, l[r], o);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float a = (k & 1 ? hi_of(acc[r][k / 2]) : lo_of(acc[r][k / 2])) * f;
+#pragma unroll
+      for (int o = 16; o >= LPK; o >>= 1) a += __shfl_xor_sync(kFull, a, o);
+      if (sub == 0) sacc[warp][r][c * 8 + k] = a;
+    }
+    if (lane == 0) sml[warp][r] = make_float2(mx, l[r]);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n * D; e += 32 * kFewWarps) {
+    const int r = e / D, d = e % D;
+    float mx = -INFINITY;
+    for (int k = 0; k < kFewWarps; ++k) mx = fmaxf(mx, sml[k][r].x);
+    float ls = 0.f, o = 0.f;
+    for (int k = 0; k < kFewWarps; ++k) {
+      const float2 s = sml[k][r];
+      const float f = s.x > -INFINITY ? ex2(s.x - mx) : s.y != s.y ? 1.f : 0.f;
+      ls = fmaf(s.y, f, ls);
+      o = fmaf(sacc[k][r][d], f, o);
+    }
+    const int64_t i = i0 + r / group;
+    const int h = hk * group + r % group;
+    const bool on = A.q_mask == nullptr || A.q_mask[i] != 0;
+    const bool any = on && (ls > 0.f || ls != ls);
+    const float ref = mx > -INFINITY ? mx : 0.f;
+    const int64_t at = (i * A.heads + h) * D + d;
+    if (splits > 1) {
+      part_o[split * A.num_q * A.heads * D + at] = any ? o : 0.f;
+      if (d == 0)
+        part_s[((int64_t)split * A.heads + h) * A.num_q + i] =
+            make_float2(any ? ref : -INFINITY, any ? ls : 0.f);
+    } else {
+      const float rl = any ? 1.f / ls : 0.f;
+      const float v = any ? o * rl : 0.f;
+      put((T *)A.out + at, v);
+      if (A.out32) A.out32[at] = v;
+      if (d == 0 && A.neg_m) A.put_stats(h, i, any ? ref : INFINITY, rl);
+    }
+  }
+}
+
+}  // namespace ra

@@ -214,18 +214,17 @@ template <class Kind>
 __device__ __forceinline__ uint32_t pack_kind(float a, float b) {
   if (Kind::bf16) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&v);
+    return bits_as<uint32_t>(v);
   }
   const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&v);
+  return bits_as<uint32_t>(v);
 }
 template <class Kind>
 __device__ __forceinline__ float2 unpack_kind(uint32_t u) {
   if (Kind::bf16) {
-    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&u);
-    return __bfloat1622float2(v);
+    return __bfloat1622float2(bits_as<__nv_bfloat162>(u));
   }
-  return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+  return __half22float2(bits_as<__half2>(u));
 }
 // 32 weights of this lane's row to TMEM: hi, and lo where a pair is wanted
 template <class Kind>
@@ -368,10 +367,12 @@ __device__ __forceinline__ void write_row(uint32_t taddr, float f, bool on, bool
           *reinterpret_cast<float4 *>(out + c + j + 4) =
               make_float4(v[j + 4], v[j + 5], v[j + 6], v[j + 7]);
         } else {
-          alignas(16) T t[8];
+          T t[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) put(t + k, v[j + k]);
-          *reinterpret_cast<uint4 *>(out + c + j) = *reinterpret_cast<const uint4 *>(t);
+          uint4 u;
+          memcpy(&u, t, 16);
+          *reinterpret_cast<uint4 *>(out + c + j) = u;
         }
       }
       if (out32 != nullptr) {
@@ -416,10 +417,11 @@ struct PrepAt {
 template <class T>
 __device__ __forceinline__ void load8(const T *x, bool wide, float (&v)[8]) {
   if (wide) {
-    alignas(16) T t[8];
+    uint4 u[sizeof(T) / 2];
 #pragma unroll
-    for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-      reinterpret_cast<uint4 *>(t)[k] = reinterpret_cast<const uint4 *>(x)[k];
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) u[k] = reinterpret_cast<const uint4 *>(x)[k];
+    T t[8];
+    memcpy(t, u, sizeof(t));
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = to_f(t[k]);
   } else {
@@ -465,16 +467,18 @@ __global__ void __launch_bounds__(256) attn_halves_kernel(const AttnPrep p, cons
     const PrepAt at(e, p.heads[t], dim8, small);
     float v[8];
     load8((const float *)p.x[t] + at.i * p.row[t] + at.h * p.head[t] + at.c * 8, wide, v);
-    alignas(16) __half hi[8];
-    alignas(16) __half lo[8];
+    __half hi[8], lo[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float y = v[k] * sc;
       hi[k] = __float2half_rn(y);
       lo[k] = __float2half_rn(y - __half2float(hi[k]));
     }
-    reinterpret_cast<uint4 *>(p.hi[t])[e] = *reinterpret_cast<const uint4 *>(hi);
-    reinterpret_cast<uint4 *>(p.lo[t])[e] = *reinterpret_cast<const uint4 *>(lo);
+    uint4 u[2];
+    memcpy(u, hi, 16);
+    memcpy(u + 1, lo, 16);
+    reinterpret_cast<uint4 *>(p.hi[t])[e] = u[0];
+    reinterpret_cast<uint4 *>(p.lo[t])[e] = u[1];
   }
 }
 
@@ -737,41 +741,51 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
   }
 }
 
-// Joins the key ranges of a row: one warp a row and head, ranges in order.
+// Joins the key ranges of a row: one CTA a row and head; its warps take every
+// eighth range, in order, and are joined in order.
 template <class T>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs A, int splits,
                                                         const float *part_o, const float2 *part_s) {
-  const int lane = threadIdx.x & 31;
-  const int64_t n = A.num_q * A.heads;
-  for (int64_t r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < n; r += gridDim.x * 8LL) {
-    const int64_t i = r / A.heads;
-    const int h = (int)(r % A.heads);
-    float m = -INFINITY;
-    for (int s = lane; s < splits; s += 32) m = fmaxf(m, part_s[((int64_t)s * A.heads + h) * A.num_q + i].x);
+  __shared__ float so[8][kAttnMaxDim];
+  __shared__ float sl[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n = A.num_q * A.heads, r = blockIdx.x, i = r / A.heads;
+  const int h = (int)(r % A.heads);
+  const float2 *ps = part_s + (int64_t)h * A.num_q + i;
+  float m = -INFINITY;
+  for (int s = lane; s < splits; s += 32) m = fmaxf(m, ps[s * n].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-    float l = 0.f, acc[kAttnMaxDim / 32] = {};
-    for (int s = 0; s < splits; ++s) {
-      const float2 st = part_s[((int64_t)s * A.heads + h) * A.num_q + i];
-      if (!(st.x > -INFINITY)) continue;
-      const float f = ex2(st.x - m);
-      l = fmaf(st.y, f, l);
-      const float *po = part_o + (s * n + r) * A.dim;
-#pragma unroll
-      for (int c = 0; c < kAttnMaxDim / 32; ++c)
-        if (lane + 32 * c < A.dim) acc[c] = fmaf(f, po[lane + 32 * c], acc[c]);
-    }
-    const bool any = l > 0.f || l != l;
-    const float rl = any ? 1.f / l : 0.f;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+  float l = 0.f, acc[kAttnMaxDim / 32] = {};
+#pragma unroll 4
+  for (int s = warp; s < splits; s += 8) {
+    const float2 st = ps[s * n];
+    const float f = st.x > -INFINITY ? ex2(st.x - m) : 0.f;  // else l and o are 0
+    l = fmaf(st.y, f, l);
+    const float *po = part_o + (s * n + r) * A.dim;
 #pragma unroll
     for (int c = 0; c < kAttnMaxDim / 32; ++c)
-      if (lane + 32 * c < A.dim) {
-        const float o = any ? acc[c] * rl : 0.f;
-        put((T *)A.out + r * A.dim + lane + 32 * c, o);
-        if (A.out32) A.out32[r * A.dim + lane + 32 * c] = o;
-      }
-    if (lane == 0 && A.neg_m) A.put_stats(h, i, any ? m : INFINITY, rl);
+      if (lane + 32 * c < A.dim) acc[c] = fmaf(f, po[lane + 32 * c], acc[c]);
   }
+#pragma unroll
+  for (int c = 0; c < kAttnMaxDim / 32; ++c)
+    if (lane + 32 * c < A.dim) so[warp][lane + 32 * c] = acc[c];
+  if (lane == 0) sl[warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) l += sl[k];
+  const bool any = l > 0.f || l != l;
+  const float rl = any ? 1.f / l : 0.f;
+  for (int d = threadIdx.x; d < A.dim; d += 256) {
+    float o = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o += so[k][d];
+    o = any ? o * rl : 0.f;
+    put((T *)A.out + r * A.dim + d, o);
+    if (A.out32) A.out32[r * A.dim + d] = o;
+  }
+  if (threadIdx.x == 0 && A.neg_m) A.put_stats(h, i, any ? m : INFINITY, rl);
 }
 
 // ---- backward -------------------------------------------------------------------

@@ -272,11 +272,11 @@ __global__ void __launch_bounds__(256) ce_coef_kernel(const int64_t *target, int
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&v);
+  return bits_as<uint32_t>(v);
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&v);
+  return bits_as<uint32_t>(v);
 }
 
 template <bool BF16>
@@ -336,7 +336,7 @@ struct CeEpiGrad {
       if (SPLIT) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+          const float2 b = __half22float2(bits_as<__half2>(h[j]));
           h[j] = pack_f16(v[2 * j] - b.x, v[2 * j + 1] - b.y);
         }
 #pragma unroll
@@ -394,10 +394,12 @@ struct CeEpiOut {
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              alignas(16) T t[8];
+              T t[8];
 #pragma unroll
               for (int k = 0; k < 8; ++k) store_as(t + k, v[8 * j + k] * al);
-              reinterpret_cast<uint4 *>(po + c)[j] = *reinterpret_cast<const uint4 *>(t);
+              uint4 u;
+              memcpy(&u, t, 16);
+              reinterpret_cast<uint4 *>(po + c)[j] = u;
             }
           }
         } else {

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <string.h>
 
 namespace ra {
 
@@ -72,6 +73,15 @@ __host__ __device__ __forceinline__ float scale_of_sigma(double sigma) {
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The bits of one value as another type of the same size.
+template <class To, class From>
+__device__ __forceinline__ To bits_as(const From &v) {
+  static_assert(sizeof(To) == sizeof(From), "same size");
+  To r;
+  memcpy(&r, &v, sizeof(To));
   return r;
 }
 

@@ -114,7 +114,9 @@ def exact(d, nq, nk, scale, cap, q_mask=None, k_mask=None):
         edp = edp + s_el["g"] * v.abs().sum(-1)[:, None] + s_el["v"] * go.abs().sum(-1)[:, :, None]
         eD = (go.abs() * (bo(fine) + (D + 4) * E * o.abs())).sum(-1, keepdim=True)
         dS = P * (dP - Di)
-        eS = P * (rp * (dP.abs() + Di.abs()) + edp + eD + 4 * E * (dP - Di).abs())
+        # exponentials below 2^-126 are flushed to zero
+        eS = 2.0 ** -126 * (dP.abs() + Di.abs())
+        eS = eS + P * (rp * (dP.abs() + Di.abs()) + edp + eD + 4 * E * (dP - Di).abs())
         if "sigma" in w:
             s2 = w["sigma"][:, None, None] ** 2
             for name, idx, dim, sgn in (("q_pos", I, 1, -1), ("k_pos", J, 0, 1)):
@@ -278,6 +280,27 @@ def test_neighbours_do_not_leak(dtype, cuda_device):
 def test_long_keys_few_queries(dtype, cuda_device):
     nq, nk = [1, 3], [40000, 5000]
     check(make(nq, nk, 8, 2, 64, dtype, 3, seed=9), nq, nk)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [8, 24, 64, 104])
+@pytest.mark.parametrize("nq,heads,kv", [([1, 1, 1, 1], 1, 1), ([1, 0, 1, 1], 4, 2),
+                                         ([2, 1, 0, 2], 2, 1), ([1, 1, 1, 1], 8, 1),
+                                         ([8, 3, 1, 0], 3, 3)])
+def test_few_rows(nq, heads, kv, dim, dtype, cuda_device):
+    """Up to eight rows a graph and key head, short and long key ranges,
+    masks, the cap."""
+    nk = [3000, 5, 600, 0]
+    d = make(nq, nk, heads, kv, dim, dtype, 3, seed=dim + heads)
+    check(d, nq, nk)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    mq = torch.rand(sum(nq), generator=g, device="cuda") > 0.2
+    mk = torch.rand(sum(nk), generator=g, device="cuda") > 0.3
+    mk[3000:3005] = False
+    for n in ("k", "v"):
+        d[n][~mk] = math.nan
+    d["k_pos"][~mk] = math.inf
+    check(d, nq, nk, masks=(mq, mk), cap=4.0)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
