@@ -50,10 +50,9 @@ CeState ce_state(const ra_ce_desc *d) {
 }
 
 // Width of the tiles over n columns: 256 unless half of a last tile or of
-// the last wave of CTAs would idle.  Logits of pairs take 128: their rounds
-// and the epilogue's arithmetic share the registers (256 spills 5 KB).
-int tile_width(int64_t m_tiles, int64_t n, int sms, bool pair_logits = false) {
-  if (pair_logits) return 128;
+// the last wave of CTAs would idle; 128 for pairs (TMEM).
+int tile_width(int64_t m_tiles, int64_t n, int sms, bool pairs) {
+  if (pairs) return 128;
   auto waves = [&](int tn) {
     const int64_t t = m_tiles * ceil_div(n, (int64_t)tn);
     return (double)(ceil_div(t, (int64_t)sms) * tn);
@@ -109,7 +108,7 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   p.piece = ceil_div(ceil_div(all, p.pieces), (int64_t)256) * 256;  // even pieces
   p.pieces = ceil_div(d->vocab, p.piece);
   p.ldg = p.piece;
-  p.tn_d = d->dim <= 128 ? 128 : tile_width(p.mt, d->dim, sms);
+  p.tn_d = d->dim <= 128 ? 128 : tile_width(p.mt, d->dim, sms, split);
   const int64_t nt = ceil_div((int64_t)d->dim, (int64_t)p.tn_d);
   p.sx = k_slices(p.mt * nt, ceil_div(std::min<int64_t>(p.piece, d->vocab), (int64_t)kGmK), sms);
   p.sw = k_slices(ceil_div(std::min<int64_t>(p.piece, d->vocab), (int64_t)kGmM) * nt,
@@ -134,7 +133,7 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
 
 template <int TN, bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
 int launch_gemm(const GmMaps &maps, const GmShape &s, const Epi &epi, int sms, cudaStream_t st) {
-  const size_t smem = gm_smem_bytes(TN);
+  const size_t smem = kGmSmem;
   auto k = gemm16_kernel<TN, BF16, PAIRS, A_MN, B_MN, Epi>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
@@ -148,8 +147,11 @@ int launch_gemm(const GmMaps &maps, const GmShape &s, const Epi &epi, int sms, c
 template <bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
 int launch_gemm(int tn, const GmMaps &maps, const GmShape &s, const Epi &epi, int sms,
                 cudaStream_t st) {
-  return tn == 256 ? launch_gemm<256, BF16, PAIRS, A_MN, B_MN>(maps, s, epi, sms, st)
-                   : launch_gemm<128, BF16, PAIRS, A_MN, B_MN>(maps, s, epi, sms, st);
+  if constexpr (PAIRS)
+    return launch_gemm<128, BF16, true, A_MN, B_MN>(maps, s, epi, sms, st);
+  else
+    return tn == 256 ? launch_gemm<256, BF16, false, A_MN, B_MN>(maps, s, epi, sms, st)
+                     : launch_gemm<128, BF16, false, A_MN, B_MN>(maps, s, epi, sms, st);
 }
 
 struct Operands {  // 16-bit x and w, or their halves
@@ -181,8 +183,9 @@ bool logit_maps(GmMaps *m, bool bf16, const Operands &op, int dim, int64_t r0, i
          map16(&m->b_lo, bf16, op.wl + v0 * op.ldw, cols, dim, op.ldw, tn);
 }
 
-CeLogit logit_of(const ra_ce_desc *d, const CeHead *head) {
-  return {d->scale, d->softcap, d->dtype == RA_F32 ? head : nullptr};
+template <bool PAIRS>
+CeLogit<PAIRS> logit_of(const ra_ce_desc *d, const CeHead *head) {
+  return {d->scale, d->softcap, head};
 }
 
 GmShape shape_of(const ra_ce_desc *d, const CePlan &p, int64_t mt, int64_t nt, int64_t k, int slices,
@@ -208,15 +211,12 @@ int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int
     GmMaps m;
     const int tn = tile_width(p.mt, cols, p.sms, SPLIT);
     if (!logit_maps(&m, BF16, op, dim, 0, d->rows, v0, cols, tn)) return RA_ERR_INVALID_ARGUMENT;
-    CeEpiGrad<BF16, SPLIT> eg{logit_of(d, head), d->rows, d->vocab, v0, target,
+    CeEpiGrad<BF16, SPLIT> eg{logit_of<SPLIT>(d, head), d->rows, d->vocab, v0, target,
                               (const float2 *)(state + sl.stats), (const float2 *)(ws + p.b_coef),
                               head, gh, gl, p.ldg};
     int rc;
     const GmShape sz = shape_of(d, p, p.mt, ceil_div(cols, (int64_t)tn), dim, 1, 1);
-    if constexpr (SPLIT)
-      rc = launch_gemm<128, BF16, true, false, false>(m, sz, eg, p.sms, st);
-    else
-      rc = launch_gemm<BF16, false, false, false>(tn, m, sz, eg, p.sms, st);
+    rc = launch_gemm<BF16, SPLIT, false, false>(tn, m, sz, eg, p.sms, st);
     if (rc) return rc;
     if (dx != nullptr) {
       if (!map16(&m.a_hi, BF16, gh, d->rows, cols, p.ldg, kGmM) ||
@@ -317,12 +317,18 @@ int ra_ce_forward(const ra_ce_desc *d, const void *x, const void *w, const int64
     GmMaps m;
     if (!logit_maps(&m, bf16, op, d->dim, r0, rows, 0, d->vocab, p.tn_z))
       return RA_ERR_INVALID_ARGUMENT;
-    CeEpiLse e{logit_of(d, head), rows, d->vocab, target + r0, part, mt * kGmM, zt + r0};
     const GmShape s =
         shape_of(d, p, mt, ceil_div(d->vocab, (int64_t)p.tn_z), d->dim, 1, 1);
-    rc = d->dtype == RA_F32 ? launch_gemm<128, false, true, false, false>(m, s, e, p.sms, st)
-         : bf16             ? launch_gemm<true, false, false, false>(p.tn_z, m, s, e, p.sms, st)
-                            : launch_gemm<false, false, false, false>(p.tn_z, m, s, e, p.sms, st);
+    if (d->dtype == RA_F32) {
+      const CeEpiLse<true> e{logit_of<true>(d, head), rows, d->vocab, target + r0, part, mt * kGmM,
+                             zt + r0};
+      rc = launch_gemm<false, true, false, false>(p.tn_z, m, s, e, p.sms, st);
+    } else {
+      const CeEpiLse<false> e{logit_of<false>(d, head), rows, d->vocab, target + r0, part,
+                              mt * kGmM, zt + r0};
+      rc = bf16 ? launch_gemm<true, false, false, false>(p.tn_z, m, s, e, p.sms, st)
+                : launch_gemm<false, false, false, false>(p.tn_z, m, s, e, p.sms, st);
+    }
     if (rc) return rc;
     ce_rows_kernel<<<(unsigned)ceil_div(rows, (int64_t)32), 1024, 0, st>>>(
         part, mt * kGmM, p.parts, r0, rows, d->rows, d->vocab, target, d->ignore_index, zt,

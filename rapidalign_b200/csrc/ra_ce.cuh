@@ -90,71 +90,93 @@ __global__ void __launch_bounds__(256) ce_split_kernel(const float *a, int64_t r
   }
 }
 
-// z = s acc or c tanh(s acc / c), in units of log 2
+// z = s acc or c tanh(s acc / c), in units of log 2.  PAIRS: fp32 inputs.
+template <bool PAIRS>
 struct CeLogit {
   float scale, cap;
-  const CeHead *head;  // split scales; null for 16-bit inputs
-  __device__ __forceinline__ float factor() const {
-    const float f = head ? ce_pow2(-ce_exp(head->amax_x) - ce_exp(head->amax_w)) : 1.f;
-    return cap > 0.f ? scale * f / cap : scale * f * kLog2e;
+  const CeHead *head;  // split scales of pairs
+  struct Fixed {
+    float f, capl;  // t = acc f, or capl tanh(acc f)
+  };
+  __device__ __forceinline__ Fixed fixed() const {
+    const float f = PAIRS ? ce_pow2(-ce_exp(head->amax_x) - ce_exp(head->amax_w)) : 1.f;
+    return cap > 0.f ? Fixed{scale * f / cap, cap * kLog2e} : Fixed{scale * f * kLog2e, 0.f};
   }
-  // acc times factor() -> t; `th` is tanh where capped
-  __device__ __forceinline__ float logit2(float u, float &th) const {
-    if (cap > 0.f) {
-      th = tanhf(u);
-      return th * (cap * kLog2e);
-    }
-    th = 0.f;
-    return u;
+  // to a few steps for fp32 inputs, to 2^-22 of 1 for 16-bit ones
+  static __device__ __forceinline__ float tanh_of(float u) {
+    if (PAIRS) return tanhf(u);
+    const float big = 1.f - __fdividef(2.f, 1.f + ex2(u * (2.f * kLog2e)));
+    const float u2 = u * u;
+    const float small =
+        u * fmaf(u2, fmaf(u2, fmaf(u2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+    return fabsf(u) < 0.1f ? small : big;
   }
 };
 
 // Forward epilogue: maximum and sum of 2^(t - m) over the thread's columns.
+template <bool PAIRS>
 struct CeEpiLse {
-  CeLogit lg;
+  CeLogit<PAIRS> lg;
   int64_t rows, vocab;
   const int64_t *target;
   float2 *part;  // [2 n_tiles][ld]
   int64_t ld;
   float *zt;  // [rows] t at the label
+  using Fixed = typename CeLogit<PAIRS>::Fixed;
+  struct Row {
+    int64_t target;
+  };
+  __device__ __forceinline__ Fixed fixed() const { return lg.fixed(); }
+  __device__ __forceinline__ Row begin(const GmUnit &w, int row) const {
+    const int64_t r = (int64_t)w.m * kGmM + row;
+    return {r < rows ? target[r] : -1};
+  }
   template <int TN, class Src>
-  __device__ __forceinline__ void run(const GmUnit &w, int row, int col, const Src &src) const {
+  __device__ __forceinline__ void run(const Fixed &F, const Row &R, const GmUnit &w, int row,
+                                      int col, const Src &src) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
-    const float f = lg.factor();
-    const int64_t tg = r < rows ? target[r] : -1;
+    const f2_t f2 = pk(F.f, F.f);
     float m = -INFINITY, s = 0.f;
 #pragma unroll Src::unroll
-    for (int c = 0; c < TN / 2; c += 32) {
-      float v[32];
+    for (int c = 0; c < TN / 2; c += 64) {
+      float v[64];
       src.get(c, v);
       const int64_t left = vocab - (c0 + c);
-      float th;
+      if (F.capl > 0.f) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = lg.logit2(v[j] * f, th);
-      if (left < 32) {
+        for (int j = 0; j < 64; ++j) v[j] = F.capl * lg.tanh_of(v[j] * F.f);
+      } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 64; j += 2) upk(mul2(pk(v[j], v[j + 1]), f2), v[j], v[j + 1]);
+      }
+      if (left < 64) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
           if (j >= left) v[j] = -INFINITY;
       }
-      const int64_t at = tg - (c0 + c);
-      if (at >= 0 && at < 32 && at < left) {
+      const int64_t at = R.target - (c0 + c);
+      if (at >= 0 && at < 64 && at < left) {
         float z = 0.f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) z = j == (int)at ? v[j] : z;
+        for (int j = 0; j < 64; ++j) z = j == (int)at ? v[j] : z;
         zt[r] = z;
       }
-      float mx = v[0];
+      float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-      for (int j = 1; j < 32; ++j) mx = fmaxf(mx, v[j]);
-      const float mn = fmaxf(m, mx);
-      if (mn > -INFINITY || mx != mx) {
-        float a = 0.f, b = 0.f;
+      for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+      mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const float mn = fmaxf(m, mx[0]);
+      if (mn > -INFINITY || mx[0] != mx[0]) {
+        const f2_t ref = pk(-mn, -mn);
+        f2_t sum[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          a += ex2(v[j] - mn);
-          b += ex2(v[j + 1] - mn);
+        for (int j = 0; j < 64; j += 2) {
+          float x, y;
+          upk(add2(pk(v[j], v[j + 1]), ref), x, y);
+          sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pk(ex2(x), ex2(y)));
         }
-        s = s * (m > -INFINITY ? ex2(m - mn) : 0.f) + (a + b);
+        const f2_t both = add2(sum[0], sum[1]);
+        s = s * (m > -INFINITY ? ex2(m - mn) : 0.f) + (lo_of(both) + hi_of(both));
         m = mn;
       }
     }
@@ -283,66 +305,88 @@ template <bool BF16>
 constexpr float kCeGradScale = BF16 ? 1.f : 8192.f;  // |du| < 2 times this
 
 // Backward epilogue: du of one piece of the vocabulary, in 16 bits.
-template <bool BF16, bool SPLIT>
+template <bool BF16, bool PAIRS>
 struct CeEpiGrad {
-  CeLogit lg;
+  CeLogit<PAIRS> lg;
   int64_t rows, vocab, v0;  // v0: the piece's first column
   const int64_t *target;
   const float2 *stats, *coef;
   const CeHead *head;
   uint16_t *hi, *lo;  // [128 m_tiles, ldg]
   int64_t ldg;
+  struct Fixed {
+    typename CeLogit<PAIRS>::Fixed lg;
+    float top;  // the largest coefficient
+  };
+  struct Row {
+    float2 cf, st;
+    int64_t target;
+  };
+  __device__ __forceinline__ Fixed fixed() const {
+    return {lg.fixed(), __uint_as_float(head->amax_g)};
+  }
+  __device__ __forceinline__ Row begin(const GmUnit &w, int row) const {
+    const int64_t r = (int64_t)w.m * kGmM + row;
+    if (r >= rows) return {make_float2(0.f, 0.f), make_float2(0.f, 1.f), -1};
+    return {coef[r], stats[r], target[r] - v0};
+  }
   template <int TN, class Src>
-  __device__ __forceinline__ void run(const GmUnit &w, int row, int col, const Src &src) const {
+  __device__ __forceinline__ void run(const Fixed &F, const Row &R, const GmUnit &w, int row,
+                                      int col, const Src &src) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
-    const float f = lg.factor();
-    float2 cf = make_float2(0.f, 0.f), st = make_float2(0.f, 1.f);
-    int64_t tg = -1;
-    if (r < rows) {
-      cf = coef[r];
-      st = stats[r];
-      tg = target[r] - v0;
-    }
-    const bool off = cf.x == 0.f && cf.y == 0.f;
-    const float top = __uint_as_float(head->amax_g);
-    cf.x = cf.x / top * kCeGradScale<BF16>;
-    cf.y = cf.y / top * kCeGradScale<BF16>;
-    const float pc = cf.x / st.y;
     uint16_t *ph = hi + r * ldg + c0;
-    uint16_t *pl = SPLIT ? lo + r * ldg + c0 : nullptr;
+    uint16_t *pl = PAIRS ? lo + r * ldg + c0 : nullptr;
+    // c / top before the scale: 1 where all coefficients are alike
+    const float gl = R.cf.y / F.top * kCeGradScale<BF16>, m = -R.st.x;
+    const float cp = R.cf.x / F.top * kCeGradScale<BF16> / R.st.y;
+    const bool off = R.cf.x == 0.f && R.cf.y == 0.f;
+    const f2_t f2 = pk(F.lg.f, F.lg.f), nm = pk(m, m), pc = pk(cp, cp);
 #pragma unroll Src::unroll
-    for (int c = 0; c < TN / 2; c += 32) {
-      float v[32];
+    for (int c = 0; c < TN / 2; c += 64) {
+      float v[64];
       src.get(c, v);
-      const int64_t at = tg - (c0 + c);
-      const bool hit = at >= 0 && at < 32;
+      const int64_t at = R.target - (c0 + c);
+      const bool hit = at >= 0 && at < 64;
+      if (F.lg.capl > 0.f) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        float th;
-        const float t = lg.logit2(v[j] * f, th);
-        float g = ex2(t - st.x) * pc;
-        if (hit && j == (int)at) g -= cf.y;
-        if (lg.cap > 0.f) g *= 1.f - th * th;
-        v[j] = off ? 0.f : g;
-      }
-      uint32_t h[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        h[j] = BF16 ? pack_bf16(v[2 * j], v[2 * j + 1]) : pack_f16(v[2 * j], v[2 * j + 1]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        reinterpret_cast<uint4 *>(ph + c)[j] =
-            make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
-      if (SPLIT) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float2 b = __half22float2(bits_as<__half2>(h[j]));
-          h[j] = pack_f16(v[2 * j] - b.x, v[2 * j + 1] - b.y);
+        for (int j = 0; j < 64; ++j) {
+          const float th = lg.tanh_of(v[j] * F.lg.f);
+          float g = ex2(fmaf(th, F.lg.capl, m)) * cp;
+          if (hit && j == (int)at) g -= gl;
+          v[j] = g * fmaf(-th, th, 1.f);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 64; j += 2) {
+          float x, y;
+          upk(fma2(pk(v[j], v[j + 1]), f2, nm), x, y);
+          upk(mul2(pk(ex2(x), ex2(y)), pc), v[j], v[j + 1]);
+        }
+        if (hit) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = j == (int)at ? v[j] - gl : v[j];
+        }
+      }
+      if (off) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < 64; q += 8) {
+        uint32_t h[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          reinterpret_cast<uint4 *>(pl + c)[j] =
-              make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+          h[j] = BF16 ? pack_bf16(v[q + 2 * j], v[q + 2 * j + 1])
+                      : pack_f16(v[q + 2 * j], v[q + 2 * j + 1]);
+        *reinterpret_cast<uint4 *>(ph + c + q) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (PAIRS) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 b = __half22float2(bits_as<__half2>(h[j]));
+            h[j] = pack_f16(v[q + 2 * j] - b.x, v[q + 2 * j + 1] - b.y);
+          }
+          *reinterpret_cast<uint4 *>(pl + c + q) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
       }
     }
   }
@@ -371,29 +415,36 @@ struct CeEpiOut {
   T *out;       // [rows, cols], or null
   float *part;  // [slices][rows, cols]
   int add;
+  struct Fixed {
+    float al;
+  };
+  struct Row {};
+  __device__ __forceinline__ Fixed fixed() const { return {out ? alpha.value() : 1.f}; }
+  __device__ __forceinline__ Row begin(const GmUnit &, int) const { return {}; }
   template <int TN, class Src>
-  __device__ __forceinline__ void run(const GmUnit &w, int row, int col, const Src &src) const {
+  __device__ __forceinline__ void run(const Fixed &F, const Row &, const GmUnit &w, int row,
+                                      int col, const Src &src) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
-    const float al = out ? alpha.value() : 1.f;
+    const float al = F.al;
     float *pp = part + ((int64_t)w.slice * rows + r) * cols + c0;
     T *po = out + r * cols + c0;
     const bool wide = (cols & 3) == 0;  // 16-byte aligned fp32 rows
 #pragma unroll Src::unroll
-    for (int c = 0; c < TN / 2; c += 32) {
-      float v[32];
+    for (int c = 0; c < TN / 2; c += 64) {
+      float v[64];
       src.get(c, v);
       const int64_t left = cols - (c0 + c);
       if (r >= rows || left <= 0) continue;
       if (out != nullptr) {
-        if (left >= 32 && (cols & 7) == 0) {
+        if (left >= 64 && (cols & 7) == 0) {
           if (sizeof(T) == 4) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 16; ++j)
               reinterpret_cast<float4 *>(po + c)[j] = make_float4(
                   v[4 * j] * al, v[4 * j + 1] * al, v[4 * j + 2] * al, v[4 * j + 3] * al);
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 8; ++j) {
               T t[8];
 #pragma unroll
               for (int k = 0; k < 8; ++k) store_as(t + k, v[8 * j + k] * al);
@@ -404,12 +455,12 @@ struct CeEpiOut {
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
+          for (int j = 0; j < 64; ++j)
             if (j < left) store_as(po + c + j, v[j] * al);
         }
-      } else if (wide && left >= 32) {
+      } else if (wide && left >= 64) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 16; ++j) {
           float4 *q = reinterpret_cast<float4 *>(pp + c) + j;
           float4 o = add ? *q : make_float4(0.f, 0.f, 0.f, 0.f);
           *q = make_float4(o.x + v[4 * j], o.y + v[4 * j + 1], o.z + v[4 * j + 2],
@@ -417,7 +468,7 @@ struct CeEpiOut {
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 64; ++j)
           if (j < left) pp[c + j] = v[j] + (add ? pp[c + j] : 0.f);
       }
     }

@@ -9,21 +9,23 @@
 // so no edge of M, N or K is special before the epilogue.
 //
 // fp32 inputs come as two fp16 halves (a = hi + lo, 22 significant bits, one
-// power-of-two scale per tensor) and three products lo hi + hi lo + hi hi,
-// which are three passes over K into the same accumulators, the small ones
-// first.  The tensor core drops the bits below an accumulator's last one
+// power-of-two scale per tensor) and three products, hi hi, hi lo and lo hi,
+// from one copy of the four tiles; the two small ones have an accumulator of
+// their own.  The tensor core drops the bits below an accumulator's last one
 // instead of rounding them: over a long K the loss adds up (2.5e-5 of dw at
-// K = 65537 in one chain, where fp32 sums keep 1e-6).  So a unit of pairs is
-// cut into rounds of kGmRound k steps; each round starts a fresh accumulator
-// and the epilogue adds the rounds in registers, rounding to nearest.
+// K = 65537 in one chain of all three, where fp32 sums keep 1e-6).  So a unit of
+// pairs is cut into rounds of kGmRound k steps; each round starts fresh
+// accumulators and the epilogue adds the rounds in registers, rounding to
+// nearest.
 //
 // Roles (320 threads, one CTA per SM, persistent over (tile, K slice) units):
 //   warps 0-7  epilogue: warp w reads TMEM lanes 32 (w % 4).. and half w / 4
 //              of the tile's columns
 //   warp 8     lane 0 copies operand tiles into the shared-memory ring
 //   warp 9     lane 0 issues the MMAs
-// Two accumulators in TMEM: the epilogue of one unit runs under the MMAs of
-// the next.  Every wait is bounded; on expiry the CTA records the timeout,
+// Two accumulators in TMEM (two pairs of them): the epilogue of one unit runs
+// under the MMAs of the next; what it reads of its rows besides is loaded before
+// it waits.  Every wait is bounded; on expiry the CTA records the timeout,
 // drains its copies, frees its TMEM and returns.
 #pragma once
 
@@ -36,15 +38,20 @@
 
 namespace ra {
 
-constexpr int kGmM = 128, kGmK = 64, kGmStages = 4;
+constexpr int kGmM = 128, kGmK = 64;
 constexpr int kGmThreads = 320, kGmEpiWarps = 8;
 constexpr int kGmABytes = kGmM * kGmK * 2;
 constexpr int kGmRound = 4;  // k steps (of 64) of a round of pairs
 
-__host__ __device__ constexpr int gm_stage_bytes(int TN) { return kGmABytes + TN * kGmK * 2; }
-__host__ __device__ constexpr size_t gm_smem_bytes(int TN) {
-  return 1024 + (size_t)kGmStages * gm_stage_bytes(TN) + 256;
+// 192 KB of operand tiles: 4 stages of 128 x 256 tiles, 6 of 128 x 128, 3 of
+// pairs (128 x 128 only)
+__host__ __device__ constexpr int gm_stage_bytes(int TN, bool pairs) {
+  return (kGmABytes + TN * kGmK * 2) * (pairs ? 2 : 1);
 }
+__host__ __device__ constexpr int gm_stages(int TN, bool pairs) {
+  return 192 * 1024 / gm_stage_bytes(TN, pairs);
+}
+constexpr size_t kGmSmem = 1024 + 192 * 1024 + 256;
 
 // The units of one launch: tiles of 128 x TN, each cut into `slices` of K.
 // m runs fastest where the B operand is the large one (m_fast), so that
@@ -109,26 +116,27 @@ __device__ __forceinline__ GmUnit gm_unit(const GmShape &s, int u) {
   return r;
 }
 
-// The thread's row of a finished tile, 32 columns at a time: straight from
+// The thread's row of a finished tile, 64 columns at a time: straight from
 // TMEM, or from the registers that joined the rounds.
 struct GmFromTmem {
   uint32_t taddr;
   static constexpr int unroll = 1;
-  __device__ __forceinline__ void get(int c, float (&v)[32]) const { tmem_ld32(taddr + c, v); }
+  __device__ __forceinline__ void get(int c, float (&v)[64]) const { tmem_ld64(taddr + c, v); }
 };
 template <int NC>
 struct GmFromRegs {
   const float (&acc)[NC];
-  static constexpr int unroll = NC / 32;
-  __device__ __forceinline__ void get(int c, float (&v)[32]) const {
+  static constexpr int unroll = NC / 64;
+  __device__ __forceinline__ void get(int c, float (&v)[64]) const {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = acc[c + j];
+    for (int j = 0; j < 64; ++j) v[j] = acc[c + j];
   }
 };
 
-// Epi: run<TN>(unit, row in tile, first column in tile, source) for one
-// thread's row and its half of the tile's columns.  PAIRS: three products, in
-// rounds; else one product and one round.
+// Epi: `Fixed fixed()` once per thread; `Row begin(unit, row, col)` loads what
+// the row needs; run<TN>(fixed, row state, unit, row, col, source) works on one
+// thread's row of the tile and its half of the columns.  PAIRS: three products,
+// in rounds; else one product and one round.
 template <int TN, bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
 __global__ void __launch_bounds__(kGmThreads, 1)
     gemm16_kernel(const __grid_constant__ GmMaps maps, const GmShape s,
@@ -136,12 +144,14 @@ __global__ void __launch_bounds__(kGmThreads, 1)
   extern __shared__ uint8_t gm_raw[];
   const uint32_t raw = smem_u32(gm_raw);
   const uint32_t base = (raw + 1023) & ~1023u;
-  constexpr int kStage = gm_stage_bytes(TN);
-  constexpr int kTmemCols = 2 * TN;
-  constexpr int kProducts = PAIRS ? 3 : 1;
+  static_assert(!PAIRS || TN == 128, "TMEM holds two pairs of 128 columns");
+  constexpr int kStage = gm_stage_bytes(TN, PAIRS), kGmStages = gm_stages(TN, PAIRS);
+  constexpr int kAccCols = PAIRS ? 2 * TN : TN;  // PAIRS: hi hi, then the small ones
+  constexpr int kTmemCols = 2 * kAccCols;
+  constexpr int kBBytes = TN * kGmK * 2;
   constexpr int kRound = PAIRS ? kGmRound : 1 << 30;
   const uint32_t bars = base + kGmStages * kStage;
-  // full[4] empty[4] accfull[2] accempty[2], then the TMEM address and abort flag
+  // full, empty [stages], accfull[2] accempty[2], then the TMEM address and abort flag
   const uint32_t full = bars, empty = bars + 8 * kGmStages, accfull = bars + 16 * kGmStages,
                  accempty = accfull + 16, tmem_slot = accempty + 16;
   volatile int *abort_flag = (volatile int *)(gm_raw + (tmem_slot + 4 - raw));
@@ -178,34 +188,32 @@ __global__ void __launch_bounds__(kGmThreads, 1)
       bool ok = true;
       for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
         const GmUnit w = gm_unit(s, u);
-        for (int k0 = w.k0; ok && k0 < w.k1; k0 += kRound)
-        for (int p = 0; ok && p < kProducts; ++p) {
-          const CUtensorMap *ma = PAIRS && p == 0 ? &maps.a_lo : &maps.a_hi;
-          const CUtensorMap *mb = PAIRS && p == 1 ? &maps.b_lo : &maps.b_hi;
-          const int k1 = min(k0 + kRound, w.k1);
-          for (int k = k0; k < k1; ++k, ++issued) {
-            const int st = issued % kGmStages;
-            if (issued >= kGmStages &&
-                !ws_wait(empty + 8 * st, ((issued / kGmStages) - 1) & 1, abort_flag,
-                         s.spin_limit)) {
-              ok = false;
-              break;
-            }
-            const uint32_t a = base + st * kStage, b = a + kGmABytes, bar = full + 8 * st;
-            mbar_expect_tx(bar, kStage);
+        for (int k = w.k0; k < w.k1; ++k, ++issued) {
+          const int st = issued % kGmStages;
+          if (issued >= kGmStages &&
+              !ws_wait(empty + 8 * st, ((issued / kGmStages) - 1) & 1, abort_flag, s.spin_limit)) {
+            ok = false;
+            break;
+          }
+          const uint32_t a = base + st * kStage, b = a + (PAIRS ? 2 : 1) * kGmABytes,
+                         bar = full + 8 * st;
+          mbar_expect_tx(bar, kStage);
+#pragma unroll
+          for (int p = 0; p < (PAIRS ? 2 : 1); ++p) {
+            const CUtensorMap *ma = p ? &maps.a_lo : &maps.a_hi, *mb = p ? &maps.b_lo : &maps.b_hi;
             if (A_MN) {
 #pragma unroll
               for (int c = 0; c < kGmM / 64; ++c)
-                tma_2d(a + c * 8192, ma, w.m * kGmM + c * 64, k * kGmK, bar);
+                tma_2d(a + p * kGmABytes + c * 8192, ma, w.m * kGmM + c * 64, k * kGmK, bar);
             } else {
-              tma_2d(a, ma, k * kGmK, w.m * kGmM, bar);
+              tma_2d(a + p * kGmABytes, ma, k * kGmK, w.m * kGmM, bar);
             }
             if (B_MN) {
 #pragma unroll
               for (int c = 0; c < TN / 64; ++c)
-                tma_2d(b + c * 8192, mb, w.n * TN + c * 64, k * kGmK, bar);
+                tma_2d(b + p * kBBytes + c * 8192, mb, w.n * TN + c * 64, k * kGmK, bar);
             } else {
-              tma_2d(b, mb, k * kGmK, w.n * TN, bar);
+              tma_2d(b + p * kBBytes, mb, k * kGmK, w.n * TN, bar);
             }
           }
         }
@@ -232,8 +240,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t acc = tmem + buf * TN;
-          const int steps = kProducts * (min(k0 + kRound, w.k1) - k0);
+          const uint32_t acc = tmem + buf * kAccCols;
+          const int steps = min(k0 + kRound, w.k1) - k0;
           for (int i = 0; i < steps; ++i, ++used) {
             const int st = used % kGmStages;
             if (!ws_wait(full + 8 * st, (used / kGmStages) & 1, abort_flag, s.spin_limit)) {
@@ -241,13 +249,18 @@ __global__ void __launch_bounds__(kGmThreads, 1)
               break;
             }
             tc_fence_after();
-            const uint32_t a = base + st * kStage, b = a + kGmABytes;
+            const uint32_t a = base + st * kStage, b = a + (PAIRS ? 2 : 1) * kGmABytes;
             const uint64_t da = gm_desc(a, A_MN), db = gm_desc(b, B_MN);
 #pragma unroll
             for (int kk = 0; kk < kGmK / 16; ++kk) {
               // 16 k: 32 bytes along a K-major row, two 8-k groups MN-major
-              gm_mma(acc, da + (uint64_t)(kk * (A_MN ? 2048 : 32) >> 4),
-                     db + (uint64_t)(kk * (B_MN ? 2048 : 32) >> 4), idesc, i > 0 || kk > 0);
+              const uint64_t ka = da + (uint64_t)(kk * (A_MN ? 2048 : 32) >> 4),
+                             kb = db + (uint64_t)(kk * (B_MN ? 2048 : 32) >> 4);
+              gm_mma(acc, ka, kb, idesc, i > 0 || kk > 0);
+              if (PAIRS) {
+                gm_mma(acc + TN, ka + (kGmABytes >> 4), kb, idesc, i > 0 || kk > 0);
+                gm_mma(acc + TN, ka, kb + (kBBytes >> 4), idesc, 1);
+              }
             }
             tc_commit(empty + 8 * st);
           }
@@ -283,26 +296,34 @@ __global__ void __launch_bounds__(kGmThreads, 1)
       ++t;
     };
     bool ok = true;
+    const auto fixed = epi.fixed();
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
       const GmUnit w = gm_unit(s, u);
+      const auto state = epi.begin(w, row);
       if constexpr (PAIRS) {
         float acc[TN / 2];
         for (int k0 = w.k0; k0 < w.k1; k0 += kRound) {
           if (!(ok = ready())) break;
-          const uint32_t from = lane_addr + (t & 1) * TN;
+          const uint32_t from = lane_addr + (t & 1) * kAccCols;
 #pragma unroll
           for (int c = 0; c < TN / 2; c += 32) {
-            float v[32];
+            float v[32], x[32];
             tmem_ld32(from + c, v);
+            tmem_ld32(from + TN + c, x);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[c + j] = k0 == w.k0 ? v[j] : acc[c + j] + v[j];
+            for (int j = 0; j < 32; ++j) {
+              v[j] += x[j];
+              acc[c + j] = k0 == w.k0 ? v[j] : acc[c + j] + v[j];
+            }
           }
           release();
         }
-        if (ok) epi.template run<TN>(w, row, half * (TN / 2), GmFromRegs<TN / 2>{acc});
+        if (ok)
+          epi.template run<TN>(fixed, state, w, row, half * (TN / 2), GmFromRegs<TN / 2>{acc});
       } else {
         if (!(ok = ready())) break;
-        epi.template run<TN>(w, row, half * (TN / 2), GmFromTmem{lane_addr + (t & 1) * TN});
+        epi.template run<TN>(fixed, state, w, row, half * (TN / 2),
+                             GmFromTmem{lane_addr + (t & 1) * kAccCols});
         release();
       }
     }
