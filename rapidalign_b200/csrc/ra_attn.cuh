@@ -135,7 +135,7 @@ struct AttnScore {
     float t = dot * su;
     slope = 1.f;
     if (capl > 0.f) {
-      const float th = tanhf(t);
+      const float th = tanh_step(t);
       slope = 1.f - th * th;
       t = th * capl;
     }

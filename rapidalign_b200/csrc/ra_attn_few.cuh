@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       float s = t[e];
-      if (capped) s = capl * tanhf(s);
+      if (capped) s = capl * tanh_step(s);
       if (pos) {
         const float dx = pi.x - pj[e].x, dy = pi.y - pj[e].y, dz = pi.z - pj[e].z;
         s = fmaf(-w, fmaf(dz, dz, fmaf(dy, dy, dx * dx)), s);

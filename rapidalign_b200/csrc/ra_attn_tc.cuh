@@ -243,17 +243,6 @@ __device__ __forceinline__ void put_weights(uint32_t taddr, const float (&v)[32]
   }
 }
 
-// tanh to 2^-22 of 1 (16-bit inputs) or to a few steps (fp32)
-template <class Kind>
-__device__ __forceinline__ float tanh_kind(float u) {
-  if (Kind::pair) return tanhf(u);
-  const float e = ex2(u * (2.f * kAttnLog2e));
-  const float big = 1.f - __fdividef(2.f, 1.f + e);
-  const float u2 = u * u;
-  const float small = u * fmaf(u2, fmaf(u2, fmaf(u2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
-  return fabsf(u) < 0.1f ? small : big;
-}
-
 // Positions of a streamed tile in shared memory: x, y, z of its rows.
 template <int R>
 struct TilePos {
@@ -294,8 +283,8 @@ __device__ __forceinline__ void scores32(const float (&v)[32], f2_t (&t)[16], co
   if (sc.capl > 0.f) {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      t[j] = pk(sc.capl * tanh_kind<Kind>(v[2 * j] * sc.su),
-                sc.capl * tanh_kind<Kind>(v[2 * j + 1] * sc.su));
+      t[j] = pk(sc.capl * tanh_step(v[2 * j] * sc.su),
+                sc.capl * tanh_step(v[2 * j + 1] * sc.su));
   } else {
 #pragma unroll
     for (int j = 0; j < 16; ++j) t[j] = mul2(pk(v[2 * j], v[2 * j + 1]), su);
@@ -821,7 +810,7 @@ __device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], con
       const int e = j + 2 * k;
       f2_t t, th;
       if (CAP) {
-        th = pk(tanh_kind<Kind>(v[e] * B.sc.su), tanh_kind<Kind>(v[e + 1] * B.sc.su));
+        th = pk(tanh_step(v[e] * B.sc.su), tanh_step(v[e + 1] * B.sc.su));
         t = fma2(th, two(B.sc.capl), nm);
       } else {
         t = fma2(pk(v[e], v[e + 1]), su, nm);
@@ -872,7 +861,7 @@ __device__ __forceinline__ void dkv_elements(float (&v)[32], float (&dp)[32], co
       const int e = j + 2 * k;
       f2_t t, th;
       if (CAP) {
-        th = pk(tanh_kind<Kind>(v[e] * B.sc.su), tanh_kind<Kind>(v[e + 1] * B.sc.su));
+        th = pk(tanh_step(v[e] * B.sc.su), tanh_step(v[e + 1] * B.sc.su));
         t = fma2(th, two(B.sc.capl), k ? nm.y : nm.x);
       } else {
         t = fma2(pk(v[e], v[e + 1]), su, k ? nm.y : nm.x);

@@ -90,7 +90,7 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   p.mt = ceil_div(d->rows, (int64_t)kGmM);
   const int64_t pass = std::min<int64_t>(d->rows, kCeRowsPerPass);
   p.tn_z = tile_width(ceil_div(pass, (int64_t)kGmM), d->vocab, sms, split);
-  p.parts = 2 * (int)ceil_div(d->vocab, (int64_t)p.tn_z);
+  p.parts = kGmParts * (int)ceil_div(d->vocab, (int64_t)p.tn_z);
   size_t o = 0;
   p.f_part = o;
   o += align256(sizeof(float2) * (size_t)p.parts * (size_t)(ceil_div(pass, (int64_t)kGmM) * kGmM));
@@ -131,10 +131,10 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   return p;
 }
 
-template <int TN, bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
+template <int TN, bool BF16, GmOp OP, bool A_MN, bool B_MN, class Epi>
 int launch_gemm(const GmMaps &maps, const GmShape &s, const Epi &epi, int sms, cudaStream_t st) {
   const size_t smem = kGmSmem;
-  auto k = gemm16_kernel<TN, BF16, PAIRS, A_MN, B_MN, Epi>;
+  auto k = gemm16_kernel<TN, BF16, OP, A_MN, B_MN, Epi>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
     return RA_ERR_CUDA;
@@ -147,11 +147,16 @@ int launch_gemm(const GmMaps &maps, const GmShape &s, const Epi &epi, int sms, c
 template <bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
 int launch_gemm(int tn, const GmMaps &maps, const GmShape &s, const Epi &epi, int sms,
                 cudaStream_t st) {
-  if constexpr (PAIRS)
-    return launch_gemm<128, BF16, true, A_MN, B_MN>(maps, s, epi, sms, st);
-  else
-    return tn == 256 ? launch_gemm<256, BF16, false, A_MN, B_MN>(maps, s, epi, sms, st)
-                     : launch_gemm<128, BF16, false, A_MN, B_MN>(maps, s, epi, sms, st);
+  if constexpr (PAIRS) {
+    // a gradient's K is long; the logits' is often one round
+    if constexpr (!A_MN && !B_MN)
+      if (s.k_steps <= kGmRound)
+        return launch_gemm<128, BF16, kGmPairs1, A_MN, B_MN>(maps, s, epi, sms, st);
+    return launch_gemm<128, BF16, kGmPairs, A_MN, B_MN>(maps, s, epi, sms, st);
+  } else {
+    return tn == 256 ? launch_gemm<256, BF16, kGmOne, A_MN, B_MN>(maps, s, epi, sms, st)
+                     : launch_gemm<128, BF16, kGmOne, A_MN, B_MN>(maps, s, epi, sms, st);
+  }
 }
 
 struct Operands {  // 16-bit x and w, or their halves

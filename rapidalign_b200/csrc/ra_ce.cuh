@@ -9,7 +9,7 @@
 // with gl, ge the upstream gradients of loss and lse.
 //
 // Forward: one product (ra_gemm16.cuh) whose epilogue keeps a running maximum
-// and sum of exponentials of each row over its 128 columns; `ce_rows_kernel`
+// and sum of exponentials of each row over its columns; `ce_rows_kernel`
 // joins the column tiles.  All in base 2: t = z log2 e, 2^(t - m).
 // Backward: the vocabulary in pieces; per piece the logits again, du in 16
 // bits (with the rows' coefficients, so both products read it as it is), then
@@ -102,15 +102,6 @@ struct CeLogit {
     const float f = PAIRS ? ce_pow2(-ce_exp(head->amax_x) - ce_exp(head->amax_w)) : 1.f;
     return cap > 0.f ? Fixed{scale * f / cap, cap * kLog2e} : Fixed{scale * f * kLog2e, 0.f};
   }
-  // to a few steps for fp32 inputs, to 2^-22 of 1 for 16-bit ones
-  static __device__ __forceinline__ float tanh_of(float u) {
-    if (PAIRS) return tanhf(u);
-    const float big = 1.f - __fdividef(2.f, 1.f + ex2(u * (2.f * kLog2e)));
-    const float u2 = u * u;
-    const float small =
-        u * fmaf(u2, fmaf(u2, fmaf(u2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
-    return fabsf(u) < 0.1f ? small : big;
-  }
 };
 
 // Forward epilogue: maximum and sum of 2^(t - m) over the thread's columns.
@@ -119,7 +110,7 @@ struct CeEpiLse {
   CeLogit<PAIRS> lg;
   int64_t rows, vocab;
   const int64_t *target;
-  float2 *part;  // [2 n_tiles][ld]
+  float2 *part;  // [kGmParts n_tiles][ld]
   int64_t ld;
   float *zt;  // [rows] t at the label
   using Fixed = typename CeLogit<PAIRS>::Fixed;
@@ -133,44 +124,47 @@ struct CeEpiLse {
   }
   template <int TN, class Src>
   __device__ __forceinline__ void run(const Fixed &F, const Row &R, const GmUnit &w, int row,
-                                      int col, const Src &src) const {
+                                      int col, const Src &src, const GmOut &out_rows) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
     const f2_t f2 = pk(F.f, F.f);
     float m = -INFINITY, s = 0.f;
 #pragma unroll Src::unroll
-    for (int c = 0; c < TN / 2; c += 64) {
-      float v[64];
+    for (int c = 0; c < TN / kGmParts; c += 32) {
+      float v[32];
       src.get(c, v);
       const int64_t left = vocab - (c0 + c);
       if (F.capl > 0.f) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] = F.capl * lg.tanh_of(v[j] * F.f);
+        for (int j = 0; j < 32; ++j) v[j] = F.capl * tanh_step(v[j] * F.f);
       } else {
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) upk(mul2(pk(v[j], v[j + 1]), f2), v[j], v[j + 1]);
+        for (int j = 0; j < 32; j += 2) upk(mul2(pk(v[j], v[j + 1]), f2), v[j], v[j + 1]);
       }
-      if (left < 64) {
+      if (left < 32) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j)
+        for (int j = 0; j < 32; ++j)
           if (j >= left) v[j] = -INFINITY;
       }
       const int64_t at = R.target - (c0 + c);
-      if (at >= 0 && at < 64 && at < left) {
+      if (at >= 0 && at < 32 && at < left) {
         float z = 0.f;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) z = j == (int)at ? v[j] : z;
+        for (int j = 0; j < 32; ++j)  // not v[at]: that would put v into local memory
+          asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, %2;\n\t@p mov.f32 %0, %3;\n\t}"
+                       : "+f"(z)
+                       : "r"((int)at), "r"(j), "f"(v[j]));
         zt[r] = z;
       }
       float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-      for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+      for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
       mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const float mn = fmaxf(m, mx[0]);
       if (mn > -INFINITY || mx[0] != mx[0]) {
         const f2_t ref = pk(-mn, -mn);
         f2_t sum[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) {
+        for (int j = 0; j < 32; j += 2) {
           float x, y;
           upk(add2(pk(v[j], v[j + 1]), ref), x, y);
           sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pk(ex2(x), ex2(y)));
@@ -180,7 +174,7 @@ struct CeEpiLse {
         m = mn;
       }
     }
-    part[((int64_t)w.n * 2 + (col ? 1 : 0)) * ld + r] = make_float2(m, s);
+    part[((int64_t)w.n * kGmParts + col / (TN / kGmParts)) * ld + r] = make_float2(m, s);
   }
 };
 
@@ -330,63 +324,72 @@ struct CeEpiGrad {
     if (r >= rows) return {make_float2(0.f, 0.f), make_float2(0.f, 1.f), -1};
     return {coef[r], stats[r], target[r] - v0};
   }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return BF16 ? pack_bf16(a, b) : pack_f16(a, b);
+  }
+  // the halves that `hi` left over
+  static __device__ __forceinline__ uint32_t rest(uint32_t hi, float a, float b) {
+    const float2 f = __half22float2(bits_as<__half2>(hi));
+    return pack_f16(a - f.x, b - f.y);
+  }
   template <int TN, class Src>
   __device__ __forceinline__ void run(const Fixed &F, const Row &R, const GmUnit &w, int row,
-                                      int col, const Src &src) const {
+                                      int col, const Src &src, const GmOut &out_rows) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
-    uint16_t *ph = hi + r * ldg + c0;
-    uint16_t *pl = PAIRS ? lo + r * ldg + c0 : nullptr;
     // c / top before the scale: 1 where all coefficients are alike
     const float gl = R.cf.y / F.top * kCeGradScale<BF16>, m = -R.st.x;
     const float cp = R.cf.x / F.top * kCeGradScale<BF16> / R.st.y;
     const bool off = R.cf.x == 0.f && R.cf.y == 0.f;
     const f2_t f2 = pk(F.lg.f, F.lg.f), nm = pk(m, m), pc = pk(cp, cp);
 #pragma unroll Src::unroll
-    for (int c = 0; c < TN / 2; c += 64) {
-      float v[64];
+    for (int c = 0; c < TN / kGmParts; c += 32) {
+      float v[32];
       src.get(c, v);
       const int64_t at = R.target - (c0 + c);
-      const bool hit = at >= 0 && at < 64;
+      const bool hit = at >= 0 && at < 32;
       if (F.lg.capl > 0.f) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-          const float th = lg.tanh_of(v[j] * F.lg.f);
+        for (int j = 0; j < 32; ++j) {
+          const float th = tanh_step(v[j] * F.lg.f);
           float g = ex2(fmaf(th, F.lg.capl, m)) * cp;
           if (hit && j == (int)at) g -= gl;
           v[j] = g * fmaf(-th, th, 1.f);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) {
+        for (int j = 0; j < 32; j += 2) {
           float x, y;
           upk(fma2(pk(v[j], v[j + 1]), f2, nm), x, y);
           upk(mul2(pk(ex2(x), ex2(y)), pc), v[j], v[j + 1]);
         }
         if (hit) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = j == (int)at ? v[j] - gl : v[j];
+          for (int j = 0; j < 32; ++j) v[j] = j == (int)at ? v[j] - gl : v[j];
         }
       }
       if (off) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] = 0.f;
+        for (int j = 0; j < 32; ++j) v[j] = 0.f;
       }
+      uint4 h[4];
 #pragma unroll
-      for (int q = 0; q < 64; q += 8) {
-        uint32_t h[4];
+      for (int q = 0; q < 4; ++q)
+        h[q] = make_uint4(pack(v[8 * q], v[8 * q + 1]), pack(v[8 * q + 2], v[8 * q + 3]),
+                          pack(v[8 * q + 4], v[8 * q + 5]), pack(v[8 * q + 6], v[8 * q + 7]));
+      const int64_t at0 = (r - (threadIdx.x & 31)) * ldg + c0 + c;
+      out_rows.rows64(h, [&](int row_, int j, uint4 x) {
+        *reinterpret_cast<uint4 *>(hi + at0 + row_ * ldg + 8 * j) = x;
+      });
+      if (PAIRS) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          h[j] = BF16 ? pack_bf16(v[q + 2 * j], v[q + 2 * j + 1])
-                      : pack_f16(v[q + 2 * j], v[q + 2 * j + 1]);
-        *reinterpret_cast<uint4 *>(ph + c + q) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (PAIRS) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 b = __half22float2(bits_as<__half2>(h[j]));
-            h[j] = pack_f16(v[q + 2 * j] - b.x, v[q + 2 * j + 1] - b.y);
-          }
-          *reinterpret_cast<uint4 *>(pl + c + q) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
+        for (int q = 0; q < 4; ++q)
+          h[q] = make_uint4(rest(h[q].x, v[8 * q], v[8 * q + 1]),
+                            rest(h[q].y, v[8 * q + 2], v[8 * q + 3]),
+                            rest(h[q].z, v[8 * q + 4], v[8 * q + 5]),
+                            rest(h[q].w, v[8 * q + 6], v[8 * q + 7]));
+        out_rows.rows64(h, [&](int row_, int j, uint4 x) {
+          *reinterpret_cast<uint4 *>(lo + at0 + row_ * ldg + 8 * j) = x;
+        });
       }
     }
   }
@@ -423,53 +426,64 @@ struct CeEpiOut {
   __device__ __forceinline__ Row begin(const GmUnit &, int) const { return {}; }
   template <int TN, class Src>
   __device__ __forceinline__ void run(const Fixed &F, const Row &, const GmUnit &w, int row,
-                                      int col, const Src &src) const {
+                                      int col, const Src &src, const GmOut &out_rows) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
-    const float al = F.al;
-    float *pp = part + ((int64_t)w.slice * rows + r) * cols + c0;
-    T *po = out + r * cols + c0;
-    const bool wide = (cols & 3) == 0;  // 16-byte aligned fp32 rows
+    const int64_t w0 = r - (threadIdx.x & 31);  // the warp's first row
+    // 16-byte aligned rows: fp32 sums, or results
+    const bool wide = cols % (out != nullptr ? 16 / (int)sizeof(T) : 4) == 0;
 #pragma unroll Src::unroll
-    for (int c = 0; c < TN / 2; c += 64) {
-      float v[64];
+    for (int c = 0; c < TN / kGmParts; c += 32) {
+      float v[32];
       src.get(c, v);
       const int64_t left = cols - (c0 + c);
-      if (r >= rows || left <= 0) continue;
-      if (out != nullptr) {
-        if (left >= 64 && (cols & 7) == 0) {
-          if (sizeof(T) == 4) {
+      if (left <= 0) break;  // the same for the warp
+      if (!wide || left < 32) {
+        if (r < rows) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              reinterpret_cast<float4 *>(po + c)[j] = make_float4(
-                  v[4 * j] * al, v[4 * j + 1] * al, v[4 * j + 2] * al, v[4 * j + 3] * al);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              T t[8];
-#pragma unroll
-              for (int k = 0; k < 8; ++k) store_as(t + k, v[8 * j + k] * al);
-              uint4 u;
-              memcpy(&u, t, 16);
-              reinterpret_cast<uint4 *>(po + c)[j] = u;
+          for (int j = 0; j < 32; ++j) {
+            if (j >= left) continue;
+            if (out != nullptr) {
+              store_as(out + r * cols + c0 + c + j, v[j] * F.al);
+            } else {
+              float *q = part + ((int64_t)w.slice * rows + r) * cols + c0 + c + j;
+              *q = v[j] + (add ? *q : 0.f);
             }
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (j < left) store_as(po + c + j, v[j] * al);
         }
-      } else if (wide && left >= 64) {
+      } else if (out != nullptr && sizeof(T) == 2) {
+        uint4 x[4];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float4 *q = reinterpret_cast<float4 *>(pp + c) + j;
-          float4 o = add ? *q : make_float4(0.f, 0.f, 0.f, 0.f);
-          *q = make_float4(o.x + v[4 * j], o.y + v[4 * j + 1], o.z + v[4 * j + 2],
-                           o.w + v[4 * j + 3]);
+        for (int q = 0; q < 4; ++q) {
+          T t[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) store_as(t + k, v[8 * q + k] * F.al);
+          memcpy(&x[q], t, 16);
         }
+        out_rows.rows64(x, [&](int row_, int j, uint4 u) {
+          if (w0 + row_ < rows)
+            *reinterpret_cast<uint4 *>(out + (w0 + row_) * cols + c0 + c + 8 * j) = u;
+        });
       } else {
+        float *base = out != nullptr ? reinterpret_cast<float *>(out)
+                                     : part + (int64_t)w.slice * rows * cols;
+        const bool more = out == nullptr && add;
 #pragma unroll
-        for (int j = 0; j < 64; ++j)
-          if (j < left) pp[c + j] = v[j] + (add ? pp[c + j] : 0.f);
+        for (int hf = 0; hf < 2; ++hf) {
+          uint4 x[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            x[q] = make_uint4(__float_as_uint(v[16 * hf + 4 * q] * F.al),
+                              __float_as_uint(v[16 * hf + 4 * q + 1] * F.al),
+                              __float_as_uint(v[16 * hf + 4 * q + 2] * F.al),
+                              __float_as_uint(v[16 * hf + 4 * q + 3] * F.al));
+          out_rows.rows64(x, [&](int row_, int j, uint4 u) {
+            if (w0 + row_ >= rows) return;
+            float4 *q = reinterpret_cast<float4 *>(base + (w0 + row_) * cols + c0 + c + 16 * hf) + j;
+            float4 o = more ? *q : make_float4(0.f, 0.f, 0.f, 0.f);
+            *q = make_float4(o.x + __uint_as_float(u.x), o.y + __uint_as_float(u.y),
+                             o.z + __uint_as_float(u.z), o.w + __uint_as_float(u.w));
+          });
+        }
       }
     }
   }

@@ -76,6 +76,25 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// tanh to about a step: below 0.6 the quotient that the continued fraction
+// u / (1 + u^2 / (3 + u^2 / (5 + u^2 / (7 + u^2 / 9)))) comes to (off by less
+// than 3e-9 there), above 1 - 2 / (1 + e^(2u)).  Straight-line, where tanhf
+// branches.
+__device__ __forceinline__ float tanh_step(float u) {
+  const float x = u * u;
+  const float num = fmaf(x, x + 105.f, 945.f) * u;
+  const float den = fmaf(x, fmaf(x, 15.f, 420.f), 945.f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
+  float q = num * r;
+  q = fmaf(fmaf(-q, den, num), r, q);
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u * 2.885390081777927f));
+  float s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return fabsf(u) < 0.6f ? q : fmaf(-2.f, s, 1.f);
+}
+
 // The bits of one value as another type of the same size.
 template <class To, class From>
 __device__ __forceinline__ To bits_as(const From &v) {

@@ -18,11 +18,13 @@
 // accumulators and the epilogue adds the rounds in registers, rounding to
 // nearest.
 //
-// Roles (320 threads, one CTA per SM, persistent over (tile, K slice) units):
-//   warps 0-7  epilogue: warp w reads TMEM lanes 32 (w % 4).. and half w / 4
-//              of the tile's columns
-//   warp 8     lane 0 copies operand tiles into the shared-memory ring
-//   warp 9     lane 0 issues the MMAs
+// Roles (576 threads, one CTA per SM, persistent over (tile, K slice) units):
+//   warps 0-15 epilogue: warp w reads TMEM lanes 32 (w % 4).. and quarter w / 4
+//              of the tile's columns.  Sixteen, because over a short K (D = 128:
+//              1,500 cycles of MMAs a tile) the epilogue's own latency is what
+//              a tile takes.
+//   warp 16    lane 0 copies operand tiles into the shared-memory ring
+//   warp 17    lane 0 issues the MMAs
 // Two accumulators in TMEM (two pairs of them): the epilogue of one unit runs
 // under the MMAs of the next; what it reads of its rows besides is loaded before
 // it waits.  Every wait is bounded; on expiry the CTA records the timeout,
@@ -39,7 +41,8 @@
 namespace ra {
 
 constexpr int kGmM = 128, kGmK = 64;
-constexpr int kGmThreads = 320, kGmEpiWarps = 8;
+constexpr int kGmEpiWarps = 16, kGmLoadWarp = 16, kGmMmaWarp = 17, kGmThreads = 576;
+constexpr int kGmParts = kGmEpiWarps / 4;  // column parts of a tile
 constexpr int kGmABytes = kGmM * kGmK * 2;
 constexpr int kGmRound = 4;  // k steps (of 64) of a round of pairs
 
@@ -51,7 +54,8 @@ __host__ __device__ constexpr int gm_stage_bytes(int TN, bool pairs) {
 __host__ __device__ constexpr int gm_stages(int TN, bool pairs) {
   return 192 * 1024 / gm_stage_bytes(TN, pairs);
 }
-constexpr size_t kGmSmem = 1024 + 192 * 1024 + 256;
+constexpr int kGmStageOut = 2048;  // a warp's 32 rows of 64 bytes on their way out
+constexpr size_t kGmSmem = 1024 + 192 * 1024 + kGmEpiWarps * kGmStageOut + 256;
 
 // The units of one launch: tiles of 128 x TN, each cut into `slices` of K.
 // m runs fastest where the B operand is the large one (m_fast), so that
@@ -116,41 +120,74 @@ __device__ __forceinline__ GmUnit gm_unit(const GmShape &s, int u) {
   return r;
 }
 
-// The thread's row of a finished tile, 64 columns at a time: straight from
+// The thread's row of a finished tile, 32 columns at a time: straight from
 // TMEM, or from the registers that joined the rounds.
 struct GmFromTmem {
   uint32_t taddr;
   static constexpr int unroll = 1;
-  __device__ __forceinline__ void get(int c, float (&v)[64]) const { tmem_ld64(taddr + c, v); }
+  __device__ __forceinline__ void get(int c, float (&v)[32]) const { tmem_ld32(taddr + c, v); }
+};
+struct GmFromPairs {  // one round of pairs: both accumulators
+  uint32_t taddr, small;
+  static constexpr int unroll = 1;
+  __device__ __forceinline__ void get(int c, float (&v)[32]) const {
+    float x[32];
+    tmem_ld32(taddr + c, v);
+    tmem_ld32(small + c, x);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += x[j];
+  }
 };
 template <int NC>
 struct GmFromRegs {
   const float (&acc)[NC];
-  static constexpr int unroll = NC / 64;
-  __device__ __forceinline__ void get(int c, float (&v)[64]) const {
+  static constexpr int unroll = NC / 32;
+  __device__ __forceinline__ void get(int c, float (&v)[32]) const {
 #pragma unroll
-    for (int j = 0; j < 64; ++j) v[j] = acc[c + j];
+    for (int j = 0; j < 32; ++j) v[j] = acc[c + j];
+  }
+};
+// A warp's way to global memory: every lane gives 64 bytes of its row, and four
+// lanes at a time take a whole row's (a lane's own 16-byte stores would write
+// half sectors of 32 rows).  put(row of the warp, 16-byte chunk, bits).
+struct GmOut {
+  uint8_t *p;  // kGmStageOut bytes of this warp
+  template <class Put>
+  __device__ __forceinline__ void rows64(const uint4 (&x)[4], Put put) const {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint4 *>(p + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = x[j];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = (lane >> 2) + 8 * k, j = lane & 3;
+      put(row, j, *reinterpret_cast<const uint4 *>(p + row * 64 + ((j ^ ((row >> 1) & 3)) << 4)));
+    }
   }
 };
 
-// Epi: `Fixed fixed()` once per thread; `Row begin(unit, row, col)` loads what
-// the row needs; run<TN>(fixed, row state, unit, row, col, source) works on one
-// thread's row of the tile and its half of the columns.  PAIRS: three products,
-// in rounds; else one product and one round.
-template <int TN, bool BF16, bool PAIRS, bool A_MN, bool B_MN, class Epi>
+// Epi: `Fixed fixed()` once per thread; `Row begin(unit, row)` loads what the
+// row needs; run<TN>(fixed, row state, unit, row, col, source, out) works on one
+// thread's row of the tile and its quarter of the columns, all lanes of a warp
+// together.  OP: one product; three products of pairs in one round, or in more.
+enum GmOp { kGmOne, kGmPairs1, kGmPairs };
+template <int TN, bool BF16, GmOp OP, bool A_MN, bool B_MN, class Epi>
 __global__ void __launch_bounds__(kGmThreads, 1)
     gemm16_kernel(const __grid_constant__ GmMaps maps, const GmShape s,
                   const __grid_constant__ Epi epi) {
   extern __shared__ uint8_t gm_raw[];
   const uint32_t raw = smem_u32(gm_raw);
   const uint32_t base = (raw + 1023) & ~1023u;
+  constexpr bool PAIRS = OP != kGmOne;
   static_assert(!PAIRS || TN == 128, "TMEM holds two pairs of 128 columns");
   constexpr int kStage = gm_stage_bytes(TN, PAIRS), kGmStages = gm_stages(TN, PAIRS);
   constexpr int kAccCols = PAIRS ? 2 * TN : TN;  // PAIRS: hi hi, then the small ones
   constexpr int kTmemCols = 2 * kAccCols;
   constexpr int kBBytes = TN * kGmK * 2;
-  constexpr int kRound = PAIRS ? kGmRound : 1 << 30;
-  const uint32_t bars = base + kGmStages * kStage;
+  constexpr int kRound = OP == kGmPairs ? kGmRound : 1 << 30;
+  const uint32_t outs = base + kGmStages * kStage, bars = outs + kGmEpiWarps * kGmStageOut;
   // full, empty [stages], accfull[2] accempty[2], then the TMEM address and abort flag
   const uint32_t full = bars, empty = bars + 8 * kGmStages, accfull = bars + 16 * kGmStages,
                  accempty = accfull + 16, tmem_slot = accempty + 16;
@@ -159,7 +196,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = s.m_tiles * s.n_tiles * s.slices;
 
-  if (warp == 9) {
+  if (warp == kGmMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      tmem_slot),
                  "r"(kTmemCols)
@@ -182,7 +219,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_addr;
 
-  if (warp == 8) {
+  if (warp == kGmLoadWarp) {
     if (lane == 0) {
       int issued = 0;  // operand tiles issued; tile i sits in stage i % kGmStages
       bool ok = true;
@@ -225,7 +262,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         if (!mbar_wait(full + 8 * (i % kGmStages), (i / kGmStages) & 1, s.spin_limit)) ok = false;
       if (!ok) atomicOr(s.status, 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == kGmMmaWarp) {
     if (lane == 0) {
       constexpr uint32_t idesc = gm_idesc(TN, BF16, A_MN, B_MN);
       int used = 0, t = 0;
@@ -273,10 +310,12 @@ __global__ void __launch_bounds__(kGmThreads, 1)
       }
     }
   } else {
-    const int half = warp >> 2;
+    constexpr int kCols = TN / kGmParts;  // columns of a thread
+    const int col = (warp >> 2) * kCols;
+    const GmOut out{gm_raw + (outs - raw) + warp * kGmStageOut};
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lane_addr =
-        tmem + half * (TN / 2) + ((uint32_t)(32 * (warp & 3)) << 16);
+        tmem + col + ((uint32_t)(32 * (warp & 3)) << 16);
     int t = 0;
     // waits for round t's accumulator; false (for the whole warp) on expiry
     auto ready = [&]() {
@@ -300,13 +339,13 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
       const GmUnit w = gm_unit(s, u);
       const auto state = epi.begin(w, row);
-      if constexpr (PAIRS) {
-        float acc[TN / 2];
+      if constexpr (OP == kGmPairs) {
+        float acc[kCols];
         for (int k0 = w.k0; k0 < w.k1; k0 += kRound) {
           if (!(ok = ready())) break;
           const uint32_t from = lane_addr + (t & 1) * kAccCols;
 #pragma unroll
-          for (int c = 0; c < TN / 2; c += 32) {
+          for (int c = 0; c < kCols; c += 32) {
             float v[32], x[32];
             tmem_ld32(from + c, v);
             tmem_ld32(from + TN + c, x);
@@ -319,18 +358,21 @@ __global__ void __launch_bounds__(kGmThreads, 1)
           release();
         }
         if (ok)
-          epi.template run<TN>(fixed, state, w, row, half * (TN / 2), GmFromRegs<TN / 2>{acc});
+          epi.template run<TN>(fixed, state, w, row, col, GmFromRegs<kCols>{acc}, out);
       } else {
         if (!(ok = ready())) break;
-        epi.template run<TN>(fixed, state, w, row, half * (TN / 2),
-                             GmFromTmem{lane_addr + (t & 1) * kAccCols});
+        const uint32_t from = lane_addr + (t & 1) * kAccCols;
+        if constexpr (OP == kGmPairs1)
+          epi.template run<TN>(fixed, state, w, row, col, GmFromPairs{from, from + TN}, out);
+        else
+          epi.template run<TN>(fixed, state, w, row, col, GmFromTmem{from}, out);
         release();
       }
     }
   }
   __syncwarp();
   __syncthreads();
-  if (*abort_flag && warp == 9 && lane == 0) {
+  if (*abort_flag && warp == kGmMmaWarp && lane == 0) {
     // products in flight still write TMEM and read shared memory: one more
     // commit completes after all of them
     const uint32_t bar = accempty;  // no role uses it any more
@@ -341,7 +383,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     mbar_wait(bar, 0, s.spin_limit);
   }
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kGmMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(kTmemCols));
