@@ -281,10 +281,16 @@ __device__ __forceinline__ void scores32(const float (&v)[32], f2_t (&t)[16], co
                                          const RowPos &rp) {
   const f2_t su = two(sc.su);
   if (sc.capl > 0.f) {
+    const f2_t capl = two(sc.capl);
+    if (all_small(v, sc.su)) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      t[j] = pk(sc.capl * tanh_step(v[2 * j] * sc.su),
-                sc.capl * tanh_step(v[2 * j + 1] * sc.su));
+      for (int j = 0; j < 16; ++j)
+        t[j] = mul2(capl, tanh_small2(mul2(pk(v[2 * j], v[2 * j + 1]), su)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        t[j] = mul2(capl, tanh2(mul2(pk(v[2 * j], v[2 * j + 1]), su)));
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 16; ++j) t[j] = mul2(pk(v[2 * j], v[2 * j + 1]), su);
@@ -782,7 +788,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs A, int sp
 // The elementwise part of 32 scores of a row, four at a time, all in one pass
 // so that only the scores and dP are held.  `v` raw products, `dp` raw dP; out:
 // dU in dp (and P in v where the rows are keys).
-// CAP, POS, PG: the cap, positions and their gradients are there.
+// CAP: no cap; capped, all products small; capped.  POS, PG: positions and
+// their gradients are there.
+enum AttnCap { kNoCap, kCapSmall, kCapAny };
+template <AttnCap CAP>
+__device__ __forceinline__ f2_t cap_tanh(f2_t u) {
+  return CAP == kCapSmall ? tanh_small2(u) : tanh2(u);
+}
 struct BwdRow {
   AttnScore sc;
   float dps, up;  // of raw dP; of dU
@@ -793,7 +805,7 @@ struct BwdRow {
 struct DqSums {
   f2_t ds = 0, g[4] = {}, q[4] = {};
 };
-template <class Kind, bool CAP, bool POS, bool PG, int R>
+template <class Kind, AttnCap CAP, bool POS, bool PG, int R>
 __device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], const BwdRow &B,
                                             float m, float rl, float delta, unsigned bits,
                                             const TilePos<R> &tp, int c0, DqSums &S) {
@@ -809,8 +821,8 @@ __device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], con
     for (int k = 0; k < 2; ++k) {
       const int e = j + 2 * k;
       f2_t t, th;
-      if (CAP) {
-        th = pk(tanh_step(v[e] * B.sc.su), tanh_step(v[e + 1] * B.sc.su));
+      if (CAP != kNoCap) {
+        th = cap_tanh<CAP>(mul2(pk(v[e], v[e + 1]), su));
         t = fma2(th, two(B.sc.capl), nm);
       } else {
         t = fma2(pk(v[e], v[e + 1]), su, nm);
@@ -832,7 +844,7 @@ __device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], con
         S.g[2] = fma2(ds, d->z[k], S.g[2]), S.q[2] = fma2(p, d->z[k], S.q[2]);
         S.g[3] = fma2(ds, d->r2[k], S.g[3]), S.q[3] = fma2(p, d->r2[k], S.q[3]);
       }
-      if (CAP) ds = mul2(ds, fma2(mul2(th, two(-1.f)), th, two(1.f)));
+      if (CAP != kNoCap) ds = mul2(ds, fma2(mul2(th, two(-1.f)), th, two(1.f)));
       if (!Kind::bf16) ds = mul2(ds, up);
       upk(ds, dp[e], dp[e + 1]);
     }
@@ -843,7 +855,7 @@ template <int R>
 struct TileStat {
   float nm[R], rl[R], nd[R];  // -m, 1 / l, -D
 };
-template <class Kind, bool CAP, bool POS, bool PG, int R>
+template <class Kind, AttnCap CAP, bool POS, bool PG, int R>
 __device__ __forceinline__ void dkv_elements(float (&v)[32], float (&dp)[32], const BwdRow &B,
                                              float p_up, const TileStat<R> &st,
                                              const TilePos<R> &tp, int c0, f2_t (&g)[3]) {
@@ -860,8 +872,8 @@ __device__ __forceinline__ void dkv_elements(float (&v)[32], float (&dp)[32], co
     for (int k = 0; k < 2; ++k) {
       const int e = j + 2 * k;
       f2_t t, th;
-      if (CAP) {
-        th = pk(tanh_step(v[e] * B.sc.su), tanh_step(v[e + 1] * B.sc.su));
+      if (CAP != kNoCap) {
+        th = cap_tanh<CAP>(mul2(pk(v[e], v[e + 1]), su));
         t = fma2(th, two(B.sc.capl), k ? nm.y : nm.x);
       } else {
         t = fma2(pk(v[e], v[e + 1]), su, k ? nm.y : nm.x);
@@ -876,7 +888,7 @@ __device__ __forceinline__ void dkv_elements(float (&v)[32], float (&dp)[32], co
         g[1] = fma2(ds, d->y[k], g[1]);
         g[2] = fma2(ds, d->z[k], g[2]);
       }
-      if (CAP) ds = mul2(ds, fma2(mul2(th, two(-1.f)), th, two(1.f)));
+      if (CAP != kNoCap) ds = mul2(ds, fma2(mul2(th, two(-1.f)), th, two(1.f)));
       if (!Kind::bf16) {
         ds = mul2(ds, up);
         p = mul2(p, two(p_up));
@@ -1023,15 +1035,16 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     const unsigned bits = live ? kval[2 * pb + part] : 0u;
 #define RA_DQ(C, P, G)                                                                       \
   dq_elements<Kind, C, P, G>(v, dp, B, st.x, st.y, delta, bits, kpos[pb], 32 * part, S)
-    if (B.sc.capl > 0.f) {
-      if (pos_grad) RA_DQ(true, true, true);
-      else if (A.pos_dim > 0) RA_DQ(true, true, false);
-      else RA_DQ(true, false, false);
-    } else {
-      if (pos_grad) RA_DQ(false, true, true);
-      else if (A.pos_dim > 0) RA_DQ(false, true, false);
-      else RA_DQ(false, false, false);
-    }
+#define RA_DQ_POS(C)                             \
+  do {                                           \
+    if (pos_grad) RA_DQ(C, true, true);          \
+    else if (A.pos_dim > 0) RA_DQ(C, true, false); \
+    else RA_DQ(C, false, false);                 \
+  } while (0)
+    if (!(B.sc.capl > 0.f)) RA_DQ_POS(kNoCap);
+    else if (all_small(v, B.sc.su)) RA_DQ_POS(kCapSmall);
+    else RA_DQ_POS(kCapAny);
+#undef RA_DQ_POS
 #undef RA_DQ
     put_weights<Kind>(tS + lane_off + 32 * part, dp, Kind::pair);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -1258,15 +1271,16 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     tmem_ld32(tP + lane_off + 32 * part, dp);
 #define RA_DKV(C, P, G) \
   dkv_elements<Kind, C, P, G>(v, dp, B, kUp, qst[pb], qpos[pb], 32 * part, g)
-    if (B.sc.capl > 0.f) {
-      if (pos_grad) RA_DKV(true, true, true);
-      else if (A.pos_dim > 0) RA_DKV(true, true, false);
-      else RA_DKV(true, false, false);
-    } else {
-      if (pos_grad) RA_DKV(false, true, true);
-      else if (A.pos_dim > 0) RA_DKV(false, true, false);
-      else RA_DKV(false, false, false);
-    }
+#define RA_DKV_POS(C)                             \
+  do {                                           \
+    if (pos_grad) RA_DKV(C, true, true);          \
+    else if (A.pos_dim > 0) RA_DKV(C, true, false); \
+    else RA_DKV(C, false, false);                 \
+  } while (0)
+    if (!(B.sc.capl > 0.f)) RA_DKV_POS(kNoCap);
+    else if (all_small(v, B.sc.su)) RA_DKV_POS(kCapSmall);
+    else RA_DKV_POS(kCapAny);
+#undef RA_DKV_POS
 #undef RA_DKV
     put_weights<Kind>(tS + lane_off + 32 * part, v, Kind::pair);
     put_weights<Kind>(tP + lane_off + 32 * part, dp, Kind::pair);

@@ -134,8 +134,16 @@ struct CeEpiLse {
       src.get(c, v);
       const int64_t left = vocab - (c0 + c);
       if (F.capl > 0.f) {
+        const f2_t capl = pk(F.capl, F.capl);
+        if (all_small(v, F.f)) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = F.capl * tanh_step(v[j] * F.f);
+          for (int j = 0; j < 32; j += 2)
+            upk(mul2(capl, tanh_small2(mul2(pk(v[j], v[j + 1]), f2))), v[j], v[j + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2)
+            upk(mul2(capl, tanh2(mul2(pk(v[j], v[j + 1]), f2))), v[j], v[j + 1]);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 32; j += 2) upk(mul2(pk(v[j], v[j + 1]), f2), v[j], v[j + 1]);
@@ -348,12 +356,20 @@ struct CeEpiGrad {
       const int64_t at = R.target - (c0 + c);
       const bool hit = at >= 0 && at < 32;
       if (F.lg.capl > 0.f) {
+        const f2_t capl = pk(F.lg.capl, F.lg.capl), one = pk(1.f, 1.f), neg = pk(-1.f, -1.f);
+        const bool small = all_small(v, F.lg.f);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float th = tanh_step(v[j] * F.lg.f);
-          float g = ex2(fmaf(th, F.lg.capl, m)) * cp;
-          if (hit && j == (int)at) g -= gl;
-          v[j] = g * fmaf(-th, th, 1.f);
+        for (int j = 0; j < 32; j += 2) {
+          const f2_t u = mul2(pk(v[j], v[j + 1]), f2);
+          const f2_t th = small ? tanh_small2(u) : tanh2(u);
+          float x, y;
+          upk(fma2(th, capl, nm), x, y);
+          f2_t g = mul2(pk(ex2(x), ex2(y)), pc);
+          if (hit) {
+            upk(g, x, y);
+            g = pk(j == (int)at ? x - gl : x, j + 1 == (int)at ? y - gl : y);
+          }
+          upk(mul2(g, fma2(mul2(th, neg), th, one)), v[j], v[j + 1]);
         }
       } else {
 #pragma unroll

@@ -76,23 +76,44 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// tanh to about a step: below 0.6 the quotient that the continued fraction
-// u / (1 + u^2 / (3 + u^2 / (5 + u^2 / (7 + u^2 / 9)))) comes to (off by less
-// than 3e-9 there), above 1 - 2 / (1 + e^(2u)).  Straight-line, where tanhf
-// branches.
-__device__ __forceinline__ float tanh_step(float u) {
-  const float x = u * u;
-  const float num = fmaf(x, x + 105.f, 945.f) * u;
-  const float den = fmaf(x, fmaf(x, 15.f, 420.f), 945.f);
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(den));
-  float q = num * r;
-  q = fmaf(fmaf(-q, den, num), r, q);
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u * 2.885390081777927f));
-  float s;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
-  return fabsf(u) < 0.6f ? q : fmaf(-2.f, s, 1.f);
+// tanh(u) for |u| < kTanhSmall, two at a time, to about a step (7e-8 relative):
+// u + u x P(x) with x = u^2, P the polynomial of degree 5 that has the least
+// largest relative error there (weighted least squares on Chebyshev nodes,
+// reweighted towards the largest error; 7e-10 before rounding).  No EX2 and no
+// reciprocal: the units for those are what binds the capped softmaxes.
+constexpr float kTanhSmall = 0.7f;
+__device__ __forceinline__ f2_t tanh_small2(f2_t u) {
+  const f2_t x = mul2(u, u);
+  f2_t p = pk(1.895663794e-3f, 1.895663794e-3f);
+  p = fma2(p, x, pk(-7.883305662e-3f, -7.883305662e-3f));
+  p = fma2(p, x, pk(2.157105878e-2f, 2.157105878e-2f));
+  p = fma2(p, x, pk(-5.392095447e-2f, -5.392095447e-2f));
+  p = fma2(p, x, pk(1.333298385e-1f, 1.333298385e-1f));
+  p = fma2(p, x, pk(-3.333332539e-1f, -3.333332539e-1f));
+  return fma2(mul2(p, x), u, u);
+}
+// any u: the same, or 1 - 2 / (1 + e^(2u)) (2e-7 relative).  Straight-line,
+// where tanhf branches.
+__device__ __forceinline__ f2_t tanh2(f2_t u) {
+  float a, b, x, y;
+  upk(tanh_small2(u), a, b);
+  upk(u, x, y);
+  float r[2] = {x, y};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float s;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + ex2(r[k] * 2.885390081777927f)));
+    r[k] = fmaf(-2.f, s, 1.f);
+  }
+  return pk(fabsf(x) < kTanhSmall ? a : r[0], fabsf(y) < kTanhSmall ? b : r[1]);
+}
+__device__ __forceinline__ float tanh_step(float u) { return lo_of(tanh2(pk(u, u))); }
+// whether 32 products, times f, are all small
+__device__ __forceinline__ bool all_small(const float (&v)[32], float f) {
+  float m[2] = {fabsf(v[0]), fabsf(v[1])};
+#pragma unroll
+  for (int j = 2; j < 32; ++j) m[j & 1] = fmaxf(m[j & 1], fabsf(v[j]));
+  return fmaxf(m[0], m[1]) * fabsf(f) < kTanhSmall;  // a NaN counts as small, and stays one
 }
 
 // The bits of one value as another type of the same size.
