@@ -230,15 +230,18 @@ bool operands(const ra_attn_desc *d, const ra_attn_inputs *in, char *state, Attn
          map_operand(d, &x->v, state + s.vh, state + s.vl, d->num_k, d->kv_heads, kr, d->dim);
 }
 
-template <class K>
-int launch(K kernel, int64_t grid, int threads, int smem, const AttnArgs &a, const AttnTcArgs &x,
+template <auto kernel>
+int launch(int64_t grid, int threads, int smem, const AttnArgs &a, const AttnTcArgs &x,
            cudaStream_t st) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-      cudaSuccess)
-    return RA_ERR_CUDA;
   // as much shared memory as there is: the CTAs of an SM hide each other's waits
-  cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                       cudaSharedmemCarveoutMaxShared);
+  static OncePerDevice once;
+  if (!once([&] {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+                   cudaSuccess &&
+               cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared) == cudaSuccess;
+      }))
+    return RA_ERR_CUDA;
   if (grid > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
   if (grid < 1) return RA_OK;
   kernel<<<(unsigned)grid, threads, smem, st>>>(a, x);
@@ -247,17 +250,17 @@ int launch(K kernel, int64_t grid, int threads, int smem, const AttnArgs &a, con
 
 template <class Kind, int DP>
 int tc_forward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
-  return launch(attn_tc_fwd_kernel<Kind, DP>, a.n_q_tiles * a.heads * x.splits, 128,
+  return launch<attn_tc_fwd_kernel<Kind, DP>>(a.n_q_tiles * a.heads * x.splits, 128,
                 FwdCfg<Kind, DP>::smem, a, x, st);
 }
 template <class Kind, int DP>
 int tc_backward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
   int rc = RA_OK;
   if (a.dq || a.pos_q || a.dk)  // dk reads the D that this kernel puts right
-    rc = launch(attn_tc_dq_kernel<Kind, DP>, a.n_q_tiles * a.heads, DqCfg<Kind, DP>::NT,
+    rc = launch<attn_tc_dq_kernel<Kind, DP>>(a.n_q_tiles * a.heads, DqCfg<Kind, DP>::NT,
                 DqCfg<Kind, DP>::smem, a, x, st);
   if (!rc && (a.dk || a.dv || a.pos_k))
-    rc = launch(attn_tc_dkv_kernel<Kind, DP>, a.n_k_tiles * a.kv_heads, DkvCfg<Kind, DP>::NT,
+    rc = launch<attn_tc_dkv_kernel<Kind, DP>>(a.n_k_tiles * a.kv_heads, DkvCfg<Kind, DP>::NT,
                 DkvCfg<Kind, DP>::smem, a, x, st);
   return rc;
 }

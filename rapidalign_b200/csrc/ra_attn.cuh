@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 
 #include "ra_common.cuh"
+#include "ra_few.cuh"
 
 namespace ra {
 
@@ -85,20 +86,6 @@ struct AttnArgs {
   }
 };
 
-template <class T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f<float>(float v) {
-  return v;
-}
-template <>
-__device__ __forceinline__ float to_f<__half>(__half v) {
-  return __half2float(v);
-}
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) {
-  return __bfloat162float(v);
-}
 __device__ __forceinline__ void put(float *p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }

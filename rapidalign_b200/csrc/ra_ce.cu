@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "ra_ce.cuh"
+#include "ra_ce_few.cuh"
 #include "ra_host.h"
 #include "ra_tmap.h"
 
@@ -28,6 +29,17 @@ bool ce_ok(const ra_ce_desc *d) {
 
 int pad8(int n) { return (n + 7) & ~7; }
 
+// A few rows: bound by the table's bytes (ra_ce_few.cuh).  Whole eights of
+// columns, and x in shared memory.
+bool use_few(const ra_ce_desc *d) {
+  return d->rows <= kCeFewRows && d->dim % 8 == 0 &&
+         (size_t)d->rows * d->dim * 4 <= kCeFewSmem;
+}
+// its 16-byte loads of the table
+bool few_aligned(const ra_ce_desc *d, const void *w) {
+  return d->dtype != RA_F32 || (((uintptr_t)w & 15) == 0 && d->ld_w % 4 == 0);
+}
+
 struct CeState {
   size_t stats, xh, xl, wh, wl, total;
 };
@@ -50,14 +62,15 @@ CeState ce_state(const ra_ce_desc *d) {
 }
 
 // Width of the tiles over n columns: 256 unless half of a last tile or of
-// the last wave of CTAs would idle; 128 for pairs (TMEM).
+// the last wave of CTAs would idle; 128 for pairs (TMEM).  One row of tiles
+// reads the table once and is bound by its bytes: any better fit counts.
 int tile_width(int64_t m_tiles, int64_t n, int sms, bool pairs) {
   if (pairs) return 128;
   auto waves = [&](int tn) {
     const int64_t t = m_tiles * ceil_div(n, (int64_t)tn);
     return (double)(ceil_div(t, (int64_t)sms) * tn);
   };
-  return waves(128) < 0.85 * waves(256) ? 128 : 256;
+  return waves(128) < (m_tiles == 1 ? 1.0 : 0.85) * waves(256) ? 128 : 256;
 }
 
 // K slices that fill the SMs when there are few tiles, each at least four
@@ -73,6 +86,7 @@ struct CePlan {
   int sms, elem;
   int64_t mt;             // 128-row tiles of x
   int tn_z, parts;        // forward
+  int few_ctas;
   int64_t piece, ldg;     // vocabulary piece (columns of du)
   int64_t pieces;
   int tn_d;               // tiles over the embedding width
@@ -91,13 +105,15 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   const int64_t pass = std::min<int64_t>(d->rows, kCeRowsPerPass);
   p.tn_z = tile_width(ceil_div(pass, (int64_t)kGmM), d->vocab, sms, split);
   p.parts = kGmParts * (int)ceil_div(d->vocab, (int64_t)p.tn_z);
+  p.few_ctas = (int)std::min<int64_t>(ceil_div(d->vocab, (int64_t)kCeFewWarps * kCeFewTable), 2 * sms);
   size_t o = 0;
   p.f_part = o;
   o += align256(sizeof(float2) * (size_t)p.parts * (size_t)(ceil_div(pass, (int64_t)kGmM) * kGmM));
+  o += align256(sizeof(float2) * (size_t)p.few_ctas * kCeFewRows);
   p.f_zt = o;
   o += align256(sizeof(float) * (size_t)d->rows);
   p.f_blocks = o;
-  o += align256(sizeof(double2) * (size_t)ceil_div(d->rows, (int64_t)32));
+  o += align256(sizeof(double2) * (size_t)ceil_div(d->rows, (int64_t)8));
   p.f_total = o;
 
   const int64_t rows_pad = p.mt * kGmM;
@@ -135,8 +151,11 @@ template <int TN, bool BF16, GmOp OP, bool A_MN, bool B_MN, class Epi>
 int launch_gemm(const GmMaps &maps, const GmShape &s, const Epi &epi, int sms, cudaStream_t st) {
   const size_t smem = kGmSmem;
   auto k = gemm16_kernel<TN, BF16, OP, A_MN, B_MN, Epi>;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess)
+  static OncePerDevice once;
+  if (!once([&] {
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) ==
+               cudaSuccess;
+      }))
     return RA_ERR_CUDA;
   const int64_t units = (int64_t)s.m_tiles * s.n_tiles * s.slices;
   if (units < 1 || units > (int64_t)0x7ff00000) return RA_ERR_INVALID_ARGUMENT;
@@ -197,6 +216,79 @@ GmShape shape_of(const ra_ce_desc *d, const CePlan &p, int64_t mt, int64_t nt, i
                  int m_fast) {
   return {(int)mt, (int)nt, (int)ceil_div(k, (int64_t)kGmK), slices, m_fast,
           kTcSpinLimit, d->status};
+}
+
+// fp32 inputs as pairs of halves, in the state
+int halves(const ra_ce_desc *d, const CePlan &p, const void *x, const void *w, char *sb,
+           cudaStream_t st) {
+  const CeState sl = ce_state(d);
+  CeHead *head = (CeHead *)sb;
+  const CeMatrix mx{(const float *)x, d->rows, d->ld_x, d->dim, &head->amax_x,
+                    (__half *)(sb + sl.xh), (__half *)(sb + sl.xl)};
+  const CeMatrix mw{(const float *)w, d->vocab, d->ld_w, d->dim, &head->amax_w,
+                    (__half *)(sb + sl.wh), (__half *)(sb + sl.wl)};
+  const dim3 grid(grid_for(std::max(d->rows, d->vocab) * (pad8(d->dim) / 8), p.sms), 2);
+  ce_amax_kernel<<<grid, 256, 0, st>>>(mx, mw);
+  int rc = launched();
+  if (rc) return rc;
+  ce_split_kernel<<<grid, 256, 0, st>>>(mx, mw);
+  return launched();
+}
+
+template <class T, int N>
+int few_launch(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w, const int64_t *target,
+               char *ws, cudaStream_t st) {
+  auto k = ce_few_kernel<T, N>;
+  static OncePerDevice once;
+  if (!once([&] {
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)kCeFewSmem) == cudaSuccess;
+      }))
+    return RA_ERR_CUDA;
+  k<<<(unsigned)p.few_ctas, 32 * kCeFewWarps, (size_t)N * d->dim * 4, st>>>(
+      x, d->ld_x, w, d->ld_w, (int)d->rows, d->vocab, d->dim, d->scale, d->softcap, target,
+      (float2 *)(ws + p.f_part), (float *)(ws + p.f_zt));
+  return launched();
+}
+template <class T>
+int few_forward(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w,
+                const int64_t *target, char *ws, cudaStream_t st) {
+  switch (d->rows) {
+    case 1: return few_launch<T, 1>(d, p, x, w, target, ws, st);
+    case 2: return few_launch<T, 2>(d, p, x, w, target, ws, st);
+    case 3: return few_launch<T, 3>(d, p, x, w, target, ws, st);
+    case 4: return few_launch<T, 4>(d, p, x, w, target, ws, st);
+    case 5: return few_launch<T, 5>(d, p, x, w, target, ws, st);
+    case 6: return few_launch<T, 6>(d, p, x, w, target, ws, st);
+    case 7: return few_launch<T, 7>(d, p, x, w, target, ws, st);
+    default: return few_launch<T, 8>(d, p, x, w, target, ws, st);
+  }
+}
+
+// The rows' losses from their parts.  Many rows: 8 threads a row in CTAs of 256
+// (65537 rows of 132 parts: ROWS1 us, with 32 threads a row 65 us); few: all of
+// 1024 threads on 8 rows.
+int join_rows(const ra_ce_desc *d, const float2 *part, int64_t ld, int parts, int64_t r0,
+              int64_t rows, const int64_t *target, float *loss, float *lse, char *sb, char *ws,
+              const CePlan &p, cudaStream_t st) {
+  const CeState sl = ce_state(d);
+  CeHead *head = (CeHead *)sb;
+  const float *zt = (const float *)(ws + p.f_zt);
+  float2 *stats = (float2 *)(sb + sl.stats);
+  double2 *blocks = (double2 *)(ws + p.f_blocks);
+  if (d->rows <= 8)
+    ce_rows_kernel<8, 128><<<1, 1024, 0, st>>>(part, ld, parts, r0, rows, d->rows, d->vocab, target,
+                                               d->ignore_index, zt, d->reduction, loss, lse, stats,
+                                               head, blocks);
+  else if (d->rows <= 4096)
+    ce_rows_kernel<32, 32><<<(unsigned)ceil_div(rows, (int64_t)32), 1024, 0, st>>>(
+        part, ld, parts, r0, rows, d->rows, d->vocab, target, d->ignore_index, zt, d->reduction,
+        loss, lse, stats, head, blocks);
+  else
+    ce_rows_kernel<32, 8><<<(unsigned)ceil_div(rows, (int64_t)32), 256, 0, st>>>(
+        part, ld, parts, r0, rows, d->rows, d->vocab, target, d->ignore_index, zt, d->reduction,
+        loss, lse, stats, head, blocks);
+  return launched();
 }
 
 template <class T, bool BF16, bool SPLIT>
@@ -297,21 +389,17 @@ int ra_ce_forward(const ra_ce_desc *d, const void *x, const void *w, const int64
                ? RA_OK
                : RA_ERR_CUDA;
   }
-  if (d->dtype == RA_F32) {
-    const int ldp = pad8(d->dim);
-    const float *src[2] = {(const float *)x, (const float *)w};
-    const int64_t n[2] = {d->rows, d->vocab}, ld[2] = {d->ld_x, d->ld_w};
-    unsigned *word[2] = {&head->amax_x, &head->amax_w};
-    const size_t hi[2] = {sl.xh, sl.wh}, lo[2] = {sl.xl, sl.wl};
-    for (int k = 0; k < 2; ++k) {
-      ce_amax_kernel<<<grid_for(n[k] * d->dim, p.sms), 256, 0, st>>>(src[k], n[k], d->dim, ld[k],
-                                                                     word[k]);
-      if ((rc = launched())) return rc;
-      ce_split_kernel<<<grid_for(n[k] * ldp, p.sms), 256, 0, st>>>(
-          src[k], n[k], d->dim, ld[k], ldp, word[k], (__half *)(sb + hi[k]), (__half *)(sb + lo[k]));
-      if ((rc = launched())) return rc;
-    }
+  const bool few = use_few(d) && few_aligned(d, w);
+  if (few) {
+    rc = d->dtype == RA_F32 ? few_forward(d, p, (const float *)x, (const float *)w, target, ws, st)
+         : d->dtype == RA_BF16
+             ? few_forward(d, p, (const __nv_bfloat16 *)x, (const __nv_bfloat16 *)w, target, ws, st)
+             : few_forward(d, p, (const __half *)x, (const __half *)w, target, ws, st);
+    if (rc) return rc;
+    return join_rows(d, (const float2 *)(ws + p.f_part), kCeFewRows, p.few_ctas, 0, d->rows, target,
+                     loss, lse, sb, ws, p, st);
   }
+  if (d->dtype == RA_F32 && (rc = halves(d, p, x, w, sb, st))) return rc;
   const bool bf16 = d->dtype == RA_BF16;
   const Operands op = operands(d, x, w, sb);
   float2 *part = (float2 *)(ws + p.f_part);
@@ -335,10 +423,8 @@ int ra_ce_forward(const ra_ce_desc *d, const void *x, const void *w, const int64
                 : launch_gemm<false, false, false, false>(p.tn_z, m, s, e, p.sms, st);
     }
     if (rc) return rc;
-    ce_rows_kernel<<<(unsigned)ceil_div(rows, (int64_t)32), 1024, 0, st>>>(
-        part, mt * kGmM, p.parts, r0, rows, d->rows, d->vocab, target, d->ignore_index, zt,
-        d->reduction, loss, lse, (float2 *)(sb + sl.stats), head, (double2 *)(ws + p.f_blocks));
-    if ((rc = launched())) return rc;
+    rc = join_rows(d, part, mt * kGmM, p.parts, r0, rows, target, loss, lse, sb, ws, p, st);
+    if (rc) return rc;
   }
   return RA_OK;
 }
@@ -373,6 +459,9 @@ int ra_ce_backward(const ra_ce_desc *d, const void *x, const void *w, const int6
                                                            g_lse, head, (float2 *)(ws + p.b_coef));
   int rc;
   if ((rc = launched())) return rc;
+  // the forward of a few rows made no halves
+  if (d->dtype == RA_F32 && use_few(d) && few_aligned(d, w) && (rc = halves(d, p, x, w, sb, st)))
+    return rc;
   const Operands op = operands(d, x, w, sb);
   if (d->dtype == RA_F32)
     return backward<float, false, true>(d, p, op, target, (float *)dx, (float *)dw, sb, ws, st);

@@ -56,37 +56,80 @@ __device__ __forceinline__ unsigned finite_bits(float v) {
   return b < 0x7f800000u ? b : 0u;
 }
 
-// largest finite |a| of a [rows, cols] fp32 matrix into *word
-__global__ void __launch_bounds__(256) ce_amax_kernel(const float *a, int64_t rows, int cols,
-                                                      int64_t ld, unsigned *word) {
+// Eight columns of a row of an fp32 matrix, zeros behind its last; `wide`: rows
+// of 16-byte aligned addresses and whole eights.
+__device__ __forceinline__ void ce_load8(const float *a, int64_t ld, int cols, int64_t r, int c,
+                                         bool wide, float (&v)[8]) {
+  const float *p = a + r * ld + c;
+  if (wide) {
+    const float4 x = __ldg(reinterpret_cast<const float4 *>(p));
+    const float4 y = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? p[k] : 0.f;
+  }
+}
+struct CeMatrix {
+  const float *a;
+  int64_t rows, ld;
+  int cols;
+  unsigned *word;
+  __half *hi, *lo;  // [rows, 8 eights]
+  __device__ __forceinline__ bool wide() const {
+    return ((uintptr_t)a & 15) == 0 && (ld & 3) == 0 && (cols & 7) == 0;
+  }
+};
+
+// largest finite |a| of x (blockIdx.y = 0) and w into their words
+__global__ void __launch_bounds__(256) ce_amax_kernel(const CeMatrix x, const CeMatrix w) {
+  const CeMatrix &m = blockIdx.y ? w : x;
+  const int eights = (m.cols + 7) >> 3;
+  const bool wide = m.wide();
   unsigned best = 0;
-  const int64_t n = rows * cols;
+  const int64_t n = m.rows * eights;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / cols;
-    const unsigned b = finite_bits(a[r * ld + (i - r * cols)]);
-    best = b > best ? b : best;
+    const int64_t r = n < ((int64_t)1 << 31) ? (unsigned)i / (unsigned)eights : i / eights;
+    float v[8];
+    ce_load8(m.a, m.ld, m.cols, r, (int)(i - r * eights) * 8, wide, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const unsigned b = finite_bits(v[k]);
+      best = b > best ? b : best;
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned b = __shfl_xor_sync(kFull, best, o);
     best = b > best ? b : best;
   }
-  if ((threadIdx.x & 31) == 0 && best) atomicMax(word, best);  // a maximum: any order
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(m.word, best);  // a maximum: any order
 }
 
-// a 2^e = hi + lo in fp16, rows padded to ldp with zeros
-__global__ void __launch_bounds__(256) ce_split_kernel(const float *a, int64_t rows, int cols,
-                                                       int64_t ld, int ldp, const unsigned *word,
-                                                       __half *hi, __half *lo) {
-  const float sc = ce_pow2(ce_exp(*word));
-  const int64_t n = rows * ldp;
+// a 2^e = hi + lo in fp16, rows padded with zeros to whole eights
+__global__ void __launch_bounds__(256) ce_split_kernel(const CeMatrix x, const CeMatrix w) {
+  const CeMatrix &m = blockIdx.y ? w : x;
+  const int eights = (m.cols + 7) >> 3;
+  const bool wide = m.wide();
+  const float sc = ce_pow2(ce_exp(*m.word));
+  const int64_t n = m.rows * eights;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / ldp;
-    const int c = (int)(i - r * ldp);
-    const float v = c < cols ? a[r * ld + c] * sc : 0.f;
-    const __half h = __float2half_rn(v);
-    hi[i] = h;
-    lo[i] = __float2half_rn(v - __half2float(h));
+    const int64_t r = n < ((int64_t)1 << 31) ? (unsigned)i / (unsigned)eights : i / eights;
+    float v[8];
+    ce_load8(m.a, m.ld, m.cols, r, (int)(i - r * eights) * 8, wide, v);
+    __half h[8], l[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float y = v[k] * sc;
+      h[k] = __float2half_rn(y);
+      l[k] = __float2half_rn(y - __half2float(h[k]));
+    }
+    uint4 u;
+    memcpy(&u, h, 16);
+    reinterpret_cast<uint4 *>(m.hi)[i] = u;
+    memcpy(&u, l, 16);
+    reinterpret_cast<uint4 *>(m.lo)[i] = u;
   }
 }
 
@@ -186,46 +229,62 @@ struct CeEpiLse {
   }
 };
 
-// Joins the column tiles of 32 rows of a pass over rows [r0, r0 + pass_rows); losses, lse, the rows' (m, sum) for the
+// Joins the parts of TX rows of a pass over rows [r0, r0 + pass_rows), TY threads
+// a row; losses, lse, the rows' (m, sum) for the
 // backward, and the sum or mean of the losses (block sums in fp64, added in
 // block order by the block that finishes last).
-__global__ void __launch_bounds__(1024) ce_rows_kernel(const float2 *part, int64_t ld, int parts,
-                                                       int64_t r0, int64_t pass_rows,
-                                                       int64_t rows, int64_t vocab,
-                                                       const int64_t *target, int64_t ignore,
-                                                       const float *zt, int reduction,
-                                                       float *loss, float *lse, float2 *stats,
-                                                       CeHead *head, double2 *blocks) {
-  __shared__ float2 sh[32][33];
-  __shared__ double red[32 * 2];
+template <int TX, int TY>
+__global__ void __launch_bounds__(TX * TY) ce_rows_kernel(const float2 *part, int64_t ld, int parts,
+                                                          int64_t r0, int64_t pass_rows,
+                                                          int64_t rows, int64_t vocab,
+                                                          const int64_t *target, int64_t ignore,
+                                                          const float *zt, int reduction,
+                                                          float *loss, float *lse, float2 *stats,
+                                                          CeHead *head, double2 *blocks) {
+  __shared__ float2 sh[TY][TX + 1];
+  __shared__ double red[TX * TY / 32 * 2];
   __shared__ bool last;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t in_pass = blockIdx.x * (int64_t)32 + tx, r = r0 + in_pass;
-  const unsigned all_blocks = (unsigned)ceil_div(rows, (int64_t)32);
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const int64_t in_pass = blockIdx.x * (int64_t)TX + tx, r = r0 + in_pass;
+  const unsigned all_blocks = (unsigned)ceil_div(rows, (int64_t)TX);
   float m = -INFINITY, s = 0.f;
   if (in_pass < pass_rows) {
-    for (int p = ty; p < parts; p += 32) {
-      const float2 v = part[p * ld + in_pass];
-      const float mn = fmaxf(m, v.x);
-      if (mn > -INFINITY || v.y != v.y) {
-        s = (m > -INFINITY ? s * ex2(m - mn) : 0.f) + v.y * (v.x > -INFINITY ? ex2(v.x - mn) : 1.f);
-        m = mn;
+    for (int p = ty; p < parts; p += TY * 8) {  // eight loads in flight
+      float2 v[8];
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = p + TY * k < parts ? part[(int64_t)(p + TY * k) * ld + in_pass]
+                                  : make_float2(-INFINITY, 0.f);
+        mn = fmaxf(mn, v[k].x);
       }
+      // no finite maximum yet: the sums are 0, or NaN
+      const float ref = mn > -INFINITY ? mn : 0.f;
+      s *= m > -INFINITY ? ex2(m - ref) : 1.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fmaf(v[k].y, v[k].x > -INFINITY ? ex2(v[k].x - ref) : 1.f, s);
+      m = mn;
     }
   }
   sh[ty][tx] = make_float2(m, s);
   __syncthreads();
-  if (ty == 0) {
+  // the first warp: 32 / TX threads a row, in order
+  if (threadIdx.x < 32) {
+    constexpr int kSide = 32 / TX;
+    float M = -INFINITY;
+    for (int k = ty; k < TY; k += kSide) M = fmaxf(M, sh[k][tx].x);
+#pragma unroll
+    for (int o = TX; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, o));
+    float S = 0.f;
+    for (int k = ty; k < TY; k += kSide) {
+      const float2 v = sh[k][tx];
+      S += v.x > -INFINITY ? v.y * ex2(v.x - M) : v.y;
+    }
+#pragma unroll
+    for (int o = TX; o < 32; o <<= 1) S += __shfl_xor_sync(kFull, S, o);
     double row_loss = 0.0;
     long long labelled = 0;
-    if (in_pass < pass_rows) {
-      float M = -INFINITY;
-      for (int k = 0; k < 32; ++k) M = fmaxf(M, sh[k][tx].x);
-      float S = 0.f;
-      for (int k = 0; k < 32; ++k) {
-        const float2 v = sh[k][tx];
-        S += v.x > -INFINITY ? v.y * ex2(v.x - M) : v.y;
-      }
+    if (ty == 0 && in_pass < pass_rows) {
       const double l = (double)M * kLn2 + log((double)S);
       const int64_t t = target[r];
       if (t != ignore) {
@@ -240,8 +299,8 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2 *part, int64
     if (reduction != RA_REDUCE_NONE) {
       const double sum = warp_sum(row_loss);
       const double cnt = warp_sum((double)labelled);
-      if (tx == 0) {
-        blocks[r0 / 32 + blockIdx.x] = make_double2(sum, cnt);
+      if (threadIdx.x == 0) {
+        blocks[r0 / TX + blockIdx.x] = make_double2(sum, cnt);
         __threadfence();
         last = atomicAdd(&head->ticket, 1u) == all_blocks - 1;
       }
@@ -252,7 +311,7 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2 *part, int64
   if (!last) return;
   __threadfence();
   double acc[2] = {0.0, 0.0};
-  for (int64_t b = threadIdx.x; b < all_blocks; b += 1024) {
+  for (int64_t b = threadIdx.x; b < all_blocks; b += TX * TY) {
     const double2 v = __ldcg(blocks + b);
     acc[0] += v.x;
     acc[1] += v.y;

@@ -20,6 +20,20 @@ inline int sm_count() {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms > 0 ? sms : 1;
 }
+// Something that is done once for each device (a kernel's attributes).  Doing
+// it twice, from two threads at once, does no harm.
+struct OncePerDevice {
+  std::atomic<unsigned long long> done{0};  // devices 0 .. 63
+  template <class F>
+  bool operator()(F f) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    if (dev < 64 && (done.load() >> dev & 1)) return true;
+    if (!f()) return false;
+    if (dev < 64) done.fetch_or(1ull << dev);
+    return true;
+  }
+};
 inline int launched() {
   ++g_launches;
   return cudaGetLastError() == cudaSuccess ? RA_OK : RA_ERR_CUDA;

@@ -139,6 +139,24 @@ def test_sizes(n, v, d, dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 8, 9])
+@pytest.mark.parametrize("v,d", [(3, 8), (1000, 264), (2049, 1024), (70, 2048), (70, 2056)])
+def test_few_rows(n, v, d, dtype, cuda_device):
+    x, w, t = make(n, v, d, dtype, seed=n + d)
+    check(x, w, t, lse_weight=0.5)
+    if n > 2:
+        t[1] = v  # outside the table
+        t[2] = IGN
+        loss, lse = ra.linear_cross_entropy(x, w, t, reduction="none", softcap=3.0)
+        assert torch.isnan(loss[1]) and loss[2] == 0 and torch.isfinite(lse).all()
+    t[:] = torch.arange(n, device="cuda") % v
+    check(x, w, t, reduction="none", cap=4.0, scale=2.0)
+    x[-1, 0] = math.nan
+    loss, lse = ra.linear_cross_entropy(x, w, t, reduction="none")
+    assert torch.isnan(loss[-1]) and torch.isfinite(loss[:-1]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("cap,scale", [(0.0, 1.7), (5.0, 1.0), (30.0, -2.0)])
 def test_cap_scale_reduction(dtype, reduction, cap, scale, cuda_device):
@@ -205,7 +223,8 @@ def test_no_rows(cuda_device):
     for reduction, want in (("mean", math.nan), ("sum", 0.0)):
         loss, lse = ra.linear_cross_entropy(x, w, t, reduction=reduction)
         assert lse.shape == (0,)
-        assert math.isnan(float(loss)) if math.isnan(want) else float(loss) == want
+        got = float(loss.detach())
+        assert math.isnan(got) if math.isnan(want) else got == want
     dx, dw = torch.autograd.grad(loss, [x, w])
     assert dx.shape == (0, 8) and not dw.any()
     loss, _ = ra.linear_cross_entropy(x, w, t, reduction="none")
