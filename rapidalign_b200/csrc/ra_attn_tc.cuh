@@ -521,6 +521,9 @@ struct FwdCfg {
   static constexpr int CTAS = smem <= 56 * 1024 ? 4 : smem <= 113 * 1024 ? 2 : 1;
 };
 
+// Work for one thread, on warps of their own: issuing a tile's products takes
+// 200 to 1,400 cycles, its copies 500, and warps 0 and 1 fetch the rows.
+constexpr int kMmaThread = 64, kTmaThread = 96;
 // This thread's row of the next streamed tile, fetched an iteration ahead.
 struct NextRow {
   AttnPos p;
@@ -619,7 +622,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
   float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to
   unsigned phase = 0;
 
-  if (t0 < t1 && threadIdx.x == 0) {
+  if (t0 < t1 && threadIdx.x == kMmaThread) {
     products_rows<Kind, KT, DP>(tS, sQ, sK + (t0 & 1) * C::KV);
     tc_commit(bar);
   }
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {  // the products on its buffers are done
-      if (threadIdx.x == 0) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread) issue(t + 1, 0);
       fetch(t + 1);
     }
     f2_t s2[KT / 32][16];
@@ -696,7 +699,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == kMmaThread) {
       tc_fence_after();
       products_weighted<Kind, KT, DP, C::SMALL>(tO, tS, sV + b * C::KV, p_pair, t > t0);
       if (t + 1 < t1) products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
@@ -1015,7 +1018,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   const bool pos_grad = A.pos_q != nullptr;
   unsigned phase = 0;
 
-  if (t1 > 0 && threadIdx.x == 0) {
+  if (t1 > 0 && threadIdx.x == kMmaThread) {
     products_rows<Kind, KT, DP>(tS, sQ, sK);
     products_rows<Kind, KT, DP>(tP, sG, sV);
     tc_commit(bar);
@@ -1026,7 +1029,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
-      if (C::STAGES > 1 && threadIdx.x == 0) issue(t + 1, 0);
+      if (C::STAGES > 1 && threadIdx.x == kTmaThread) issue(t + 1, 0);
       fetch(t + 1);
     }
     float v[32], dp[32];
@@ -1054,7 +1057,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == kMmaThread) {
       tc_fence_after();
       products_weighted<Kind, KT, DP, C::SMALL>(tD, tS, sK + b * C::KV, false, t > 0);
       if (C::STAGES > 1 && t + 1 < t1) {
@@ -1066,11 +1069,11 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     if (C::STAGES == 1 && t + 1 < t1) {  // one buffer: its products first
       bad |= !mbar_wait(bar, phase);
       phase ^= 1;
-      if (threadIdx.x == 0) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread) issue(t + 1, 0);
       bad |= !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
-      if (threadIdx.x == 0) {
+      if (threadIdx.x == kMmaThread) {
         tc_fence_after();
         products_rows<Kind, KT, DP>(tS, sQ, sK);
         products_rows<Kind, KT, DP>(tP, sG, sV);
@@ -1236,7 +1239,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   unsigned phase = 0;
   int cur = -1;
 
-  if (t1 > 0 && threadIdx.x == 0) {
+  if (t1 > 0 && threadIdx.x == kMmaThread) {
     products_rows<Kind, QT, DP>(tS, sK, sQ);
     products_rows<Kind, QT, DP>(tP, sV, sG);
     tc_commit(bar);
@@ -1263,7 +1266,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
-      if (C::STAGES > 1 && threadIdx.x == 0) issue(t + 1, 0);
+      if (C::STAGES > 1 && threadIdx.x == kTmaThread) issue(t + 1, 0);
       fetch(t + 1);
     }
     float v[32], dp[32];
@@ -1291,7 +1294,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == kMmaThread) {
       tc_fence_after();
       products_weighted<Kind, QT, DP, C::SMALL>(tDv, tS, sG + b * C::QG, false, t > 0);
       products_weighted<Kind, QT, DP, C::SMALL>(tDk, tP, sQ + b * C::QG, false, t > 0);
@@ -1304,11 +1307,11 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     if (C::STAGES == 1 && t + 1 < t1) {
       bad |= !mbar_wait(bar, phase);
       phase ^= 1;
-      if (threadIdx.x == 0) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread) issue(t + 1, 0);
       bad |= !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
-      if (threadIdx.x == 0) {
+      if (threadIdx.x == kMmaThread) {
         tc_fence_after();
         products_rows<Kind, QT, DP>(tS, sK, sQ);
         products_rows<Kind, QT, DP>(tP, sV, sG);
