@@ -108,32 +108,64 @@ def attention_segments(q_ptr: Optional[Tensor] = None, k_ptr: Optional[Tensor] =
                              info[3], info[8])
 
 
+def _rows(t: Tensor) -> Tensor:
+    """`t` as rows of heads (rows, heads, dim), the leading dimensions of a padded
+    batch as one: unit stride along the head dimension, and for the 16-bit
+    tensor-core kernels (widths that are multiples of 8) 16-byte aligned rows
+    and no broadcast; copied where it is not so.  (Called without autograd: a
+    view for it costs more than a small kernel.)"""
+    if t.dim() == 4:
+        b, n = t.shape[:2]
+        if b != 1 and n != 1 and t.stride(0) != n * t.stride(1):
+            t = t.contiguous()
+        t = t.flatten(0, 1)
+    strides, shape = t.stride(), t.shape
+    ok = strides[2] == 1 or shape[2] == 1
+    if ok and t.dtype != torch.float32 and shape[2] % 8 == 0:
+        ok = t.data_ptr() % 16 == 0 and all(
+            strides[i] % 8 == 0 and (strides[i] > 0 or shape[i] == 1) for i in (0, 1))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _floats(t: Tensor) -> Tensor:
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+
+
 class _KernelAttention(torch.autograd.Function):
-    """(q, k, v, q_pos, k_pos, sigma) -> out; q, k, v as (rows, heads, dim)."""
+    """(q, k, v, q_pos, k_pos, sigma) -> out, for rows of heads or padded
+    batches of them."""
 
     @staticmethod
     def forward(ctx, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap,
                 need_grad):
         lib = _lib.load()
         dev = q.device
+        qr, kr, vr = _rows(q), _rows(k), _rows(v)
         d = _lib.RaAttnDesc()
         (d.graphs, d.num_q, d.num_k, d.max_q, d.max_k) = shape[:5]
         q_ptr, k_ptr, q_tiles, k_tiles = shape[5:]
-        d.q_row, d.q_head = q.stride(0), q.stride(1)
-        d.k_row, d.k_head = k.stride(0), k.stride(1)
-        d.v_row, d.v_head = v.stride(0), v.stride(1)
+        d.q_row, d.q_head = qr.stride()[:2]
+        d.k_row, d.k_head = kr.stride()[:2]
+        d.v_row, d.v_head = vr.stride()[:2]
         if q_ptr is None:
             d.q_tiles = d.graphs * -(-d.max_q // _TILE)
             d.k_tiles = d.graphs * -(-d.max_k // _TILE)
         else:
             d.q_tiles, d.k_tiles = q_tiles.shape[0], k_tiles.shape[0]
-        d.heads, d.dim, d.kv_heads = q.shape[1], q.shape[2], k.shape[1]
-        d.pos_dim = 0 if q_pos is None else q_pos.shape[1]
+        d.heads, d.dim, d.kv_heads = qr.shape[1], qr.shape[2], kr.shape[1]
+        pos = [None, None, None]
+        if q_pos is not None:
+            d.pos_dim = q_pos.shape[-1]
+            sig = sigma.to(device=dev, dtype=torch.float32)
+            if sig.shape != (d.heads,) or not sig.is_contiguous():
+                sig = sig.reshape(-1).expand(d.heads).contiguous()
+            pos = [_floats(q_pos), _floats(k_pos), sig]
         d.dtype, d.scale, d.softcap = _lib.DTYPES[q.dtype], scale, softcap
         d.status = _lib.status_word()
-        inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in (q, k, v, q_ptr, k_ptr, q_tiles, k_tiles,
-                                                        q_pos, k_pos, sigma, q_mask, k_mask)])
-        with torch.cuda.device(dev):
+        tensors = (qr, kr, vr, q_ptr, k_ptr, q_tiles, k_tiles, *pos, q_mask, k_mask)
+        inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in tensors])
+        ref = ctypes.byref(d)
+        with _lib.on_device(dev):
             out = torch.empty(q.shape, dtype=q.dtype, device=dev)
             out32 = stats = None
             if need_grad:
@@ -142,43 +174,58 @@ class _KernelAttention(torch.autograd.Function):
                 if q.dtype != torch.float32:
                     out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
                 stats = torch.empty((2, d.heads, d.num_q), dtype=torch.float32, device=dev)
-            state = _lib.workspace(lib.ra_attn_state_bytes(ctypes.byref(d)), dev)
-            ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 0), dev)
-            rc = lib.ra_attn_forward(ctypes.byref(d), ctypes.byref(inp), out.data_ptr(),
-                                     _lib.ptr(out32), _lib.ptr(stats), state.data_ptr(),
-                                     state.numel(), ws.data_ptr(), ws.numel(),
-                                     _lib.stream_handle(dev))
+            n_state, n_ws = lib.ra_attn_state_bytes(ref), lib.ra_attn_workspace_bytes(ref, 0)
+            # a small workspace lies behind the state
+            state = _lib.scratch(n_state + (n_ws if n_ws <= 256 else 0), dev)
+            ws = None if n_ws <= 256 else _lib.scratch(n_ws, dev)
+            rc = lib.ra_attn_forward(ref, ctypes.byref(inp), out.data_ptr(), _lib.ptr(out32),
+                                     _lib.ptr(stats), state.data_ptr(), n_state,
+                                     state.data_ptr() + n_state if ws is None else ws.data_ptr(),
+                                     n_ws, _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention")
         if need_grad:
-            ctx.desc, ctx.state, ctx.layout = d, state, (q_ptr, k_ptr, q_tiles, k_tiles)
+            ctx.desc, ctx.state, ctx.inp = d, state, inp
             ctx.save_for_backward(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask,
                                   out if out32 is None else out32, stats)
+            # what the pointers of `inp` belong to, where it is not saved above
+            ctx.keep = (*[None if t is o or t.data_ptr() == o.data_ptr() else t
+                          for t, o in ((qr, q), (kr, k), (vr, v))],
+                        pos, q_ptr, k_ptr, q_tiles, k_tiles)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         lib = _lib.load()
-        q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, out32, stats = ctx.saved_tensors
+        q, k, v, q_pos, k_pos, sigma, _, _, out32, stats = ctx.saved_tensors
         d, dev = ctx.desc, q.device
-        inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in (q, k, v, *ctx.layout, q_pos, k_pos, sigma,
-                                                        q_mask, k_mask)])
         g = g.contiguous()
         if g.data_ptr() % 16:
             g = g.clone()
         need = ctx.needs_input_grad
-        with torch.cuda.device(dev):
-            grads = [torch.empty(t.shape, dtype=t.dtype, device=dev)
-                     if t is not None and need[i] else None
-                     for i, t in enumerate((q, k, v, q_pos, k_pos, sigma))]
+        with _lib.on_device(dev):
+            grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need[i] else None
+                     for i, t in enumerate((q, k, v))]
+            grads += [torch.empty(t.shape, dtype=torch.float32, device=dev)
+                      if t is not None and need[3 + i] else None
+                      for i, t in enumerate((q_pos, k_pos))]
+            grads.append(torch.empty(d.heads, dtype=torch.float32, device=dev) if need[5] else None)
             gr = _lib.RaAttnGrads(*[_lib.ptr(t) for t in grads])
-            ws = _lib.workspace(lib.ra_attn_workspace_bytes(ctypes.byref(d), 1), dev)
+            n_ws = lib.ra_attn_workspace_bytes(ctypes.byref(d), 1)
+            ws = _lib.scratch(n_ws, dev)
             f32 = q.dtype == torch.float32
-            rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), g.data_ptr(),
+            rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(ctx.inp), g.data_ptr(),
                                       out32.data_ptr() if f32 else None,
-                                      None if f32 else out32.data_ptr(), stats.data_ptr(), ctypes.byref(gr),
-                                      ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+                                      None if f32 else out32.data_ptr(), stats.data_ptr(),
+                                      ctypes.byref(gr), ctx.state.data_ptr(), ctx.state.numel(),
+                                      ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention backward")
+        for i, t in ((3, q_pos), (4, k_pos)):
+            if grads[i] is not None and t.dtype != torch.float32:
+                grads[i] = grads[i].to(t.dtype)
+        if grads[5] is not None:
+            s = grads[5] if sigma.numel() == d.heads else grads[5].sum()
+            grads[5] = s.reshape(sigma.shape).to(device=sigma.device, dtype=sigma.dtype)
         return (*grads, None, None, None, None, None, None)
 
 
@@ -199,7 +246,8 @@ def _checked(q, k, v, ndim, shape_text):
 
 
 def _positions(q_pos, k_pos, sigma, num_q, num_k, heads, device):
-    """float32 positions (rows, c) and sigma (heads,), or three Nones."""
+    """Positions (rows, c) and sigma (heads,) or one, or three Nones.  `num`:
+    the shape of the rows."""
     if q_pos is None:
         if k_pos is not None or sigma is not None:
             raise ValueError("positions of queries and sigma go together")
@@ -208,11 +256,14 @@ def _positions(q_pos, k_pos, sigma, num_q, num_k, heads, device):
         raise ValueError("positions need a sigma")
     if k_pos is None:
         k_pos = q_pos
-    if q_pos.ndim != 2 or k_pos.ndim != 2 or q_pos.shape[1] != k_pos.shape[1] or \
-            not 1 <= q_pos.shape[1] <= 3:
+    lead = len(num_q)
+    if q_pos.ndim != lead + 1 or k_pos.ndim != lead + 1 or \
+            q_pos.shape[-1] != k_pos.shape[-1] or not 1 <= q_pos.shape[-1] <= 3:
         raise ValueError("positions must have 1 to 3 coordinates, the same for queries and keys")
-    if q_pos.shape[0] != num_q or k_pos.shape[0] != num_k:
+    if tuple(q_pos.shape[:-1]) != tuple(num_q) or tuple(k_pos.shape[:-1]) != tuple(num_k):
         raise ValueError("positions length must equal number of rows")
+    if not (q_pos.is_floating_point() and k_pos.is_floating_point()):
+        raise ValueError("positions must be floating point")
     if not isinstance(sigma, Tensor):
         if not sigma > 0:
             raise ValueError("sigma must be positive")
@@ -221,9 +272,7 @@ def _positions(q_pos, k_pos, sigma, num_q, num_k, heads, device):
         raise ValueError("sigma must be a scalar or one value per head")
     if q_pos.device != device or k_pos.device != device:
         raise ValueError("positions must be on the device of q")
-    sigma = sigma.to(device=device, dtype=torch.float32).reshape(-1).expand(heads)
-    return (q_pos.to(torch.float32).contiguous(), k_pos.to(torch.float32).contiguous(),
-            sigma.contiguous())
+    return q_pos, k_pos, sigma
 
 
 def _factors(scale, softcap, dim):
@@ -231,8 +280,8 @@ def _factors(scale, softcap, dim):
     softcap = float(softcap)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    if not (softcap >= 0.0 and math.isfinite(softcap)):
-        raise ValueError("softcap must be finite and not negative")
+    if not (softcap == 0.0 or (softcap >= 1e-6 and math.isfinite(softcap))):
+        raise ValueError("softcap must be 0 (none), or finite and at least 1e-6")
     return scale, softcap
 
 
@@ -241,26 +290,16 @@ def _mask(mask, shape, device):
         return None
     if tuple(mask.shape) != tuple(shape):
         raise ValueError(f"masks must have shape {tuple(shape)}")
-    return mask.to(device=device, dtype=torch.bool).reshape(-1).to(torch.uint8).contiguous()
-
-
-def _unit_rows(t: Tensor) -> Tensor:
-    """Unit stride along the head dimension, and 16-byte aligned rows for the
-    16-bit tensor-core kernels (widths that are multiples of 8)."""
-    unit = t.stride(-1) == 1 or t.shape[-1] == 1
-    if unit and t.dtype != torch.float32 and t.shape[-1] % 8 == 0:
-        unit = t.data_ptr() % 16 == 0 and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in
-                                              zip(t.stride()[:-1], t.shape[:-1]))
-        return t if unit else t.clone(memory_format=torch.contiguous_format)
-    return t if unit else t.contiguous()
+    mask = mask.to(device=device, dtype=torch.bool)
+    return (mask if mask.is_contiguous() else mask.contiguous()).view(torch.uint8)
 
 
 def _run(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap):
     _lib.check_status("kernel attention")
     need = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, q_pos, k_pos, sigma))
-    return _KernelAttention.apply(_unit_rows(q), _unit_rows(k), _unit_rows(v), q_pos, k_pos, sigma,
-                                  q_mask, k_mask, shape, scale, softcap, need)
+    return _KernelAttention.apply(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale,
+                                  softcap, need)
 
 
 def pyg_kernel_attention(q: Tensor, k: Tensor, v: Tensor, *, q_ptr: Optional[Tensor] = None,
@@ -306,7 +345,7 @@ def pyg_kernel_attention(q: Tensor, k: Tensor, v: Tensor, *, q_ptr: Optional[Ten
         raise ValueError("ptr[-1] must equal number of nodes")
     if segments.q_ptr.device != device:
         raise ValueError("segments must be on the device of q")
-    pos = _positions(q_pos, k_pos, sigma, q.shape[0], k.shape[0], q.shape[1], device)
+    pos = _positions(q_pos, k_pos, sigma, q.shape[:1], k.shape[:1], q.shape[1], device)
     shape = (segments.graphs, segments.num_q, segments.num_k, segments.max_q, segments.max_k,
              segments.q_ptr, segments.k_ptr, segments.q_tiles, segments.k_tiles)
     return _run(q, k, v, *pos, _mask(q_mask, q.shape[:1], device),
@@ -329,15 +368,7 @@ def kernel_attention_dense(q: Tensor, k: Tensor, v: Tensor, mask_q: Optional[Ten
         raise ValueError("q, k and v must have the same number of clouds")
     scale, softcap = _factors(scale, softcap, D)
     device = _lib.require_cuda(q, k, v)
-    for p, n in ((q_pos, N), (k_pos, M)):
-        if p is not None and (p.ndim != 3 or tuple(p.shape[:2]) != (B, n)):
-            raise ValueError("positions must have shape (B, N, c)")
-    if k_pos is None and q_pos is not None and N != M:
-        raise ValueError("positions length must equal number of rows")
-    flat = [None if p is None else p.reshape(-1, p.shape[2]) for p in (q_pos, k_pos)]
-    pos = _positions(flat[0], flat[1], sigma, B * N, B * M, H, device)
+    pos = _positions(q_pos, k_pos, sigma, (B, N), (B, M), H, device)
     shape = (B, B * N, B * M, N if B else 0, M if B else 0, None, None, None, None)
-    out = _run(q.reshape(B * N, H, D), k.reshape(B * M, k.shape[2], D),
-               v.reshape(B * M, k.shape[2], D), *pos, _mask(mask_q, (B, N), device),
-               _mask(mask_k, (B, M), device), shape, scale, softcap)
-    return out.reshape(B, N, H, D)
+    return _run(q, k, v, *pos, _mask(mask_q, (B, N), device), _mask(mask_k, (B, M), device), shape,
+                scale, softcap)

@@ -29,7 +29,6 @@ _REDUCTIONS = {"none": _lib.RA_REDUCE_NONE, "sum": _lib.RA_REDUCE_SUM,
 def _rows16(t: Tensor) -> Tensor:
     """`t` (a matrix) as the kernels read it: unit stride along its rows and,
     for the 16-bit types, 16-byte aligned rows (copied where it is not)."""
-    t = t.detach()
     if t.dtype == torch.float32:
         return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
     if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and \
@@ -57,9 +56,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         d.ld_w = wk.stride(0)
         d.ignore_index, d.dtype, d.reduction = ignore_index, _lib.DTYPES[x.dtype], reduction
         d.scale, d.softcap, d.status = scale, softcap, _lib.status_word()
-        with torch.cuda.device(dev):
-            state = _lib.workspace(lib.ra_ce_state_bytes(ctypes.byref(d)), dev)
-            ws = _lib.workspace(lib.ra_ce_workspace_bytes(ctypes.byref(d), 0), dev)
+        with _lib.on_device(dev):
+            state = _lib.scratch(lib.ra_ce_state_bytes(ctypes.byref(d)), dev)
+            ws = _lib.scratch(lib.ra_ce_workspace_bytes(ctypes.byref(d), 0), dev)
             shape = (d.rows,) if reduction == _lib.RA_REDUCE_NONE else ()
             loss = torch.empty(shape, dtype=torch.float32, device=dev)
             lse = torch.empty(d.rows, dtype=torch.float32, device=dev)
@@ -87,10 +86,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         gl = None if g_loss is None else g_loss.to(torch.float32).contiguous()
         ge = None if g_lse is None else g_lse.to(torch.float32).contiguous()
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
             dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
-            ws = _lib.workspace(lib.ra_ce_workspace_bytes(ctypes.byref(d), 1), dev)
+            ws = _lib.scratch(lib.ra_ce_workspace_bytes(ctypes.byref(d), 1), dev)
             rc = lib.ra_ce_backward(ctypes.byref(d), xk.data_ptr(), wk.data_ptr(),
                                     target.data_ptr(), _lib.ptr(gl), _lib.ptr(ge), _lib.ptr(dx),
                                     _lib.ptr(dw), ctx.state.data_ptr(), ctx.state.numel(),
@@ -141,14 +140,15 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, *, scale: fl
     scale, softcap = float(scale), float(softcap)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    if not (softcap >= 0.0 and math.isfinite(softcap)):
-        raise ValueError("softcap must be finite and not negative")
+    if not (softcap == 0.0 or (softcap >= 1e-6 and math.isfinite(softcap))):
+        raise ValueError("softcap must be 0 (none), or finite and at least 1e-6")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"Unsupported reduction: {reduction}")
     device = _lib.require_cuda(x, weight, target)
     if weight.device != device or target.device != device:
         raise ValueError("x, weight and target must be on the same device")
     _lib.check_status("linear cross entropy")
-    target = target.to(torch.long).contiguous()
+    if target.dtype != torch.long or not target.is_contiguous():
+        target = target.to(torch.long).contiguous()
     return _LinearCrossEntropy.apply(x, weight, target, scale, softcap, int(ignore_index),
                                      _REDUCTIONS[reduction])

@@ -404,18 +404,20 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
       if ((rc = launched())) return rc;
     }
   }
-  if (gr->dq_pos && a.num_q > 0) {
-    attn_pos_kernel<<<(unsigned)std::min<int64_t>(ceil_div(a.num_q, (int64_t)256), sms * 8), 256, 0,
-                      st>>>(a.pos_q, a.num_q, a.heads, a.pos_dim, gr->dq_pos);
-    if ((rc = launched())) return rc;
-  }
-  if (gr->dk_pos && a.num_k > 0) {
-    attn_pos_kernel<<<(unsigned)std::min<int64_t>(ceil_div(a.num_k, (int64_t)256), sms * 8), 256, 0,
-                      st>>>(a.pos_k, a.num_k, a.kv_heads, a.pos_dim, gr->dk_pos);
-    if ((rc = launched())) return rc;
-  }
-  if (gr->dsigma) {
-    attn_sigma_kernel<<<a.heads, 1024, 0, st>>>(a.pos_q, a.num_q, a.sigma, gr->dsigma);
+  if (gr->dq_pos || gr->dk_pos || gr->dsigma) {
+    const AttnPosGrads p{{a.pos_q, a.pos_k},
+                         {a.num_q, a.num_k},
+                         {a.heads, a.kv_heads},
+                         a.pos_dim,
+                         {gr->dq_pos, gr->dk_pos},
+                         gr->dsigma,
+                         a.sigma};
+    const int64_t rows = std::max<int64_t>(std::max(a.num_q, a.num_k), 512);
+    const dim3 grid((unsigned)std::max<int64_t>(
+                        std::min<int64_t>(ceil_div(rows, (int64_t)512), sms * 4),
+                        std::min<int64_t>(a.heads, sms)),
+                    3);
+    attn_pos_kernel<<<grid, 512, 0, st>>>(p);
     if ((rc = launched())) return rc;
   }
   return RA_OK;

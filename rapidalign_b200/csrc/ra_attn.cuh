@@ -145,34 +145,48 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const T *dout, const fl
   }
 }
 
-// positions' gradients: the heads' partials in order
-__global__ void __launch_bounds__(256) attn_pos_kernel(const float4 *part, int64_t num, int heads,
-                                                       int pos_dim, float *grad) {
-  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < num; i += gridDim.x * 256LL) {
-    float x = 0.f, y = 0.f, z = 0.f;
-    for (int h = 0; h < heads; ++h) {
-      const float4 v = part[h * num + i];
-      x += v.x;
-      y += v.y;
-      z += v.z;
+// Gradients of positions and sigmas from the rows' partials.  blockIdx.y = 0, 1:
+// queries' and keys' positions, the heads in order; 2: dsigma_h = sum_i w_i /
+// sigma^3 in fp64, one CTA a head, in a fixed order.
+struct AttnPosGrads {
+  const float4 *part[2];  // [heads][num]
+  int64_t num[2];
+  int heads[2];
+  int pos_dim;
+  float *grad[2], *dsigma;  // or null
+  const float *sigma;
+};
+__global__ void __launch_bounds__(512) attn_pos_kernel(const AttnPosGrads P) {
+  __shared__ double sh[16];
+  const int y = blockIdx.y;
+  if (y < 2) {
+    if (P.grad[y] == nullptr) return;
+    const int64_t num = P.num[y];
+    for (int64_t i = blockIdx.x * 512LL + threadIdx.x; i < num; i += gridDim.x * 512LL) {
+      float x = 0.f, yy = 0.f, z = 0.f;
+      for (int h = 0; h < P.heads[y]; ++h) {
+        const float4 v = P.part[y][h * num + i];
+        x += v.x;
+        yy += v.y;
+        z += v.z;
+      }
+      float *g = P.grad[y] + i * P.pos_dim;
+      g[0] = x;
+      if (P.pos_dim > 1) g[1] = yy;
+      if (P.pos_dim > 2) g[2] = z;
     }
-    grad[i * pos_dim] = x;
-    if (pos_dim > 1) grad[i * pos_dim + 1] = y;
-    if (pos_dim > 2) grad[i * pos_dim + 2] = z;
-  }
-}
-
-// dsigma_h = sum_i w_i / sigma^3 in fp64: one CTA a head
-__global__ void __launch_bounds__(1024) attn_sigma_kernel(const float4 *part, int64_t num,
-                                                          const float *sigma, float *grad) {
-  __shared__ double sh[32];
-  const float4 *p = part + blockIdx.x * num;
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < num; i += 1024) s += (double)p[i].w;
-  s = block_sum(s, sh);
-  if (threadIdx.x == 0) {
-    const double sg = (double)sigma[blockIdx.x];
-    grad[blockIdx.x] = (float)(s / (sg * sg * sg));
+  } else if (P.dsigma != nullptr) {
+    for (int h = blockIdx.x; h < P.heads[0]; h += gridDim.x) {
+      const float4 *p = P.part[0] + h * P.num[0];
+      double s = 0.0;
+      for (int64_t i = threadIdx.x; i < P.num[0]; i += 512) s += (double)p[i].w;
+      s = block_sum(s, sh);
+      if (threadIdx.x == 0) {
+        const double sg = (double)P.sigma[h];
+        P.dsigma[h] = (float)(s / (sg * sg * sg));
+      }
+      __syncthreads();
+    }
   }
 }
 

@@ -23,6 +23,7 @@ def qkv(n=5, m=7, h=4, hk=2, d=8, dtype=torch.float32):
     (lambda q, k, v: ((q[..., :0], k[..., :0], v[..., :0]), {}), "between 1 and 256"),
     (lambda q, k, v: ((q, k, v), {"scale": float("nan")}), "scale"),
     (lambda q, k, v: ((q, k, v), {"softcap": -2.0}), "softcap"),
+    (lambda q, k, v: ((q, k, v), {"softcap": 1e-7}), "softcap"),
     (lambda q, k, v: ((q, k, v), {"softcap": float("inf")}), "softcap"),
 ])
 def test_refuses(change, message):
@@ -58,13 +59,15 @@ def test_cpu_tensors_are_refused():
     (dict(q_pos=torch.zeros(5, 4), k_pos=torch.zeros(7, 4), sigma=1.0), "1 to 3"),
     (dict(q_pos=torch.zeros(5, 3), k_pos=torch.zeros(7, 2), sigma=1.0), "1 to 3"),
     (dict(q_pos=torch.zeros(5, 3), sigma=1.0), "length"),
+    (dict(q_pos=torch.zeros(1, 5, 3), k_pos=torch.zeros(1, 7, 3), sigma=1.0), "1 to 3"),
+    (dict(q_pos=torch.zeros(5, 3).long(), k_pos=torch.zeros(7, 3).long(), sigma=1.0), "floating"),
     (dict(q_pos=torch.zeros(5, 3), k_pos=torch.zeros(7, 3), sigma=torch.ones(3)), "per head"),
 ])
 def test_positions_are_checked(kw, message):
     from rapidalign_b200.attention import _positions
     args = [kw.get(n) for n in ("q_pos", "k_pos", "sigma")]
     with pytest.raises(ValueError, match=message):
-        _positions(*args, 5, 7, 4, torch.device("cpu"))
+        _positions(*args, (5,), (7,), 4, torch.device("cpu"))
 
 
 def test_tiles():

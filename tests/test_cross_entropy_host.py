@@ -24,6 +24,7 @@ def args(n=4, v=6, d=8, dtype=torch.float32):
     (lambda x, w, t: ((x[:, :0], w[:, :0], t), {}), "at least one row"),
     (lambda x, w, t: ((x, w, t), {"scale": float("inf")}), "scale"),
     (lambda x, w, t: ((x, w, t), {"softcap": -1.0}), "softcap"),
+    (lambda x, w, t: ((x, w, t), {"softcap": 1e-7}), "softcap"),
     (lambda x, w, t: ((x, w, t), {"softcap": float("nan")}), "softcap"),
     (lambda x, w, t: ((x, w, t), {"reduction": "max"}), "Unsupported reduction"),
 ])
