@@ -808,11 +808,11 @@ struct BwdRow {
 struct DqSums {
   f2_t ds = 0, g[4] = {}, q[4] = {};
 };
-template <class Kind, AttnCap CAP, bool POS, bool PG, int R>
+// MASKED: some of the 32 columns are not there (`bits`).
+template <class Kind, AttnCap CAP, bool POS, bool PG, bool MASKED, int R>
 __device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], const BwdRow &B,
                                             float m, float rl, float delta, unsigned bits,
                                             const TilePos<R> &tp, int c0, DqSums &S) {
-  const bool every = bits == kFull;
   const f2_t su = two(B.sc.su), nm = two(-m), nw = two(-B.sc.w), dps = two(B.dps),
              nd = two(-delta), r2l = two(rl), up = two(B.up);
 #pragma unroll
@@ -834,7 +834,7 @@ __device__ __forceinline__ void dq_elements(float (&v)[32], float (&dp)[32], con
       float x, y;
       upk(t, x, y);
       x = ex2(x), y = ex2(y);
-      if (!every) {
+      if (MASKED) {
         x = (bits >> e) & 1 ? x : 0.f;
         y = (bits >> (e + 1)) & 1 ? y : 0.f;
       }
@@ -1035,20 +1035,30 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
     tmem_ld32(tP + lane_off + 32 * part, dp);
-    const unsigned bits = live ? kval[2 * pb + part] : 0u;
-#define RA_DQ(C, P, G)                                                                       \
-  dq_elements<Kind, C, P, G>(v, dp, B, st.x, st.y, delta, bits, kpos[pb], 32 * part, S)
+    const unsigned bits = kval[2 * pb + part];  // the same for the warp
+#define RA_DQ_(C, P, G, M) \
+  dq_elements<Kind, C, P, G, M>(v, dp, B, st.x, st.y, delta, bits, kpos[pb], 32 * part, S)
+#define RA_DQ(C, P, G) RA_DQ_(C, P, G, false)
 #define RA_DQ_POS(C)                             \
   do {                                           \
     if (pos_grad) RA_DQ(C, true, true);          \
     else if (A.pos_dim > 0) RA_DQ(C, true, false); \
     else RA_DQ(C, false, false);                 \
   } while (0)
-    if (!(B.sc.capl > 0.f)) RA_DQ_POS(kNoCap);
+    // a last or masked tile: fewer forms.  (A row that is not there spoils its own
+    // lane only, which nothing reads.)
+    if (bits != kFull) {
+      const bool cap = B.sc.capl > 0.f, pos = A.pos_dim > 0;
+      if (cap && pos) RA_DQ_(kCapAny, true, true, true);
+      else if (cap) RA_DQ_(kCapAny, false, false, true);
+      else if (pos) RA_DQ_(kNoCap, true, true, true);
+      else RA_DQ_(kNoCap, false, false, true);
+    } else if (!(B.sc.capl > 0.f)) RA_DQ_POS(kNoCap);
     else if (all_small(v, B.sc.su)) RA_DQ_POS(kCapSmall);
     else RA_DQ_POS(kCapAny);
 #undef RA_DQ_POS
 #undef RA_DQ
+#undef RA_DQ_
     put_weights<Kind>(tS + lane_off + 32 * part, dp, Kind::pair);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     if (C::STAGES > 1 && t + 1 < t1) {
