@@ -209,25 +209,36 @@ bool map_heads(CUtensorMap *m, bool bf16, const void *p, int64_t rows, int heads
 }
 int padded_dim(const ra_attn_desc *d) { return d->dim <= 32 ? 32 : d->dim <= 64 ? 64 : 128; }
 bool map_operand(const ra_attn_desc *d, AttnMap *m, const void *hi, const void *lo, int64_t rows,
-                 int heads, int64_t row, int64_t head) {
-  const bool bf16 = d->dtype == RA_BF16, pair = d->dtype == RA_F32;
-  const int dp = padded_dim(d), cw = dp == 32 ? 32 : 64, br = pair && dp == 128 ? 32 : 64;
+                 int heads, int64_t row, int64_t head, int br) {
+  const bool bf16 = d->dtype == RA_BF16;
+  const int dp = padded_dim(d), cw = dp == 32 ? 32 : 64;
   return map_heads(&m->hi, bf16, hi, rows, heads, d->dim, row, head, cw, br) &&
          map_heads(&m->lo, bf16, lo, rows, heads, d->dim, row, head, cw, br);
 }
 
-// 16-bit operands of q, k, v: as given, or the halves in the state
-bool operands(const ra_attn_desc *d, const ra_attn_inputs *in, char *state, AttnTcArgs *x) {
-  x->words = (const unsigned *)state;
+// What the kernels read: q, k, v as given or the halves in the state, dout
+// (`gh`, `gl`; null in the forward).
+struct Operands {
+  const void *q[2], *k[2], *v[2], *g[2];
+  int64_t qr, qh, kr, kh, vr, vh, gr, gh;
+};
+Operands operands(const ra_attn_desc *d, const ra_attn_inputs *in, char *state, const void *gh,
+                  const void *gl) {
+  const int64_t qr = (int64_t)d->heads * d->dim, kr = (int64_t)d->kv_heads * d->dim, D = d->dim;
   if (d->dtype != RA_F32)
-    return map_operand(d, &x->q, in->q, in->q, d->num_q, d->heads, d->q_row, d->q_head) &&
-           map_operand(d, &x->k, in->k, in->k, d->num_k, d->kv_heads, d->k_row, d->k_head) &&
-           map_operand(d, &x->v, in->v, in->v, d->num_k, d->kv_heads, d->v_row, d->v_head);
+    return {{in->q, in->q}, {in->k, in->k}, {in->v, in->v}, {gh, gl}, d->q_row, d->q_head,
+            d->k_row, d->k_head, d->v_row, d->v_head, qr, D};
   const AttnState s = state_layout(d);
-  const int64_t qr = (int64_t)d->heads * d->dim, kr = (int64_t)d->kv_heads * d->dim;
-  return map_operand(d, &x->q, state + s.qh, state + s.ql, d->num_q, d->heads, qr, d->dim) &&
-         map_operand(d, &x->k, state + s.kh, state + s.kl, d->num_k, d->kv_heads, kr, d->dim) &&
-         map_operand(d, &x->v, state + s.vh, state + s.vl, d->num_k, d->kv_heads, kr, d->dim);
+  return {{state + s.qh, state + s.ql}, {state + s.kh, state + s.kl}, {state + s.vh, state + s.vl},
+          {gh, gl}, qr, D, kr, D, kr, D, qr, D};
+}
+// their maps, `br` rows a box
+bool map_operands(const ra_attn_desc *d, const Operands &o, int br, AttnTcArgs *x) {
+  return map_operand(d, &x->q, o.q[0], o.q[1], d->num_q, d->heads, o.qr, o.qh, br) &&
+         map_operand(d, &x->k, o.k[0], o.k[1], d->num_k, d->kv_heads, o.kr, o.kh, br) &&
+         map_operand(d, &x->v, o.v[0], o.v[1], d->num_k, d->kv_heads, o.vr, o.vh, br) &&
+         (o.g[0] == nullptr ||
+          map_operand(d, &x->go, o.g[0], o.g[1], d->num_q, d->heads, o.gr, o.gh, br));
 }
 
 template <auto kernel>
@@ -249,19 +260,25 @@ int launch(int64_t grid, int threads, int smem, const AttnArgs &a, const AttnTcA
 }
 
 template <class Kind, int DP>
-int tc_forward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
-  return launch<attn_tc_fwd_kernel<Kind, DP>>(a.n_q_tiles * a.heads * x.splits, 128,
-                FwdCfg<Kind, DP>::smem, a, x, st);
+int tc_forward(const ra_attn_desc *d, const Operands &o, const AttnArgs &a, AttnTcArgs *x,
+               cudaStream_t st) {
+  using C = FwdCfg<Kind, DP>;
+  if (!map_operands(d, o, C::BR, x)) return RA_ERR_INVALID_ARGUMENT;
+  return launch<attn_tc_fwd_kernel<Kind, DP>>(a.n_q_tiles * a.heads * x->splits, 128, C::smem, a,
+                                              *x, st);
 }
 template <class Kind, int DP>
-int tc_backward(const AttnArgs &a, const AttnTcArgs &x, cudaStream_t st) {
+int tc_backward(const ra_attn_desc *d, const Operands &o, const AttnArgs &a, AttnTcArgs *x,
+                cudaStream_t st) {
+  using Q = DqCfg<Kind, DP>;
+  using K = DkvCfg<Kind, DP>;
   int rc = RA_OK;
+  if (!map_operands(d, o, Q::BR, x)) return RA_ERR_INVALID_ARGUMENT;
   if (a.dq || a.pos_q || a.dk)  // dk reads the D that this kernel puts right
-    rc = launch<attn_tc_dq_kernel<Kind, DP>>(a.n_q_tiles * a.heads, DqCfg<Kind, DP>::NT,
-                DqCfg<Kind, DP>::smem, a, x, st);
+    rc = launch<attn_tc_dq_kernel<Kind, DP>>(a.n_q_tiles * a.heads, Q::NT, Q::smem, a, *x, st);
+  if (K::BR != Q::BR && !map_operands(d, o, K::BR, x)) return RA_ERR_INVALID_ARGUMENT;
   if (!rc && (a.dk || a.dv || a.pos_k))
-    rc = launch<attn_tc_dkv_kernel<Kind, DP>>(a.n_k_tiles * a.kv_heads, DkvCfg<Kind, DP>::NT,
-                DkvCfg<Kind, DP>::smem, a, x, st);
+    rc = launch<attn_tc_dkv_kernel<Kind, DP>>(a.n_k_tiles * a.kv_heads, K::NT, K::smem, a, *x, st);
   return rc;
 }
 
@@ -317,7 +334,7 @@ int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, 
     return rc ? rc : join<T>(a, f, ws, sms, st);
   }
   AttnTcArgs x{};
-  if (!operands(d, in, state, &x)) return RA_ERR_INVALID_ARGUMENT;
+  x.words = (const unsigned *)state;
   if (Kind::pair) {
     const AttnState s = state_layout(d);
     if (cudaMemsetAsync(state, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
@@ -335,9 +352,10 @@ int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, 
   x.splits = f.splits;
   x.part_o = (float *)(ws + f.part_o), x.part_s = (float2 *)(ws + f.part_s);
   x.pair_p = a.out32 != nullptr;
-  rc = d->dim <= 32   ? tc_forward<Kind, 32>(a, x, st)
-       : d->dim <= 64 ? tc_forward<Kind, 64>(a, x, st)
-                      : tc_forward<Kind, 128>(a, x, st);
+  const Operands o = operands(d, in, state, nullptr, nullptr);
+  rc = d->dim <= 32   ? tc_forward<Kind, 32>(d, o, a, &x, st)
+       : d->dim <= 64 ? tc_forward<Kind, 64>(d, o, a, &x, st)
+                      : tc_forward<Kind, 128>(d, o, a, &x, st);
   return rc ? rc : join<T>(a, f, ws, sms, st);
 }
 
@@ -369,10 +387,9 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
   if (tc) {
     AttnTcArgs x{};
     const int64_t qr = (int64_t)d->heads * d->dim;
-    const void *gh = Kind::pair ? ws + b.gh : a.dout, *gl = Kind::pair ? ws + b.gl : a.dout;
-    if (!operands(d, in, state, &x) ||
-        !map_operand(d, &x.go, gh, gl, d->num_q, d->heads, qr, d->dim))
-      return RA_ERR_INVALID_ARGUMENT;
+    const Operands o = operands(d, in, state, Kind::pair ? ws + b.gh : a.dout,
+                                Kind::pair ? ws + b.gl : a.dout);
+    x.words = (const unsigned *)state;
     unsigned *words = (unsigned *)state;
     if (!Kind::bf16) {
       AttnPrep p{};
@@ -388,9 +405,9 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
       if ((rc = bounds<T>(p, words, sms, st))) return rc;
       if (Kind::pair && (rc = halves(p, words, sms, st))) return rc;
     }
-    rc = d->dim <= 32   ? tc_backward<Kind, 32>(a, x, st)
-         : d->dim <= 64 ? tc_backward<Kind, 64>(a, x, st)
-                        : tc_backward<Kind, 128>(a, x, st);
+    rc = d->dim <= 32   ? tc_backward<Kind, 32>(d, o, a, &x, st)
+         : d->dim <= 64 ? tc_backward<Kind, 64>(d, o, a, &x, st)
+                        : tc_backward<Kind, 128>(d, o, a, &x, st);
     if (rc) return rc;
   } else {
     if (a.num_q > 0 && (a.dq || a.pos_q)) {

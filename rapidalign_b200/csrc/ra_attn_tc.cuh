@@ -502,15 +502,29 @@ __global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const f
 
 // ---- forward --------------------------------------------------------------------
 
-// rows of a TMA box
+// Rows of a streamed tile of the backward, and of its TMA boxes: 32 where four
+// CTAs of 128 threads then share an SM's TMEM (more of them wait at different
+// times than of two CTAs of 256 threads with tiles of 64; DQ32), or where 64
+// would not fit.
 template <class Kind, int DP>
-constexpr int box_rows = Kind::pair && DP == 128 ? 32 : 64;
+constexpr int dq_rows =
+    64 + (Kind::pair ? 2 : 1) * DP <= 128 || (Kind::pair && DP == 128) ? 32 : 64;
+template <class Kind, int DP>
+constexpr int dkv_rows =
+    64 + (Kind::pair ? 4 : 2) * DP <= 128 || (Kind::pair && DP == 128) ? 32 : 64;
+// CTAs that fit an SM beside each other
+constexpr int attn_ctas(int smem, int tmem, int threads) {
+  int n = 4 * 128 / threads;
+  if (n > 512 / tmem) n = 512 / tmem;
+  while (n > 1 && n * (smem + 1024) > 228 * 1024) --n;
+  return n;
+}
 
 template <class Kind, int DP>
 struct FwdCfg {
   static constexpr int KT = Kind::pair && DP == 128 ? 32 : 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
-  static constexpr int BR = box_rows<Kind, DP>;
+  static constexpr int BR = KT;  // rows of a TMA box
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
   static constexpr bool SMALL = Kind::pair;
   static constexpr int TMEM = tmem_round(KT + (SMALL ? 2 : 1) * DP);
@@ -518,7 +532,7 @@ struct FwdCfg {
   static constexpr int val = pos + 2 * KT * 12;          // unsigned [2][2]
   static constexpr int bar = val + 16, slot = bar + 24;  // slot: also the mask's extent
   static constexpr int smem = slot + 8 + 1024;           // 1024: the tiles' alignment
-  static constexpr int CTAS = smem <= 56 * 1024 ? 4 : smem <= 113 * 1024 ? 2 : 1;
+  static constexpr int CTAS = attn_ctas(smem, TMEM, 128);
 };
 
 // Work for one thread, on warps of their own: issuing a tile's products takes
@@ -905,9 +919,9 @@ __device__ __forceinline__ float sum_of(f2_t v) { return lo_of(v) + hi_of(v); }
 
 template <class Kind, int DP>
 struct DqCfg {
-  static constexpr int KT = Kind::pair && DP == 128 ? 32 : 64;
+  static constexpr int KT = dq_rows<Kind, DP>;
   static constexpr int HALF = Kind::pair ? 2 : 1;
-  static constexpr int BR = box_rows<Kind, DP>;
+  static constexpr int BR = KT;
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
   // two CTAs on an SM are worth more than a second buffer
   static constexpr int STAGES = 2 * Q + 4 * KV <= 100 * 1024 ? 2 : 1;
@@ -918,7 +932,7 @@ struct DqCfg {
   static constexpr int val = pos + 2 * KT * 12;
   static constexpr int bar = val + 16, slot = bar + 24;
   static constexpr int smem = slot + 8 + 1024;
-  static constexpr int CTAS = smem <= 113 * 1024 && TMEM <= 256 ? 2 : 1;
+  static constexpr int CTAS = attn_ctas(smem, TMEM, NT);
 };
 
 template <class Kind, int DP>
@@ -1134,9 +1148,9 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
 
 template <class Kind, int DP>
 struct DkvCfg {
-  static constexpr int QT = Kind::pair && DP == 128 ? 32 : 64;
+  static constexpr int QT = dkv_rows<Kind, DP>;
   static constexpr int HALF = Kind::pair ? 2 : 1;
-  static constexpr int BR = box_rows<Kind, DP>;
+  static constexpr int BR = QT;
   static constexpr int K = HALF * tile_bytes<128, DP>, QG = HALF * tile_bytes<QT, DP>;
   static constexpr bool SMALL = Kind::pair && DP <= 64;  // at 128 TMEM is full
   static constexpr int TMEM = tmem_round(2 * QT + (SMALL ? 4 : 2) * DP);
@@ -1146,7 +1160,7 @@ struct DkvCfg {
   static constexpr int stt = pos + 2 * QT * 12;        // TileStat<QT> [2]
   static constexpr int bar = stt + 2 * QT * 12, slot = bar + 24;
   static constexpr int smem = slot + 8 + 1024;
-  static constexpr int CTAS = smem <= 113 * 1024 && TMEM <= 256 ? 2 : 1;
+  static constexpr int CTAS = attn_ctas(smem, TMEM, NT);
 };
 
 template <class Kind, int DP>
