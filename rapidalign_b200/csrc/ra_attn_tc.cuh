@@ -502,16 +502,18 @@ __global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const f
 
 // ---- forward --------------------------------------------------------------------
 
-// Rows of a streamed tile of the backward, and of its TMA boxes: 32 where four
-// CTAs of 128 threads then share an SM's TMEM (more of them wait at different
-// times than of two CTAs of 256 threads with tiles of 64; DQ32), or where 64
-// would not fit.
+// Rows of a streamed tile of the backward, and of its TMA boxes; 4 threads of a
+// CTA work on each row of 32 columns of it (128 threads for 32).  What counts is
+// that warps wait at different times: 32 where four CTAs then share an SM's TMEM
+// (dq of 64-wide bf16 heads: 318 us, with 64 and two CTAs 387); 128 where one
+// CTA holds the TMEM anyhow (dk, dv of 128-wide heads: 671 us, with 64 756);
+// else 64.
 template <class Kind, int DP>
-constexpr int dq_rows =
-    64 + (Kind::pair ? 2 : 1) * DP <= 128 || (Kind::pair && DP == 128) ? 32 : 64;
+constexpr int dq_rows = 64 + (Kind::pair ? 2 : 1) * DP <= 128 ? 32 : 64;
 template <class Kind, int DP>
-constexpr int dkv_rows =
-    64 + (Kind::pair ? 4 : 2) * DP <= 128 || (Kind::pair && DP == 128) ? 32 : 64;
+constexpr int dkv_rows = 64 + (Kind::pair ? 4 : 2) * DP <= 128          ? 32
+                         : !Kind::pair && DP == 128 || Kind::pair && DP == 64 ? 128
+                                                                        : 64;
 // CTAs that fit an SM beside each other
 constexpr int attn_ctas(int smem, int tmem, int threads) {
   int n = 4 * 128 / threads;
@@ -522,7 +524,7 @@ constexpr int attn_ctas(int smem, int tmem, int threads) {
 
 template <class Kind, int DP>
 struct FwdCfg {
-  static constexpr int KT = Kind::pair && DP == 128 ? 32 : 64;
+  static constexpr int KT = 64;
   static constexpr int HALF = Kind::pair ? 2 : 1;
   static constexpr int BR = KT;  // rows of a TMA box
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
@@ -535,9 +537,13 @@ struct FwdCfg {
   static constexpr int CTAS = attn_ctas(smem, TMEM, 128);
 };
 
-// Work for one thread, on warps of their own: issuing a tile's products takes
-// 200 to 1,400 cycles, its copies 500, and warps 0 and 1 fetch the rows.
-constexpr int kMmaThread = 64, kTmaThread = 96;
+// Work for one thread, on the last two of NT threads' warps: issuing a tile's
+// products takes 200 to 1,400 cycles, its copies 500, and the first warps fetch
+// the rows.
+template <int NT>
+constexpr int kMmaThread = NT - 64;
+template <int NT>
+constexpr int kTmaThread = NT - 32;
 // This thread's row of the next streamed tile, fetched an iteration ahead.
 struct NextRow {
   AttnPos p;
@@ -636,7 +642,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
   float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to
   unsigned phase = 0;
 
-  if (t0 < t1 && threadIdx.x == kMmaThread) {
+  if (t0 < t1 && threadIdx.x == kMmaThread<128>) {
     products_rows<Kind, KT, DP>(tS, sQ, sK + (t0 & 1) * C::KV);
     tc_commit(bar);
   }
@@ -646,7 +652,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {  // the products on its buffers are done
-      if (threadIdx.x == kTmaThread) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread<128>) issue(t + 1, 0);
       fetch(t + 1);
     }
     f2_t s2[KT / 32][16];
@@ -713,7 +719,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == kMmaThread) {
+    if (threadIdx.x == kMmaThread<128>) {
       tc_fence_after();
       products_weighted<Kind, KT, DP, C::SMALL>(tO, tS, sV + b * C::KV, p_pair, t > t0);
       if (t + 1 < t1) products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
@@ -1032,7 +1038,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   const bool pos_grad = A.pos_q != nullptr;
   unsigned phase = 0;
 
-  if (t1 > 0 && threadIdx.x == kMmaThread) {
+  if (t1 > 0 && threadIdx.x == kMmaThread<NT>) {
     products_rows<Kind, KT, DP>(tS, sQ, sK);
     products_rows<Kind, KT, DP>(tP, sG, sV);
     tc_commit(bar);
@@ -1043,7 +1049,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
-      if (C::STAGES > 1 && threadIdx.x == kTmaThread) issue(t + 1, 0);
+      if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
       fetch(t + 1);
     }
     float v[32], dp[32];
@@ -1081,7 +1087,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == kMmaThread) {
+    if (threadIdx.x == kMmaThread<NT>) {
       tc_fence_after();
       products_weighted<Kind, KT, DP, C::SMALL>(tD, tS, sK + b * C::KV, false, t > 0);
       if (C::STAGES > 1 && t + 1 < t1) {
@@ -1093,11 +1099,11 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     if (C::STAGES == 1 && t + 1 < t1) {  // one buffer: its products first
       bad |= !mbar_wait(bar, phase);
       phase ^= 1;
-      if (threadIdx.x == kTmaThread) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
       bad |= !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
-      if (threadIdx.x == kMmaThread) {
+      if (threadIdx.x == kMmaThread<NT>) {
         tc_fence_after();
         products_rows<Kind, KT, DP>(tS, sQ, sK);
         products_rows<Kind, KT, DP>(tP, sG, sV);
@@ -1154,7 +1160,8 @@ struct DkvCfg {
   static constexpr int K = HALF * tile_bytes<128, DP>, QG = HALF * tile_bytes<QT, DP>;
   static constexpr bool SMALL = Kind::pair && DP <= 64;  // at 128 TMEM is full
   static constexpr int TMEM = tmem_round(2 * QT + (SMALL ? 4 : 2) * DP);
-  static constexpr int STAGES = 2 * K + 4 * QG <= 100 * 1024 || (TMEM == 512 && QT == 64) ? 2 : 1;
+  static constexpr int STAGES =
+      2 * K + 4 * QG <= (TMEM == 512 ? 200 : 100) * 1024 ? 2 : 1;
   static constexpr int NT = 128 * (QT / 32);
   static constexpr int pos = 2 * K + 2 * STAGES * QG;  // TilePos<QT> [2]
   static constexpr int stt = pos + 2 * QT * 12;        // TileStat<QT> [2]
@@ -1263,7 +1270,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   unsigned phase = 0;
   int cur = -1;
 
-  if (t1 > 0 && threadIdx.x == kMmaThread) {
+  if (t1 > 0 && threadIdx.x == kMmaThread<NT>) {
     products_rows<Kind, QT, DP>(tS, sK, sQ);
     products_rows<Kind, QT, DP>(tP, sV, sG);
     tc_commit(bar);
@@ -1290,7 +1297,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
-      if (C::STAGES > 1 && threadIdx.x == kTmaThread) issue(t + 1, 0);
+      if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
       fetch(t + 1);
     }
     float v[32], dp[32];
@@ -1318,7 +1325,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == kMmaThread) {
+    if (threadIdx.x == kMmaThread<NT>) {
       tc_fence_after();
       products_weighted<Kind, QT, DP, C::SMALL>(tDv, tS, sG + b * C::QG, false, t > 0);
       products_weighted<Kind, QT, DP, C::SMALL>(tDk, tP, sQ + b * C::QG, false, t > 0);
@@ -1331,11 +1338,11 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     if (C::STAGES == 1 && t + 1 < t1) {
       bad |= !mbar_wait(bar, phase);
       phase ^= 1;
-      if (threadIdx.x == kTmaThread) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
       bad |= !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
-      if (threadIdx.x == kMmaThread) {
+      if (threadIdx.x == kMmaThread<NT>) {
         tc_fence_after();
         products_rows<Kind, QT, DP>(tS, sK, sQ);
         products_rows<Kind, QT, DP>(tP, sV, sG);
@@ -1361,12 +1368,13 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     write_row<T, DP, C::SMALL>(tDv + lane_off, ldexpf(1.f, -elem_exp<Kind>(X, kWdo)) / kUp, in, zero, A.dim,
                      (T *)A.dv + at, nullptr);
   if (pos_grad) {
-    float4 *sum = reinterpret_cast<float4 *>(sm);
-    if (part > 0) sum[row] = make_float4(px, py, pz, 0.f);
+    float4 *sum = reinterpret_cast<float4 *>(sm);  // [parts - 1][128]
+    if (part > 0) sum[(part - 1) * 128 + row] = make_float4(px, py, pz, 0.f);
     __syncthreads();
     if (part == 0 && in) {
-      if (QT > 32) {
-        const float4 o = sum[row];
+#pragma unroll
+      for (int k = 0; k < QT / 32 - 1; ++k) {
+        const float4 o = sum[k * 128 + row];
         px += o.x, py += o.y, pz += o.z;
       }
       if (!live) px = py = pz = 0.f;
