@@ -287,8 +287,13 @@ int join(const AttnArgs &a, const AttnFwd &f, char *ws, int sms, cudaStream_t st
   if (f.splits == 1) return RA_OK;
   const int64_t rows = a.num_q * a.heads;
   if (rows > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
-  attn_join_kernel<T><<<(unsigned)rows, 256, 0, st>>>(a, f.splits, (float *)(ws + f.part_o),
-                                                      (float2 *)(ws + f.part_s));
+  float *po = (float *)(ws + f.part_o);
+  float2 *ps = (float2 *)(ws + f.part_s);
+  // many parts are many loads one after another, which more warps share
+  if (f.splits > 32)
+    attn_join_kernel<T, 32><<<(unsigned)rows, 1024, 0, st>>>(a, f.splits, po, ps);
+  else
+    attn_join_kernel<T, 8><<<(unsigned)rows, 256, 0, st>>>(a, f.splits, po, ps);
   return launched();
 }
 
@@ -296,7 +301,17 @@ template <class T, int N, int LPK>
 int few_launch(const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
   const int64_t grid = a.graphs * a.kv_heads * f.splits;
   if (grid > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
-  attn_few_kernel<T, N, LPK><<<(unsigned)grid, 32 * kFewWarps, 0, st>>>(
+  static OncePerDevice once;
+  if (!once([&] {
+        return cudaFuncSetAttribute(attn_few_kernel<T, N, LPK>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    few_smem<T, N>) == cudaSuccess &&
+               cudaFuncSetAttribute(attn_few_kernel<T, N, LPK>,
+                                    cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared) == cudaSuccess;
+      }))
+    return RA_ERR_CUDA;
+  attn_few_kernel<T, N, LPK><<<(unsigned)grid, 32 * kFewWarps, few_smem<T, N>, st>>>(
       a, f.splits, (float *)(ws + f.part_o), (float2 *)(ws + f.part_s));
   return launched();
 }

@@ -18,6 +18,7 @@
 
 #include "ra_attn.cuh"
 #include "ra_few.cuh"
+#include "ra_tcprim.cuh"
 
 namespace ra {
 
@@ -26,6 +27,19 @@ constexpr int kFewWarps = 4;
 
 template <class T, int N>
 constexpr int few_keys = (N == 1 ? 8 : N == 8 ? 2 : 4) / (sizeof(T) == 4 && N < 8 ? 2 : 1);
+// steps in flight: 16 KB a warp
+template <class T, int N>
+constexpr int few_stage = 2 * few_keys<T, N> * (int)sizeof(T) * 256;  // bytes of a warp's step
+template <class T, int N>
+constexpr int few_stages = 16384 / few_stage<T, N>;
+template <class T, int N>
+constexpr int few_smem = kFewWarps * few_stages<T, N> * few_stage<T, N>;
+
+__device__ __forceinline__ void few_copy(uint32_t dst, const void *src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
 
 template <class T, int N, int LPK>
 __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
@@ -33,6 +47,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
   constexpr int KPW = 32 / LPK, U = few_keys<T, N>, NV = N * U;
   constexpr int V = NV >= LPK ? NV / LPK : 1;  // scores a lane finishes, all of one row
   static_assert(V <= U, "a lane's scores are of one row");
+  extern __shared__ uint4 few_ring[];
   __shared__ float sacc[kFewWarps][N][LPK * 8];
   __shared__ float2 sml[kFewWarps][N];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -73,40 +88,78 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
   }
   float mm = -INFINITY, ml = 0.f;  // of row mr, this lane group's keys; ml: this lane's part
   f2_t acc[N][4] = {};
-  // This lane's keys of a step: rows u KPW apart from kp, vp.  Keys of the next
-  // step are loaded once the scores of this one are made, values while they are
-  // being made.
-  constexpr int kStep = kFewWarps * KPW * U;
+  // This lane's keys of a step: rows u KPW apart from kp, vp.  A lane copies its
+  // columns of S - 1 steps ahead into shared memory and reads only what it copied.
+  constexpr int kStep = kFewWarps * KPW * U, S = few_stages<T, N>, W = sizeof(T) / 2;
+  constexpr int kSlot = 2 * U * W * 32;  // 16-byte pieces of a warp's step
   const int64_t start = j0 + k0 + warp * (KPW * U) + sub;
   const T *kp = (const T *)A.k + hk * A.k_head + c * 8 + start * A.k_row;
   const T *vp = (const T *)A.v + hk * A.v_head + c * 8 + start * A.v_row;
   const float *pp = pos ? A.k_pos + (start + u0 * KPW) * A.pos_dim : nullptr;
   const uint8_t *mp = A.k_mask ? A.k_mask + start : nullptr;
-  int left = (int)(k1 - k0) - warp * (KPW * U) - sub;  // keys from this lane's first on
-  Few8<T> kx[U];
-  AttnPos pj[V];
-  unsigned on = 0;
-  auto fetch = [&]() {
-    on = 0;
+  int left = (int)(k1 - k0) - warp * (KPW * U) - sub;  // keys from the next copied on
+  const int steps = (int)((k1 - k0) - warp * (KPW * U) + kStep - 1) / kStep;  // the warp's
+  uint4 *ring = few_ring + warp * S * kSlot + lane;
+  unsigned marks = 0;  // U bits a slot
+  unsigned next = 0;   // of the step to be copied next
+  auto look = [&]() {
+    next = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool here = u * KPW < left && (mp == nullptr || mp[u * KPW] != 0);
-      on |= (unsigned)here << u;
-      kx[u].load(kp + u * KPW * A.k_row, here && cols);
+    for (int u = 0; u < U; ++u)
+      next |= (unsigned)(u * KPW < left && (mp == nullptr || mp[u * KPW] != 0)) << u;
+  };
+  auto issue = [&](int t) {
+    if (t < steps) {
+      const int slot = t % S;
+      const uint32_t at = smem_u32(ring + slot * kSlot);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool on = ((next >> u) & 1) && cols;
+        const T *ku = on ? kp + u * KPW * A.k_row : (const T *)A.k;
+        const T *vu = on ? vp + u * KPW * A.v_row : (const T *)A.v;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          few_copy(at + (u * W + w) * 512, ku + w * (16 / sizeof(T)), on);
+          few_copy(at + ((U + u) * W + w) * 512, vu + w * (16 / sizeof(T)), on);
+        }
+      }
+      marks = (marks & ~(((1u << U) - 1) << (slot * U))) | next << (slot * U);
+      kp += kStep * A.k_row;
+      vp += kStep * A.v_row;
+      if (mp) mp += kStep;
+      left -= kStep;
+      look();
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  AttnPos pj[V];
+  auto place = [&](int t) {  // positions of step t, that has been copied
+    const unsigned on = marks >> (t % S * U);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       pj[e] = AttnPos{0.f, 0.f, 0.f};
       if (pos && ((on >> (u0 + e)) & 1)) pj[e] = pos_of(pp + e * KPW * A.pos_dim, A.pos_dim, 0);
     }
+    if (pos) pp += kStep * A.pos_dim;
   };
-  int steps = (int)((k1 - k0) - warp * (KPW * U) + kStep - 1) / kStep;  // the warp's
-  if (steps > 0) fetch();
-  for (; steps > 0; --steps) {
-    Few8<T> vx[U];
+  look();
 #pragma unroll
-    for (int u = 0; u < U; ++u) vx[u].load(vp + u * KPW * A.v_row, ((on >> u) & 1) && cols);
-    vp += kStep * A.v_row;
+  for (int t = 0; t < S - 1; ++t) issue(t);
+  if (steps > 0) place(0);
+  for (int step = 0; step < steps; ++step) {
+    issue(step + S - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+    const unsigned on = marks >> (step % S * U);
+    const uint4 *at = ring + step % S * kSlot;
+    Few8<T> kx[U], vx[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        kx[u].u[w] = at[(u * W + w) * 32];
+        vx[u].u[w] = at[((U + u) * W + w) * 32];
+      }
+    }
     float t[NV];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -133,13 +186,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
       t[e] = (on >> (u0 + e)) & 1 ? s : -INFINITY;
       mx = fmaxf(mx, t[e]);
     }
-    if (steps > 1) {
-      kp += kStep * A.k_row;
-      if (pos) pp += kStep * A.pos_dim;
-      if (mp) mp += kStep;
-      left -= kStep;
-      fetch();
-    }
+    if (step + 1 < steps) place(step + 1);
     // the row's other lanes: U keys (or, of duplicates, the same)
 #pragma unroll
     for (int o = 1; o < LPK / N; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));

@@ -761,11 +761,11 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
 
 // Joins the key ranges of a row: one CTA a row and head; its warps take every
 // eighth range, in order, and are joined in order.
-template <class T>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs A, int splits,
+template <class T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const AttnArgs A, int splits,
                                                         const float *part_o, const float2 *part_s) {
-  __shared__ float so[8][kAttnMaxDim];
-  __shared__ float sl[8];
+  __shared__ float so[WARPS][kAttnMaxDim];
+  __shared__ float sl[WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n = A.num_q * A.heads, r = blockIdx.x, i = r / A.heads;
   const int h = (int)(r % A.heads);
@@ -775,8 +775,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs A, int sp
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
   float l = 0.f, acc[kAttnMaxDim / 32] = {};
-#pragma unroll 4
-  for (int s = warp; s < splits; s += 8) {
+#pragma unroll 8
+  for (int s = warp; s < splits; s += WARPS) {
     const float2 st = ps[s * n];
     const float f = st.x > -INFINITY ? ex2(st.x - m) : 0.f;  // else l and o are 0
     l = fmaf(st.y, f, l);
@@ -792,13 +792,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs A, int sp
   __syncthreads();
   l = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) l += sl[k];
+  for (int k = 0; k < WARPS; ++k) l += sl[k];
   const bool any = l > 0.f || l != l;
   const float rl = any ? 1.f / l : 0.f;
-  for (int d = threadIdx.x; d < A.dim; d += 256) {
+  for (int d = threadIdx.x; d < A.dim; d += 32 * WARPS) {
     float o = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) o += so[k][d];
+    for (int k = 0; k < WARPS; ++k) o += so[k][d];
     o = any ? o * rl : 0.f;
     put((T *)A.out + r * A.dim + d, o);
     if (A.out32) A.out32[r * A.dim + d] = o;
