@@ -3,6 +3,7 @@
 
 #include "ra_attn.cuh"
 #include "ra_attn_few.cuh"
+#include "ra_attn_few16.cuh"
 #include "ra_attn_tc.cuh"
 #include "ra_host.h"
 #include "ra_tmap.h"
@@ -115,11 +116,10 @@ bool few_aligned(const ra_attn_desc *d, const ra_attn_inputs *in) {
   return (s & (d->dtype == RA_F32 ? 3 : 7)) == 0 &&
          (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v) & 15) == 0;
 }
-// Key ranges: as many as fill the SMs once (three CTAs each, two of eight
-// rows), each at least 512 keys.
+// Key ranges: as many as fill the SMs once, each at least 512 keys.
 int few_splits(const ra_attn_desc *d, int sms) {
   const int64_t ctas = d->graphs * d->kv_heads;
-  const int64_t fit = sms * (d->max_q * (d->heads / d->kv_heads) > 4 ? 2 : 3);
+  const int64_t fit = sms * (d->dtype == RA_F32 ? few_ctas(d->max_q * (d->heads / d->kv_heads)) : kFew16Ctas);
   if (ctas < 1 || ctas >= fit) return 1;
   const int64_t s = std::min<int64_t>(fit / ctas, d->max_k / 512);
   return s < 1 ? 1 : (int)s;
@@ -297,39 +297,52 @@ int join(const AttnArgs &a, const AttnFwd &f, char *ws, int sms, cudaStream_t st
   return launched();
 }
 
-template <class T, int N, int LPK>
-int few_launch(const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
-  const int64_t grid = a.graphs * a.kv_heads * f.splits;
-  if (grid > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
-  static OncePerDevice once;
+int few_launch(void (*kernel)(AttnArgs, int, float *, float2 *), OncePerDevice &once, int smem,
+               const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
   if (!once([&] {
-        return cudaFuncSetAttribute(attn_few_kernel<T, N, LPK>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    few_smem<T, N>) == cudaSuccess &&
-               cudaFuncSetAttribute(attn_few_kernel<T, N, LPK>,
-                                    cudaFuncAttributePreferredSharedMemoryCarveout,
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+                   cudaSuccess &&
+               cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                     cudaSharedmemCarveoutMaxShared) == cudaSuccess;
       }))
     return RA_ERR_CUDA;
-  attn_few_kernel<T, N, LPK><<<(unsigned)grid, 32 * kFewWarps, few_smem<T, N>, st>>>(
-      a, f.splits, (float *)(ws + f.part_o), (float2 *)(ws + f.part_s));
+  const int64_t grid = a.graphs * a.kv_heads * f.splits;
+  if (grid > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
+  kernel<<<(unsigned)grid, 32 * kFewWarps, smem, st>>>(a, f.splits, (float *)(ws + f.part_o),
+                                                       (float2 *)(ws + f.part_s));
   return launched();
 }
-template <class T, int N>
+template <class T, int DP>
+int few16(const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
+  static OncePerDevice once;
+  return few_launch(attn_few16_kernel<T, DP>, once, Few16Cfg<DP>::smem, a, f, ws, st);
+}
+template <int N, int LPK>
+int few32(const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
+  static OncePerDevice once;
+  return few_launch(attn_few_kernel<N, LPK>, once, few_smem<N>, a, f, ws, st);
+}
+template <int N>
 int few_width(const AttnArgs &a, const AttnFwd &f, char *ws, cudaStream_t st) {
   // a row's scores need lanes of their own: N <= LPK
-  return a.dim <= 32   ? few_launch<T, N, (N > 4 ? 8 : 4)>(a, f, ws, st)
-         : a.dim <= 64 ? few_launch<T, N, 8>(a, f, ws, st)
-                       : few_launch<T, N, 16>(a, f, ws, st);
+  return a.dim <= 32   ? few32<N, (N > 4 ? 8 : 4)>(a, f, ws, st)
+         : a.dim <= 64 ? few32<N, 8>(a, f, ws, st)
+                       : few32<N, 16>(a, f, ws, st);
 }
 template <class T>
 int few_forward(const ra_attn_desc *d, const AttnArgs &a, const AttnFwd &f, char *ws,
                 cudaStream_t st) {
-  const int64_t rows = d->max_q * (d->heads / d->kv_heads);
-  return rows <= 1   ? few_width<T, 1>(a, f, ws, st)
-         : rows <= 2 ? few_width<T, 2>(a, f, ws, st)
-         : rows <= 4 ? few_width<T, 4>(a, f, ws, st)
-                     : few_width<T, 8>(a, f, ws, st);
+  if constexpr (sizeof(T) == 2) {
+    return a.dim <= 32   ? few16<T, 32>(a, f, ws, st)
+           : a.dim <= 64 ? few16<T, 64>(a, f, ws, st)
+                         : few16<T, 128>(a, f, ws, st);
+  } else {
+    const int64_t rows = d->max_q * (d->heads / d->kv_heads);
+    return rows <= 1   ? few_width<1>(a, f, ws, st)
+           : rows <= 2 ? few_width<2>(a, f, ws, st)
+           : rows <= 4 ? few_width<4>(a, f, ws, st)
+                       : few_width<8>(a, f, ws, st);
+  }
 }
 
 template <class Kind>

@@ -1,19 +1,20 @@
 // ra_attn_few.cuh -- forward of kernel attention for a few query rows a graph
-// (one query a graph: pooling, scoring, single new tokens).
+// (one query a graph: pooling, scoring, single new tokens), fp32 inputs without
+// a backward; and what it shares with the 16-bit form (ra_attn_few16.cuh).
 //
 // Bound by the bytes of the keys and values, each read once for all the
 // query heads of a key head.  A CTA takes one graph, key head and range of keys;
 // its N = queries x group rows stay in registers.  LPK lanes share a key, eight
-// columns (16 bytes of a 16-bit type) each, so a warp reads 32 / LPK whole rows
-// an instruction; U keys a lane are in flight at once.  The N U dots of a step
-// are joined over the LPK lanes by halving (each exchange leaves a lane half of
-// its values), so that every lane finishes N U / LPK scores of one row and none
-// is worked on twice; their weights go back by shuffles.  Every lane group
-// keeps the maximum and sums of its own keys, joined at the end over the warp,
-// the CTA (shared memory) and the key ranges (attn_join_kernel).
-// Measured: one query of 8 heads on 2 key heads of 64 against 262144 keys, bf16
-// (134 MB): FEW1; 1024 graphs of 64-512 keys: FEW2.  The tile kernel of
-// ra_attn_tc.cuh, 128 rows for these few, took 272 and 288 us.
+// columns (two 16-byte pieces) each, so a warp reads 32 / LPK whole rows an
+// instruction, copied steps ahead into a ring in shared memory where a lane reads
+// only what it copied itself.  The N U dots of a step are joined over the LPK
+// lanes by halving (each exchange leaves a lane half of its values), so that
+// every lane finishes N U / LPK scores of one row and none is worked on twice;
+// their weights go back by shuffles.  Every lane group keeps the maximum and sums
+// of its own keys, joined at the end over the warp, the CTA (shared memory) and
+// the key ranges (attn_join_kernel).
+// Measured: one query of 8 heads on 2 key heads of 64 against 262144 keys (272 MB
+// with positions) 84 us, 3.2 TB/s; 8 rows a key head 87 us.
 #pragma once
 
 #include "ra_attn.cuh"
@@ -25,15 +26,14 @@ namespace ra {
 constexpr int kFewRows = 8;    // most rows (queries of a graph x heads a key head)
 constexpr int kFewWarps = 4;
 
-template <class T, int N>
-constexpr int few_keys = (N == 1 ? 8 : N == 8 ? 2 : 4) / (sizeof(T) == 4 && N < 8 ? 2 : 1);
-// steps in flight: 16 KB a warp
-template <class T, int N>
-constexpr int few_stage = 2 * few_keys<T, N> * (int)sizeof(T) * 256;  // bytes of a warp's step
-template <class T, int N>
-constexpr int few_stages = 16384 / few_stage<T, N>;
-template <class T, int N>
-constexpr int few_smem = kFewWarps * few_stages<T, N> * few_stage<T, N>;
+constexpr int kFewKeys = 2;  // U: keys of a step a lane
+// CTAs of an SM, and steps in flight: 12 KB a warp of four, 16 of two
+constexpr int few_ctas(int64_t rows) { return rows > 4 ? 2 : 4; }
+constexpr int kFewStage = 2 * kFewKeys * 1024;  // bytes of a warp's step
+template <int N>
+constexpr int few_stages = (N > 4 ? 16384 : 12288) / kFewStage;
+template <int N>
+constexpr int few_smem = kFewWarps * few_stages<N> * kFewStage;
 
 __device__ __forceinline__ void few_copy(uint32_t dst, const void *src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
@@ -41,10 +41,50 @@ __device__ __forceinline__ void few_copy(uint32_t dst, const void *src, bool on)
                : "memory");
 }
 
-template <class T, int N, int LPK>
-__global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
+// Joins the warps of a CTA: their sums acc and (maximum, sum) sml of n rows.
+template <class T>
+__device__ __forceinline__ void few_finish(const AttnArgs &A, int n, int hk, int64_t i0, int splits,
+                                           int split, const float *acc, int acc_warp, int acc_row,
+                                           const float2 *sml, int ml_warp, float *part_o,
+                                           float2 *part_s) {
+  const int D = A.dim, group = A.heads / A.kv_heads;
+  for (int e = threadIdx.x; e < n * D; e += 32 * kFewWarps) {
+    const int r = e / D, d = e % D;
+    float mx = -INFINITY;
+    for (int k = 0; k < kFewWarps; ++k) mx = fmaxf(mx, sml[k * ml_warp + r].x);
+    float ls = 0.f, o = 0.f;
+    for (int k = 0; k < kFewWarps; ++k) {
+      const float2 s = sml[k * ml_warp + r];
+      const float f = s.x > -INFINITY ? ex2(s.x - mx) : s.y != s.y ? 1.f : 0.f;
+      ls = fmaf(s.y, f, ls);
+      o = fmaf(acc[k * acc_warp + r * acc_row + d], f, o);
+    }
+    const int64_t i = i0 + r / group;
+    const int h = hk * group + r % group;
+    const bool on = A.q_mask == nullptr || A.q_mask[i] != 0;
+    const bool any = on && (ls > 0.f || ls != ls);
+    const float ref = mx > -INFINITY ? mx : 0.f;
+    const int64_t at = (i * A.heads + h) * D + d;
+    if (splits > 1) {
+      part_o[split * A.num_q * A.heads * D + at] = any ? o : 0.f;
+      if (d == 0)
+        part_s[((int64_t)split * A.heads + h) * A.num_q + i] =
+            make_float2(any ? ref : -INFINITY, any ? ls : 0.f);
+    } else {
+      const float rl = any ? 1.f / ls : 0.f;
+      const float v = any ? o * rl : 0.f;
+      put((T *)A.out + at, v);
+      if (A.out32) A.out32[at] = v;
+      if (d == 0 && A.neg_m) A.put_stats(h, i, any ? ref : INFINITY, rl);
+    }
+  }
+}
+
+template <int N, int LPK>
+__global__ void __launch_bounds__(32 * kFewWarps, few_ctas(N))
     attn_few_kernel(const AttnArgs A, int splits, float *part_o, float2 *part_s) {
-  constexpr int KPW = 32 / LPK, U = few_keys<T, N>, NV = N * U;
+  using T = float;
+  constexpr int KPW = 32 / LPK, U = kFewKeys, NV = N * U;
   constexpr int V = NV >= LPK ? NV / LPK : 1;  // scores a lane finishes, all of one row
   static_assert(V <= U, "a lane's scores are of one row");
   extern __shared__ uint4 few_ring[];
@@ -90,7 +130,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
   f2_t acc[N][4] = {};
   // This lane's keys of a step: rows u KPW apart from kp, vp.  A lane copies its
   // columns of S - 1 steps ahead into shared memory and reads only what it copied.
-  constexpr int kStep = kFewWarps * KPW * U, S = few_stages<T, N>, W = sizeof(T) / 2;
+  constexpr int kStep = kFewWarps * KPW * U, S = few_stages<N>, W = sizeof(T) / 2;
   constexpr int kSlot = 2 * U * W * 32;  // 16-byte pieces of a warp's step
   const int64_t start = j0 + k0 + warp * (KPW * U) + sub;
   const T *kp = (const T *)A.k + hk * A.k_head + c * 8 + start * A.k_row;
@@ -151,20 +191,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
     asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
     const unsigned on = marks >> (step % S * U);
     const uint4 *at = ring + step % S * kSlot;
-    Few8<T> kx[U], vx[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        kx[u].u[w] = at[(u * W + w) * 32];
-        vx[u].u[w] = at[((U + u) * W + w) * 32];
-      }
-    }
     float t[NV];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       f2_t x[4];
-      kx[u].get(x);
+      Few8<T> kx;
+#pragma unroll
+      for (int e = 0; e < W; ++e) kx.u[e] = at[(u * W + e) * 32];
+      kx.get(x);
 #pragma unroll
       for (int r = 0; r < N; ++r) {
         f2_t s = mul2(q[r][0], x[0]);
@@ -210,7 +244,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       f2_t x[4];
-      vx[u].get(x);
+      Few8<T> vx;
+#pragma unroll
+      for (int e = 0; e < W; ++e) vx.u[e] = at[((U + u) * W + e) * 32];
+      vx.get(x);
 #pragma unroll
       for (int r = 0; r < N; ++r) {
         const int v = r * U + u;
@@ -250,36 +287,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, N == 8 ? 2 : 3)
     if (lane == 0) sml[warp][r] = make_float2(mx, l[r]);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < n * D; e += 32 * kFewWarps) {
-    const int r = e / D, d = e % D;
-    float mx = -INFINITY;
-    for (int k = 0; k < kFewWarps; ++k) mx = fmaxf(mx, sml[k][r].x);
-    float ls = 0.f, o = 0.f;
-    for (int k = 0; k < kFewWarps; ++k) {
-      const float2 s = sml[k][r];
-      const float f = s.x > -INFINITY ? ex2(s.x - mx) : s.y != s.y ? 1.f : 0.f;
-      ls = fmaf(s.y, f, ls);
-      o = fmaf(sacc[k][r][d], f, o);
-    }
-    const int64_t i = i0 + r / group;
-    const int h = hk * group + r % group;
-    const bool on = A.q_mask == nullptr || A.q_mask[i] != 0;
-    const bool any = on && (ls > 0.f || ls != ls);
-    const float ref = mx > -INFINITY ? mx : 0.f;
-    const int64_t at = (i * A.heads + h) * D + d;
-    if (splits > 1) {
-      part_o[split * A.num_q * A.heads * D + at] = any ? o : 0.f;
-      if (d == 0)
-        part_s[((int64_t)split * A.heads + h) * A.num_q + i] =
-            make_float2(any ? ref : -INFINITY, any ? ls : 0.f);
-    } else {
-      const float rl = any ? 1.f / ls : 0.f;
-      const float v = any ? o * rl : 0.f;
-      put((T *)A.out + at, v);
-      if (A.out32) A.out32[at] = v;
-      if (d == 0 && A.neg_m) A.put_stats(h, i, any ? ref : INFINITY, rl);
-    }
-  }
+  few_finish<T>(A, n, hk, i0, splits, split, &sacc[0][0][0], N * LPK * 8, LPK * 8, &sml[0][0], N,
+                part_o, part_s);
 }
 
 }  // namespace ra

@@ -759,49 +759,54 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
   }
 }
 
-// Joins the key ranges of a row: one CTA a row and head; its warps take every
-// eighth range, in order, and are joined in order.
+// Joins the key ranges of a row.  A warp takes every WARPS-th range in order,
+// with the maximum as it goes; then the warps, a column a warp.
 template <class T, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const AttnArgs A, int splits,
-                                                        const float *part_o, const float2 *part_s) {
-  __shared__ float so[WARPS][kAttnMaxDim];
-  __shared__ float sl[WARPS];
+__global__ void __launch_bounds__(32 * WARPS)
+    attn_join_kernel(const AttnArgs A, int splits, const float *part_o, const float2 *part_s) {
+  __shared__ float so[WARPS][kAttnMaxDim / 2 + 1];
+  __shared__ float2 sl[WARPS];
+  constexpr int COLS = kAttnMaxDim / 2 / 32;  // ranges are for widths up to 128
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n = A.num_q * A.heads, r = blockIdx.x, i = r / A.heads;
   const int h = (int)(r % A.heads);
   const float2 *ps = part_s + (int64_t)h * A.num_q + i;
-  float m = -INFINITY;
-  for (int s = lane; s < splits; s += 32) m = fmaxf(m, ps[s * n].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-  float l = 0.f, acc[kAttnMaxDim / 32] = {};
+  float m = -INFINITY, l = 0.f, acc[COLS] = {};
 #pragma unroll 8
   for (int s = warp; s < splits; s += WARPS) {
     const float2 st = ps[s * n];
-    const float f = st.x > -INFINITY ? ex2(st.x - m) : 0.f;  // else l and o are 0
-    l = fmaf(st.y, f, l);
     const float *po = part_o + (s * n + r) * A.dim;
+    float x[COLS];
 #pragma unroll
-    for (int c = 0; c < kAttnMaxDim / 32; ++c)
-      if (lane + 32 * c < A.dim) acc[c] = fmaf(f, po[lane + 32 * c], acc[c]);
+    for (int c = 0; c < COLS; ++c) x[c] = lane + 32 * c < A.dim ? po[lane + 32 * c] : 0.f;
+    const float mx = fmaxf(m, st.x);
+    const float keep = m > -INFINITY ? ex2(m - mx) : 0.f;
+    const float f = st.x > -INFINITY ? ex2(st.x - mx) : 0.f;  // else l and o are 0
+    l = fmaf(st.y, f, l * keep);
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) acc[c] = fmaf(f, x[c], acc[c] * keep);
+    m = mx;
   }
 #pragma unroll
-  for (int c = 0; c < kAttnMaxDim / 32; ++c)
+  for (int c = 0; c < COLS; ++c)
     if (lane + 32 * c < A.dim) so[warp][lane + 32 * c] = acc[c];
-  if (lane == 0) sl[warp] = l;
+  if (lane == 0) sl[warp] = make_float2(m, l);
   __syncthreads();
-  l = 0.f;
+  const float2 st = lane < WARPS ? sl[lane] : make_float2(-INFINITY, 0.f);
+  m = st.x;
 #pragma unroll
-  for (int k = 0; k < WARPS; ++k) l += sl[k];
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+  const float f = st.x > -INFINITY ? ex2(st.x - m) : 0.f;
+  l = warp_sum(st.y * f);
   const bool any = l > 0.f || l != l;
   const float rl = any ? 1.f / l : 0.f;
-  for (int d = threadIdx.x; d < A.dim; d += 32 * WARPS) {
-    float o = 0.f;
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) o += so[k][d];
+  for (int d = warp; d < A.dim; d += WARPS) {
+    float o = warp_sum(lane < WARPS ? so[lane][d] * f : 0.f);
     o = any ? o * rl : 0.f;
-    put((T *)A.out + r * A.dim + d, o);
-    if (A.out32) A.out32[r * A.dim + d] = o;
+    if (lane == 0) {
+      put((T *)A.out + r * A.dim + d, o);
+      if (A.out32) A.out32[r * A.dim + d] = o;
+    }
   }
   if (threadIdx.x == 0 && A.neg_m) A.put_stats(h, i, any ? m : INFINITY, rl);
 }

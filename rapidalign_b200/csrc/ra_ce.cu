@@ -266,7 +266,7 @@ int few_forward(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w,
 }
 
 // The rows' losses from their parts.  Many rows: 8 threads a row in CTAs of 256
-// (65537 rows of 132 parts: ROWS1 us, with 32 threads a row 65 us); few: all of
+// (65537 rows of 132 parts: 29 us, with 32 threads a row 65 us); few: all of
 // 1024 threads on 8 rows.
 int join_rows(const ra_ce_desc *d, const float2 *part, int64_t ld, int parts, int64_t r0,
               int64_t rows, const int64_t *target, float *loss, float *lse, char *sb, char *ws,
