@@ -136,9 +136,9 @@ class _KernelAttention(torch.autograd.Function):
     batches of them."""
 
     @staticmethod
-    def forward(ctx, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap,
-                need_grad):
+    def forward(ctx, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap):
         lib = _lib.load()
+        need_grad = ctx is not None
         dev = q.device
         qr, kr, vr = _rows(q), _rows(k), _rows(v)
         d = _lib.RaAttnDesc()
@@ -226,7 +226,7 @@ class _KernelAttention(torch.autograd.Function):
         if grads[5] is not None:
             s = grads[5] if sigma.numel() == d.heads else grads[5].sum()
             grads[5] = s.reshape(sigma.shape).to(device=sigma.device, dtype=sigma.dtype)
-        return (*grads, None, None, None, None, None, None)
+        return (*grads, None, None, None, None, None)
 
 
 def _checked(q, k, v, ndim, shape_text):
@@ -296,10 +296,11 @@ def _mask(mask, shape, device):
 
 def _run(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap):
     _lib.check_status("kernel attention")
-    need = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (q, k, v, q_pos, k_pos, sigma))
-    return _KernelAttention.apply(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale,
-                                  softcap, need)
+    args = (q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:6]):
+        return _KernelAttention.apply(*args)
+    # no gradient wanted: without autograd's share of a small call
+    return _KernelAttention.forward(None, *args)
 
 
 def pyg_kernel_attention(q: Tensor, k: Tensor, v: Tensor, *, q_ptr: Optional[Tensor] = None,

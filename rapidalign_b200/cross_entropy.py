@@ -67,6 +67,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
                                    state.data_ptr(), state.numel(), ws.data_ptr(), ws.numel(),
                                    _lib.stream_handle(dev))
         _lib.check(rc, "linear cross entropy")
+        if ctx is None:  # no gradient wanted: without autograd's share of a small call
+            return loss, lse
         ctx.desc, ctx.state = d, state
         ctx.save_for_backward(x, weight, target)
         # the aligned copies, where copies had to be made
@@ -150,5 +152,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, *, scale: fl
     _lib.check_status("linear cross entropy")
     if target.dtype != torch.long or not target.is_contiguous():
         target = target.to(torch.long).contiguous()
-    return _LinearCrossEntropy.apply(x, weight, target, scale, softcap, int(ignore_index),
-                                     _REDUCTIONS[reduction])
+    args = (x, weight, target, scale, softcap, int(ignore_index), _REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(*args)
+    return _LinearCrossEntropy.forward(None, *args)
