@@ -19,7 +19,6 @@
 
 #include "ra_attn.cuh"
 #include "ra_few.cuh"
-#include "ra_tcprim.cuh"
 
 namespace ra {
 
@@ -34,12 +33,6 @@ template <int N>
 constexpr int few_stages = (N > 4 ? 16384 : 12288) / kFewStage;
 template <int N>
 constexpr int few_smem = kFewWarps * few_stages<N> * kFewStage;
-
-__device__ __forceinline__ void few_copy(uint32_t dst, const void *src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(on ? 16 : 0)
-               : "memory");
-}
 
 // Joins the warps of a CTA: their sums acc and (maximum, sum) sml of n rows.
 template <class T>

@@ -19,8 +19,6 @@
 // 1024 graphs of 64-512 keys 39 us (63).
 #pragma once
 
-#include <type_traits>
-
 #include "ra_attn_few.cuh"
 
 namespace ra {
@@ -57,42 +55,6 @@ template <>
 __device__ __forceinline__ float2 few_unpack<__nv_bfloat16>(uint32_t u) {
   return __bfloat1622float2(bits_as<__nv_bfloat162>(u));
 }
-template <class T>
-__device__ __forceinline__ void few_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                        uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// four 8 x 8 matrices; lane 8 m + r gives the address of row r of matrix m
-template <bool TRANS>
-__device__ __forceinline__ void few_ldm(uint32_t (&v)[4], uint32_t at) {
-  if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "r"(at)
-                 : "memory");
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "r"(at)
-                 : "memory");
-}
-// byte of 16-byte piece c of row r: eight rows' pieces in eight bank groups
-template <int DP>
-__device__ __forceinline__ int few_at(int r, int c) {
-  return r * DP * 2 + (c ^ (DP >= 64 ? r & 7 : (r >> 1) & 3)) * 16;
-}
-
 template <class T, int DP>
 __global__ void __launch_bounds__(32 * kFewWarps, kFew16Ctas)
     attn_few16_kernel(const AttnArgs A, int splits, float *part_o, float2 *part_s) {

@@ -4,6 +4,7 @@
 
 #include "ra_ce.cuh"
 #include "ra_ce_few.cuh"
+#include "ra_ce_few16.cuh"
 #include "ra_host.h"
 #include "ra_tmap.h"
 
@@ -29,7 +30,7 @@ bool ce_ok(const ra_ce_desc *d) {
 
 int pad8(int n) { return (n + 7) & ~7; }
 
-// A few rows: bound by the table's bytes (ra_ce_few.cuh).  Whole eights of
+// A few rows: bound by the table's bytes (ra_ce_few.cuh, ra_ce_few16.cuh).  Whole eights of
 // columns, and x in shared memory.
 bool use_few(const ra_ce_desc *d) {
   return d->rows <= kCeFewRows && d->dim % 8 == 0 &&
@@ -105,7 +106,8 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   const int64_t pass = std::min<int64_t>(d->rows, kCeRowsPerPass);
   p.tn_z = tile_width(ceil_div(pass, (int64_t)kGmM), d->vocab, sms, split);
   p.parts = kGmParts * (int)ceil_div(d->vocab, (int64_t)p.tn_z);
-  p.few_ctas = (int)std::min<int64_t>(ceil_div(d->vocab, (int64_t)kCeFewWarps * kCeFewTable), 2 * sms);
+  const int few_rows = kCeFewWarps * (split ? kCeFewTable : kCeFew16Rows);
+  p.few_ctas = (int)std::min<int64_t>(ceil_div(d->vocab, (int64_t)few_rows), split ? 2 * sms : sms);
   size_t o = 0;
   p.f_part = o;
   o += align256(sizeof(float2) * (size_t)p.parts * (size_t)(ceil_div(pass, (int64_t)kGmM) * kGmM));
@@ -235,10 +237,10 @@ int halves(const ra_ce_desc *d, const CePlan &p, const void *x, const void *w, c
   return launched();
 }
 
-template <class T, int N>
-int few_launch(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w, const int64_t *target,
-               char *ws, cudaStream_t st) {
-  auto k = ce_few_kernel<T, N>;
+template <int N>
+int few32(const ra_ce_desc *d, const CePlan &p, const float *x, const float *w,
+          const int64_t *target, char *ws, cudaStream_t st) {
+  auto k = ce_few_kernel<N>;
   static OncePerDevice once;
   if (!once([&] {
         return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -251,17 +253,36 @@ int few_launch(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w, con
   return launched();
 }
 template <class T>
-int few_forward(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w,
+int few16(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w, const int64_t *target,
+          char *ws, cudaStream_t st) {
+  auto k = ce_few16_kernel<T>;
+  static OncePerDevice once;
+  if (!once([&] {
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    kCeFew16MostSmem) == cudaSuccess;
+      }))
+    return RA_ERR_CUDA;
+  k<<<(unsigned)p.few_ctas, 32 * kCeFewWarps, ce_few16_smem((int)d->rows, d->dim), st>>>(
+      x, d->ld_x, w, d->ld_w, (int)d->rows, d->vocab, d->dim, d->scale, d->softcap, target,
+      (float2 *)(ws + p.f_part), (float *)(ws + p.f_zt));
+  return launched();
+}
+int few_forward(const ra_ce_desc *d, const CePlan &p, const void *xv, const void *wv,
                 const int64_t *target, char *ws, cudaStream_t st) {
+  if (d->dtype == RA_BF16)
+    return few16(d, p, (const __nv_bfloat16 *)xv, (const __nv_bfloat16 *)wv, target, ws, st);
+  if (d->dtype == RA_F16)
+    return few16(d, p, (const __half *)xv, (const __half *)wv, target, ws, st);
+  const float *x = (const float *)xv, *w = (const float *)wv;
   switch (d->rows) {
-    case 1: return few_launch<T, 1>(d, p, x, w, target, ws, st);
-    case 2: return few_launch<T, 2>(d, p, x, w, target, ws, st);
-    case 3: return few_launch<T, 3>(d, p, x, w, target, ws, st);
-    case 4: return few_launch<T, 4>(d, p, x, w, target, ws, st);
-    case 5: return few_launch<T, 5>(d, p, x, w, target, ws, st);
-    case 6: return few_launch<T, 6>(d, p, x, w, target, ws, st);
-    case 7: return few_launch<T, 7>(d, p, x, w, target, ws, st);
-    default: return few_launch<T, 8>(d, p, x, w, target, ws, st);
+    case 1: return few32<1>(d, p, x, w, target, ws, st);
+    case 2: return few32<2>(d, p, x, w, target, ws, st);
+    case 3: return few32<3>(d, p, x, w, target, ws, st);
+    case 4: return few32<4>(d, p, x, w, target, ws, st);
+    case 5: return few32<5>(d, p, x, w, target, ws, st);
+    case 6: return few32<6>(d, p, x, w, target, ws, st);
+    case 7: return few32<7>(d, p, x, w, target, ws, st);
+    default: return few32<8>(d, p, x, w, target, ws, st);
   }
 }
 
@@ -391,11 +412,7 @@ int ra_ce_forward(const ra_ce_desc *d, const void *x, const void *w, const int64
   }
   const bool few = use_few(d) && few_aligned(d, w);
   if (few) {
-    rc = d->dtype == RA_F32 ? few_forward(d, p, (const float *)x, (const float *)w, target, ws, st)
-         : d->dtype == RA_BF16
-             ? few_forward(d, p, (const __nv_bfloat16 *)x, (const __nv_bfloat16 *)w, target, ws, st)
-             : few_forward(d, p, (const __half *)x, (const __half *)w, target, ws, st);
-    if (rc) return rc;
+    if ((rc = few_forward(d, p, x, w, target, ws, st))) return rc;
     return join_rows(d, (const float2 *)(ws + p.f_part), kCeFewRows, p.few_ctas, 0, d->rows, target,
                      loss, lse, sb, ws, p, st);
   }

@@ -1,16 +1,14 @@
 // ra_ce_few.cuh -- forward of the linear cross entropy for up to eight rows:
-// scoring a few tokens against the whole table.
+// scoring a few tokens against the whole table; fp32 inputs, and what it shares
+// with the 16-bit form (ra_ce_few16.cuh).
 //
 // Bound by the table's bytes, each read once.  x stays in shared memory in fp32;
 // a warp takes four rows of the table at a time, 32 lanes x 8 columns, with all
 // N dots of the four in registers.  The 4 N dots are joined over the lanes by
 // halving, so that each lane ends with one logit (or a copy of one) and its own
 // running maximum and sum; those are joined over the warp and the CTA, and the
-// CTAs by ce_rows_kernel.  Exact products of the inputs, fp32 sums: fp32 inputs
-// need no halves here.
-// Measured: 5 rows against 131072 x 1024 in bf16 (268 MB): 62 us (4.3 TB/s); the
-// product kernel of ra_gemm16.cuh, 128 rows for these few, 66 us, and for fp32
-// inputs two more passes over the table for their halves.
+// CTAs by ce_rows_kernel.  Exact products of the inputs, fp32 sums: no halves.
+// Measured: 5 rows against 131072 x 1024 (537 MB): CEF32.
 #pragma once
 
 #include "ra_ce.cuh"
@@ -21,10 +19,43 @@ namespace ra {
 constexpr int kCeFewRows = 8, kCeFewWarps = 8, kCeFewTable = 4;  // table rows a warp
 constexpr size_t kCeFewSmem = 64 * 1024;  // most of x in shared memory: three CTAs an SM
 
-template <class T, int N>
+// one more logit (base 2) to a running maximum and sum
+__device__ __forceinline__ void ce_few_add(float &m, float &l, float z) {
+  const float mx = fmaxf(m, z);
+  if (mx > -INFINITY) {
+    l = (m > -INFINITY ? l * ex2(m - mx) : l) + ex2(z - mx);
+    m = mx;
+  } else {
+    l += z != z ? z : 0.f;
+  }
+}
+// those of the lanes FROM, 2 FROM .. apart, below TO
+template <int FROM, int TO>
+__device__ __forceinline__ void ce_few_join(float &m, float &l) {
+  float mx = m;
+#pragma unroll
+  for (int o = FROM; o < TO; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
+  l *= m > -INFINITY ? ex2(m - mx) : 1.f;  // without a maximum: 0, or NaN
+#pragma unroll
+  for (int o = FROM; o < TO; o <<= 1) l += __shfl_xor_sync(kFull, l, o);
+  m = mx;
+}
+// and of the warps (sml[warp * ld]), to the CTA's part of row n
+__device__ __forceinline__ void ce_few_cta(const float2 *sml, int ld, float2 *part, int n) {
+  float M = -INFINITY, S = 0.f;
+  for (int k = 0; k < kCeFewWarps; ++k) M = fmaxf(M, sml[k * ld].x);
+  for (int k = 0; k < kCeFewWarps; ++k) {
+    const float2 s = sml[k * ld];
+    S += s.x > -INFINITY ? s.y * ex2(s.x - M) : s.y;
+  }
+  part[blockIdx.x * kCeFewRows + n] = make_float2(M, S);
+}
+
+template <int N>
 __global__ void __launch_bounds__(32 * kCeFewWarps, 2)
-    ce_few_kernel(const T *x, int64_t ldx, const T *w, int64_t ldw, int rows, int64_t vocab, int dim,
+    ce_few_kernel(const float *x, int64_t ldx, const float *w, int64_t ldw, int rows, int64_t vocab, int dim,
                   float scale, float cap, const int64_t *target, float2 *part, float *zt) {
+  using T = float;
   constexpr int R = kCeFewTable, NP = N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8, NV = R * NP,
                 kDup = 32 / NV;  // lanes with the same logit
   // x: of each eight columns the first four, then (dim / 2 floats on) the others,
@@ -89,33 +120,14 @@ __global__ void __launch_bounds__(32 * kCeFewWarps, 2)
     if (cap > 0.f) z = capl * tanh_step(z);
     if (mr < left) {
       if (tg == v0 + mr) zt[mn] = z;
-      const float mx = fmaxf(m, z);
-      if (mx > -INFINITY) {
-        l = (m > -INFINITY ? l * ex2(m - mx) : l) + ex2(z - mx);
-        m = mx;
-      } else {
-        l += z != z ? z : 0.f;
-      }
+      ce_few_add(m, l, z);
     }
   }
   // the R lanes of a row, then the warps
-  float mx = m;
-#pragma unroll
-  for (int o = kDup; o < kDup * R; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
-  l *= m > -INFINITY ? ex2(m - mx) : 1.f;  // without a maximum: 0, or NaN
-#pragma unroll
-  for (int o = kDup; o < kDup * R; o <<= 1) l += __shfl_xor_sync(kFull, l, o);
-  if (lane % (kDup * R) == 0) sml[warp][mn] = make_float2(mx, l);
+  ce_few_join<kDup, kDup * R>(m, l);
+  if (lane % (kDup * R) == 0) sml[warp][mn] = make_float2(m, l);
   __syncthreads();
-  if (threadIdx.x < N) {
-    float M = -INFINITY, S = 0.f;
-    for (int k = 0; k < kCeFewWarps; ++k) M = fmaxf(M, sml[k][threadIdx.x].x);
-    for (int k = 0; k < kCeFewWarps; ++k) {
-      const float2 s = sml[k][threadIdx.x];
-      S += s.x > -INFINITY ? s.y * ex2(s.x - M) : s.y;
-    }
-    part[blockIdx.x * kCeFewRows + threadIdx.x] = make_float2(M, S);
-  }
+  if (threadIdx.x < N) ce_few_cta(&sml[0][threadIdx.x], NP, part, threadIdx.x);
 }
 
 }  // namespace ra
