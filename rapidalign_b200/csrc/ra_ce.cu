@@ -106,7 +106,7 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   const int64_t pass = std::min<int64_t>(d->rows, kCeRowsPerPass);
   p.tn_z = tile_width(ceil_div(pass, (int64_t)kGmM), d->vocab, sms, split);
   p.parts = kGmParts * (int)ceil_div(d->vocab, (int64_t)p.tn_z);
-  const int few_rows = kCeFewWarps * (split ? kCeFewTable : kCeFew16Rows);
+  const int few_rows = kCeFewWarps * (split ? 2 : kCeFew16Rows);  // a CTA, at least
   p.few_ctas = (int)std::min<int64_t>(ceil_div(d->vocab, (int64_t)few_rows), split ? 2 * sms : sms);
   size_t o = 0;
   p.f_part = o;
@@ -237,20 +237,27 @@ int halves(const ra_ce_desc *d, const CePlan &p, const void *x, const void *w, c
   return launched();
 }
 
-template <int N>
+template <int N, int LPK>
 int few32(const ra_ce_desc *d, const CePlan &p, const float *x, const float *w,
           const int64_t *target, char *ws, cudaStream_t st) {
-  auto k = ce_few_kernel<N>;
+  auto k = ce_few_kernel<N, LPK>;
   static OncePerDevice once;
   if (!once([&] {
         return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     (int)kCeFewSmem) == cudaSuccess;
       }))
     return RA_ERR_CUDA;
-  k<<<(unsigned)p.few_ctas, 32 * kCeFewWarps, (size_t)N * d->dim * 4, st>>>(
+  k<<<(unsigned)p.few_ctas, 32 * kCeFewWarps, (size_t)d->rows * d->dim * 4, st>>>(
       x, d->ld_x, w, d->ld_w, (int)d->rows, d->vocab, d->dim, d->scale, d->softcap, target,
       (float2 *)(ws + p.f_part), (float *)(ws + p.f_zt));
   return launched();
+}
+template <int N>
+int few_width(const ra_ce_desc *d, const CePlan &p, const float *x, const float *w,
+              const int64_t *target, char *ws, cudaStream_t st) {
+  return d->dim <= 64    ? few32<N, 8>(d, p, x, w, target, ws, st)
+         : d->dim <= 128 ? few32<N, 16>(d, p, x, w, target, ws, st)
+                         : few32<N, 32>(d, p, x, w, target, ws, st);
 }
 template <class T>
 int few16(const ra_ce_desc *d, const CePlan &p, const T *x, const T *w, const int64_t *target,
@@ -274,16 +281,10 @@ int few_forward(const ra_ce_desc *d, const CePlan &p, const void *xv, const void
   if (d->dtype == RA_F16)
     return few16(d, p, (const __half *)xv, (const __half *)wv, target, ws, st);
   const float *x = (const float *)xv, *w = (const float *)wv;
-  switch (d->rows) {
-    case 1: return few32<1>(d, p, x, w, target, ws, st);
-    case 2: return few32<2>(d, p, x, w, target, ws, st);
-    case 3: return few32<3>(d, p, x, w, target, ws, st);
-    case 4: return few32<4>(d, p, x, w, target, ws, st);
-    case 5: return few32<5>(d, p, x, w, target, ws, st);
-    case 6: return few32<6>(d, p, x, w, target, ws, st);
-    case 7: return few32<7>(d, p, x, w, target, ws, st);
-    default: return few32<8>(d, p, x, w, target, ws, st);
-  }
+  return d->rows <= 1   ? few_width<1>(d, p, x, w, target, ws, st)
+         : d->rows <= 2 ? few_width<2>(d, p, x, w, target, ws, st)
+         : d->rows <= 4 ? few_width<4>(d, p, x, w, target, ws, st)
+                        : few_width<8>(d, p, x, w, target, ws, st);
 }
 
 // The rows' losses from their parts.  Many rows: 8 threads a row in CTAs of 256
