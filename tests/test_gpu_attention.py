@@ -18,6 +18,7 @@ element, so their elements are off by 2^-38 of it.
 Positions and sigma get dS as it is, in fp32.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -473,6 +474,70 @@ def test_other_stream_and_capture(dtype, cuda_device):
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [16, 40, 128])
+def test_few_rows_of_slices_replayed(dim, dtype, cuda_device):
+    """One query a graph against slices of a fused projection whose other
+    columns hold NaN, and a replayed graph of it on new values."""
+    nq, nk = [1, 1, 1], [9000, 1, 33]
+    d = make(nq, nk, 6, 2, dim, dtype, 2, seed=dim)
+    fused = torch.full((sum(nk), 2, 2 * dim + 24), math.nan, dtype=dtype, device="cuda")
+    k, v = fused[..., 8:8 + dim], fused[..., 16 + dim:16 + 2 * dim]
+    k.copy_(d["k"]), v.copy_(d["v"])
+    d["k"], d["v"] = k, v
+    seg = ra.attention_segments(ptr(nq), ptr(nk))
+
+    def step():
+        return ra.pyg_kernel_attention(d["q"], k, v, segments=seg, q_pos=d["q_pos"],
+                                       k_pos=d["k_pos"], sigma=d["sigma"])
+
+    (o64, bo), _ = exact(d, nq, nk, dim ** -0.5, 0.0)
+    close(step(), o64, bo, "out")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for n, t in make(nq, nk, 6, 2, dim, dtype, 2, seed=dim + 1).items():
+        d[n].copy_(t)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, step())
+    (o64, bo), _ = exact(d, nq, nk, dim ** -0.5, 0.0)
+    close(held, o64, bo, "replayed out")
+
+
+def test_calls_from_two_threads(cuda_device):
+    """Calls at the same time, each on its own stream: what each is alone."""
+    sizes = [([1] * 5, [700, 3, 64, 65, 2000]), ([90, 200], [90, 200])]
+    data = [make(*n, 4, 2, 64, torch.bfloat16, 3, seed=i) for i, n in enumerate(sizes)]
+    segs = [ra.attention_segments(ptr(a), ptr(b)) for a, b in sizes]
+
+    def step(i):
+        x = {n: t.detach().requires_grad_(n != "g") for n, t in data[i].items()}
+        o = ra.pyg_kernel_attention(x["q"], x["k"], x["v"], segments=segs[i], q_pos=x["q_pos"],
+                                    k_pos=x["k_pos"], sigma=x["sigma"])
+        return (o.detach(), *torch.autograd.grad(o, [x["q"], x["k"], x["v"]], x["g"]))
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i].extend(step(i) for _ in range(20))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 20
+        assert all(torch.equal(a, b) for g in got[i] for a, b in zip(g, want[i]))
 
 
 def test_refusals_on_the_device(cuda_device):

@@ -338,6 +338,37 @@ def test_other_stream_and_capture(dtype, cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(held, step()))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(1, 1, 8), (3, 15, 24), (5, 17, 56), (8, 4097, 72),
+                                   (6, 300, 128), (7, 129, 136), (8, 20000, 64)])
+def test_few_rows_of_a_wider_table(n, v, d, dtype, cuda_device):
+    """Tables and rows as slices, NaN in what lies between; every row's target
+    in turn at the ends of the table; replayed from a graph."""
+    x, w, t = make(n, v, d, dtype, seed=v, ignore=0)
+    wide = torch.full((v, d + 8), math.nan, dtype=dtype, device="cuda")
+    wide[:, :d] = w
+    rows = torch.full((n, d + 16), math.nan, dtype=dtype, device="cuda")
+    rows[:, 8:8 + d] = x
+    t[-1], t[0] = 0, v - 1
+    w, x = wide[:, :d], rows[:, 8:8 + d]
+    check(x, w, t, reduction="none", lse_weight=0.3)
+    step = lambda: ra.linear_cross_entropy(x, w, t, softcap=3.0, reduction="none")  # noqa: E731
+    want = step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    x.copy_(make(n, v, d, dtype, seed=v + 1)[0])
+    graph.replay()
+    torch.cuda.synchronize()
+    got = step()
+    assert all(torch.equal(a, b) for a, b in zip(held, got))
+    assert not torch.equal(got[1], want[1]) or v == 1
+    (r64, l64, _, _), (br, bl, _, _) = exact(x, w, t, 1.0, 3.0, torch.ones(n, device="cuda"),
+                                             torch.zeros(n, device="cuda"))
+    close(got[0], r64, br, "loss")
+    close(got[1], l64, bl, "lse")
+
+
 def test_launches_are_counted(cuda_device):
     x, w, t = make(50, 60, 32, torch.bfloat16)
     before = _lib.launch_count()
