@@ -264,8 +264,8 @@ int tc_forward(const ra_attn_desc *d, const Operands &o, const AttnArgs &a, Attn
                cudaStream_t st) {
   using C = FwdCfg<Kind, DP>;
   if (!map_operands(d, o, C::BR, x)) return RA_ERR_INVALID_ARGUMENT;
-  return launch<attn_tc_fwd_kernel<Kind, DP>>(a.n_q_tiles * a.heads * x->splits, 128, C::smem, a,
-                                              *x, st);
+  return launch<attn_tc_fwd_kernel<Kind, DP>>(a.n_q_tiles * a.heads * x->splits, C::NT, C::smem,
+                                              a, *x, st);
 }
 template <class Kind, int DP>
 int tc_backward(const ra_attn_desc *d, const Operands &o, const AttnArgs &a, AttnTcArgs *x,

@@ -339,9 +339,9 @@ __host__ __device__ constexpr int tmem_round(int c) {
 // dim of a row's fp32 values (from TMEM, times f) to T and to fp32
 template <class T, int DP, bool SMALL>
 __device__ __forceinline__ void write_row(uint32_t taddr, float f, bool on, bool zero, int dim,
-                                          T *out, float *out32) {
+                                          T *out, float *out32, int c0 = 0, int c1 = DP) {
 #pragma unroll 1
-  for (int c = 0; c < DP; c += 32) {
+  for (int c = c0; c < c1; c += 32) {
     float v[32];
     tmem_ld32(taddr + c, v);
     if (SMALL) {
@@ -514,9 +514,9 @@ template <class Kind, int DP>
 constexpr int dkv_rows = 64 + (Kind::pair ? 4 : 2) * DP <= 128          ? 32
                          : !Kind::pair && DP == 128 || Kind::pair && DP == 64 ? 128
                                                                         : 64;
-// CTAs that fit an SM beside each other
-constexpr int attn_ctas(int smem, int tmem, int threads) {
-  int n = 4 * 128 / threads;
+// CTAs that fit an SM beside each other, with `regs` registers a thread
+constexpr int attn_ctas(int smem, int tmem, int threads, int regs = 128) {
+  int n = 65536 / (regs * threads);
   if (n > 512 / tmem) n = 512 / tmem;
   while (n > 1 && n * (smem + 1024) > 228 * 1024) --n;
   return n;
@@ -533,8 +533,13 @@ struct FwdCfg {
   static constexpr int pos = Q + 4 * KV;                 // TilePos<KT> [2]
   static constexpr int val = pos + 2 * KT * 12;          // unsigned [2][2]
   static constexpr int bar = val + 16, slot = bar + 24;  // slot: also the mask's extent
-  static constexpr int smem = slot + 8 + 1024;           // 1024: the tiles' alignment
-  static constexpr int CTAS = attn_ctas(smem, TMEM, 128);
+  static constexpr int top = slot + 8;                   // float [PARTS][128]
+  // threads of a row: half of the columns each where TMEM or shared memory holds
+  // fewer than four CTAs
+  static constexpr int PARTS = attn_ctas(Q + 4 * KV, TMEM, 128) < 4 ? 2 : 1;
+  static constexpr int NT = 128 * PARTS, C = KT / 32 / PARTS;  // 32-column chunks a thread
+  static constexpr int smem = top + PARTS * 512 + 1024;        // 1024: the tiles' alignment
+  static constexpr int CTAS = attn_ctas(smem, TMEM, NT, 128);
 };
 
 // Work for one thread, on the last two of NT threads' warps: issuing a tile's
@@ -555,10 +560,10 @@ __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
 }
 
 template <class Kind, int DP>
-__global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
+__global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     attn_tc_fwd_kernel(const AttnArgs A, const __grid_constant__ AttnTcArgs X) {
   using C = FwdCfg<Kind, DP>;
-  constexpr int KT = C::KT;
+  constexpr int KT = C::KT, NT = C::NT, PARTS = C::PARTS;
   extern __shared__ uint8_t raw_sm[];
   uint8_t *sm = align1024(raw_sm);
   const uint32_t base = smem_u32(sm);
@@ -566,16 +571,18 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
                  full = bar + 8;
   TilePos<KT> *kpos = reinterpret_cast<TilePos<KT> *>(sm + C::pos);
   unsigned *kval = reinterpret_cast<unsigned *>(sm + C::val);
+  float *top = reinterpret_cast<float *>(sm + C::top);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = threadIdx.x & 127, part = warp >> 2;  // its share of the columns
 
   const int64_t item = blockIdx.x;
   const int split = (int)(item % X.splits);
   const int h = (int)(item / X.splits % A.heads), hk = h / (A.heads / A.kv_heads);
   const int4 tile = A.qs.tile(item / X.splits / A.heads, A.ks);
   const int i0 = tile.x, nq = tile.y, j0 = tile.z;
-  const int64_t i = i0 + (int)threadIdx.x;
-  const bool row_on = threadIdx.x < nq && (A.q_mask == nullptr || A.q_mask[i] != 0);
-  const int nk = (int)masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, tile.w, 128,
+  const int64_t i = i0 + row;
+  const bool row_on = row < nq && (A.q_mask == nullptr || A.q_mask[i] != 0);
+  const int nk = (int)masked_extent(A.k_mask ? A.k_mask + j0 : nullptr, tile.w, NT,
                                     reinterpret_cast<unsigned long long *>(sm + C::slot));
   // no row to work for: no keys to see
   const int64_t all = __syncthreads_or(row_on) ? (nk + KT - 1) / KT : 0;
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + C::slot);
-  const uint32_t tS = tmem, tO = tmem + KT, lane_off = (uint32_t)(32 * warp) << 16;
+  const uint32_t tS = tmem, tO = tmem + KT, lane_off = (uint32_t)(32 * (warp & 3)) << 16;
 
   AttnScore sc;
   sc.init(A, h);
@@ -639,10 +646,10 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
   rp.set(row_on ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
   constexpr float kUp = Kind::bf16 ? 0.f : 7.f;  // P is held 2^kUp up
   const bool p_pair = Kind::pair || X.pair_p;
-  float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to
+  float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to; l: this part's
   unsigned phase = 0;
 
-  if (t0 < t1 && threadIdx.x == kMmaThread<128>) {
+  if (t0 < t1 && threadIdx.x == kMmaThread<NT>) {
     products_rows<Kind, KT, DP>(tS, sQ, sK + (t0 & 1) * C::KV);
     tc_commit(bar);
   }
@@ -652,17 +659,18 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {  // the products on its buffers are done
-      if (threadIdx.x == kTmaThread<128>) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
       fetch(t + 1);
     }
-    f2_t s2[KT / 32][16];
+    f2_t s2[C::C][16];
     float mx = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < KT / 32; ++c) {
+    for (int c = 0; c < C::C; ++c) {
+      const int at = C::C * part + c;
       float v[32];
-      tmem_ld32(tS + lane_off + 32 * c, v);
-      scores32<Kind>(v, s2[c], sc, A.pos_dim > 0, kpos[b], 32 * c, rp);
-      const unsigned bits = kval[2 * b + c];
+      tmem_ld32(tS + lane_off + 32 * at, v);
+      scores32<Kind>(v, s2[c], sc, A.pos_dim > 0, kpos[b], 32 * at, rp);
+      const unsigned bits = kval[2 * b + at];
       if (bits != kFull) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -675,6 +683,11 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
 #pragma unroll
       for (int j = 0; j < 16; ++j) mx = fmaxf(mx, fmaxf(lo_of(s2[c][j]), hi_of(s2[c][j])));
     }
+    if (PARTS > 1) {  // the row's: the four pairs of warps that share rows
+      top[part * 128 + row] = mx;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+      mx = fmaxf(mx, top[(part ^ 1) * 128 + row]);
+    }
     // the reference follows the maximum only where it grew by more than 2^8:
     // sums and O stay relative to one reference, whichever it is
     const bool grow = mx > m + 8.f;  // also from -inf
@@ -684,7 +697,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
       l *= f;
       if (t > t0) {
 #pragma unroll 1
-        for (int c = 0; c < (C::SMALL ? 2 : 1) * DP; c += 32) {
+        for (int c = 32 * part; c < (C::SMALL ? 2 : 1) * DP; c += 32 * PARTS) {
           float o[32];
           tmem_ld32(tO + lane_off + c, o);
           uint32_t u[32];
@@ -698,7 +711,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
     const f2_t ref = two(kUp - (m > -INFINITY ? m : 0.f));
     f2_t sum[2] = {0, 0};
 #pragma unroll
-    for (int c = 0; c < KT / 32; ++c) {
+    for (int c = 0; c < C::C; ++c) {
       float v[32];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -708,7 +721,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
         v[2 * j + 1] = ex2(y);
         sum[j & 1] = add2(sum[j & 1], pk(v[2 * j], v[2 * j + 1]));
       }
-      put_weights<Kind>(tS + lane_off + 32 * c, v, p_pair);
+      put_weights<Kind>(tS + lane_off + 32 * (C::C * part + c), v, p_pair);
     }
     const f2_t both = add2(sum[0], sum[1]);
     l += lo_of(both) + hi_of(both);
@@ -719,7 +732,7 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == kMmaThread<128>) {
+    if (threadIdx.x == kMmaThread<NT>) {
       tc_fence_after();
       products_weighted<Kind, KT, DP, C::SMALL>(tO, tS, sV + b * C::KV, p_pair, t > t0);
       if (t + 1 < t1) products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
@@ -733,23 +746,33 @@ __global__ void __launch_bounds__(128, FwdCfg<Kind, DP>::CTAS)
   bad = __syncthreads_or(bad);
   if (bad && threadIdx.x == 0) atomicOr(A.status, 1);
 
+  if (PARTS > 1) {
+    if (part > 0) top[row] = l;
+    __syncthreads();
+    if (part == 0) top[row] = l += top[row];
+    __syncthreads();
+    l = top[row];
+  }
   const bool any = l > 0.f || l != l;
   const bool empty = !row_on || !any || t0 >= t1;
   using T = typename Kind::T;
   const float unscale = ldexpf(1.f, -elem_exp<Kind>(X, kWv));
-  const bool in = threadIdx.x < nq;
+  const bool in = row < nq;
+  // the row's columns: every PARTS-th 32, or what there is
+  constexpr int W = DP / PARTS < 32 ? 32 : DP / PARTS;
+  const int c0 = W * part, c1 = DP < c0 + W ? DP : c0 + W;
   if (X.splits > 1) {
     float *po = X.part_o + ((split * A.num_q + i) * A.heads + h) * A.dim;
-    write_row<float, DP, C::SMALL>(tO + lane_off, unscale, in, empty, A.dim, po, nullptr);
-    if (in)
+    write_row<float, DP, C::SMALL>(tO + lane_off, unscale, in, empty, A.dim, po, nullptr, c0, c1);
+    if (in && part == 0)
       X.part_s[((int64_t)split * A.heads + h) * A.num_q + i] =
           make_float2(empty ? -INFINITY : (m > -INFINITY ? m : 0.f) - kUp, empty ? 0.f : l);
   } else {
     const float r = empty ? 0.f : 1.f / l;
     const int64_t at = (i * A.heads + h) * A.dim;
     write_row<T, DP, C::SMALL>(tO + lane_off, unscale * r, in, empty, A.dim, (T *)A.out + at,
-                     A.out32 ? A.out32 + at : nullptr);
-    if (in && A.neg_m) A.put_stats(h, i, empty ? INFINITY : (m > -INFINITY ? m : 0.f) - kUp, r);
+                     A.out32 ? A.out32 + at : nullptr, c0, c1);
+    if (in && part == 0 && A.neg_m) A.put_stats(h, i, empty ? INFINITY : (m > -INFINITY ? m : 0.f) - kUp, r);
   }
   tc_fence_before();
   __syncthreads();
