@@ -272,7 +272,9 @@ def check(code: int, what: str = "") -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: a Stream object costs as much as a kernel launch
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -291,6 +293,11 @@ def scratch(nbytes: int, device: torch.device) -> torch.Tensor:
     as they are (a few microseconds of a small call)."""
     buf = torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
     return buf if buf.data_ptr() % 256 == 0 else workspace(nbytes, device)
+
+
+def empty_as(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape and device."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 _HERE_ALREADY = contextlib.nullcontext()

@@ -166,13 +166,13 @@ class _KernelAttention(torch.autograd.Function):
         inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in tensors])
         ref = ctypes.byref(d)
         with _lib.on_device(dev):
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            out = _lib.empty_as(q)
             out32 = stats = None
             if need_grad:
                 # unrounded outputs: the backward's do.o would carry the
                 # rounding of 16 bits into every score's gradient
                 if q.dtype != torch.float32:
-                    out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
+                    out32 = _lib.empty_as(q, torch.float32)
                 stats = torch.empty((2, d.heads, d.num_q), dtype=torch.float32, device=dev)
             n_state, n_ws = lib.ra_attn_state_bytes(ref), lib.ra_attn_workspace_bytes(ref, 0)
             # a small workspace lies behind the state
@@ -204,10 +204,8 @@ class _KernelAttention(torch.autograd.Function):
             g = g.clone()
         need = ctx.needs_input_grad
         with _lib.on_device(dev):
-            grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need[i] else None
-                     for i, t in enumerate((q, k, v))]
-            grads += [torch.empty(t.shape, dtype=torch.float32, device=dev)
-                      if t is not None and need[3 + i] else None
+            grads = [_lib.empty_as(t) if need[i] else None for i, t in enumerate((q, k, v))]
+            grads += [_lib.empty_as(t, torch.float32) if t is not None and need[3 + i] else None
                       for i, t in enumerate((q_pos, k_pos))]
             grads.append(torch.empty(d.heads, dtype=torch.float32, device=dev) if need[5] else None)
             gr = _lib.RaAttnGrads(*[_lib.ptr(t) for t in grads])
@@ -223,7 +221,8 @@ class _KernelAttention(torch.autograd.Function):
         for i, t in ((3, q_pos), (4, k_pos)):
             if grads[i] is not None and t.dtype != torch.float32:
                 grads[i] = grads[i].to(t.dtype)
-        if grads[5] is not None:
+        if grads[5] is not None and not (sigma.shape == grads[5].shape and sigma.device == dev
+                                         and sigma.dtype == torch.float32):
             s = grads[5] if sigma.numel() == d.heads else grads[5].sum()
             grads[5] = s.reshape(sigma.shape).to(device=sigma.device, dtype=sigma.dtype)
         return (*grads, None, None, None, None, None)

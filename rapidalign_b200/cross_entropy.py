@@ -89,8 +89,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         gl = None if g_loss is None else g_loss.to(torch.float32).contiguous()
         ge = None if g_lse is None else g_lse.to(torch.float32).contiguous()
         with _lib.on_device(dev):
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-            dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
+            dx = _lib.empty_as(x) if need_x else None
+            dw = _lib.empty_as(weight) if need_w else None
             ws = _lib.scratch(lib.ra_ce_workspace_bytes(ctypes.byref(d), 1), dev)
             rc = lib.ra_ce_backward(ctypes.byref(d), xk.data_ptr(), wk.data_ptr(),
                                     target.data_ptr(), _lib.ptr(gl), _lib.ptr(ge), _lib.ptr(dx),

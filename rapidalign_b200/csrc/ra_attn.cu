@@ -213,7 +213,8 @@ bool map_operand(const ra_attn_desc *d, AttnMap *m, const void *hi, const void *
   const bool bf16 = d->dtype == RA_BF16;
   const int dp = padded_dim(d), cw = dp == 32 ? 32 : 64;
   return map_heads(&m->hi, bf16, hi, rows, heads, d->dim, row, head, cw, br) &&
-         map_heads(&m->lo, bf16, lo, rows, heads, d->dim, row, head, cw, br);
+         (d->dtype != RA_F32 ||
+          map_heads(&m->lo, bf16, lo, rows, heads, d->dim, row, head, cw, br));
 }
 
 // What the kernels read: q, k, v as given or the halves in the state, dout
