@@ -167,26 +167,31 @@ class _KernelAttention(torch.autograd.Function):
         ref = ctypes.byref(d)
         with _lib.on_device(dev):
             out = _lib.empty_as(q)
-            out32 = stats = None
+            out32 = None
+            n_stats = 0
             if need_grad:
                 # unrounded outputs: the backward's do.o would carry the
                 # rounding of 16 bits into every score's gradient
                 if q.dtype != torch.float32:
                     out32 = _lib.empty_as(q, torch.float32)
-                stats = torch.empty((2, d.heads, d.num_q), dtype=torch.float32, device=dev)
+                n_stats = 8 * d.heads * d.num_q
             n_state, n_ws = lib.ra_attn_state_bytes(ref), lib.ra_attn_workspace_bytes(ref, 0)
-            # a small workspace lies behind the state
-            state = _lib.scratch(n_state + (n_ws if n_ws <= 256 else 0), dev)
+            # the state, a small workspace and the statistics share a buffer
+            held = (n_state + 255) // 256 * 256
+            at_stats = held + (n_ws if n_ws <= 256 else 0)
+            state = _lib.scratch(at_stats + n_stats, dev)
             ws = None if n_ws <= 256 else _lib.scratch(n_ws, dev)
+            base = state.data_ptr()
+            stats = base + at_stats if n_stats else None
             rc = lib.ra_attn_forward(ref, ctypes.byref(inp), out.data_ptr(), _lib.ptr(out32),
-                                     _lib.ptr(stats), state.data_ptr(), n_state,
-                                     state.data_ptr() + n_state if ws is None else ws.data_ptr(),
-                                     n_ws, _lib.stream_handle(dev))
+                                     stats, base, n_state,
+                                     base + held if ws is None else ws.data_ptr(), n_ws,
+                                     _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention")
         if need_grad:
-            ctx.desc, ctx.state, ctx.inp = d, state, inp
+            ctx.desc, ctx.state, ctx.inp, ctx.stats = d, state, inp, stats
             ctx.save_for_backward(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask,
-                                  out if out32 is None else out32, stats)
+                                  out if out32 is None else out32)
             # what the pointers of `inp` belong to, where it is not saved above
             ctx.keep = (*[None if t is o or t.data_ptr() == o.data_ptr() else t
                           for t, o in ((qr, q), (kr, k), (vr, v))],
@@ -197,7 +202,7 @@ class _KernelAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         lib = _lib.load()
-        q, k, v, q_pos, k_pos, sigma, _, _, out32, stats = ctx.saved_tensors
+        q, k, v, q_pos, k_pos, sigma, _, _, out32 = ctx.saved_tensors
         d, dev = ctx.desc, q.device
         g = g.contiguous()
         if g.data_ptr() % 16:
@@ -214,7 +219,7 @@ class _KernelAttention(torch.autograd.Function):
             f32 = q.dtype == torch.float32
             rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(ctx.inp), g.data_ptr(),
                                       out32.data_ptr() if f32 else None,
-                                      None if f32 else out32.data_ptr(), stats.data_ptr(),
+                                      None if f32 else out32.data_ptr(), ctx.stats,
                                       ctypes.byref(gr), ctx.state.data_ptr(), ctx.state.numel(),
                                       ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention backward")

@@ -25,6 +25,8 @@ __all__ = ["linear_cross_entropy"]
 _REDUCTIONS = {"none": _lib.RA_REDUCE_NONE, "sum": _lib.RA_REDUCE_SUM,
                "mean": _lib.RA_REDUCE_MEAN}
 
+_SMALL = 1 << 20  # bytes of a workspace that may live as long as its call's state
+
 
 def _rows16(t: Tensor) -> Tensor:
     """`t` (a matrix) as the kernels read it: unit stride along its rows and,
@@ -57,14 +59,19 @@ class _LinearCrossEntropy(torch.autograd.Function):
         d.ignore_index, d.dtype, d.reduction = ignore_index, _lib.DTYPES[x.dtype], reduction
         d.scale, d.softcap, d.status = scale, softcap, _lib.status_word()
         with _lib.on_device(dev):
-            state = _lib.scratch(lib.ra_ce_state_bytes(ctypes.byref(d)), dev)
-            ws = _lib.scratch(lib.ra_ce_workspace_bytes(ctypes.byref(d), 0), dev)
+            n_state = lib.ra_ce_state_bytes(ctypes.byref(d))
+            n_ws = lib.ra_ce_workspace_bytes(ctypes.byref(d), 0)
+            # a small workspace lies behind the state
+            held = (n_state + 255) // 256 * 256
+            ws = _lib.scratch(n_ws, dev) if n_ws > _SMALL else None
+            state = _lib.scratch(held if ws is not None else held + n_ws, dev)
             shape = (d.rows,) if reduction == _lib.RA_REDUCE_NONE else ()
             loss = torch.empty(shape, dtype=torch.float32, device=dev)
             lse = torch.empty(d.rows, dtype=torch.float32, device=dev)
             rc = lib.ra_ce_forward(ctypes.byref(d), xk.data_ptr(), wk.data_ptr(),
                                    target.data_ptr(), loss.data_ptr(), lse.data_ptr(),
-                                   state.data_ptr(), state.numel(), ws.data_ptr(), ws.numel(),
+                                   state.data_ptr(), n_state,
+                                   state.data_ptr() + held if ws is None else ws.data_ptr(), n_ws,
                                    _lib.stream_handle(dev))
         _lib.check(rc, "linear cross entropy")
         if ctx is None:  # no gradient wanted: without autograd's share of a small call

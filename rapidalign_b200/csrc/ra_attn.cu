@@ -277,7 +277,7 @@ int tc_backward(const ra_attn_desc *d, const Operands &o, const AttnArgs &a, Att
   if (!map_operands(d, o, Q::BR, x)) return RA_ERR_INVALID_ARGUMENT;
   if (a.dq || a.pos_q || a.dk)  // dk reads the D that this kernel puts right
     rc = launch<attn_tc_dq_kernel<Kind, DP>>(a.n_q_tiles * a.heads, Q::NT, Q::smem, a, *x, st);
-  if (K::BR != Q::BR && !map_operands(d, o, K::BR, x)) return RA_ERR_INVALID_ARGUMENT;
+  static_assert(K::BR == Q::BR, "one set of maps");
   if (!rc && (a.dk || a.dv || a.pos_k))
     rc = launch<attn_tc_dkv_kernel<Kind, DP>>(a.n_k_tiles * a.kv_heads, K::NT, K::smem, a, *x, st);
   return rc;

@@ -961,7 +961,7 @@ template <class Kind, int DP>
 struct DqCfg {
   static constexpr int KT = dq_rows<Kind, DP>;
   static constexpr int HALF = Kind::pair ? 2 : 1;
-  static constexpr int BR = KT;
+  static constexpr int BR = KT < dkv_rows<Kind, DP> ? KT : dkv_rows<Kind, DP>;
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
   // two CTAs on an SM are worth more than a second buffer
   static constexpr int STAGES = 2 * Q + 4 * KV <= 100 * 1024 ? 2 : 1;
@@ -1190,7 +1190,8 @@ template <class Kind, int DP>
 struct DkvCfg {
   static constexpr int QT = dkv_rows<Kind, DP>;
   static constexpr int HALF = Kind::pair ? 2 : 1;
-  static constexpr int BR = QT;
+  // one set of maps for both backward kernels
+  static constexpr int BR = QT < dq_rows<Kind, DP> ? QT : dq_rows<Kind, DP>;
   static constexpr int K = HALF * tile_bytes<128, DP>, QG = HALF * tile_bytes<QT, DP>;
   static constexpr bool SMALL = Kind::pair && DP <= 64;  // at 128 TMEM is full
   static constexpr int TMEM = tmem_round(2 * QT + (SMALL ? 4 : 2) * DP);
