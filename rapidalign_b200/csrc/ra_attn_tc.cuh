@@ -508,8 +508,8 @@ __global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const f
 
 // ---- forward --------------------------------------------------------------------
 
-// Rows of a streamed tile of the backward, and of its TMA boxes; 4 threads of a
-// CTA work on each row of 32 columns of it (128 threads for 32).  What counts is
+// Rows of a streamed tile of the backward, with 128 threads of the CTA for every 32
+// of them (32 columns of the scores a thread).  What counts is
 // that warps wait at different times: 32 where four CTAs then share an SM's TMEM
 // (dq of 64-wide bf16 heads: 318 us, with 64 and two CTAs 387); 128 where one
 // CTA holds the TMEM anyhow (dk, dv of 128-wide heads: 671 us, with 64 756);
