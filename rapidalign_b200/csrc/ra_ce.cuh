@@ -508,28 +508,16 @@ struct CeEpiOut {
                                       int col, const Src &src, const GmOut &out_rows) const {
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
     const int64_t w0 = r - (threadIdx.x & 31);  // the warp's first row
-    // 16-byte aligned rows: fp32 sums, or results
+    // 16-byte aligned rows: fp32 sums, or results; 8-byte ones of 16-bit results
     const bool wide = cols % (out != nullptr ? 16 / (int)sizeof(T) : 4) == 0;
+    const bool half = cols % 4 == 0;
 #pragma unroll Src::unroll
     for (int c = 0; c < TN / kGmParts; c += 32) {
       float v[32];
       src.get(c, v);
       const int64_t left = cols - (c0 + c);
       if (left <= 0) break;  // the same for the warp
-      if (!wide || left < 32) {
-        if (r < rows) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j >= left) continue;
-            if (out != nullptr) {
-              store_as(out + r * cols + c0 + c + j, v[j] * F.al);
-            } else {
-              float *q = part + ((int64_t)w.slice * rows + r) * cols + c0 + c + j;
-              *q = v[j] + (add ? *q : 0.f);
-            }
-          }
-        }
-      } else if (out != nullptr && sizeof(T) == 2) {
+      if (out != nullptr && sizeof(T) == 2) {
         uint4 x[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -539,8 +527,21 @@ struct CeEpiOut {
           memcpy(&x[q], t, 16);
         }
         out_rows.rows64(x, [&](int row_, int j, uint4 u) {
-          if (w0 + row_ < rows)
-            *reinterpret_cast<uint4 *>(out + (w0 + row_) * cols + c0 + c + 8 * j) = u;
+          if (w0 + row_ >= rows) return;
+          T *q = out + (w0 + row_) * cols + c0 + c + 8 * j;
+          const int n = (int)min((int64_t)8, left - 8 * j);
+          if (wide && n == 8) {
+            *reinterpret_cast<uint4 *>(q) = u;
+          } else if (half) {  // n is a multiple of 4
+            if (n >= 4) *reinterpret_cast<uint2 *>(q) = make_uint2(u.x, u.y);
+            if (n == 8) *reinterpret_cast<uint2 *>(q + 4) = make_uint2(u.z, u.w);
+          } else {
+            T t[8];
+            memcpy(t, &u, 16);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k < n) q[k] = t[k];
+          }
         });
       } else {
         float *base = out != nullptr ? reinterpret_cast<float *>(out)
@@ -557,10 +558,20 @@ struct CeEpiOut {
                               __float_as_uint(v[16 * hf + 4 * q + 3] * F.al));
           out_rows.rows64(x, [&](int row_, int j, uint4 u) {
             if (w0 + row_ >= rows) return;
-            float4 *q = reinterpret_cast<float4 *>(base + (w0 + row_) * cols + c0 + c + 16 * hf) + j;
-            float4 o = more ? *q : make_float4(0.f, 0.f, 0.f, 0.f);
-            *q = make_float4(o.x + __uint_as_float(u.x), o.y + __uint_as_float(u.y),
-                             o.z + __uint_as_float(u.z), o.w + __uint_as_float(u.w));
+            float *q = base + (w0 + row_) * cols + c0 + c + 16 * hf + 4 * j;
+            const int64_t n = left - 16 * hf - 4 * j;
+            if (wide && n >= 4) {
+              float4 *q4 = reinterpret_cast<float4 *>(q);
+              float4 o = more ? *q4 : make_float4(0.f, 0.f, 0.f, 0.f);
+              *q4 = make_float4(o.x + __uint_as_float(u.x), o.y + __uint_as_float(u.y),
+                                o.z + __uint_as_float(u.z), o.w + __uint_as_float(u.w));
+            } else {
+              const float t[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z),
+                                  __uint_as_float(u.w)};
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < n) q[k] = (more ? q[k] : 0.f) + t[k];
+            }
           });
         }
       }
