@@ -292,9 +292,9 @@ int join(const AttnArgs &a, const AttnFwd &f, char *ws, int sms, cudaStream_t st
   float2 *ps = (float2 *)(ws + f.part_s);
   // many parts are many loads one after another, which more warps share
   if (f.splits > 32)
-    attn_join_kernel<T, 32><<<(unsigned)rows, 1024, 0, st>>>(a, f.splits, po, ps);
+    attn_join_many_kernel<T><<<(unsigned)rows, 1024, 0, st>>>(a, f.splits, po, ps);
   else
-    attn_join_kernel<T, 8><<<(unsigned)rows, 256, 0, st>>>(a, f.splits, po, ps);
+    attn_join_kernel<T><<<grid_rows(rows, 8), 256, 0, st>>>(a, f.splits, po, ps);
   return launched();
 }
 

@@ -788,14 +788,58 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   }
 }
 
-// Joins the key ranges of a row.  A warp takes every WARPS-th range in order,
-// with the maximum as it goes; then the warps, a column a warp.
-template <class T, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS)
+// One more key range (its maximum and sum st, its values x) joined to a row's.
+template <int COLS>
+__device__ __forceinline__ void join_range(float2 st, const float (&x)[COLS], float &m, float &l,
+                                           float (&acc)[COLS]) {
+  const float mx = fmaxf(m, st.x);
+  const float keep = m > -INFINITY ? ex2(m - mx) : 0.f;
+  const float f = st.x > -INFINITY ? ex2(st.x - mx) : 0.f;  // else l and o are 0
+  l = fmaf(st.y, f, l * keep);
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) acc[c] = fmaf(f, x[c], acc[c] * keep);
+  m = mx;
+}
+constexpr int kJoinCols = 128 / 32;  // columns a lane: ranges are for widths up to 128
+// Joins the key ranges of the rows, a warp a row, the maximum as it goes.
+template <class T>
+__global__ void __launch_bounds__(256)
     attn_join_kernel(const AttnArgs A, int splits, const float *part_o, const float2 *part_s) {
-  __shared__ float so[WARPS][kAttnMaxDim / 2 + 1];
+  const int lane = threadIdx.x & 31;
+  const int64_t n = A.num_q * A.heads, r = blockIdx.x * 8LL + (threadIdx.x >> 5), i = r / A.heads;
+  if (r >= n) return;
+  const int h = (int)(r % A.heads);
+  const float2 *ps = part_s + (int64_t)h * A.num_q + i;
+  float m = -INFINITY, l = 0.f, acc[kJoinCols] = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float *po = part_o + (s * n + r) * A.dim;
+    float x[kJoinCols];
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c)
+      x[c] = lane + 32 * c < A.dim ? po[lane + 32 * c] : 0.f;
+    join_range(ps[s * n], x, m, l, acc);
+  }
+  const bool any = l > 0.f || l != l;
+  const float rl = any ? 1.f / l : 0.f;
+#pragma unroll
+  for (int c = 0; c < kJoinCols; ++c)
+    if (lane + 32 * c < A.dim) {
+      const float o = any ? acc[c] * rl : 0.f;
+      put((T *)A.out + r * A.dim + lane + 32 * c, o);
+      if (A.out32) A.out32[r * A.dim + lane + 32 * c] = o;
+    }
+  if (lane == 0 && A.neg_m) A.put_stats(h, i, any ? m : INFINITY, rl);
+}
+// The same with 32 warps a row, for many ranges: a warp takes every 32nd, then
+// the warps are joined, a column a warp.
+template <class T>
+__global__ void __launch_bounds__(1024)
+    attn_join_many_kernel(const AttnArgs A, int splits, const float *part_o, const float2 *part_s) {
+  constexpr int WARPS = 32;
+  __shared__ float so[WARPS][kJoinCols * 32 + 1];
   __shared__ float2 sl[WARPS];
-  constexpr int COLS = kAttnMaxDim / 2 / 32;  // ranges are for widths up to 128
+  constexpr int COLS = kJoinCols;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n = A.num_q * A.heads, r = blockIdx.x, i = r / A.heads;
   const int h = (int)(r % A.heads);
@@ -808,20 +852,14 @@ __global__ void __launch_bounds__(32 * WARPS)
     float x[COLS];
 #pragma unroll
     for (int c = 0; c < COLS; ++c) x[c] = lane + 32 * c < A.dim ? po[lane + 32 * c] : 0.f;
-    const float mx = fmaxf(m, st.x);
-    const float keep = m > -INFINITY ? ex2(m - mx) : 0.f;
-    const float f = st.x > -INFINITY ? ex2(st.x - mx) : 0.f;  // else l and o are 0
-    l = fmaf(st.y, f, l * keep);
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) acc[c] = fmaf(f, x[c], acc[c] * keep);
-    m = mx;
+    join_range(st, x, m, l, acc);
   }
 #pragma unroll
   for (int c = 0; c < COLS; ++c)
     if (lane + 32 * c < A.dim) so[warp][lane + 32 * c] = acc[c];
   if (lane == 0) sl[warp] = make_float2(m, l);
   __syncthreads();
-  const float2 st = lane < WARPS ? sl[lane] : make_float2(-INFINITY, 0.f);
+  const float2 st = sl[lane];
   m = st.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
@@ -830,7 +868,7 @@ __global__ void __launch_bounds__(32 * WARPS)
   const bool any = l > 0.f || l != l;
   const float rl = any ? 1.f / l : 0.f;
   for (int d = warp; d < A.dim; d += WARPS) {
-    float o = warp_sum(lane < WARPS ? so[lane][d] * f : 0.f);
+    float o = warp_sum(so[lane][d] * f);
     o = any ? o * rl : 0.f;
     if (lane == 0) {
       put((T *)A.out + r * A.dim + d, o);
