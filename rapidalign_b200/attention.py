@@ -131,6 +131,32 @@ def _floats(t: Tensor) -> Tensor:
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
+def _dense16(t: Tensor) -> Tensor:
+    """`t` contiguous, on a 16-byte boundary."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _operands(d, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, plan):
+    """What the kernels read of one pass's tensors: the strides into `d`, the
+    addresses, and the tensors these belong to (copies among them), which have to
+    live until the pass is launched."""
+    qr, kr, vr = _rows(q), _rows(k), _rows(v)
+    d.q_row, d.q_head = qr.stride()[:2]
+    d.k_row, d.k_head = kr.stride()[:2]
+    d.v_row, d.v_head = vr.stride()[:2]
+    pos = [None, None, None]
+    if q_pos is not None:
+        d.pos_dim = q_pos.shape[-1]
+        sig = sigma.to(device=q.device, dtype=torch.float32)
+        if sig.shape != (d.heads,) or not sig.is_contiguous():
+            sig = sig.reshape(-1).expand(d.heads).contiguous()
+        pos = [_floats(q_pos), _floats(k_pos), sig]
+    masks = [m if m is None or m.is_contiguous() else m.contiguous() for m in (q_mask, k_mask)]
+    tensors = (qr, kr, vr, *plan, *pos, *masks)
+    return _lib.RaAttnInputs(*[_lib.ptr(t) for t in tensors]), tensors
+
+
 class _KernelAttention(torch.autograd.Function):
     """(q, k, v, q_pos, k_pos, sigma) -> out, for rows of heads or padded
     batches of them."""
@@ -140,30 +166,18 @@ class _KernelAttention(torch.autograd.Function):
         lib = _lib.load()
         need_grad = ctx is not None
         dev = q.device
-        qr, kr, vr = _rows(q), _rows(k), _rows(v)
         d = _lib.RaAttnDesc()
         (d.graphs, d.num_q, d.num_k, d.max_q, d.max_k) = shape[:5]
-        q_ptr, k_ptr, q_tiles, k_tiles = shape[5:]
-        d.q_row, d.q_head = qr.stride()[:2]
-        d.k_row, d.k_head = kr.stride()[:2]
-        d.v_row, d.v_head = vr.stride()[:2]
+        q_ptr, k_ptr, q_tiles, k_tiles = plan = shape[5:]
         if q_ptr is None:
             d.q_tiles = d.graphs * -(-d.max_q // _TILE)
             d.k_tiles = d.graphs * -(-d.max_k // _TILE)
         else:
             d.q_tiles, d.k_tiles = q_tiles.shape[0], k_tiles.shape[0]
-        d.heads, d.dim, d.kv_heads = qr.shape[1], qr.shape[2], kr.shape[1]
-        pos = [None, None, None]
-        if q_pos is not None:
-            d.pos_dim = q_pos.shape[-1]
-            sig = sigma.to(device=dev, dtype=torch.float32)
-            if sig.shape != (d.heads,) or not sig.is_contiguous():
-                sig = sig.reshape(-1).expand(d.heads).contiguous()
-            pos = [_floats(q_pos), _floats(k_pos), sig]
+        d.heads, d.kv_heads, d.dim = q.shape[-2], k.shape[-2], q.shape[-1]
         d.dtype, d.scale, d.softcap = _lib.DTYPES[q.dtype], scale, softcap
         d.status = _lib.status_word()
-        tensors = (qr, kr, vr, q_ptr, k_ptr, q_tiles, k_tiles, *pos, q_mask, k_mask)
-        inp = _lib.RaAttnInputs(*[_lib.ptr(t) for t in tensors])
+        inp, kept = _operands(d, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, plan)
         ref = ctypes.byref(d)
         with _lib.on_device(dev):
             out = _lib.empty_as(q)
@@ -189,24 +203,22 @@ class _KernelAttention(torch.autograd.Function):
                                      _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention")
         if need_grad:
-            ctx.desc, ctx.state, ctx.inp, ctx.stats = d, state, inp, stats
+            ctx.desc, ctx.state, ctx.plan, ctx.stats = d, state, plan, stats
             ctx.save_for_backward(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask,
                                   out if out32 is None else out32)
-            # what the pointers of `inp` belong to, where it is not saved above
-            ctx.keep = (*[None if t is o or t.data_ptr() == o.data_ptr() else t
-                          for t, o in ((qr, q), (kr, k), (vr, v))],
-                        pos, q_ptr, k_ptr, q_tiles, k_tiles)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         lib = _lib.load()
-        q, k, v, q_pos, k_pos, sigma, _, _, out32 = ctx.saved_tensors
+        # not always the forward's tensors: a checkpoint makes them again, hooks
+        # on saved tensors may bring them back elsewhere and with other strides
+        *saved, out32 = ctx.saved_tensors
+        q, k, v, q_pos, k_pos, sigma = saved[:6]
         d, dev = ctx.desc, q.device
-        g = g.contiguous()
-        if g.data_ptr() % 16:
-            g = g.clone()
+        inp, kept = _operands(d, *saved, ctx.plan)
+        g, out32 = _dense16(g), _dense16(out32)
         need = ctx.needs_input_grad
         with _lib.on_device(dev):
             grads = [_lib.empty_as(t) if need[i] else None for i, t in enumerate((q, k, v))]
@@ -217,7 +229,7 @@ class _KernelAttention(torch.autograd.Function):
             n_ws = lib.ra_attn_workspace_bytes(ctypes.byref(d), 1)
             ws = _lib.scratch(n_ws, dev)
             f32 = q.dtype == torch.float32
-            rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(ctx.inp), g.data_ptr(),
+            rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), g.data_ptr(),
                                       out32.data_ptr() if f32 else None,
                                       None if f32 else out32.data_ptr(), ctx.stats,
                                       ctypes.byref(gr), ctx.state.data_ptr(), ctx.state.numel(),

@@ -1,0 +1,78 @@
+"""Gradients of the softmax operators where PyTorch gives the backward other
+tensors than the forward saved: checkpoints and hooks.  Bitwise what they are
+without, since the values are the same and the backward repeats bitwise."""
+import contextlib
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import rapidalign_b200 as ra
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def moved(t):
+    """The same values elsewhere: in wider rows where it is a matrix or more."""
+    if t.dim() < 2 or not t.is_floating_point():
+        return t.clone()
+    wide = torch.full((*t.shape[:-1], t.shape[-1] + 16), 7.0, dtype=t.dtype, device=t.device)
+    out = wide[..., 8:8 + t.shape[-1]]
+    out.copy_(t)
+    return out
+
+
+def hooks(unpack):
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack)
+
+
+CONTEXTS = {
+    "clones": lambda: hooks(lambda t: t.clone()),
+    "wider rows": lambda: hooks(moved),
+    "dense": lambda: hooks(lambda t: t.clone(memory_format=torch.contiguous_format)),
+    "on the host": lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
+}
+
+
+def compare(step, leaves, up):
+    def grads(context, fn):
+        with context:
+            out = fn(*leaves)
+        # what the forward freed is written over
+        torch.full((1 << 22,), float("nan"), device="cuda")
+        return (out.detach(), *torch.autograd.grad(out, leaves, up))
+
+    want = grads(contextlib.nullcontext(), step)
+    for name, context in CONTEXTS.items():
+        for a, b in zip(grads(context(), step), want):
+            assert torch.equal(a, b), name
+    again = grads(contextlib.nullcontext(),
+                  lambda *a: checkpoint(step, *a, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [32, 20])
+@pytest.mark.parametrize("nq", [[70, 150], [2, 1]])
+def test_attention(dtype, dim, nq, cuda_device):
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    H, HK, n = 4, 2, [90, 700]
+
+    def rn(*s):
+        return torch.randn(*s, generator=gen, device="cuda")
+
+    x = [rn(sum(nq), H, dim), rn(sum(n), 2 * HK, dim), rn(sum(nq), 3), rn(sum(n), 3),
+         torch.rand(H, generator=gen, device="cuda") + 0.5]
+    leaves = [t.requires_grad_(True) for t in x]
+    mask = torch.rand(sum(n), generator=gen, device="cuda") > 0.2
+    seg = ra.attention_segments(*(torch.tensor([0, *m], device="cuda").cumsum(0) for m in (nq, n)))
+
+    def step(q, kv, q_pos, k_pos, sigma):  # operands made inside, k and v slices
+        kv = (kv * 1.5).to(dtype)
+        return ra.pyg_kernel_attention((q * 1.25).to(dtype), kv[:, :HK], kv[:, HK:], segments=seg,
+                                       q_pos=q_pos * 1.0, k_pos=k_pos * 1.0, sigma=sigma * 1.0,
+                                       k_mask=mask.clone())
+
+    compare(step, leaves, rn(sum(nq), H, dim).to(dtype))
