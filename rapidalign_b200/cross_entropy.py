@@ -42,6 +42,14 @@ def _rows16(t: Tensor) -> Tensor:
     return padded
 
 
+def _operands(d, x: Tensor, weight: Tensor) -> Tuple[Tensor, Tensor]:
+    """Both matrices as one pass of the kernels reads them, their strides into `d`."""
+    xk, wk = _rows16(x), _rows16(weight)
+    d.ld_x = max(xk.stride(0), d.dim) if d.rows else (d.dim + 7) // 8 * 8
+    d.ld_w = wk.stride(0)
+    return xk, wk
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     """(x, weight) -> (loss, lse), both float32."""
 
@@ -50,12 +58,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
                 ignore_index: int, reduction: int):
         lib = _lib.load()
         dev = x.device
-        xk, wk = _rows16(x), _rows16(weight)
         d = _lib.RaCeDesc()
         d.rows, d.dim = x.shape
         d.vocab = weight.shape[0]
-        d.ld_x = max(xk.stride(0), d.dim) if d.rows else (d.dim + 7) // 8 * 8
-        d.ld_w = wk.stride(0)
+        xk, wk = _operands(d, x, weight)
         d.ignore_index, d.dtype, d.reduction = ignore_index, _lib.DTYPES[x.dtype], reduction
         d.scale, d.softcap, d.status = scale, softcap, _lib.status_word()
         with _lib.on_device(dev):
@@ -78,9 +84,6 @@ class _LinearCrossEntropy(torch.autograd.Function):
             return loss, lse
         ctx.desc, ctx.state = d, state
         ctx.save_for_backward(x, weight, target)
-        # the aligned copies, where copies had to be made
-        ctx.copies = (None if xk.data_ptr() == x.data_ptr() else xk,
-                      None if wk.data_ptr() == weight.data_ptr() else wk)
         ctx.set_materialize_grads(False)
         return loss, lse
 
@@ -88,10 +91,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, g_lse):
         lib = _lib.load()
+        # not always the forward's tensors: a checkpoint makes them again, hooks
+        # on saved tensors may bring them back elsewhere and with other strides
         x, weight, target = ctx.saved_tensors
         d, dev = ctx.desc, x.device
-        xk = x if ctx.copies[0] is None else ctx.copies[0]
-        wk = weight if ctx.copies[1] is None else ctx.copies[1]
+        xk, wk = _operands(d, x, weight)
+        target = target.contiguous()
         need_x, need_w = ctx.needs_input_grad[:2]
         gl = None if g_loss is None else g_loss.to(torch.float32).contiguous()
         ge = None if g_lse is None else g_lse.to(torch.float32).contiguous()

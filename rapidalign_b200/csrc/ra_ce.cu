@@ -477,9 +477,9 @@ int ra_ce_backward(const ra_ce_desc *d, const void *x, const void *w, const int6
                                                            g_lse, head, (float2 *)(ws + p.b_coef));
   int rc;
   if ((rc = launched())) return rc;
-  // the forward of a few rows made no halves
-  if (d->dtype == RA_F32 && use_few(d) && few_aligned(d, w) && (rc = halves(d, p, x, w, sb, st)))
-    return rc;
+  // The forward of a few rows made no halves if w lay aligned then; where it
+  // lies now says nothing about that.
+  if (d->dtype == RA_F32 && use_few(d) && (rc = halves(d, p, x, w, sb, st))) return rc;
   const Operands op = operands(d, x, w, sb);
   if (d->dtype == RA_F32)
     return backward<float, false, true>(d, p, op, target, (float *)dx, (float *)dw, sb, ws, st);

@@ -8,6 +8,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import rapidalign_b200 as ra
+from test_gpu_cross_entropy import close, exact
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +77,46 @@ def test_attention(dtype, dim, nq, cuda_device):
                                        k_mask=mask.clone())
 
     compare(step, leaves, rn(sum(nq), H, dim).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(3, 700, 64), (200, 500, 36), (150, 90, 72)])
+def test_cross_entropy(dtype, n, v, d, cuda_device):
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    leaves = [torch.randn(m, 2 * d, generator=gen, device="cuda").requires_grad_(True)
+              for m in (n, v)]
+    target = torch.randint(0, v, (n,), generator=gen, device="cuda")
+
+    def step(x, w):  # both are slices of wider rows
+        x, w = ((t * 0.5).to(dtype)[:, :d] for t in (x, w))
+        loss, lse = ra.linear_cross_entropy(x, w, target + 0, reduction="none")
+        return loss + 0.1 * lse
+
+    compare(step, leaves, torch.randn(n, generator=gen, device="cuda"))
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_cross_entropy_alignment_changes(first, cuda_device):
+    """fp32, few rows: the forward's choice of kernel is by the table's alignment,
+    which the backward may not find again."""
+    gen = torch.Generator(device="cuda").manual_seed(first)
+    n, v, d = 3, 800, 64
+    x, w = (torch.randn(m, d, generator=gen, device="cuda") for m in (n, v))
+    target = torch.tensor([0, 5, v - 1], device="cuda")
+
+    def placed(t, at):
+        wide = torch.zeros(t.shape[0], d + 4, device="cuda")
+        wide[:, at:at + d] = t
+        return wide[:, at:at + d]
+
+    def grads(start, end):
+        a = x.clone().requires_grad_(True)
+        b = placed(w, start).requires_grad_(True)
+        with hooks(lambda t: placed(t, end) if t.shape == (v, d) else t):
+            loss, _ = ra.linear_cross_entropy(a, b, target)
+        return torch.autograd.grad(loss, [a, b])
+
+    gl = torch.full((n,), 1 / n, device="cuda").double()
+    (_, _, *want), (_, _, *bound) = exact(x, w, target, 1.0, 0.0, gl, torch.zeros_like(gl))
+    for got, t, b in zip(grads(first, 1 - first), want, bound):
+        close(got, t, b, "gradient")

@@ -142,3 +142,43 @@ def test_attention_strides_of_what_is_given_back(recorder):
         t = hooks.owner(inputs[n])
         assert (desc[n + "_row"], desc[n + "_head"]) == t.stride()[:2]
     assert desc["q_row"] == H * D and desc["k_row"] == (HK + 1) * (D + 8)
+
+
+def cross_entropy(leaf, weight, target):
+    return ra.linear_cross_entropy(leaf * 2, weight * 3, target)[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_cross_entropy_under_a_checkpoint(recorder, dtype):
+    x, w = (torch.randn(n, 16, dtype=dtype, requires_grad=True) for n in (9, 20))
+    loss = checkpoint(cross_entropy, x, w, torch.zeros(9, dtype=torch.long), use_reentrant=False)
+    loss.backward()
+    forwards = [got for n, got in recorder.calls if n == "ra_ce_forward"]
+    assert len(forwards) == 2
+    assert recorder.last("ra_ce_backward")[:4] == forwards[1][:4]  # desc, x, w, target
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_cross_entropy_strides_of_what_is_given_back(recorder, dtype):
+    """Strided operands come back contiguous, and the other way round."""
+    for wide_first in (True, False):
+        def again(t, wide=not wide_first):
+            if not wide or t.dim() < 2:
+                return t.clone(memory_format=torch.contiguous_format)
+            rows = torch.zeros(t.shape[0], 40, dtype=t.dtype)
+            rows[:, :16] = t
+            return rows[:, :16]
+
+        hooks = Clones(again)
+        leaves = [torch.randn(n, 40 if wide_first else 16, dtype=dtype, requires_grad=True)
+                  for n in (9, 20)]
+        with hooks:
+            x, w = ((t * 2)[:, :16] for t in leaves)
+            loss, _ = ra.linear_cross_entropy(x, w, torch.zeros(9, dtype=torch.long))
+        before = recorder.last("ra_ce_forward")[0]
+        assert before["ld_x"] == before["ld_w"] == (40 if wide_first else 16)
+        loss.backward()
+        desc, x, w, target = recorder.last("ra_ce_backward")[:4]
+        assert desc["ld_x"] == hooks.owner(x).stride(0) == (16 if wide_first else 40)
+        assert desc["ld_w"] == hooks.owner(w).stride(0) == (16 if wide_first else 40)
+        assert hooks.owner(target).dtype == torch.long
