@@ -15,6 +15,7 @@ import threading
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librapidalign_b200.so")
@@ -330,6 +331,15 @@ def check_status(what: str) -> None:
     if _STATUS is not None and ctypes.c_int32.from_address(_STATUS.data_ptr()).value:
         _STATUS.zero_()
         check(RA_ERR_DEVICE_TIMEOUT, what + " (an earlier call)")
+
+
+def past_autograd(tensors) -> bool:
+    """Whether a call on `tensors` may go past its autograd function: no gradient is
+    wanted, no forward-mode level is open (its tangents are not gradients: the
+    function refuses them) and no function transform is at work."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return False
+    return forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()
 
 
 def launch_count() -> int:

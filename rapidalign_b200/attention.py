@@ -313,10 +313,9 @@ def _mask(mask, shape, device):
 def _run(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap):
     _lib.check_status("kernel attention")
     args = (q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, shape, scale, softcap)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:6]):
-        return _KernelAttention.apply(*args)
-    # no gradient wanted: without autograd's share of a small call
-    return _KernelAttention.forward(None, *args)
+    if _lib.past_autograd(args[:6]):  # without autograd's share of a small call
+        return _KernelAttention.forward(None, *args)
+    return _KernelAttention.apply(*args)
 
 
 def pyg_kernel_attention(q: Tensor, k: Tensor, v: Tensor, *, q_ptr: Optional[Tensor] = None,

@@ -165,6 +165,6 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, *, scale: fl
     if target.dtype != torch.long or not target.is_contiguous():
         target = target.to(torch.long).contiguous()
     args = (x, weight, target, scale, softcap, int(ignore_index), _REDUCTIONS[reduction])
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        return _LinearCrossEntropy.apply(*args)
-    return _LinearCrossEntropy.forward(None, *args)
+    if _lib.past_autograd((x, weight)):
+        return _LinearCrossEntropy.forward(None, *args)
+    return _LinearCrossEntropy.apply(*args)
