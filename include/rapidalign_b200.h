@@ -124,7 +124,7 @@ typedef struct ra_kde_desc {
                           library's own failure paths only. */
 } ra_kde_desc;
 
-/* Test hooks (ra_kde_desc.test_hooks).  RA_TEST_NO_MMA: the tensor-core kernels
+/* Test hooks (test_hooks of the descriptors).  RA_TEST_NO_MMA: the tensor-core kernels
  * (dim >= 4 on the tensor-core engine) issue no MMA at all and bound each wait
  * to 4096 polls, so their first wait for a GEMM expires with nothing in flight:
  * the kernel records the timeout, frees its tensor memory and returns, and
@@ -132,7 +132,9 @@ typedef struct ra_kde_desc {
  * passes that stream rows by bulk copies (padded dim 32-128, equal weights, no
  * mask) copy nothing and bound each wait to 4096 polls, so their consumers'
  * first wait expires: the same status, from the forward (sums and packing)
- * or the backward (write pass).  The results of such a call are invalid. */
+ * or the backward (write pass).  The results of such a call are invalid.
+ * ra_ce_desc and ra_attn_desc take RA_TEST_NO_MMA too: their tensor-core kernels
+ * then add bit 0 to the status word. */
 enum ra_test_hook { RA_TEST_NO_MMA = 1, RA_TEST_RING_IDLE = 2 };
 
 typedef struct ra_kde_inputs {
@@ -467,7 +469,7 @@ typedef struct ra_ce_desc {
   int32_t reduction;
   float scale;
   float softcap;
-  int32_t reserved;
+  int32_t test_hooks; /* 0, or RA_TEST_NO_MMA */
   int32_t *status;
 } ra_ce_desc;
 
@@ -514,7 +516,7 @@ typedef struct ra_attn_desc {
   int32_t heads, kv_heads, dim, pos_dim;
   int32_t dtype;
   float scale, softcap;
-  int32_t reserved;
+  int32_t test_hooks; /* 0, or RA_TEST_NO_MMA */
   int32_t *status;
 } ra_attn_desc;
 typedef struct ra_attn_inputs {

@@ -96,7 +96,7 @@ class RaCeDesc(ctypes.Structure):
         ("reduction", ctypes.c_int32),
         ("scale", ctypes.c_float),
         ("softcap", ctypes.c_float),
-        ("reserved", ctypes.c_int32),
+        ("test_hooks", ctypes.c_int32),
         ("status", ctypes.c_void_p),
     ]
 
@@ -107,7 +107,7 @@ class RaAttnDesc(ctypes.Structure):
                                        "k_head", "v_row", "v_head", "q_tiles", "k_tiles",
                                        "max_q", "max_k")] +
         [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "pos_dim", "dtype")] +
-        [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("reserved", ctypes.c_int32),
+        [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("test_hooks", ctypes.c_int32),
          ("status", ctypes.c_void_p)])
 
 

@@ -25,6 +25,7 @@ bool attn_ok(const ra_attn_desc *d) {
       d->v_head < 0)
     return false;
   if (d->max_q < 0 || d->max_k < 0 || d->max_q > d->num_q || d->max_k > d->num_k) return false;
+  if ((d->test_hooks & ~RA_TEST_NO_MMA) != 0) return false;
   return d->q_tiles >= 0 && d->k_tiles >= 0 && d->status != nullptr;
 }
 
@@ -62,6 +63,14 @@ AttnArgs args_of(const ra_attn_desc *d, const ra_attn_inputs *in) {
   a.scale = d->scale, a.cap = d->softcap;
   a.status = d->status;
   return a;
+}
+
+AttnTcArgs tc_args(const ra_attn_desc *d, const char *state) {
+  AttnTcArgs x{};
+  x.words = (const unsigned *)state;
+  x.no_mma = (d->test_hooks & RA_TEST_NO_MMA) != 0;
+  x.spin_limit = x.no_mma ? 4096u : kTcSpinLimit;
+  return x;
 }
 
 // Head widths the tensor-core kernels take (ra_attn_tc.cuh); other widths and
@@ -362,8 +371,7 @@ int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, 
     rc = few_forward<T>(d, a, f, ws, st);
     return rc ? rc : join<T>(a, f, ws, sms, st);
   }
-  AttnTcArgs x{};
-  x.words = (const unsigned *)state;
+  AttnTcArgs x = tc_args(d, state);
   if (Kind::pair) {
     const AttnState s = state_layout(d);
     if (cudaMemsetAsync(state, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
@@ -414,11 +422,10 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
     if ((rc = launched())) return rc;
   }
   if (tc) {
-    AttnTcArgs x{};
+    AttnTcArgs x = tc_args(d, state);
     const int64_t qr = (int64_t)d->heads * d->dim;
     const Operands o = operands(d, in, state, Kind::pair ? ws + b.gh : a.dout,
                                 Kind::pair ? ws + b.gl : a.dout);
-    x.words = (const unsigned *)state;
     unsigned *words = (unsigned *)state;
     if (!Kind::bf16) {
       AttnPrep p{};

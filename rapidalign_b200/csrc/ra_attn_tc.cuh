@@ -65,6 +65,8 @@ struct AttnTcArgs {
   float *part_o;          // [splits][num_q][heads][dim], unnormalised
   float2 *part_s;         // [splits][heads][num_q] (m, l)
   int pair_p;             // forward of 16-bit inputs: P as a pair
+  unsigned spin_limit;    // polls of one wait before giving up
+  int no_mma;             // test hook: no products, so that the waits for them expire
 };
 
 struct KindBf16 {
@@ -538,7 +540,7 @@ struct FwdCfg {
   static constexpr int TMEM = tmem_round(KT + (SMALL ? 2 : 1) * DP);
   static constexpr int pos = Q + 4 * KV;                 // TilePos<KT> [2]
   static constexpr int val = pos + 2 * KT * 12;          // unsigned [2][2]
-  static constexpr int bar = val + 16, slot = bar + 24;  // slot: also the mask's extent
+  static constexpr int bar = val + 16, slot = bar + 40;  // slot: also the mask's extent
   static constexpr int top = slot + 8;                   // float [PARTS][128]
   // threads of a row: half of the columns each where TMEM or shared memory holds
   // fewer than four CTAs
@@ -555,6 +557,25 @@ template <int NT>
 constexpr int kMmaThread = NT - 64;
 template <int NT>
 constexpr int kTmaThread = NT - 32;
+// After an expired wait: a CTA does not leave while its copies write its shared
+// memory, nor free TMEM that its products write.  The last copies of either
+// buffer (`full`: the barriers; tiles t0 .. copied were asked for), and one more
+// commit, which arrives after all products.
+template <int NT>
+__device__ __forceinline__ void drain(uint32_t full, int copied, int t0, int stages) {
+  if (threadIdx.x == kTmaThread<NT> && copied >= t0) {
+    if (stages == 1) mbar_wait(full, copied & 1);
+    else
+      for (int t = copied > t0 ? copied - 1 : t0; t <= copied; ++t)
+        mbar_wait(full + 8 * (t & 1), ((t - t0) >> 1) & 1);
+  }
+  if (threadIdx.x == kMmaThread<NT>) {
+    tc_commit(full + 16);
+    mbar_wait(full + 16, 0);
+  }
+  __syncthreads();
+  tc_fence_after();
+}
 // This thread's row of the next streamed tile, fetched an iteration ahead.
 struct NextRow {
   AttnPos p;
@@ -592,10 +613,13 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
                                     reinterpret_cast<unsigned long long *>(sm + C::slot));
   // no row to work for: no keys to see
   const int64_t all = __syncthreads_or(row_on) ? (nk + KT - 1) / KT : 0;
-  const int t0 = (int)(all * split / X.splits), t1 = (int)(all * (split + 1) / X.splits);
+  const int t0 = (int)(all * split / X.splits);
+  int t1 = (int)(all * (split + 1) / X.splits);
 
+  volatile int *copied = reinterpret_cast<int *>(sm + C::bar + 32);  // the last tile asked for
   auto issue = [&](int t, uint32_t more) {
     const uint32_t fb = full + 8 * (t & 1);
+    *copied = t;
     mbar_expect_tx(fb, more + 2 * C::KV);
     load_tile<Kind, KT, DP, C::BR>(sK + (t & 1) * C::KV, X.k, hk, j0 + t * KT, fb);
     load_tile<Kind, KT, DP, C::BR>(sV + (t & 1) * C::KV, X.v, hk, j0 + t * KT, fb);
@@ -626,6 +650,8 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     mbar_init(bar, 1);
     mbar_init(full, 1);
     mbar_init(full + 8, 1);
+    mbar_init(full + 16, 1);
+    *copied = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (t0 < t1) {
       issue(t0, C::Q);
@@ -636,11 +662,11 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   if (t0 < t1) fetch(t0);
   __syncthreads();
   if (t0 < t1) {
-    bad = !mbar_wait(full + 8 * (t0 & 1), 0);
+    bad = !mbar_wait(full + 8 * (t0 & 1), 0, X.spin_limit);
     settle(t0);
   }
   tc_fence_before();
-  __syncthreads();
+  if ((bad = __syncthreads_or(bad))) t1 = t0;  // no first tile
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + C::slot);
   const uint32_t tS = tmem, tO = tmem + KT, lane_off = (uint32_t)(32 * (warp & 3)) << 16;
@@ -655,17 +681,18 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to; l: this part's
   unsigned phase = 0;
 
-  if (t0 < t1 && threadIdx.x == kMmaThread<NT>) {
+  auto mma = [&]() { return threadIdx.x == kMmaThread<NT> && !X.no_mma; };
+  if (t0 < t1 && mma()) {
     products_rows<Kind, KT, DP>(tS, sQ, sK + (t0 & 1) * C::KV);
     tc_commit(bar);
   }
   for (int t = t0; t < t1; ++t) {
     const int b = t & 1;
-    bad |= !mbar_wait(bar, phase);
+    bad |= !mbar_wait(bar, phase, X.spin_limit);
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {  // the products on its buffers are done
-      if (threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
     f2_t s2[C::C][16];
@@ -733,12 +760,12 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     l += lo_of(both) + hi_of(both);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     if (t + 1 < t1) {
-      bad |= !mbar_wait(full + 8 * (b ^ 1), ((t + 1 - t0) >> 1) & 1);
+      bad |= !mbar_wait(full + 8 * (b ^ 1), ((t + 1 - t0) >> 1) & 1, X.spin_limit);
       settle(t + 1);
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == kMmaThread<NT>) {
+    if (mma()) {
       tc_fence_after();
       products_weighted<Kind, KT, DP, C::SMALL>(tO, tS, sV + b * C::KV, p_pair, t > t0);
       if (t + 1 < t1) products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
@@ -746,11 +773,13 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     }
   }
   if (t0 < t1 && !bad) {
-    bad = !mbar_wait(bar, phase);
+    bad = !mbar_wait(bar, phase, X.spin_limit);
     tc_fence_after();
   }
-  bad = __syncthreads_or(bad);
-  if (bad && threadIdx.x == 0) atomicOr(A.status, 1);
+  if ((bad = __syncthreads_or(bad))) {
+    if (threadIdx.x == 0) atomicOr(A.status, 1);
+    drain<NT>(full, *copied, t0, 2);
+  }
 
   if (PARTS > 1) {
     if (part > 0) top[row] = l;
@@ -1008,7 +1037,7 @@ struct DqCfg {
   static constexpr int NT = 128 * (KT / 32);
   static constexpr int pos = 2 * Q + 2 * STAGES * KV;  // TilePos<KT> [2]
   static constexpr int val = pos + 2 * KT * 12;
-  static constexpr int bar = val + 16, slot = bar + 24;
+  static constexpr int bar = val + 16, slot = bar + 40;
   static constexpr int smem = slot + 8 + 1024;
   static constexpr int CTAS = attn_ctas(smem, TMEM, NT);
 };
@@ -1039,11 +1068,13 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   float2 st = make_float2(INFINITY, 0.f);
   if (in) st = A.stats(h, i);
   const bool live = st.y != 0.f;  // has keys, and is not masked
-  const int t1 = __syncthreads_or(live) ? (nk + KT - 1) / KT : 0;
+  int t1 = __syncthreads_or(live) ? (nk + KT - 1) / KT : 0;
 
+  volatile int *copied = reinterpret_cast<int *>(sm + C::bar + 32);  // the last tile asked for
   auto issue = [&](int t, uint32_t more) {
     const int b = C::STAGES == 1 ? 0 : t & 1;
     const uint32_t fb = full + 8 * b;
+    *copied = t;
     mbar_expect_tx(fb, more + 2 * C::KV);
     load_tile<Kind, KT, DP, C::BR>(sK + b * C::KV, X.k, hk, j0 + t * KT, fb);
     load_tile<Kind, KT, DP, C::BR>(sV + b * C::KV, X.v, hk, j0 + t * KT, fb);
@@ -1070,13 +1101,16 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     fence_async_smem();
   };
   auto landed = [&](int t) {
-    return C::STAGES == 1 ? mbar_wait(full, t & 1) : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1);
+    return C::STAGES == 1 ? mbar_wait(full, t & 1, X.spin_limit)
+                          : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1, X.spin_limit);
   };
   if (warp == 1) tmem_alloc<C::TMEM>(base + C::slot);
   if (threadIdx.x == 0) {
     mbar_init(bar, 1);
     mbar_init(full, 1);
     mbar_init(full + 8, 1);
+    mbar_init(full + 16, 1);
+    *copied = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (t1 > 0) {
       issue(0, 2 * C::Q);
@@ -1092,7 +1126,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     settle(0);
   }
   tc_fence_before();
-  __syncthreads();
+  if ((bad = __syncthreads_or(bad))) t1 = 0;  // no first tile
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + C::slot);
   const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
@@ -1110,18 +1144,19 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   const bool pos_grad = A.pos_q != nullptr;
   unsigned phase = 0;
 
-  if (t1 > 0 && threadIdx.x == kMmaThread<NT>) {
+  auto mma = [&]() { return threadIdx.x == kMmaThread<NT> && !X.no_mma; };
+  if (t1 > 0 && mma()) {
     products_rows<Kind, KT, DP>(tS, sQ, sK);
     products_rows<Kind, KT, DP>(tP, sG, sV);
     tc_commit(bar);
   }
   for (int t = 0; t < t1; ++t) {
     const int pb = t & 1, b = C::STAGES == 1 ? 0 : pb;
-    bad |= !mbar_wait(bar, phase);
+    bad |= !mbar_wait(bar, phase, X.spin_limit);
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
-      if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
+      if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
     float v[32], dp[32];
@@ -1159,7 +1194,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == kMmaThread<NT>) {
+    if (mma()) {
       tc_fence_after();
       products_weighted<Kind, KT, DP, C::SMALL>(tD, tS, sK + b * C::KV, false, t > 0);
       if (C::STAGES > 1 && t + 1 < t1) {
@@ -1169,13 +1204,13 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
       tc_commit(bar);
     }
     if (C::STAGES == 1 && t + 1 < t1) {  // one buffer: its products first
-      bad |= !mbar_wait(bar, phase);
+      bad |= !mbar_wait(bar, phase, X.spin_limit);
       phase ^= 1;
-      if (threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       bad |= !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
-      if (threadIdx.x == kMmaThread<NT>) {
+      if (mma()) {
         tc_fence_after();
         products_rows<Kind, KT, DP>(tS, sQ, sK);
         products_rows<Kind, KT, DP>(tP, sG, sV);
@@ -1184,11 +1219,13 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     }
   }
   if (t1 > 0 && !bad) {
-    bad = !mbar_wait(bar, phase);
+    bad = !mbar_wait(bar, phase, X.spin_limit);
     tc_fence_after();
   }
-  bad = __syncthreads_or(bad);
-  if (bad && threadIdx.x == 0) atomicOr(A.status, 1);
+  if ((bad = __syncthreads_or(bad))) {
+    if (threadIdx.x == 0) atomicOr(A.status, 1);
+    drain<NT>(full, *copied, 0, C::STAGES);
+  }
   using T = typename Kind::T;
   if (A.dq != nullptr && part == 0)
     write_row<T, DP, C::SMALL>(tD + lane_off, A.scale * ldexpf(1.f, -eu - elem_exp<Kind>(X, kWk)), in,
@@ -1238,7 +1275,7 @@ struct DkvCfg {
   static constexpr int NT = 128 * (QT / 32);
   static constexpr int pos = 2 * K + 2 * STAGES * QG;  // TilePos<QT> [2]
   static constexpr int stt = pos + 2 * QT * 12;        // TileStat<QT> [2]
-  static constexpr int bar = stt + 2 * QT * 12, slot = bar + 24;
+  static constexpr int bar = stt + 2 * QT * 12, slot = bar + 40;
   static constexpr int smem = slot + 8 + 1024;
   static constexpr int CTAS = attn_ctas(smem, TMEM, NT);
 };
@@ -1268,11 +1305,13 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   const int nq = (int)masked_extent(A.q_mask ? A.q_mask + i0 : nullptr, tile.w, NT,
                                     reinterpret_cast<unsigned long long *>(sm + C::slot));
   const int per = (nq + QT - 1) / QT;
-  const int t1 = __syncthreads_or(live) ? per * group : 0;  // query tiles, head by head
+  int t1 = __syncthreads_or(live) ? per * group : 0;  // query tiles, head by head
 
+  volatile int *copied = reinterpret_cast<int *>(sm + C::bar + 32);  // the last tile asked for
   auto issue = [&](int t, uint32_t more) {
     const int b = C::STAGES == 1 ? 0 : t & 1, h = hk * group + t / per, r0 = i0 + t % per * QT;
     const uint32_t fb = full + 8 * b;
+    *copied = t;
     mbar_expect_tx(fb, more + 2 * C::QG);
     load_tile<Kind, QT, DP, C::BR>(sQ + b * C::QG, X.q, h, r0, fb);
     load_tile<Kind, QT, DP, C::BR>(sG + b * C::QG, X.go, h, r0, fb);
@@ -1302,13 +1341,16 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     fence_async_smem();
   };
   auto landed = [&](int t) {
-    return C::STAGES == 1 ? mbar_wait(full, t & 1) : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1);
+    return C::STAGES == 1 ? mbar_wait(full, t & 1, X.spin_limit)
+                          : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1, X.spin_limit);
   };
   if (warp == 1) tmem_alloc<C::TMEM>(base + C::slot);
   if (threadIdx.x == 0) {
     mbar_init(bar, 1);
     mbar_init(full, 1);
     mbar_init(full + 8, 1);
+    mbar_init(full + 16, 1);
+    *copied = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (t1 > 0) {
       issue(0, 2 * C::K);
@@ -1324,7 +1366,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     settle(0);
   }
   tc_fence_before();
-  __syncthreads();
+  if ((bad = __syncthreads_or(bad))) t1 = 0;  // no first tile
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + C::slot);
   const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
@@ -1343,7 +1385,8 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   unsigned phase = 0;
   int cur = -1;
 
-  if (t1 > 0 && threadIdx.x == kMmaThread<NT>) {
+  auto mma = [&]() { return threadIdx.x == kMmaThread<NT> && !X.no_mma; };
+  if (t1 > 0 && mma()) {
     products_rows<Kind, QT, DP>(tS, sK, sQ);
     products_rows<Kind, QT, DP>(tP, sV, sG);
     tc_commit(bar);
@@ -1366,11 +1409,11 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
       B.sc.init(A, h);
       B.sc.su *= us;
     }
-    bad |= !mbar_wait(bar, phase);
+    bad |= !mbar_wait(bar, phase, X.spin_limit);
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
-      if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
+      if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
     float v[32], dp[32];
@@ -1398,7 +1441,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     }
     tc_fence_before();
     if ((bad = __syncthreads_or(bad))) break;
-    if (threadIdx.x == kMmaThread<NT>) {
+    if (mma()) {
       tc_fence_after();
       products_weighted<Kind, QT, DP, C::SMALL>(tDv, tS, sG + b * C::QG, false, t > 0);
       products_weighted<Kind, QT, DP, C::SMALL>(tDk, tP, sQ + b * C::QG, false, t > 0);
@@ -1409,13 +1452,13 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
       tc_commit(bar);
     }
     if (C::STAGES == 1 && t + 1 < t1) {
-      bad |= !mbar_wait(bar, phase);
+      bad |= !mbar_wait(bar, phase, X.spin_limit);
       phase ^= 1;
-      if (threadIdx.x == kTmaThread<NT>) issue(t + 1, 0);
+      if (threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       bad |= !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
-      if (threadIdx.x == kMmaThread<NT>) {
+      if (mma()) {
         tc_fence_after();
         products_rows<Kind, QT, DP>(tS, sK, sQ);
         products_rows<Kind, QT, DP>(tP, sV, sG);
@@ -1425,11 +1468,13 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   }
   close_head();
   if (t1 > 0 && !bad) {
-    bad = !mbar_wait(bar, phase);
+    bad = !mbar_wait(bar, phase, X.spin_limit);
     tc_fence_after();
   }
-  bad = __syncthreads_or(bad);
-  if (bad && threadIdx.x == 0) atomicOr(A.status, 1);
+  if ((bad = __syncthreads_or(bad))) {
+    if (threadIdx.x == 0) atomicOr(A.status, 1);
+    drain<NT>(full, *copied, 0, C::STAGES);
+  }
   using T = typename Kind::T;
   const int64_t at = (j * A.kv_heads + hk) * A.dim;
   const bool zero = !live || t1 == 0;

@@ -25,6 +25,7 @@ bool ce_ok(const ra_ce_desc *d) {
   if (d->reduction < RA_REDUCE_NONE || d->reduction > RA_REDUCE_MEAN) return false;
   if (!(d->softcap >= 0.f) || !(d->softcap < INFINITY) || !(d->scale - d->scale == 0.f))
     return false;
+  if ((d->test_hooks & ~RA_TEST_NO_MMA) != 0) return false;
   return d->status != nullptr;
 }
 
@@ -216,8 +217,9 @@ CeLogit<PAIRS> logit_of(const ra_ce_desc *d, const CeHead *head) {
 
 GmShape shape_of(const ra_ce_desc *d, const CePlan &p, int64_t mt, int64_t nt, int64_t k, int slices,
                  int m_fast) {
+  const bool no_mma = (d->test_hooks & RA_TEST_NO_MMA) != 0;
   return {(int)mt, (int)nt, (int)ceil_div(k, (int64_t)kGmK), slices, m_fast,
-          kTcSpinLimit, d->status};
+          no_mma ? 4096u : kTcSpinLimit, no_mma, d->status};
 }
 
 // fp32 inputs as pairs of halves, in the state

@@ -63,7 +63,8 @@ constexpr size_t kGmSmem = 1024 + 192 * 1024 + kGmEpiWarps * kGmStageOut + 256;
 struct GmShape {
   int m_tiles, n_tiles, k_steps, slices;
   int m_fast;
-  unsigned spin_limit;
+  unsigned spin_limit;  // polls of one wait before giving up
+  int no_mma;           // test hook: no products, so that the waits for them expire
   int *status;
 };
 
@@ -259,11 +260,11 @@ __global__ void __launch_bounds__(kGmThreads, 1)
       // a CTA does not leave while copies into its shared memory are in flight
       const int first = issued > kGmStages ? issued - kGmStages : 0;
       for (int i = first; i < issued; ++i)
-        if (!mbar_wait(full + 8 * (i % kGmStages), (i / kGmStages) & 1, s.spin_limit)) ok = false;
+        if (!mbar_wait(full + 8 * (i % kGmStages), (i / kGmStages) & 1)) ok = false;
       if (!ok) atomicOr(s.status, 1);
     }
   } else if (warp == kGmMmaWarp) {
-    if (lane == 0) {
+    if (lane == 0 && !s.no_mma) {
       constexpr uint32_t idesc = gm_idesc(TN, BF16, A_MN, B_MN);
       int used = 0, t = 0;
       bool ok = true;
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     mbar_init(bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tc_commit(bar);
-    mbar_wait(bar, 0, s.spin_limit);
+    mbar_wait(bar, 0);
   }
   __syncthreads();
   if (warp == kGmMmaWarp) {
