@@ -158,10 +158,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, kFew16Ctas)
         kpos[2 * KT + lane] = np.z;
       }
       issue(step + S - 1, (slot + S - 1) % S, marks[(slot + S - 1) % S]);
+      if (step + 1 < steps) place(step + 1, marks[(slot + 1) % S]);
       asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
       __syncwarp();
       const unsigned bits = marks[slot];
-      if (step + 1 < steps) place(step + 1, marks[(slot + 1) % S]);
       const uint32_t sk = ring + slot * 2 * C::TILE, sv = sk + C::TILE;
       const int lr = lane & 7, lm = lane >> 3;
       float s[NT][4] = {};

@@ -351,6 +351,7 @@ __device__ __forceinline__ void write_row(uint32_t taddr, float f, bool on, bool
 #pragma unroll 1
   for (int c = c0; c < c1; c += 32) {
     float v[32];
+    __syncwarp();  // TMEM is read by whole warps
     tmem_ld32(taddr + c, v);
     if (SMALL) {
       float u[32];
@@ -695,6 +696,7 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
       if (threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
+    __syncwarp();
     f2_t s2[C::C][16];
     float mx = -INFINITY;
 #pragma unroll
@@ -1159,6 +1161,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
       if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
+    __syncwarp();
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
     tmem_ld32(tP + lane_off + 32 * part, dp);
@@ -1416,6 +1419,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
       if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
+    __syncwarp();
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
     tmem_ld32(tP + lane_off + 32 * part, dp);

@@ -108,12 +108,15 @@ __device__ __forceinline__ f2_t tanh2(f2_t u) {
   return pk(fabsf(x) < kTanhSmall ? a : r[0], fabsf(y) < kTanhSmall ? b : r[1]);
 }
 __device__ __forceinline__ float tanh_step(float u) { return lo_of(tanh2(pk(u, u))); }
-// whether 32 products, times f, are all small
+// Whether 32 products of every lane, times f, are small: one answer for the warp,
+// whose next TMEM access all lanes have to make together.  (tanh2 gives a small
+// element the same value, so a row's results do not depend on its neighbours.)
 __device__ __forceinline__ bool all_small(const float (&v)[32], float f) {
   float m[2] = {fabsf(v[0]), fabsf(v[1])};
 #pragma unroll
   for (int j = 2; j < 32; ++j) m[j & 1] = fmaxf(m[j & 1], fabsf(v[j]));
-  return fmaxf(m[0], m[1]) * fabsf(f) < kTanhSmall;  // a NaN counts as small, and stays one
+  // a NaN counts as small, and stays one
+  return __all_sync(kFull, fmaxf(m[0], m[1]) * fabsf(f) < kTanhSmall);
 }
 
 // The bits of one value as another type of the same size.

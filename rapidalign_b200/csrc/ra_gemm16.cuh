@@ -122,17 +122,22 @@ __device__ __forceinline__ GmUnit gm_unit(const GmShape &s, int u) {
 }
 
 // The thread's row of a finished tile, 32 columns at a time: straight from
-// TMEM, or from the registers that joined the rounds.
+// TMEM (which a warp reads together, whatever branches its lanes took before), or
+// from the registers that joined the rounds.
 struct GmFromTmem {
   uint32_t taddr;
   static constexpr int unroll = 1;
-  __device__ __forceinline__ void get(int c, float (&v)[32]) const { tmem_ld32(taddr + c, v); }
+  __device__ __forceinline__ void get(int c, float (&v)[32]) const {
+    __syncwarp();
+    tmem_ld32(taddr + c, v);
+  }
 };
 struct GmFromPairs {  // one round of pairs: both accumulators
   uint32_t taddr, small;
   static constexpr int unroll = 1;
   __device__ __forceinline__ void get(int c, float (&v)[32]) const {
     float x[32];
+    __syncwarp();
     tmem_ld32(taddr + c, v);
     tmem_ld32(small + c, x);
 #pragma unroll
