@@ -87,13 +87,18 @@ bool operands_aligned(const ra_attn_desc *d, const ra_attn_inputs *in) {
          (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v) & 15) == 0;
 }
 
-// The state a backward needs: bounds, and the halves of fp32 inputs.
+// The state a backward needs: bounds (fp32 inputs; the backward writes fp16's),
+// and the halves of fp32 inputs.
 struct AttnState {
   size_t qh, ql, kh, kl, vh, vl, total;
 };
+size_t words_of(const ra_attn_desc *d, int tensors) {
+  return (size_t)tensors * (size_t)d->graphs * (size_t)d->kv_heads;
+}
 AttnState state_layout(const ra_attn_desc *d) {
   AttnState s{};
   size_t o = 256;
+  if (d->dtype != RA_BF16 && use_tc(d)) o = std::max(o, align256(4 * words_of(d, 4)));
   if (d->dtype == RA_F32 && use_tc(d)) {
     const size_t q = align256(2 * (size_t)d->num_q * d->heads * d->dim);
     const size_t k = align256(2 * (size_t)d->num_k * d->kv_heads * d->dim);
@@ -154,13 +159,15 @@ AttnFwd fwd_layout(const ra_attn_desc *d, int sms) {
 }
 
 struct AttnBwd {
-  size_t delta, pos_q, pos_k, gh, gl, total;
+  size_t delta, do_top, pos_q, pos_k, gh, gl, total;
 };
 AttnBwd bwd_layout(const ra_attn_desc *d) {
   AttnBwd b{};
   size_t o = 0;
   b.delta = o;
   o += align256(sizeof(float) * (size_t)d->num_q * d->heads);
+  b.do_top = o;
+  if (d->dtype != RA_BF16 && use_tc(d)) o += align256(sizeof(float) * (size_t)d->num_q * d->heads);
   b.pos_q = o;
   if (d->pos_dim) o += align256(sizeof(float4) * (size_t)d->num_q * d->heads);
   b.pos_k = o;
@@ -175,27 +182,40 @@ AttnBwd bwd_layout(const ra_attn_desc *d) {
 
 unsigned grid_rows(int64_t n, int per) { return (unsigned)ceil_div(n, (int64_t)per); }
 
+AttnPrep prep_of(const AttnArgs &a) {
+  AttnPrep p{};
+  p.graphs = a.graphs, p.kv_heads = a.kv_heads, p.dim = a.dim;
+  return p;
+}
+int64_t prep_grid(const AttnPrep &p) {
+  int64_t tiles = 0;
+  for (int t = 0; t < p.count; ++t) tiles = std::max(tiles, p.tiles[t]);
+  return tiles * p.kv_heads;
+}
 template <class T>
-int bounds(const AttnPrep &p, unsigned *words, int sms, cudaStream_t st) {
-  int64_t rows = 1;
-  for (int t = 0; t < p.count; ++t) rows = std::max(rows, p.rows[t] * p.heads[t]);
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows * (p.dim / 8), (int64_t)1024), sms * 8),
-                  p.count);
-  attn_bounds_kernel<T><<<grid, 256, 0, st>>>(p, words);
+int bounds(const AttnPrep &p, unsigned *words, cudaStream_t st) {
+  const int64_t n = prep_grid(p);
+  if (n > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
+  if (n < 1) return RA_OK;
+  attn_bounds_kernel<T><<<dim3((unsigned)n, p.count), kPrepThreads, 0, st>>>(p, words);
   return launched();
 }
-int halves(const AttnPrep &p, const unsigned *words, int sms, cudaStream_t st) {
-  int64_t n = 1;
-  for (int t = 0; t < p.count; ++t) n = std::max(n, p.rows[t] * p.heads[t] * p.dim);
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, (int64_t)4096), sms * 16), p.count);
-  attn_halves_kernel<<<grid, 256, 0, st>>>(p, words);
+int halves(const AttnPrep &p, unsigned *words, cudaStream_t st) {
+  const int64_t n = prep_grid(p);
+  if (n > (int64_t)0x7fffffff) return RA_ERR_INVALID_ARGUMENT;
+  if (n < 1) return RA_OK;
+  attn_halves_kernel<<<dim3((unsigned)n, p.count), kPrepThreads, 0, st>>>(p, words);
   return launched();
 }
-void add(AttnPrep &p, const void *x, int64_t rows, int heads, int64_t row, int64_t head,
-         const uint8_t *mask, int word, void *hi, void *lo) {
+// a tensor of the queries' or the keys' rows
+void add(AttnPrep &p, const void *x, bool keys, const AttnArgs &a, int64_t row, int64_t head,
+         int word, void *hi, void *lo) {
   const int t = p.count++;
-  p.x[t] = x, p.rows[t] = rows, p.heads[t] = heads, p.row[t] = row, p.head[t] = head;
-  p.mask[t] = mask, p.word[t] = word, p.hi[t] = (uint16_t *)hi, p.lo[t] = (uint16_t *)lo;
+  p.x[t] = x, p.row[t] = row, p.head[t] = head;
+  p.heads[t] = keys ? a.kv_heads : a.heads;
+  p.segs[t] = keys ? a.ks : a.qs, p.tiles[t] = keys ? a.n_k_tiles : a.n_q_tiles;
+  p.mask[t] = keys ? a.k_mask : a.q_mask;
+  p.word[t] = word, p.hi[t] = (uint16_t *)hi, p.lo[t] = (uint16_t *)lo;
 }
 
 // Tensor maps [rows][heads][dim] of an operand, or of its halves.
@@ -374,17 +394,14 @@ int forward(const ra_attn_desc *d, const ra_attn_inputs *in, const AttnArgs &a, 
   AttnTcArgs x = tc_args(d, state);
   if (Kind::pair) {
     const AttnState s = state_layout(d);
-    if (cudaMemsetAsync(state, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
-    AttnPrep p{};
-    p.dim = d->dim;
-    add(p, in->q, d->num_q, d->heads, d->q_row, d->q_head, in->q_mask, kWq, state + s.qh,
-        state + s.ql);
-    add(p, in->k, d->num_k, d->kv_heads, d->k_row, d->k_head, in->k_mask, kWk, state + s.kh,
-        state + s.kl);
-    add(p, in->v, d->num_k, d->kv_heads, d->v_row, d->v_head, in->k_mask, kWv, state + s.vh,
-        state + s.vl);
-    if ((rc = bounds<float>(p, (unsigned *)state, sms, st))) return rc;
-    if ((rc = halves(p, (const unsigned *)state, sms, st))) return rc;
+    unsigned *words = (unsigned *)state;
+    if (cudaMemsetAsync(words, 0, 4 * words_of(d, 3), st) != cudaSuccess) return RA_ERR_CUDA;
+    AttnPrep p = prep_of(a);
+    add(p, in->q, false, a, d->q_row, d->q_head, kWq, state + s.qh, state + s.ql);
+    add(p, in->k, true, a, d->k_row, d->k_head, kWk, state + s.kh, state + s.kl);
+    add(p, in->v, true, a, d->v_row, d->v_head, kWv, state + s.vh, state + s.vl);
+    if ((rc = bounds<float>(p, words, st))) return rc;
+    if ((rc = halves(p, words, st))) return rc;
   }
   x.splits = f.splits;
   x.part_o = (float *)(ws + f.part_o), x.part_s = (float2 *)(ws + f.part_s);
@@ -404,6 +421,7 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
   const int sms = sm_count();
   const AttnBwd b = bwd_layout(d);
   const bool tc = use_tc(d) && operands_aligned(d, in);
+  if (tc && !Kind::bf16) a.do_top = (float *)(ws + b.do_top);
   if (a.num_q > 0) {
     const float *o32 = Kind::pair ? (const float *)a.out : a.out32;
     if (tc) {
@@ -412,7 +430,7 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
       const unsigned grid = (unsigned)std::min<int64_t>(
           ceil_div(a.num_q * a.heads * lanes, (int64_t)512), (int64_t)sms * 16);
       attn_delta8_kernel<T><<<grid, 256, 0, st>>>((const T *)a.dout, o32, a.num_q, a.heads, a.dim,
-                                                  lanes, a.neg_d);
+                                                  lanes, a.neg_d, a.do_top);
     } else {
       const unsigned grid =
           (unsigned)std::min<int64_t>(ceil_div(a.num_q * a.heads, (int64_t)8), (int64_t)sms * 16);
@@ -426,20 +444,17 @@ int backward(const ra_attn_desc *d, const ra_attn_inputs *in, AttnArgs a, const 
     const int64_t qr = (int64_t)d->heads * d->dim;
     const Operands o = operands(d, in, state, Kind::pair ? ws + b.gh : a.dout,
                                 Kind::pair ? ws + b.gl : a.dout);
-    unsigned *words = (unsigned *)state;
     if (!Kind::bf16) {
-      AttnPrep p{};
-      p.dim = d->dim;
-      add(p, a.dout, d->num_q, d->heads, qr, d->dim, in->q_mask, kWdo, ws + b.gh, ws + b.gl);
-      if (Kind::pair) {
-        if (cudaMemsetAsync(words + kWdo, 0, 8, st) != cudaSuccess) return RA_ERR_CUDA;
-      } else {
-        if (cudaMemsetAsync(words, 0, 256, st) != cudaSuccess) return RA_ERR_CUDA;
-        add(p, in->v, d->num_k, d->kv_heads, d->v_row, d->v_head, in->k_mask, kWv, nullptr,
-            nullptr);
-      }
-      if ((rc = bounds<T>(p, words, sms, st))) return rc;
-      if (Kind::pair && (rc = halves(p, words, sms, st))) return rc;
+      unsigned *words = (unsigned *)state;
+      const int first = Kind::pair ? kWdo : kWv;  // kept from the forward: the others
+      if (cudaMemsetAsync(words + words_of(d, first), 0, 4 * words_of(d, 4 - first), st) !=
+          cudaSuccess)
+        return RA_ERR_CUDA;
+      AttnPrep p = prep_of(a);
+      add(p, a.dout, false, a, qr, d->dim, kWdo, ws + b.gh, ws + b.gl);
+      if (!Kind::pair) add(p, in->v, true, a, d->v_row, d->v_head, kWv, nullptr, nullptr);
+      if ((rc = bounds<T>(p, words, st))) return rc;
+      if (Kind::pair && (rc = halves(p, words, st))) return rc;
     }
     rc = d->dim <= 32   ? tc_backward<Kind, 32>(d, o, a, &x, st)
          : d->dim <= 64 ? tc_backward<Kind, 64>(d, o, a, &x, st)

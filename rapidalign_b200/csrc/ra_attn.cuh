@@ -43,6 +43,19 @@ struct AttnSegs {
     return make_int4((int)(g * per + 128 * n), (int)min((int64_t)128, per - 128 * n),
                      (int)(g * other.per), (int)other.per);
   }
+  // the graph of tile t, whose first row is `row`: a search with the whole warp,
+  // two dependent loads for a thousand graphs
+  __device__ __forceinline__ int64_t graph_of_tile(int64_t graphs, int64_t t, int64_t row) const {
+    if (!ptr) return t / ((per + 127) >> 7);
+    int64_t lo = 0, hi = graphs;
+    while (hi - lo > 1) {
+      const int64_t step = (hi - lo + 31) >> 5, at = lo + (threadIdx.x & 31) * step;
+      const int under = __popc(__ballot_sync(kFull, at < hi && ptr[at] <= row));
+      lo += (under - 1) * step;  // the first probe always is
+      hi = min(hi, lo + step);
+    }
+    return lo;
+  }
   // the graph of row i (skips empty graphs)
   __device__ __forceinline__ int64_t graph_of(int64_t graphs, int64_t i) const {
     if (!ptr) return i / per;
@@ -73,6 +86,7 @@ struct AttnArgs {
   // backward
   const void *dout;         // [num_q][heads][dim]
   float *neg_d;             // [heads][num_q]: -D
+  float *do_top;            // [heads][num_q]: largest finite |do|; null where nothing is scaled
   void *dq, *dk, *dv;       // contiguous
   float4 *pos_q, *pos_k;    // [heads][num_q], [kv_heads][num_k]; or null
   int *status;

@@ -30,17 +30,20 @@
 // those hold reaches none.  What a tile needs of its rows besides (positions,
 // statistics) is loaded into registers an iteration ahead.
 //
-// fp32 inputs are fp16 pairs (hi + lo, one power of two per tensor), three
-// products for one; the two small ones have an accumulator of their own where
-// TMEM has room (the tensor core drops the bits below an accumulator's last one
-// at each step: a third of the steps on the large sums, a third of the loss).
+// fp32 inputs are fp16 pairs (hi + lo, one power of two for each graph and key head
+// of a tensor, so that a graph's precision is its own), three products for one; the
+// two small ones have an accumulator of their own where TMEM has room (the tensor
+// core drops the bits below an accumulator's last one at each step: a third of the
+// steps on the large sums, a third of the loss).
 // P of 16-bit inputs is a pair too where the output is kept unrounded for a
 // backward (D_i = do.o wants it); dU is one 16-bit number for 16-bit inputs (half
 // a step, independent between elements).  The dq kernel also sums dS: the sum
 // is what D_i was off by, since each row's P add up to 1, and it puts D_i right
 // for the positions and for the dk, dv kernel.
 // In fp16 P is held 2^7 up, and dU in units of the power of two that keeps
-// 2 dim max |do| max |v| >= |dU| / slope below 2^14.
+// 2 dim max |do| max |v| >= |dU| / slope below 2^14: v of the graph and key head,
+// do of the row for dq (rows are lanes, the unit comes out of a lane's results) and
+// of the graph's rows for dk, which adds them up.
 #pragma once
 
 #include <new>
@@ -52,7 +55,8 @@
 
 namespace ra {
 
-// words of the bounds: bits of the largest finite magnitude of each tensor
+// Bounds: bits of the largest finite magnitude of each tensor in each graph and key
+// head (for q and do: in the heads that share it), [4][graphs][kv_heads].
 enum AttnWord { kWq = 0, kWk = 1, kWv = 2, kWdo = 3 };
 
 struct AttnMap {  // 16-bit operand, or its halves
@@ -60,7 +64,7 @@ struct AttnMap {  // 16-bit operand, or its halves
 };
 struct AttnTcArgs {
   AttnMap q, k, v, go;
-  const unsigned *words;  // null where nothing is scaled
+  const unsigned *words;  // bounds; not read where nothing is scaled
   int splits;             // forward: key ranges of a row tile
   float *part_o;          // [splits][num_q][heads][dim], unnormalised
   float2 *part_s;         // [splits][heads][num_q] (m, l)
@@ -90,16 +94,25 @@ __device__ __forceinline__ int attn_exp(float top) {
   e = 14 - e;
   return e > 100 ? 100 : (e < -100 ? -100 : e);
 }
+// Scales of one graph and key head.
 template <class Kind>
-__device__ __forceinline__ int elem_exp(const AttnTcArgs &X, int w) {
-  return Kind::pair ? attn_exp(__uint_as_float(X.words[w])) : 0;
-}
-// of dU: 2 dim max |do| max |v| bounds |dP - D|
-template <class Kind>
-__device__ __forceinline__ int du_exp(const AttnTcArgs &X, int dim) {
-  if (Kind::bf16) return 0;
-  return attn_exp(2.f * dim * __uint_as_float(X.words[kWdo]) * __uint_as_float(X.words[kWv]));
-}
+struct AttnScales {
+  const unsigned *words;  // of this graph and head
+  int64_t n;
+  __device__ __forceinline__ void init(const AttnArgs &A, const AttnTcArgs &X, const AttnSegs &rows,
+                                       int64_t tile, int64_t row, int hk) {
+    if (Kind::bf16) return;
+    n = A.graphs * A.kv_heads;
+    words = X.words + rows.graph_of_tile(A.graphs, tile, row) * A.kv_heads + hk;
+  }
+  __device__ __forceinline__ float top(int w) const { return __uint_as_float(words[w * n]); }
+  // of a tensor's halves
+  __device__ __forceinline__ int elem(int w) const { return Kind::pair ? attn_exp(top(w)) : 0; }
+  // of dU: 2 dim max |do| max |v| bounds |dP - D|
+  __device__ __forceinline__ int du(float top_do, int dim) const {
+    return Kind::bf16 ? 0 : attn_exp(2.f * dim * top_do * top(kWv));
+  }
+};
 
 // Swizzled tiles: [chunk of CW columns][row][CW]; eight rows make an atom.
 template <int DP>
@@ -392,30 +405,42 @@ __device__ __forceinline__ void write_row(uint32_t taddr, float f, bool on, bool
 
 struct AttnPrep {
   const void *x[4];
-  int64_t rows[4], row[4], head[4];
+  int64_t row[4], head[4];
   int heads[4];
+  AttnSegs segs[4];
+  int64_t tiles[4];
   const uint8_t *mask[4];
   int word[4];
   uint16_t *hi[4], *lo[4];  // [rows][heads][dim]
-  int dim, count;
+  int64_t graphs;
+  int kv_heads, dim, count;
 };
 
-// (row, head, chunk of 8) of the e-th chunk
-struct PrepAt {
-  int64_t i;
-  int h, c;
-  __device__ __forceinline__ PrepAt(int64_t e, int heads, int dim8, bool small) {
-    if (small) {
-      const unsigned u = (unsigned)e, r = u / dim8;
-      c = u - r * dim8;
-      i = r / heads;
-      h = r - (unsigned)i * heads;
-    } else {
-      const int64_t r = e / dim8;
-      c = (int)(e - r * dim8);
-      i = r / heads;
-      h = (int)(r - i * heads);
-    }
+// A CTA's share: a tile of 128 rows of a graph and the heads of a key head.
+struct PrepUnit {
+  int64_t tile_no, row0;
+  int hk, group, dim8, n;  // n chunks of 8
+  __device__ __forceinline__ PrepUnit(const AttnPrep &p, int t) {
+    hk = (int)(blockIdx.x % p.kv_heads);
+    tile_no = blockIdx.x / p.kv_heads;
+    n = 0;
+    if (tile_no >= p.tiles[t]) return;
+    const int4 tile = p.segs[t].tile(tile_no, p.segs[t]);
+    group = p.heads[t] / p.kv_heads;
+    dim8 = p.dim >> 3;
+    row0 = tile.x;
+    n = tile.y * group * dim8;
+  }
+  __device__ __forceinline__ unsigned *word(const AttnPrep &p, int t, unsigned *words) const {
+    const int64_t g = p.segs[t].graph_of_tile(p.graphs, tile_no, row0);
+    return words + (p.word[t] * p.graphs + g) * p.kv_heads + hk;
+  }
+  // row, head and chunk of the e-th chunk
+  __device__ __forceinline__ void at(int e, int64_t &i, int &h, int &c) const {
+    const unsigned r = (unsigned)e / dim8, k = r / group;
+    c = e - r * dim8;
+    i = row0 + k;
+    h = hk * group + (r - k * group);
   }
 };
 template <class T>
@@ -439,38 +464,51 @@ __device__ __forceinline__ bool rows_wide(const AttnPrep &p, int t) {
   return ((uintptr_t)p.x[t] & 15) == 0 && p.row[t] % e == 0 && p.head[t] % e == 0;
 }
 
-// largest finite magnitude of each tensor
+constexpr int kPrepThreads = 128;
+// largest finite magnitude of each tensor in each graph and key head
 template <class T>
-__global__ void __launch_bounds__(256) attn_bounds_kernel(const AttnPrep p, unsigned *words) {
-  const int t = blockIdx.y, dim8 = p.dim >> 3;
-  const int64_t n = p.rows[t] * p.heads[t] * dim8;
-  const bool small = n < ((int64_t)1 << 31), wide = rows_wide<T>(p, t);
+__global__ void __launch_bounds__(kPrepThreads)
+    attn_bounds_kernel(const AttnPrep p, unsigned *words) {
+  const int t = blockIdx.y;
+  const PrepUnit u(p, t);
+  if (u.n == 0) return;
+  const bool wide = rows_wide<T>(p, t);
   float top = 0.f;
-  for (int64_t e = blockIdx.x * 256LL + threadIdx.x; e < n; e += gridDim.x * 256LL) {
-    const PrepAt at(e, p.heads[t], dim8, small);
-    if (p.mask[t] != nullptr && p.mask[t][at.i] == 0) continue;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < u.n; e += kPrepThreads) {
+    int64_t i;
+    int h, c;
+    u.at(e, i, h, c);
+    if (p.mask[t] != nullptr && p.mask[t][i] == 0) continue;
     float v[8];
-    load8((const T *)p.x[t] + at.i * p.row[t] + at.h * p.head[t] + at.c * 8, wide, v);
+    load8((const T *)p.x[t] + i * p.row[t] + h * p.head[t] + c * 8, wide, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (fabsf(v[k]) < INFINITY) top = fmaxf(top, fabsf(v[k]));
   }
+  __syncwarp();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+  unsigned *word = u.word(p, t, words);
   // maxima of bits: any order
-  if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(words + p.word[t], __float_as_uint(top));
+  if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(word, __float_as_uint(top));
 }
 
 // x 2^e = hi + lo in fp16
-__global__ void __launch_bounds__(256) attn_halves_kernel(const AttnPrep p, const unsigned *words) {
-  const int t = blockIdx.y, dim8 = p.dim >> 3;
-  const float sc = ldexpf(1.f, attn_exp(__uint_as_float(words[p.word[t]])));
-  const int64_t n = p.rows[t] * p.heads[t] * dim8;
-  const bool small = n < ((int64_t)1 << 31), wide = rows_wide<float>(p, t);
-  for (int64_t e = blockIdx.x * 256LL + threadIdx.x; e < n; e += gridDim.x * 256LL) {
-    const PrepAt at(e, p.heads[t], dim8, small);
+__global__ void __launch_bounds__(kPrepThreads)
+    attn_halves_kernel(const AttnPrep p, unsigned *words) {
+  const int t = blockIdx.y;
+  const PrepUnit u(p, t);
+  if (u.n == 0) return;
+  const bool wide = rows_wide<float>(p, t);
+  const float sc = ldexpf(1.f, attn_exp(__uint_as_float(*u.word(p, t, words))));
+#pragma unroll 4
+  for (int e = threadIdx.x; e < u.n; e += kPrepThreads) {
+    int64_t i;
+    int h, c;
+    u.at(e, i, h, c);
     float v[8];
-    load8((const float *)p.x[t] + at.i * p.row[t] + at.h * p.head[t] + at.c * 8, wide, v);
+    load8((const float *)p.x[t] + i * p.row[t] + h * p.head[t] + c * 8, wide, v);
     __half hi[8], lo[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -478,34 +516,46 @@ __global__ void __launch_bounds__(256) attn_halves_kernel(const AttnPrep p, cons
       hi[k] = __float2half_rn(y);
       lo[k] = __float2half_rn(y - __half2float(hi[k]));
     }
-    uint4 u[2];
-    memcpy(u, hi, 16);
-    memcpy(u + 1, lo, 16);
-    reinterpret_cast<uint4 *>(p.hi[t])[e] = u[0];
-    reinterpret_cast<uint4 *>(p.lo[t])[e] = u[1];
+    uint4 w[2];
+    memcpy(w, hi, 16);
+    memcpy(w + 1, lo, 16);
+    const int64_t to = (i * p.heads[t] + h) * u.dim8 + c;
+    reinterpret_cast<uint4 *>(p.hi[t])[to] = w[0];
+    reinterpret_cast<uint4 *>(p.lo[t])[to] = w[1];
   }
 }
 
-// D_i = do_i . o_i: 2^k lanes a row and head, 8 elements each
+// D_i = do_i . o_i, and the largest finite |do_i|: 2^k lanes a row and head, 8
+// elements each
 template <class T>
 __global__ void __launch_bounds__(256) attn_delta8_kernel(const T *dout, const float *out32,
                                                           int64_t num_q, int heads, int dim,
-                                                          int lanes, float *neg_d) {
+                                                          int lanes, float *neg_d,
+                                                          float *do_top) {
   const int l = threadIdx.x % lanes;
   const int64_t n = num_q * heads, step = gridDim.x * 256LL / lanes;
   // all lanes of a warp go round together: the shuffles need them
   for (int64_t r0 = (blockIdx.x * 256LL + (threadIdx.x & ~31)) / lanes; r0 < n; r0 += step) {
     const int64_t r = r0 + (threadIdx.x & 31) / lanes;
-    float s = 0.f;
+    float s = 0.f, top = 0.f;
     if (r < n && l * 8 < dim) {
       float a[8], b[8];
       load8(dout + r * dim + l * 8, true, a);
       load8(out32 + r * dim + l * 8, true, b);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s = fmaf(a[k], b[k], s);
+      for (int k = 0; k < 8; ++k) {
+        s = fmaf(a[k], b[k], s);
+        if (fabsf(a[k]) < INFINITY) top = fmaxf(top, fabsf(a[k]));
+      }
     }
-    for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
-    if (r < n && l == 0) neg_d[(r % heads) * num_q + r / heads] = -s;
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(kFull, s, o);
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    }
+    if (r < n && l == 0) {
+      neg_d[(r % heads) * num_q + r / heads] = -s;
+      if (do_top != nullptr) do_top[(r % heads) * num_q + r / heads] = top;
+    }
   }
 }
 
@@ -661,6 +711,9 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   }
   bool bad = false;
   if (t0 < t1) fetch(t0);
+  __syncwarp();
+  AttnScales<Kind> scl;
+  scl.init(A, X, A.qs, item / X.splits / A.heads, i0, hk);
   __syncthreads();
   if (t0 < t1) {
     bad = !mbar_wait(full + 8 * (t0 & 1), 0, X.spin_limit);
@@ -674,7 +727,8 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
 
   AttnScore sc;
   sc.init(A, h);
-  sc.su *= ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
+  sc.su *= ldexpf(1.f, -scl.elem(kWq) - scl.elem(kWk));
+  const int ev = scl.elem(kWv);
   RowPos rp;
   rp.set(row_on ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
   constexpr float kUp = Kind::bf16 ? 0.f : 7.f;  // P is held 2^kUp up
@@ -793,7 +847,7 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   const bool any = l > 0.f || l != l;
   const bool empty = !row_on || !any || t0 >= t1;
   using T = typename Kind::T;
-  const float unscale = ldexpf(1.f, -elem_exp<Kind>(X, kWv));
+  const float unscale = ldexpf(1.f, -ev);
   const bool in = row < nq;
   // the row's columns: every PARTS-th 32, or what there is
   constexpr int W = DP / PARTS < 32 ? 32 : DP / PARTS;
@@ -1122,6 +1176,9 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   }
   bool bad = false;
   if (t1 > 0) fetch(0);
+  __syncwarp();
+  AttnScales<Kind> scl;
+  scl.init(A, X, A.qs, item / A.heads, i0, hk);
   __syncthreads();
   if (t1 > 0) {
     bad = !landed(0);
@@ -1137,9 +1194,10 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   const float delta = live ? -A.neg_d[h * A.num_q + i] : 0.f;
   BwdRow B;
   B.sc.init(A, h);
-  B.sc.su *= ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
-  const int eu = du_exp<Kind>(X, A.dim);
-  B.dps = ldexpf(1.f, -elem_exp<Kind>(X, kWdo) - elem_exp<Kind>(X, kWv));
+  B.sc.su *= ldexpf(1.f, -scl.elem(kWq) - scl.elem(kWk));
+  const int eu = Kind::bf16 || !live ? 0 : scl.du(A.do_top[h * A.num_q + i], A.dim);
+  const int ek = scl.elem(kWk);
+  B.dps = ldexpf(1.f, -scl.elem(kWdo) - scl.elem(kWv));
   B.up = ldexpf(1.f, eu);
   B.p.set(live ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
   DqSums S;
@@ -1231,7 +1289,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   }
   using T = typename Kind::T;
   if (A.dq != nullptr && part == 0)
-    write_row<T, DP, C::SMALL>(tD + lane_off, A.scale * ldexpf(1.f, -eu - elem_exp<Kind>(X, kWk)), in,
+    write_row<T, DP, C::SMALL>(tD + lane_off, A.scale * ldexpf(1.f, -eu - ek), in,
                      !live || t1 == 0, A.dim, (T *)A.dq + (i * A.heads + h) * A.dim, nullptr);
   // both halves of the columns; what the row's dS add up to is D's error
   float all[9] = {sum_of(S.ds)};
@@ -1363,6 +1421,9 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   }
   bool bad = false;
   if (t1 > 0) fetch(0);
+  __syncwarp();
+  AttnScales<Kind> scl;
+  scl.init(A, X, A.ks, item / A.kv_heads, j0, hk);
   __syncthreads();
   if (t1 > 0) {
     bad = !landed(0);
@@ -1375,11 +1436,12 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
   const uint32_t tS = tmem, tP = tmem + QT, tDk = tmem + 2 * QT, tDv = tDk + (C::SMALL ? 2 : 1) * DP;
 
-  const float us = ldexpf(1.f, -elem_exp<Kind>(X, kWq) - elem_exp<Kind>(X, kWk));
-  const int eu = du_exp<Kind>(X, A.dim);
+  const int eu = Kind::bf16 ? 0 : scl.du(scl.top(kWdo), A.dim);
+  const int eq = scl.elem(kWq), eg = scl.elem(kWdo);
   constexpr float kUp = Kind::bf16 ? 1.f : 8192.f;  // of P
   BwdRow B;
-  B.dps = ldexpf(1.f, -elem_exp<Kind>(X, kWdo) - elem_exp<Kind>(X, kWv));
+  const float us = ldexpf(1.f, -eq - scl.elem(kWk));
+  B.dps = ldexpf(1.f, -eg - scl.elem(kWv));
   B.up = ldexpf(1.f, eu);
   B.p.set(live ? pos_of(A.k_pos, A.pos_dim, j) : AttnPos{0.f, 0.f, 0.f});
   float px = 0.f, py = 0.f, pz = 0.f;  // over all heads, times 1 / sigma^2
@@ -1484,10 +1546,10 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   const bool zero = !live || t1 == 0;
   constexpr int last = QT / 32 - 1;
   if (A.dk != nullptr && part == 0)
-    write_row<T, DP, C::SMALL>(tDk + lane_off, A.scale * ldexpf(1.f, -eu - elem_exp<Kind>(X, kWq)), in, zero,
+    write_row<T, DP, C::SMALL>(tDk + lane_off, A.scale * ldexpf(1.f, -eu - eq), in, zero,
                      A.dim, (T *)A.dk + at, nullptr);
   if (A.dv != nullptr && part == last)
-    write_row<T, DP, C::SMALL>(tDv + lane_off, ldexpf(1.f, -elem_exp<Kind>(X, kWdo)) / kUp, in, zero, A.dim,
+    write_row<T, DP, C::SMALL>(tDv + lane_off, ldexpf(1.f, -eg) / kUp, in, zero, A.dim,
                      (T *)A.dv + at, nullptr);
   if (pos_grad) {
     float4 *sum = reinterpret_cast<float4 *>(sm);  // [parts - 1][128]
