@@ -95,7 +95,7 @@ struct CePlan {
   int sx, sw;             // K slices of dx and dw
   bool direct_x, direct_w;
   size_t f_part, f_zt, f_blocks, f_total;
-  size_t b_coef, b_hi, b_lo, b_px, b_pw, b_total;
+  size_t b_coef, b_unit, b_xh, b_xl, b_hi, b_lo, b_px, b_pw, b_total;
 };
 
 CePlan ce_plan(const ra_ce_desc *d, int sms) {
@@ -137,6 +137,15 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   o = 0;
   p.b_coef = o;
   o += align256(sizeof(float2) * (size_t)d->rows);
+  p.b_unit = o;  // rows in units: the units, and x in them
+  if (d->dtype != RA_BF16) {
+    o += align256(sizeof(float) * (size_t)d->rows);
+    const size_t x = align256(2 * (size_t)d->rows * pad8(d->dim));
+    p.b_xh = o;
+    o += x;
+    p.b_xl = o;
+    if (split) o += x;
+  }
   const size_t g = align256(2 * (size_t)rows_pad * (size_t)p.ldg);
   p.b_hi = o;
   o += g;
@@ -227,15 +236,31 @@ int halves(const ra_ce_desc *d, const CePlan &p, const void *x, const void *w, c
            cudaStream_t st) {
   const CeState sl = ce_state(d);
   CeHead *head = (CeHead *)sb;
-  const CeMatrix mx{(const float *)x, d->rows, d->ld_x, d->dim, &head->amax_x,
-                    (__half *)(sb + sl.xh), (__half *)(sb + sl.xl)};
-  const CeMatrix mw{(const float *)w, d->vocab, d->ld_w, d->dim, &head->amax_w,
-                    (__half *)(sb + sl.wh), (__half *)(sb + sl.wl)};
+  const CeMatrix<float> mx{(const float *)x, d->rows, d->ld_x, d->dim, nullptr, &head->amax_x,
+                           (__half *)(sb + sl.xh), (__half *)(sb + sl.xl)};
+  const CeMatrix<float> mw{(const float *)w, d->vocab, d->ld_w, d->dim, nullptr, &head->amax_w,
+                           (__half *)(sb + sl.wh), (__half *)(sb + sl.wl)};
   const dim3 grid(grid_for(std::max(d->rows, d->vocab) * (pad8(d->dim) / 8), p.sms), 2);
   ce_amax_kernel<<<grid, 256, 0, st>>>(mx, mw);
   int rc = launched();
   if (rc) return rc;
   ce_split_kernel<<<grid, 256, 0, st>>>(mx, mw);
+  return launched();
+}
+
+// x in its rows' units, in the workspace: what dw multiplies
+template <class T>
+int rows_in_units(const ra_ce_desc *d, const CePlan &p, const void *x, CeHead *head, char *ws,
+                  cudaStream_t st) {
+  if (cudaMemsetAsync(&head->amax_xu, 0, 4, st) != cudaSuccess) return RA_ERR_CUDA;
+  const CeMatrix<T> m{(const T *)x, d->rows, d->ld_x, d->dim, (const float *)(ws + p.b_unit),
+                      &head->amax_xu, (__half *)(ws + p.b_xh),
+                      sizeof(T) == 4 ? (__half *)(ws + p.b_xl) : nullptr};
+  const unsigned grid = grid_for(d->rows * (pad8(d->dim) / 8), p.sms);
+  ce_amax_kernel<T><<<grid, 256, 0, st>>>(m, m);
+  int rc = launched();
+  if (rc) return rc;
+  ce_split_kernel<T><<<grid, 256, 0, st>>>(m, m);
   return launched();
 }
 
@@ -316,8 +341,8 @@ int join_rows(const ra_ce_desc *d, const float2 *part, int64_t ld, int parts, in
 }
 
 template <class T, bool BF16, bool SPLIT>
-int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int64_t *target, T *dx,
-             T *dw, char *state, char *ws, cudaStream_t st) {
+int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, bool units,
+             const int64_t *target, T *dx, T *dw, char *state, char *ws, cudaStream_t st) {
   const CeState sl = ce_state(d);
   CeHead *head = (CeHead *)state;
   uint16_t *gh = (uint16_t *)(ws + p.b_hi), *gl = (uint16_t *)(ws + (SPLIT ? p.b_lo : p.b_hi));
@@ -326,7 +351,13 @@ int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int
   const int64_t nt = ceil_div((int64_t)dim, (int64_t)p.tn_d);
   const float undo = d->scale / kCeGradScale<BF16>;
   const CeAlpha al_x{undo, &head->amax_g, SPLIT ? &head->amax_w : nullptr};
-  const CeAlpha al_w{undo, &head->amax_g, SPLIT ? &head->amax_x : nullptr};
+  const CeAlpha al_w{undo, &head->amax_g,
+                     units ? &head->amax_xu : SPLIT ? &head->amax_x : nullptr};
+  const float *unit = units ? (const float *)(ws + p.b_unit) : nullptr;
+  // x as dw multiplies it
+  const uint16_t *xh = units ? (const uint16_t *)(ws + p.b_xh) : op.xh;
+  const uint16_t *xl = !units ? op.xl : SPLIT ? (const uint16_t *)(ws + p.b_xl) : xh;
+  const int64_t ldx = units ? pad8(dim) : op.ldx;
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, cols = std::min<int64_t>(p.piece, d->vocab - v0);
     GmMaps m;
@@ -346,7 +377,7 @@ int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int
           !map16(&m.b_lo, BF16, op.wl + v0 * op.ldw, cols, dim, op.ldw, kGmK))
         return RA_ERR_INVALID_ARGUMENT;
       const int slices = std::min<int>(p.sx, (int)ceil_div(cols, (int64_t)kGmK));
-      CeEpiOut<T> eo{al_x, d->rows, dim, p.direct_x ? dx : nullptr, px, i > 0};
+      CeEpiOut<T> eo{al_x, d->rows, dim, p.direct_x ? dx : nullptr, px, i > 0, unit};
       const GmShape s = shape_of(d, p, p.mt, nt, cols, slices, 0);
       rc = launch_gemm<BF16, SPLIT, false, true>(p.tn_d, m, s, eo, p.sms, st);
       if (rc) return rc;
@@ -354,10 +385,10 @@ int backward(const ra_ce_desc *d, const CePlan &p, const Operands &op, const int
     if (dw != nullptr) {
       if (!map16(&m.a_hi, BF16, gh, d->rows, cols, p.ldg, kGmK) ||
           !map16(&m.a_lo, BF16, gl, d->rows, cols, p.ldg, kGmK) ||
-          !map16(&m.b_hi, BF16, op.xh, d->rows, dim, op.ldx, kGmK) ||
-          !map16(&m.b_lo, BF16, op.xl, d->rows, dim, op.ldx, kGmK))
+          !map16(&m.b_hi, BF16, xh, d->rows, dim, ldx, kGmK) ||
+          !map16(&m.b_lo, BF16, xl, d->rows, dim, ldx, kGmK))
         return RA_ERR_INVALID_ARGUMENT;
-      CeEpiOut<T> eo{al_w, cols, dim, p.direct_w ? dw + v0 * dim : nullptr, pw, 0};
+      CeEpiOut<T> eo{al_w, cols, dim, p.direct_w ? dw + v0 * dim : nullptr, pw, 0, nullptr};
       const GmShape s = shape_of(d, p, ceil_div(cols, (int64_t)kGmM), nt, d->rows, p.sw, 0);
       rc = launch_gemm<BF16, SPLIT, true, true>(p.tn_d, m, s, eo, p.sms, st);
       if (rc) return rc;
@@ -473,22 +504,32 @@ int ra_ce_backward(const ra_ce_desc *d, const void *x, const void *w, const int6
       return RA_ERR_CUDA;
     return RA_OK;
   }
+  // Coefficients of rows that may lie apart: fp16 holds each row in its own unit.
+  // (Those of a sum or mean of the losses are all alike; bf16 has the range.)
+  const bool units = d->dtype != RA_BF16 && (d->reduction == RA_REDUCE_NONE || g_lse != nullptr);
   if (cudaMemsetAsync(&head->amax_g, 0, 4, st) != cudaSuccess) return RA_ERR_CUDA;
-  ce_coef_kernel<<<grid_for(d->rows, p.sms), 256, 0, st>>>(target, d->rows, d->vocab,
-                                                           d->ignore_index, d->reduction, g_loss,
-                                                           g_lse, head, (float2 *)(ws + p.b_coef));
+  ce_coef_kernel<<<grid_for(d->rows, p.sms), 256, 0, st>>>(
+      target, d->rows, d->vocab, d->ignore_index, d->reduction, g_loss, g_lse, head,
+      (float2 *)(ws + p.b_coef), units ? (float *)(ws + p.b_unit) : nullptr);
   int rc;
   if ((rc = launched())) return rc;
+  if (units && dw != nullptr) {
+    rc = d->dtype == RA_F32 ? rows_in_units<float>(d, p, x, head, ws, st)
+                            : rows_in_units<__half>(d, p, x, head, ws, st);
+    if (rc) return rc;
+  }
   // The forward of a few rows made no halves if w lay aligned then; where it
   // lies now says nothing about that.
   if (d->dtype == RA_F32 && use_few(d) && (rc = halves(d, p, x, w, sb, st))) return rc;
   const Operands op = operands(d, x, w, sb);
   if (d->dtype == RA_F32)
-    return backward<float, false, true>(d, p, op, target, (float *)dx, (float *)dw, sb, ws, st);
+    return backward<float, false, true>(d, p, op, units, target, (float *)dx, (float *)dw, sb, ws,
+                                        st);
   if (d->dtype == RA_BF16)
-    return backward<__nv_bfloat16, true, false>(d, p, op, target, (__nv_bfloat16 *)dx,
+    return backward<__nv_bfloat16, true, false>(d, p, op, units, target, (__nv_bfloat16 *)dx,
                                                 (__nv_bfloat16 *)dw, sb, ws, st);
-  return backward<__half, false, false>(d, p, op, target, (__half *)dx, (__half *)dw, sb, ws, st);
+  return backward<__half, false, false>(d, p, op, units, target, (__half *)dx, (__half *)dw, sb, ws,
+                                        st);
 }
 
 }  // extern "C"

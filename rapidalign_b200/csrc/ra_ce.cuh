@@ -20,8 +20,11 @@
 // have coefficient 1, and the label's element, which outweighs the others, is
 // near -1 and exact, where 1 / count would round alike in every row (bf16
 // gradients off by 3.9e-3 instead of 2e-3).  In fp16 2^13 more keeps small
-// elements normal.  For fp32 inputs du, x and w are fp16 pairs hi + lo (22
-// bits).
+// elements normal, and where the rows' coefficients may lie apart (a loss of each
+// row, gradients of lse) each row has a power of two of its own in the place of the
+// largest: dx takes it back by rows, and dw multiplies a copy of x whose rows have
+// taken it, so that a row of small coefficients keeps its bits.  For fp32 inputs
+// du, x and w are fp16 pairs hi + lo (22 bits).
 // Bound by the tensor cores over a long width, by du's bytes over a short one.
 // Measured, logits / du / dx / dw: 8192 x 131072 x 1024 bf16 1.55 / 1.78 / 1.74 /
 // 1.64 ms (1.42 to 1.23 PFLOP/s); 65537 x 4099 x 128 fp32 270 / 410 / 290 / 241 us
@@ -42,6 +45,7 @@ struct CeHead {
   unsigned amax_g;          // bits of the largest finite coefficient (backward)
   unsigned ticket;          // blocks of ce_rows_kernel done
   long long count;          // rows with a label
+  unsigned amax_xu;         // bits of the largest finite |x_i| u_i (rows in units u_i)
 };
 
 // Power of two that brings a largest magnitude into [2^13, 2^14), below the
@@ -60,8 +64,8 @@ __device__ __forceinline__ unsigned finite_bits(float v) {
   return b < 0x7f800000u ? b : 0u;
 }
 
-// Eight columns of a row of an fp32 matrix, zeros behind its last; `wide`: rows
-// of 16-byte aligned addresses and whole eights.
+// Eight columns of a row, zeros behind its last; `wide`: rows of 16-byte aligned
+// addresses and whole eights.
 __device__ __forceinline__ void ce_load8(const float *a, int64_t ld, int cols, int64_t r, int c,
                                          bool wide, float (&v)[8]) {
   const float *p = a + r * ld + c;
@@ -75,20 +79,45 @@ __device__ __forceinline__ void ce_load8(const float *a, int64_t ld, int cols, i
     for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? p[k] : 0.f;
   }
 }
+__device__ __forceinline__ void ce_load8(const __half *a, int64_t ld, int cols, int64_t r, int c,
+                                         bool wide, float (&v)[8]) {
+  const __half *p = a + r * ld + c;
+  if (wide) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+    __half h[8];
+    memcpy(h, &u, 16);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = __half2float(h[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? __half2float(p[k]) : 0.f;
+  }
+}
+template <class T>
 struct CeMatrix {
-  const float *a;
+  const T *a;
   int64_t rows, ld;
   int cols;
+  const float *unit;  // of each row, or null: 1
   unsigned *word;
-  __half *hi, *lo;  // [rows, 8 eights]
+  __half *hi, *lo;  // [rows, 8 eights]; lo null: hi alone
   __device__ __forceinline__ bool wide() const {
-    return ((uintptr_t)a & 15) == 0 && (ld & 3) == 0 && (cols & 7) == 0;
+    return ((uintptr_t)a & 15) == 0 && ld % (16 / (int)sizeof(T)) == 0 && (cols & 7) == 0;
+  }
+  __device__ __forceinline__ void load(int64_t r, int c, bool wide, float (&v)[8]) const {
+    ce_load8(a, ld, cols, r, c, wide, v);
+    if (unit != nullptr) {
+      const float u = unit[r];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= u;
+    }
   }
 };
 
 // largest finite |a| of x (blockIdx.y = 0) and w into their words
-__global__ void __launch_bounds__(256) ce_amax_kernel(const CeMatrix x, const CeMatrix w) {
-  const CeMatrix &m = blockIdx.y ? w : x;
+template <class T>
+__global__ void __launch_bounds__(256) ce_amax_kernel(const CeMatrix<T> x, const CeMatrix<T> w) {
+  const CeMatrix<T> &m = blockIdx.y ? w : x;
   const int eights = (m.cols + 7) >> 3;
   const bool wide = m.wide();
   unsigned best = 0;
@@ -96,7 +125,7 @@ __global__ void __launch_bounds__(256) ce_amax_kernel(const CeMatrix x, const Ce
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = n < ((int64_t)1 << 31) ? (unsigned)i / (unsigned)eights : i / eights;
     float v[8];
-    ce_load8(m.a, m.ld, m.cols, r, (int)(i - r * eights) * 8, wide, v);
+    m.load(r, (int)(i - r * eights) * 8, wide, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const unsigned b = finite_bits(v[k]);
@@ -112,8 +141,9 @@ __global__ void __launch_bounds__(256) ce_amax_kernel(const CeMatrix x, const Ce
 }
 
 // a 2^e = hi + lo in fp16, rows padded with zeros to whole eights
-__global__ void __launch_bounds__(256) ce_split_kernel(const CeMatrix x, const CeMatrix w) {
-  const CeMatrix &m = blockIdx.y ? w : x;
+template <class T>
+__global__ void __launch_bounds__(256) ce_split_kernel(const CeMatrix<T> x, const CeMatrix<T> w) {
+  const CeMatrix<T> &m = blockIdx.y ? w : x;
   const int eights = (m.cols + 7) >> 3;
   const bool wide = m.wide();
   const float sc = ce_pow2(ce_exp(*m.word));
@@ -121,7 +151,7 @@ __global__ void __launch_bounds__(256) ce_split_kernel(const CeMatrix x, const C
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = n < ((int64_t)1 << 31) ? (unsigned)i / (unsigned)eights : i / eights;
     float v[8];
-    ce_load8(m.a, m.ld, m.cols, r, (int)(i - r * eights) * 8, wide, v);
+    m.load(r, (int)(i - r * eights) * 8, wide, v);
     __half h[8], l[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -132,6 +162,7 @@ __global__ void __launch_bounds__(256) ce_split_kernel(const CeMatrix x, const C
     uint4 u;
     memcpy(&u, h, 16);
     reinterpret_cast<uint4 *>(m.hi)[i] = u;
+    if (m.lo == nullptr) continue;
     memcpy(&u, l, 16);
     reinterpret_cast<uint4 *>(m.lo)[i] = u;
   }
@@ -328,11 +359,12 @@ __global__ void __launch_bounds__(TX * TY) ce_rows_kernel(const float2 *part, in
 }
 
 // Per row (gl + ge, gl) of the backward; 0 for a row without a label, NaN
-// for a label outside the table (as its loss).
+// for a label outside the table (as its loss).  `unit`: null, or the rows' powers
+// of two, that are taken out here; the largest coefficient then counts as 1.
 __global__ void __launch_bounds__(256) ce_coef_kernel(const int64_t *target, int64_t rows,
                                                       int64_t vocab, int64_t ignore, int reduction,
                                                       const float *g_loss, const float *g_lse,
-                                                      CeHead *head, float2 *coef) {
+                                                      CeHead *head, float2 *coef, float *unit) {
   unsigned best = 0;
   for (int64_t r = blockIdx.x * (int64_t)256 + threadIdx.x; r < rows;
        r += (int64_t)gridDim.x * 256) {
@@ -343,11 +375,29 @@ __global__ void __launch_bounds__(256) ce_coef_kernel(const int64_t *target, int
       if (reduction == RA_REDUCE_MEAN) gl = (float)((double)gl / (double)head->count);
       if (t < 0 || t >= vocab) gl = NAN;
     }
-    const float c = gl + (g_lse != nullptr ? g_lse[r] : 0.f);
+    float c = gl + (g_lse != nullptr ? g_lse[r] : 0.f);
+    const unsigned a = finite_bits(c), b = finite_bits(gl), top = a > b ? a : b;
+    if (unit != nullptr) {
+      // in [1/2, 1) of the unit; of a row without coefficients 0, so that its x
+      // counts for nothing
+      int e = 0;
+      if (top) frexpf(__uint_as_float(top), &e);
+      e = e > 127 ? 127 : (e < -100 ? -100 : e);
+      const float u = top ? ce_pow2(e) : c == 0.f && gl == 0.f ? 0.f : 1.f;
+      unit[r] = u;
+      if (top) {
+        const float inv = ce_pow2(-e);
+        c *= inv;
+        gl *= inv;
+      }
+    } else {
+      best = top > best ? top : best;
+    }
     coef[r] = make_float2(c, gl);
-    const unsigned a = finite_bits(c), b = finite_bits(gl);
-    best = a > best ? a : best;
-    best = b > best ? b : best;
+  }
+  if (unit != nullptr) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) head->amax_g = __float_as_uint(1.f);
+    return;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -497,15 +547,22 @@ struct CeEpiOut {
   T *out;       // [rows, cols], or null
   float *part;  // [slices][rows, cols]
   int add;
+  const float *unit;  // of the rows, or null
   struct Fixed {
     float al;
   };
-  struct Row {};
+  struct Row {
+    float unit;
+  };
   __device__ __forceinline__ Fixed fixed() const { return {out ? alpha.value() : 1.f}; }
-  __device__ __forceinline__ Row begin(const GmUnit &, int) const { return {}; }
+  __device__ __forceinline__ Row begin(const GmUnit &w, int row) const {
+    const int64_t r = (int64_t)w.m * kGmM + row;
+    return {unit != nullptr && r < rows ? unit[r] : 1.f};
+  }
   template <int TN, class Src>
-  __device__ __forceinline__ void run(const Fixed &F, const Row &, const GmUnit &w, int row,
+  __device__ __forceinline__ void run(const Fixed &F, const Row &R, const GmUnit &w, int row,
                                       int col, const Src &src, const GmOut &out_rows) const {
+    const float al = F.al * R.unit;
     const int64_t r = (int64_t)w.m * kGmM + row, c0 = (int64_t)w.n * TN + col;
     const int64_t w0 = r - (threadIdx.x & 31);  // the warp's first row
     // 16-byte aligned rows: fp32 sums, or results; 8-byte ones of 16-bit results
@@ -523,7 +580,7 @@ struct CeEpiOut {
         for (int q = 0; q < 4; ++q) {
           T t[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) store_as(t + k, v[8 * q + k] * F.al);
+          for (int k = 0; k < 8; ++k) store_as(t + k, v[8 * q + k] * al);
           memcpy(&x[q], t, 16);
         }
         out_rows.rows64(x, [&](int row_, int j, uint4 u) {
@@ -552,10 +609,10 @@ struct CeEpiOut {
           uint4 x[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            x[q] = make_uint4(__float_as_uint(v[16 * hf + 4 * q] * F.al),
-                              __float_as_uint(v[16 * hf + 4 * q + 1] * F.al),
-                              __float_as_uint(v[16 * hf + 4 * q + 2] * F.al),
-                              __float_as_uint(v[16 * hf + 4 * q + 3] * F.al));
+            x[q] = make_uint4(__float_as_uint(v[16 * hf + 4 * q] * al),
+                              __float_as_uint(v[16 * hf + 4 * q + 1] * al),
+                              __float_as_uint(v[16 * hf + 4 * q + 2] * al),
+                              __float_as_uint(v[16 * hf + 4 * q + 3] * al));
           out_rows.rows64(x, [&](int row_, int j, uint4 u) {
             if (w0 + row_ >= rows) return;
             float *q = base + (w0 + row_) * cols + c0 + c + 16 * hf + 4 * j;
