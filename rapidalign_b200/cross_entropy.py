@@ -45,8 +45,9 @@ def _rows16(t: Tensor) -> Tensor:
 def _operands(d, x: Tensor, weight: Tensor) -> Tuple[Tensor, Tensor]:
     """Both matrices as one pass of the kernels reads them, their strides into `d`."""
     xk, wk = _rows16(x), _rows16(weight)
+    # of a single row PyTorch keeps any stride, and calls it contiguous
     d.ld_x = max(xk.stride(0), d.dim) if d.rows else (d.dim + 7) // 8 * 8
-    d.ld_w = wk.stride(0)
+    d.ld_w = max(wk.stride(0), d.dim)
     return xk, wk
 
 
