@@ -296,6 +296,14 @@ def scratch(nbytes: int, device: torch.device) -> torch.Tensor:
     return buf if buf.data_ptr() % 256 == 0 else workspace(nbytes, device)
 
 
+def aligned(buf: torch.Tensor) -> torch.Tensor:
+    """A buffer of ``scratch`` that was saved for a backward, on a boundary of 256
+    bytes again wherever a hook brought it back to."""
+    if buf.data_ptr() % 256 == 0 and buf.is_contiguous():
+        return buf
+    return scratch(buf.numel(), buf.device).copy_(buf)
+
+
 def empty_as(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """An uninitialised contiguous tensor of t's shape and device."""
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)

@@ -203,9 +203,10 @@ class _KernelAttention(torch.autograd.Function):
                                      _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention")
         if need_grad:
-            ctx.desc, ctx.state, ctx.plan, ctx.stats = d, state, plan, stats
-            ctx.save_for_backward(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask,
-                                  out if out32 is None else out32)
+            ctx.desc, ctx.at_stats = d, at_stats
+            # all of it saved, so that it is freed with the graph
+            ctx.save_for_backward(q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, *plan,
+                                  out if out32 is None else out32, state)
         return out
 
     @staticmethod
@@ -214,13 +215,15 @@ class _KernelAttention(torch.autograd.Function):
         lib = _lib.load()
         # not always the forward's tensors: a checkpoint makes them again, hooks
         # on saved tensors may bring them back elsewhere and with other strides
-        *saved, out32 = ctx.saved_tensors
+        *saved, out32, state = ctx.saved_tensors
         q, k, v, q_pos, k_pos, sigma = saved[:6]
         d, dev = ctx.desc, q.device
-        inp, kept = _operands(d, *saved, ctx.plan)
+        inp, kept = _operands(d, *saved[:8], saved[8:])
         g, out32 = _dense16(g), _dense16(out32)
         need = ctx.needs_input_grad
         with _lib.on_device(dev):
+            state = _lib.aligned(state)
+            stats = state.data_ptr() + ctx.at_stats if d.num_q else None
             grads = [_lib.empty_as(t) if need[i] else None for i, t in enumerate((q, k, v))]
             grads += [_lib.empty_as(t, torch.float32) if t is not None and need[3 + i] else None
                       for i, t in enumerate((q_pos, k_pos))]
@@ -231,8 +234,8 @@ class _KernelAttention(torch.autograd.Function):
             f32 = q.dtype == torch.float32
             rc = lib.ra_attn_backward(ctypes.byref(d), ctypes.byref(inp), g.data_ptr(),
                                       out32.data_ptr() if f32 else None,
-                                      None if f32 else out32.data_ptr(), ctx.stats,
-                                      ctypes.byref(gr), ctx.state.data_ptr(), ctx.state.numel(),
+                                      None if f32 else out32.data_ptr(), stats,
+                                      ctypes.byref(gr), state.data_ptr(), state.numel(),
                                       ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
         _lib.check(rc, "kernel attention backward")
         for i, t in ((3, q_pos), (4, k_pos)):

@@ -83,8 +83,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         _lib.check(rc, "linear cross entropy")
         if ctx is None:  # no gradient wanted: without autograd's share of a small call
             return loss, lse
-        ctx.desc, ctx.state = d, state
-        ctx.save_for_backward(x, weight, target)
+        ctx.desc = d
+        ctx.save_for_backward(x, weight, target, state)  # freed with the graph
         ctx.set_materialize_grads(False)
         return loss, lse
 
@@ -94,7 +94,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         lib = _lib.load()
         # not always the forward's tensors: a checkpoint makes them again, hooks
         # on saved tensors may bring them back elsewhere and with other strides
-        x, weight, target = ctx.saved_tensors
+        x, weight, target, state = ctx.saved_tensors
         d, dev = ctx.desc, x.device
         xk, wk = _operands(d, x, weight)
         target = target.contiguous()
@@ -102,12 +102,13 @@ class _LinearCrossEntropy(torch.autograd.Function):
         gl = None if g_loss is None else g_loss.to(torch.float32).contiguous()
         ge = None if g_lse is None else g_lse.to(torch.float32).contiguous()
         with _lib.on_device(dev):
+            state = _lib.aligned(state)
             dx = _lib.empty_as(x) if need_x else None
             dw = _lib.empty_as(weight) if need_w else None
             ws = _lib.scratch(lib.ra_ce_workspace_bytes(ctypes.byref(d), 1), dev)
             rc = lib.ra_ce_backward(ctypes.byref(d), xk.data_ptr(), wk.data_ptr(),
                                     target.data_ptr(), _lib.ptr(gl), _lib.ptr(ge), _lib.ptr(dx),
-                                    _lib.ptr(dw), ctx.state.data_ptr(), ctx.state.numel(),
+                                    _lib.ptr(dw), state.data_ptr(), state.numel(),
                                     ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
         _lib.check(rc, "linear cross entropy backward")
         return dx, dw, None, None, None, None, None

@@ -120,3 +120,22 @@ def test_cross_entropy_alignment_changes(first, cuda_device):
     (_, _, *want), (_, _, *bound) = exact(x, w, target, 1.0, 0.0, gl, torch.zeros_like(gl))
     for got, t, b in zip(grads(first, 1 - first), want, bound):
         close(got, t, b, "gradient")
+
+
+def test_memory_after_the_backward(cuda_device):
+    """With the results alive, nothing of a pass is left but results and gradients."""
+    q = torch.randn(4096, 4, 64, device="cuda", requires_grad=True)
+    x = torch.randn(2048, 256, device="cuda", requires_grad=True)
+    w = torch.randn(8192, 256, device="cuda", requires_grad=True)
+    t = torch.randint(0, 8192, (2048,), device="cuda")
+    seg = ra.attention_segments(torch.tensor([0, 4096], device="cuda"))
+    calls = (lambda: ra.pyg_kernel_attention(q, q, q, segments=seg),
+             lambda: ra.linear_cross_entropy(x, w, t, reduction="sum")[0])
+    for call, leaves in zip(calls, ([q], [x, w])):
+        call().sum().backward()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = call()
+        torch.autograd.backward(out.sum())  # into gradients that are there
+        left = torch.cuda.memory_allocated() - before
+        assert left <= out.numel() * out.element_size() + 8192

@@ -182,3 +182,42 @@ def test_cross_entropy_strides_of_what_is_given_back(recorder, dtype):
         assert desc["ld_x"] == hooks.owner(x).stride(0) == (16 if wide_first else 40)
         assert desc["ld_w"] == hooks.owner(w).stride(0) == (16 if wide_first else 40)
         assert hooks.owner(target).dtype == torch.long
+
+
+def tensors_of(node):
+    held = [v for v in vars(node).values()]
+    return [v for h in held for v in (h if isinstance(h, (tuple, list)) else [h])
+            if isinstance(v, torch.Tensor)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nothing_is_held_after_the_backward(recorder, dtype):
+    """What the passes keep between them is saved, and freed with the rest."""
+    leaf = torch.randn(N * H * D, requires_grad=True)
+    x, w = (torch.randn(n, 16, dtype=dtype, requires_grad=True) for n in (9, 20))
+    for out in (attention(leaf, dtype), cross_entropy(x, w, torch.zeros(9, dtype=torch.long))):
+        assert not tensors_of(out.grad_fn)
+        out.sum().backward()
+        with pytest.raises(RuntimeError, match="already been freed"):
+            out.grad_fn.saved_tensors
+
+
+def test_state_is_aligned_again(recorder):
+    def again(t):
+        if t.dtype != torch.uint8:
+            return t.clone()
+        odd = torch.zeros(t.numel() + 264, dtype=torch.uint8)
+        at = (-odd.data_ptr()) % 256 + 8
+        return odd[at:at + t.numel()].copy_(t)
+
+    leaf = torch.randn(N * H * D, requires_grad=True)
+    x, w = (torch.randn(n, 16, requires_grad=True) for n in (9, 20))
+    with Clones(again):
+        outs = [attention(leaf, mask=False),
+                cross_entropy(x, w, torch.zeros(9, dtype=torch.long))]
+    for out in outs:
+        out.sum().backward()
+    got = recorder.last("ra_attn_backward")
+    assert got[7] % 256 == 0 and got[8] > 0 and (got[5] - got[7]) % 256 == 0
+    got = recorder.last("ra_ce_backward")
+    assert got[8] % 256 == 0 and got[9] > 0
