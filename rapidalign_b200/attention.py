@@ -137,24 +137,28 @@ def _dense16(t: Tensor) -> Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _operands(d, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, plan):
     """What the kernels read of one pass's tensors: the strides into `d`, the
     addresses, and the tensors these belong to (copies among them), which have to
     live until the pass is launched."""
     qr, kr, vr = _rows(q), _rows(k), _rows(v)
-    d.q_row, d.q_head = qr.stride()[:2]
-    d.k_row, d.k_head = kr.stride()[:2]
-    d.v_row, d.v_head = vr.stride()[:2]
-    pos = [None, None, None]
+    d.q_row, d.q_head, _ = qr.stride()
+    d.k_row, d.k_head, _ = kr.stride()
+    d.v_row, d.v_head, _ = vr.stride()
+    q_mask, k_mask = _dense(q_mask), _dense(k_mask)
     if q_pos is not None:
         d.pos_dim = q_pos.shape[-1]
-        sig = sigma.to(device=q.device, dtype=torch.float32)
-        if sig.shape != (d.heads,) or not sig.is_contiguous():
-            sig = sig.reshape(-1).expand(d.heads).contiguous()
-        pos = [_floats(q_pos), _floats(k_pos), sig]
-    masks = [m if m is None or m.is_contiguous() else m.contiguous() for m in (q_mask, k_mask)]
-    tensors = (qr, kr, vr, *plan, *pos, *masks)
-    return _lib.RaAttnInputs(*[_lib.ptr(t) for t in tensors]), tensors
+        q_pos, k_pos = _floats(q_pos), _floats(k_pos)
+        if sigma.dtype != torch.float32 or sigma.device != q.device:
+            sigma = sigma.to(device=q.device, dtype=torch.float32)
+        if sigma.shape != (d.heads,) or not sigma.is_contiguous():
+            sigma = sigma.reshape(-1).expand(d.heads).contiguous()
+    kept = (qr, kr, vr, *plan, q_pos, k_pos, sigma, q_mask, k_mask)
+    return _lib.RaAttnInputs(*[None if t is None else t.data_ptr() for t in kept]), kept
 
 
 class _KernelAttention(torch.autograd.Function):
