@@ -471,6 +471,10 @@ typedef struct ra_ce_desc {
   float softcap;
   int32_t test_hooks; /* 0, or RA_TEST_NO_MMA */
   int32_t *status;
+  int32_t forward_only; /* 1: no backward follows, and the state is smaller where the forward
+                           itself makes no halves of fp32 inputs (few rows); their
+                           table's address and strides are then
+                           multiples of 16 bytes.  A backward is RA_ERR_STATE. */
 } ra_ce_desc;
 
 RA_API size_t ra_ce_state_bytes(const ra_ce_desc *desc);
@@ -518,6 +522,10 @@ typedef struct ra_attn_desc {
   float scale, softcap;
   int32_t test_hooks; /* 0, or RA_TEST_NO_MMA */
   int32_t *status;
+  int32_t forward_only; /* 1: no backward follows, and the state is smaller where the forward
+                           itself makes no halves of fp32 inputs (few rows); their
+                           addresses and strides are then
+                           multiples of 16 bytes.  A backward is RA_ERR_STATE. */
 } ra_attn_desc;
 typedef struct ra_attn_inputs {
   const void *q, *k, *v;

@@ -98,6 +98,7 @@ class RaCeDesc(ctypes.Structure):
         ("softcap", ctypes.c_float),
         ("test_hooks", ctypes.c_int32),
         ("status", ctypes.c_void_p),
+        ("forward_only", ctypes.c_int32),
     ]
 
 
@@ -108,7 +109,7 @@ class RaAttnDesc(ctypes.Structure):
                                        "max_q", "max_k")] +
         [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "dim", "pos_dim", "dtype")] +
         [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("test_hooks", ctypes.c_int32),
-         ("status", ctypes.c_void_p)])
+         ("status", ctypes.c_void_p), ("forward_only", ctypes.c_int32)])
 
 
 class RaAttnInputs(ctypes.Structure):

@@ -182,6 +182,10 @@ class _KernelAttention(torch.autograd.Function):
         d.dtype, d.scale, d.softcap = _lib.DTYPES[q.dtype], scale, softcap
         d.status = _lib.status_word()
         inp, kept = _operands(d, q, k, v, q_pos, k_pos, sigma, q_mask, k_mask, plan)
+        if not need_grad and (q.dtype != torch.float32 or all(
+                t.data_ptr() % 16 == 0 and t.stride(0) % 4 == 0 and t.stride(1) % 4 == 0
+                for t in kept[:3])):
+            d.forward_only = 1
         ref = ctypes.byref(d)
         with _lib.on_device(dev):
             out = _lib.empty_as(q)

@@ -65,6 +65,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         xk, wk = _operands(d, x, weight)
         d.ignore_index, d.dtype, d.reduction = ignore_index, _lib.DTYPES[x.dtype], reduction
         d.scale, d.softcap, d.status = scale, softcap, _lib.status_word()
+        if ctx is None and (x.dtype != torch.float32
+                            or wk.data_ptr() % 16 == 0 and d.ld_w % 4 == 0):
+            d.forward_only = 1
         with _lib.on_device(dev):
             n_state = lib.ra_ce_state_bytes(ctypes.byref(d))
             n_ws = lib.ra_ce_workspace_bytes(ctypes.byref(d), 0)

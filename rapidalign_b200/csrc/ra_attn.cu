@@ -26,6 +26,7 @@ bool attn_ok(const ra_attn_desc *d) {
     return false;
   if (d->max_q < 0 || d->max_k < 0 || d->max_q > d->num_q || d->max_k > d->num_k) return false;
   if ((d->test_hooks & ~RA_TEST_NO_MMA) != 0) return false;
+  if (d->forward_only != 0 && d->forward_only != 1) return false;
   return d->q_tiles >= 0 && d->k_tiles >= 0 && d->status != nullptr;
 }
 
@@ -87,6 +88,10 @@ bool operands_aligned(const ra_attn_desc *d, const ra_attn_inputs *in) {
          (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v) & 15) == 0;
 }
 
+// A few rows a graph: bound by the keys' bytes (ra_attn_few.cuh).
+bool use_few(const ra_attn_desc *d) {
+  return use_tc(d) && d->max_q * (d->heads / d->kv_heads) <= kFewRows;
+}
 // The state a backward needs: bounds (fp32 inputs; the backward writes fp16's),
 // and the halves of fp32 inputs.
 struct AttnState {
@@ -98,6 +103,10 @@ size_t words_of(const ra_attn_desc *d, int tensors) {
 AttnState state_layout(const ra_attn_desc *d) {
   AttnState s{};
   size_t o = 256;
+  if (d->forward_only && use_few(d)) {  // reads the inputs as they are
+    s.total = o;
+    return s;
+  }
   if (d->dtype != RA_BF16 && use_tc(d)) o = std::max(o, align256(4 * words_of(d, 4)));
   if (d->dtype == RA_F32 && use_tc(d)) {
     const size_t q = align256(2 * (size_t)d->num_q * d->heads * d->dim);
@@ -120,10 +129,6 @@ int key_splits(const ra_attn_desc *d, int sms) {
   return s < 1 ? 1 : (int)s;
 }
 
-// A few rows a graph: bound by the keys' bytes (ra_attn_few.cuh).
-bool use_few(const ra_attn_desc *d) {
-  return use_tc(d) && d->max_q * (d->heads / d->kv_heads) <= kFewRows;
-}
 // 16-byte loads of eight columns
 bool few_aligned(const ra_attn_desc *d, const ra_attn_inputs *in) {
   const int64_t s = d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head;
@@ -509,6 +514,9 @@ int ra_attn_forward(const ra_attn_desc *d, const ra_attn_inputs *in, void *out, 
                     size_t workspace_bytes, ra_stream_t stream) {
   if (!attn_ok(d) || !inputs_ok(d, in)) return RA_ERR_INVALID_ARGUMENT;
   if (d->num_q == 0) return RA_OK;
+  if (d->forward_only &&
+      (stats != nullptr || (use_few(d) && d->dtype == RA_F32 && !few_aligned(d, in))))
+    return RA_ERR_INVALID_ARGUMENT;
   if (out == nullptr || (((uintptr_t)out | (uintptr_t)out32) & 15)) return RA_ERR_INVALID_ARGUMENT;
   if (workspace == nullptr || !aligned256(workspace) ||
       workspace_bytes < ra_attn_workspace_bytes(d, 0) || state == nullptr || !aligned256(state) ||
@@ -529,6 +537,7 @@ int ra_attn_backward(const ra_attn_desc *d, const ra_attn_inputs *in, const void
                      const ra_attn_grads *grads, void *state, size_t state_bytes, void *workspace,
                      size_t workspace_bytes, ra_stream_t stream) {
   if (!attn_ok(d) || !inputs_ok(d, in) || grads == nullptr) return RA_ERR_INVALID_ARGUMENT;
+  if (d->forward_only) return RA_ERR_STATE;
   if (d->num_q > 0 && (dout == nullptr || stats == nullptr || (d->dtype == RA_F32 ? out : out32) == nullptr))
     return RA_ERR_INVALID_ARGUMENT;
   if (d->pos_dim == 0 && (grads->dq_pos || grads->dk_pos || grads->dsigma))

@@ -12,7 +12,10 @@ namespace {
 
 using namespace ra;
 
-constexpr int64_t kCeRowsPerPass = 32768;         // rows of a forward launch: bounds the partials
+// Rows of a forward launch, and bytes of its partials (8 for each row and 64 or 32
+// columns): a table of 131072 takes 8192 rows at a time.
+constexpr int64_t kCeRowsPerPass = 32768;
+constexpr int64_t kCePartBytes = (int64_t)128 << 20;
 constexpr size_t kCePieceBytes = (size_t)512 << 20;  // du of one piece of the vocabulary
 
 bool ce_ok(const ra_ce_desc *d) {
@@ -26,6 +29,7 @@ bool ce_ok(const ra_ce_desc *d) {
   if (!(d->softcap >= 0.f) || !(d->softcap < INFINITY) || !(d->scale - d->scale == 0.f))
     return false;
   if ((d->test_hooks & ~RA_TEST_NO_MMA) != 0) return false;
+  if (d->forward_only != 0 && d->forward_only != 1) return false;
   return d->status != nullptr;
 }
 
@@ -50,7 +54,8 @@ CeState ce_state(const ra_ce_desc *d) {
   size_t o = 256;
   s.stats = o;
   o += align256(sizeof(float2) * (size_t)d->rows);
-  if (d->dtype == RA_F32) {
+  // the forward of a few rows reads the inputs as they are
+  if (d->dtype == RA_F32 && !(d->forward_only && use_few(d))) {
     const size_t x = align256(2 * (size_t)d->rows * pad8(d->dim));
     const size_t w = align256(2 * (size_t)d->vocab * pad8(d->dim));
     s.xh = o;
@@ -87,7 +92,8 @@ int k_slices(int64_t tiles, int64_t steps, int sms) {
 struct CePlan {
   int sms, elem;
   int64_t mt;             // 128-row tiles of x
-  int tn_z, parts;        // forward
+  int64_t pass;           // forward: rows of a launch
+  int tn_z, parts;
   int few_ctas;
   int64_t piece, ldg;     // vocabulary piece (columns of du)
   int64_t pieces;
@@ -104,9 +110,12 @@ CePlan ce_plan(const ra_ce_desc *d, int sms) {
   const bool split = d->dtype == RA_F32;
   p.elem = split ? 4 : 2;
   p.mt = ceil_div(d->rows, (int64_t)kGmM);
-  const int64_t pass = std::min<int64_t>(d->rows, kCeRowsPerPass);
-  p.tn_z = tile_width(ceil_div(pass, (int64_t)kGmM), d->vocab, sms, split);
+  p.tn_z = tile_width(ceil_div(std::min<int64_t>(d->rows, kCeRowsPerPass), (int64_t)kGmM), d->vocab,
+                      sms, split);
   p.parts = kGmParts * (int)ceil_div(d->vocab, (int64_t)p.tn_z);
+  p.pass = kCePartBytes / ((int64_t)sizeof(float2) * p.parts) / kGmM * kGmM;
+  p.pass = std::min<int64_t>(std::max<int64_t>(p.pass, kGmM), kCeRowsPerPass);
+  const int64_t pass = std::min<int64_t>(d->rows, p.pass);
   const int few_rows = kCeFewWarps * (split ? 2 : kCeFew16Rows);  // a CTA, at least
   p.few_ctas = (int)std::min<int64_t>(ceil_div(d->vocab, (int64_t)few_rows), split ? 2 * sms : sms);
   size_t o = 0;
@@ -445,6 +454,7 @@ int ra_ce_forward(const ra_ce_desc *d, const void *x, const void *w, const int64
                : RA_ERR_CUDA;
   }
   const bool few = use_few(d) && few_aligned(d, w);
+  if (d->forward_only && use_few(d) && !few) return RA_ERR_INVALID_ARGUMENT;
   if (few) {
     if ((rc = few_forward(d, p, x, w, target, ws, st))) return rc;
     return join_rows(d, (const float2 *)(ws + p.f_part), kCeFewRows, p.few_ctas, 0, d->rows, target,
@@ -455,8 +465,8 @@ int ra_ce_forward(const ra_ce_desc *d, const void *x, const void *w, const int64
   const Operands op = operands(d, x, w, sb);
   float2 *part = (float2 *)(ws + p.f_part);
   float *zt = (float *)(ws + p.f_zt);
-  for (int64_t r0 = 0; r0 < d->rows; r0 += kCeRowsPerPass) {
-    const int64_t rows = std::min<int64_t>(kCeRowsPerPass, d->rows - r0);
+  for (int64_t r0 = 0; r0 < d->rows; r0 += p.pass) {
+    const int64_t rows = std::min<int64_t>(p.pass, d->rows - r0);
     const int64_t mt = ceil_div(rows, (int64_t)kGmM);
     GmMaps m;
     if (!logit_maps(&m, bf16, op, d->dim, r0, rows, 0, d->vocab, p.tn_z))
@@ -485,6 +495,7 @@ int ra_ce_backward(const ra_ce_desc *d, const void *x, const void *w, const int6
                    size_t state_bytes, void *workspace, size_t workspace_bytes,
                    ra_stream_t stream) {
   if (!ce_ok(d) || w == nullptr) return RA_ERR_INVALID_ARGUMENT;
+  if (d->forward_only) return RA_ERR_STATE;
   if (d->rows > 0 && (x == nullptr || target == nullptr)) return RA_ERR_INVALID_ARGUMENT;
   if (d->dtype != RA_F32 && (!aligned(x, 16) || !aligned(w, 16))) return RA_ERR_INVALID_ARGUMENT;
   if (!aligned(dx, 16) || !aligned(dw, 16)) return RA_ERR_INVALID_ARGUMENT;
