@@ -70,7 +70,6 @@ AttnTcArgs tc_args(const ra_attn_desc *d, const char *state) {
   AttnTcArgs x{};
   x.words = (const unsigned *)state;
   x.no_mma = (d->test_hooks & RA_TEST_NO_MMA) != 0;
-  x.spin_limit = x.no_mma ? 4096u : kTcSpinLimit;
   return x;
 }
 

@@ -69,9 +69,22 @@ struct AttnTcArgs {
   float *part_o;          // [splits][num_q][heads][dim], unnormalised
   float2 *part_s;         // [splits][heads][num_q] (m, l)
   int pair_p;             // forward of 16-bit inputs: P as a pair
-  unsigned spin_limit;    // polls of one wait before giving up
   int no_mma;             // test hook: no products, so that the waits for them expire
 };
+
+// Bounded waits, which end early where no products are made (the test hook).  With
+// a limit in a register the dq kernel spilled, 11 % of its time at 64-wide heads;
+// with tile_wait's test in its loop the dk, dv kernel did, 4 %.
+__device__ __forceinline__ bool tile_wait(const AttnTcArgs &X, uint32_t bar, uint32_t parity) {
+  for (unsigned it = 0; it < kTcSpinLimit; ++it) {
+    if (mbar_wait(bar, parity, 1)) return true;
+    if ((it & 4095) == 4095 && X.no_mma) return false;
+  }
+  return false;
+}
+__device__ __forceinline__ bool products_done(const AttnTcArgs &X, uint32_t bar, uint32_t parity) {
+  return !X.no_mma && mbar_wait(bar, parity);
+}
 
 struct KindBf16 {
   using T = __nv_bfloat16;
@@ -501,27 +514,42 @@ __global__ void __launch_bounds__(kPrepThreads)
   const PrepUnit u(p, t);
   if (u.n == 0) return;
   const bool wide = rows_wide<float>(p, t);
-  const float sc = ldexpf(1.f, attn_exp(__uint_as_float(*u.word(p, t, words))));
-#pragma unroll 4
-  for (int e = threadIdx.x; e < u.n; e += kPrepThreads) {
-    int64_t i;
-    int h, c;
-    u.at(e, i, h, c);
-    float v[8];
-    load8((const float *)p.x[t] + i * p.row[t] + h * p.head[t] + c * 8, wide, v);
-    __half hi[8], lo[8];
+  constexpr int B = 4;  // chunks in flight, the first ones during the search
+  float v[B][8];
+  int64_t to[B];
+  auto load = [&](int e0) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float y = v[k] * sc;
-      hi[k] = __float2half_rn(y);
-      lo[k] = __float2half_rn(y - __half2float(hi[k]));
+    for (int b = 0; b < B; ++b) {
+      const int e = e0 + b * kPrepThreads;
+      if (e >= u.n) break;
+      int64_t i;
+      int h, c;
+      u.at(e, i, h, c);
+      load8((const float *)p.x[t] + i * p.row[t] + h * p.head[t] + c * 8, wide, v[b]);
+      to[b] = (i * p.heads[t] + h) * u.dim8 + c;
     }
-    uint4 w[2];
-    memcpy(w, hi, 16);
-    memcpy(w + 1, lo, 16);
-    const int64_t to = (i * p.heads[t] + h) * u.dim8 + c;
-    reinterpret_cast<uint4 *>(p.hi[t])[to] = w[0];
-    reinterpret_cast<uint4 *>(p.lo[t])[to] = w[1];
+  };
+  load(threadIdx.x);
+  __syncwarp();
+  const float sc = ldexpf(1.f, attn_exp(__uint_as_float(*u.word(p, t, words))));
+  for (int e0 = threadIdx.x; e0 < u.n; e0 += B * kPrepThreads) {
+    if (e0 != threadIdx.x) load(e0);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      if (e0 + b * kPrepThreads >= u.n) break;
+      __half hi[8], lo[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float y = v[b][k] * sc;
+        hi[k] = __float2half_rn(y);
+        lo[k] = __float2half_rn(y - __half2float(hi[k]));
+      }
+      uint4 w[2];
+      memcpy(w, hi, 16);
+      memcpy(w + 1, lo, 16);
+      reinterpret_cast<uint4 *>(p.hi[t])[to[b]] = w[0];
+      reinterpret_cast<uint4 *>(p.lo[t])[to[b]] = w[1];
+    }
   }
 }
 
@@ -714,9 +742,10 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   __syncwarp();
   AttnScales<Kind> scl;
   scl.init(A, X, A.qs, item / X.splits / A.heads, i0, hk);
+  const int es = scl.elem(kWq) + scl.elem(kWk), ev = scl.elem(kWv);
   __syncthreads();
   if (t0 < t1) {
-    bad = !mbar_wait(full + 8 * (t0 & 1), 0, X.spin_limit);
+    bad = !tile_wait(X, full + 8 * (t0 & 1), 0);
     settle(t0);
   }
   tc_fence_before();
@@ -727,8 +756,7 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
 
   AttnScore sc;
   sc.init(A, h);
-  sc.su *= ldexpf(1.f, -scl.elem(kWq) - scl.elem(kWk));
-  const int ev = scl.elem(kWv);
+  sc.su *= ldexpf(1.f, -es);
   RowPos rp;
   rp.set(row_on ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
   constexpr float kUp = Kind::bf16 ? 0.f : 7.f;  // P is held 2^kUp up
@@ -743,7 +771,7 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   }
   for (int t = t0; t < t1; ++t) {
     const int b = t & 1;
-    bad |= !mbar_wait(bar, phase, X.spin_limit);
+    bad |= !tile_wait(X, bar, phase);
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {  // the products on its buffers are done
@@ -816,7 +844,8 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     l += lo_of(both) + hi_of(both);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     if (t + 1 < t1) {
-      bad |= !mbar_wait(full + 8 * (b ^ 1), ((t + 1 - t0) >> 1) & 1, X.spin_limit);
+      // (copies that are not asked for any more are not waited for)
+      bad = bad || !tile_wait(X, full + 8 * (b ^ 1), ((t + 1 - t0) >> 1) & 1);
       settle(t + 1);
     }
     tc_fence_before();
@@ -829,7 +858,7 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     }
   }
   if (t0 < t1 && !bad) {
-    bad = !mbar_wait(bar, phase, X.spin_limit);
+    bad = !tile_wait(X, bar, phase);
     tc_fence_after();
   }
   if ((bad = __syncthreads_or(bad))) {
@@ -1157,8 +1186,8 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     fence_async_smem();
   };
   auto landed = [&](int t) {
-    return C::STAGES == 1 ? mbar_wait(full, t & 1, X.spin_limit)
-                          : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1, X.spin_limit);
+    return C::STAGES == 1 ? tile_wait(X, full, t & 1)
+                          : tile_wait(X, full + 8 * (t & 1), (t >> 1) & 1);
   };
   if (warp == 1) tmem_alloc<C::TMEM>(base + C::slot);
   if (threadIdx.x == 0) {
@@ -1179,6 +1208,8 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   __syncwarp();
   AttnScales<Kind> scl;
   scl.init(A, X, A.qs, item / A.heads, i0, hk);
+  const int ek = scl.elem(kWk), es = scl.elem(kWq) + ek, ep = scl.elem(kWdo) + scl.elem(kWv);
+  const int eu = Kind::bf16 || !live ? 0 : scl.du(A.do_top[h * A.num_q + i], A.dim);
   __syncthreads();
   if (t1 > 0) {
     bad = !landed(0);
@@ -1194,10 +1225,8 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   const float delta = live ? -A.neg_d[h * A.num_q + i] : 0.f;
   BwdRow B;
   B.sc.init(A, h);
-  B.sc.su *= ldexpf(1.f, -scl.elem(kWq) - scl.elem(kWk));
-  const int eu = Kind::bf16 || !live ? 0 : scl.du(A.do_top[h * A.num_q + i], A.dim);
-  const int ek = scl.elem(kWk);
-  B.dps = ldexpf(1.f, -scl.elem(kWdo) - scl.elem(kWv));
+  B.sc.su *= ldexpf(1.f, -es);
+  B.dps = ldexpf(1.f, -ep);
   B.up = ldexpf(1.f, eu);
   B.p.set(live ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
   DqSums S;
@@ -1212,7 +1241,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   }
   for (int t = 0; t < t1; ++t) {
     const int pb = t & 1, b = C::STAGES == 1 ? 0 : pb;
-    bad |= !mbar_wait(bar, phase, X.spin_limit);
+    bad |= !tile_wait(X, bar, phase);
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
@@ -1250,7 +1279,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     put_weights<Kind>(tS + lane_off + 32 * part, dp, Kind::pair);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     if (C::STAGES > 1 && t + 1 < t1) {
-      bad |= !landed(t + 1);
+      bad = bad || !landed(t + 1);
       settle(t + 1);
     }
     tc_fence_before();
@@ -1265,10 +1294,10 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
       tc_commit(bar);
     }
     if (C::STAGES == 1 && t + 1 < t1) {  // one buffer: its products first
-      bad |= !mbar_wait(bar, phase, X.spin_limit);
+      bad |= !tile_wait(X, bar, phase);
       phase ^= 1;
       if (threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
-      bad |= !landed(t + 1);
+      bad = bad || !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
       if (mma()) {
@@ -1280,7 +1309,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     }
   }
   if (t1 > 0 && !bad) {
-    bad = !mbar_wait(bar, phase, X.spin_limit);
+    bad = !tile_wait(X, bar, phase);
     tc_fence_after();
   }
   if ((bad = __syncthreads_or(bad))) {
@@ -1402,8 +1431,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     fence_async_smem();
   };
   auto landed = [&](int t) {
-    return C::STAGES == 1 ? mbar_wait(full, t & 1, X.spin_limit)
-                          : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1, X.spin_limit);
+    return C::STAGES == 1 ? mbar_wait(full, t & 1) : mbar_wait(full + 8 * (t & 1), (t >> 1) & 1);
   };
   if (warp == 1) tmem_alloc<C::TMEM>(base + C::slot);
   if (threadIdx.x == 0) {
@@ -1436,6 +1464,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
   const uint32_t tS = tmem, tP = tmem + QT, tDk = tmem + 2 * QT, tDv = tDk + (C::SMALL ? 2 : 1) * DP;
 
+  // (read here: before the first wait, as the other kernels do, they spill)
   const int eu = Kind::bf16 ? 0 : scl.du(scl.top(kWdo), A.dim);
   const int eq = scl.elem(kWq), eg = scl.elem(kWdo);
   constexpr float kUp = Kind::bf16 ? 1.f : 8192.f;  // of P
@@ -1474,7 +1503,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
       B.sc.init(A, h);
       B.sc.su *= us;
     }
-    bad |= !mbar_wait(bar, phase, X.spin_limit);
+    bad |= !products_done(X, bar, phase);
     phase ^= 1;
     tc_fence_after();
     if (t + 1 < t1) {
@@ -1502,7 +1531,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     put_weights<Kind>(tP + lane_off + 32 * part, dp, Kind::pair);
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     if (C::STAGES > 1 && t + 1 < t1) {
-      bad |= !landed(t + 1);
+      bad = bad || !landed(t + 1);
       settle(t + 1);
     }
     tc_fence_before();
@@ -1518,10 +1547,10 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
       tc_commit(bar);
     }
     if (C::STAGES == 1 && t + 1 < t1) {
-      bad |= !mbar_wait(bar, phase, X.spin_limit);
+      bad |= !products_done(X, bar, phase);
       phase ^= 1;
       if (threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
-      bad |= !landed(t + 1);
+      bad = bad || !landed(t + 1);
       settle(t + 1);
       if ((bad = __syncthreads_or(bad))) break;
       if (mma()) {
@@ -1534,7 +1563,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
   }
   close_head();
   if (t1 > 0 && !bad) {
-    bad = !mbar_wait(bar, phase, X.spin_limit);
+    bad = !products_done(X, bar, phase);
     tc_fence_after();
   }
   if ((bad = __syncthreads_or(bad))) {

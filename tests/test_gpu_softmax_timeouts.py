@@ -1,6 +1,6 @@
 """Waits of the softmax operators that run out, without faulting the GPU: with
-the test hook RA_TEST_NO_MMA the kernels issue no product and bound each wait to
-4096 polls.  The call returns, the next one raises, and what runs after it is
+the test hook RA_TEST_NO_MMA the kernels issue no product, and the waits for
+them run out after 4096 polls or sooner.  The call returns, the next one raises, and what runs after it is
 what it was before (an aborted launch that kept tensor memory, or copies that
 still land, would show there)."""
 import pytest
