@@ -205,6 +205,9 @@ __global__ void __launch_bounds__(512) attn_pos_kernel(const AttnPosGrads P) {
 }
 
 // ---- one warp a row ---------------------------------------------------------
+// For any width and strides, not for speed: every lane reads another row of the
+// other side, an element at a time (64 graphs of 64-512 points, 4 heads of 100, bf16:
+// 5.2 ms forward, 26 ms forward and backward).
 
 template <class T>
 __global__ void __launch_bounds__(32 * kAttnWarps) attn_row_fwd_kernel(const AttnArgs A) {

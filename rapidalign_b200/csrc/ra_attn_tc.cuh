@@ -15,12 +15,12 @@
 // packed two-lane forms counted once), barrier.  So the flow within a CTA is
 // simple -- all threads wait for the products, work on the scores, one thread
 // issues the next products -- and two to four CTAs on an SM hide each other's
-// waits: 0.39 to 0.47 instructions a cycle and scheduler, 10 % less with three
+// waits: 0.41 to 0.47 instructions a cycle and scheduler, 10 % less with three
 // CTAs in place of four.
 // Measured, forward / dq / dk, dv in us: 512 graphs of 64-512 points, 4 heads on 2
-// of 64, positions, bf16 295 / 315 / 380; 32 graphs of 33-2048, 8 heads of 128, cap,
-// bf16 510 / 535 / 671 (324 TFLOP/s of 14 D operations a score); 256 graphs of
-// 64-512, 4 heads of 32, positions, fp32 132 / 200 / 267.
+// of 64, positions, bf16 293 / 329 / 368; 32 graphs of 33-2048, 8 heads of 128, cap,
+// bf16 500 / 539 / 680 (322 TFLOP/s of 14 D operations a score); 256 graphs of
+// 64-512, 4 heads of 32, positions, fp32 135 / 202 / 271.
 //
 // Tiles come by TMA in boxes of 64 columns (32 at DP = 32) with 128-byte (64)
 // swizzle and are read K-major (S, dP) and MN-major (P V, dU K) from one copy.
@@ -477,6 +477,8 @@ __device__ __forceinline__ bool rows_wide(const AttnPrep &p, int t) {
   return ((uintptr_t)p.x[t] & 15) == 0 && p.row[t] % e == 0 && p.head[t] % e == 0;
 }
 
+// Bounds and halves, of q, k, v and do of 256 graphs of 64-512 points, 4 heads of 32:
+// 43 and 50 us (one scale a tensor, without tiles: 45 and 40).
 constexpr int kPrepThreads = 128;
 // largest finite magnitude of each tensor in each graph and key head
 template <class T>
