@@ -378,11 +378,12 @@ __global__ void __launch_bounds__(256) ce_coef_kernel(const int64_t *target, int
     float c = gl + (g_lse != nullptr ? g_lse[r] : 0.f);
     const unsigned a = finite_bits(c), b = finite_bits(gl), top = a > b ? a : b;
     if (unit != nullptr) {
-      // in [1/2, 1) of the unit; of a row without coefficients 0, so that its x
-      // counts for nothing
-      int e = 0;
+      // in [1, 2) of the unit, so that fp16's smallest step is no more of it than of
+      // the largest coefficient elsewhere; of a row without coefficients 0, so that
+      // its x counts for nothing
+      int e = 1;
       if (top) frexpf(__uint_as_float(top), &e);
-      e = e > 127 ? 127 : (e < -100 ? -100 : e);
+      e = e > 127 ? 126 : (e < -99 ? -100 : e - 1);
       const float u = top ? ce_pow2(e) : c == 0.f && gl == 0.f ? 0.f : 1.f;
       unit[r] = u;
       if (top) {
@@ -417,7 +418,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 
 template <bool BF16>
-constexpr float kCeGradScale = BF16 ? 1.f : 8192.f;  // |du| < 2 times this
+constexpr float kCeGradScale = BF16 ? 1.f : 8192.f;  // |du| < 2 times this (4, in rows' units)
 
 // Backward epilogue: du of one piece of the vocabulary, in 16 bits.
 template <bool BF16, bool PAIRS>
