@@ -19,8 +19,8 @@
 // CTAs in place of four.
 // Measured, forward / dq / dk, dv in us: 512 graphs of 64-512 points, 4 heads on 2
 // of 64, positions, bf16 293 / 329 / 368; 32 graphs of 33-2048, 8 heads of 128, cap,
-// bf16 500 / 539 / 680 (322 TFLOP/s of 14 D operations a score); 256 graphs of
-// 64-512, 4 heads of 32, positions, fp32 135 / 202 / 271.
+// bf16 498 / 539 / 682 (322 TFLOP/s of 14 D operations a score); 256 graphs of
+// 64-512, 4 heads of 32, positions, fp32 143 / 218 / 276.
 //
 // Tiles come by TMA in boxes of 64 columns (32 at DP = 32) with 128-byte (64)
 // swizzle and are read K-major (S, dP) and MN-major (P V, dU K) from one copy.
@@ -34,7 +34,12 @@
 // of a tensor, so that a graph's precision is its own), three products for one; the
 // two small ones have an accumulator of their own where TMEM has room (the tensor
 // core drops the bits below an accumulator's last one at each step: a third of the
-// steps on the large sums, a third of the loss).
+// steps on the large sums, a third of the loss).  That loss grows with the sum (of
+// dk over 5000 queries 5e-6, of 128-wide heads 1.5e-5), so a sum of fp32 is taken
+// in rounds, which are added up in the results' memory with rounding: 512 rows for
+// the output, dk and dv, 256 for dq, whose D and dP add their own errors, 128 for dk
+// and dv without the second accumulator.  Then each is off by 3e-7 to 9e-7 at any
+// length.  (256 rows for all cost 12 % of a step on graphs of 64-512 points.)
 // P of 16-bit inputs is a pair too where the output is kept unrounded for a
 // backward (D_i = do.o wants it); dU is one 16-bit number for 16-bit inputs (half
 // a step, independent between elements).  The dq kernel also sums dS: the sum
@@ -414,6 +419,39 @@ __device__ __forceinline__ void write_row(uint32_t taddr, float f, bool on, bool
   }
 }
 
+// A round of this lane's row to the sums in global memory, which only this thread
+// writes: out = (keep out + f v) post, or zeros; keep 0: nothing is there yet.
+template <int DP, bool SMALL>
+__device__ __forceinline__ void add_round(uint32_t taddr, float f, float keep, float post, bool on,
+                                          bool zero, int dim, float *out, int c0 = 0,
+                                          int c1 = DP) {
+#pragma unroll 1
+  for (int c = c0; c < c1; c += 32) {
+    float v[32];
+    __syncwarp();
+    tmem_ld32(taddr + c, v);
+    if (SMALL) {
+      float u[32];
+      tmem_ld32(taddr + DP + c, u);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += u[j];
+    }
+    if (!on || c >= dim) continue;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      if (c + j >= dim) break;
+      float4 *at = reinterpret_cast<float4 *>(out + c + j);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (keep != 0.f) o = *at;
+      o.x = fmaf(o.x, keep, v[j] * f) * post;
+      o.y = fmaf(o.y, keep, v[j + 1] * f) * post;
+      o.z = fmaf(o.z, keep, v[j + 2] * f) * post;
+      o.w = fmaf(o.w, keep, v[j + 3] * f) * post;
+      *at = zero ? make_float4(0.f, 0.f, 0.f, 0.f) : o;
+    }
+  }
+}
+
 // ---- bounds and halves ---------------------------------------------------------
 
 struct AttnPrep {
@@ -603,6 +641,12 @@ template <class Kind, int DP>
 constexpr int dkv_rows = 64 + (Kind::pair ? 4 : 2) * DP <= 128          ? 32
                          : !Kind::pair && DP == 128 || Kind::pair && DP == 64 ? 128
                                                                         : 64;
+// Tiles of a round of `rows` (a power of two): 16-bit inputs have one, whose loss
+// stays below their own rounding.
+template <class Kind, int ROWS>
+constexpr int round_tiles(int rows) {
+  return Kind::pair ? rows / ROWS : 1 << 30;
+}
 // CTAs that fit an SM beside each other, with `regs` registers a thread
 constexpr int attn_ctas(int smem, int tmem, int threads, int regs = 128) {
   int n = 65536 / (regs * threads);
@@ -618,6 +662,7 @@ struct FwdCfg {
   static constexpr int BR = KT;  // rows of a TMA box
   static constexpr int Q = HALF * tile_bytes<128, DP>, KV = HALF * tile_bytes<KT, DP>;
   static constexpr bool SMALL = Kind::pair;
+  static constexpr int ROUND = round_tiles<Kind, KT>(512);
   static constexpr int TMEM = tmem_round(KT + (SMALL ? 2 : 1) * DP);
   static constexpr int pos = Q + 4 * KV;                 // TilePos<KT> [2]
   static constexpr int val = pos + 2 * KT * 12;          // unsigned [2][2]
@@ -764,6 +809,14 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   constexpr float kUp = Kind::bf16 ? 0.f : 7.f;  // P is held 2^kUp up
   const bool p_pair = Kind::pair || X.pair_p;
   float m = -INFINITY, l = 0.f;  // m: the reference the sums are relative to; l: this part's
+  float keep = 0.f;              // of earlier rounds, which are relative to earlier references
+  // the row's columns: every PARTS-th 32, or what there is
+  constexpr int W = DP / PARTS < 32 ? 32 : DP / PARTS;
+  const int c0 = W * part, c1 = DP < c0 + W ? DP : c0 + W;
+  auto dest = [&]() {  // of the sums: the output, or this range's
+    return X.splits > 1 ? X.part_o + ((split * A.num_q + i) * A.heads + h) * A.dim
+                        : (float *)A.out + (i * A.heads + h) * A.dim;
+  };
   unsigned phase = 0;
 
   auto mma = [&]() { return threadIdx.x == kMmaThread<NT> && !X.no_mma; };
@@ -779,6 +832,11 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     if (t + 1 < t1) {  // the products on its buffers are done
       if (threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
+    }
+    if (Kind::pair && t > t0 && (t - t0) % C::ROUND == 0) {
+      add_round<DP, C::SMALL>(tO + lane_off, ldexpf(1.f, -ev), keep, 1.f, row_on, false, A.dim,
+                              dest(), c0, c1);
+      keep = 1.f;
     }
     __syncwarp();
     f2_t s2[C::C][16];
@@ -814,7 +872,8 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     if (__any_sync(kFull, grow)) {
       const float f = m > -INFINITY ? ex2(m - mn) : 0.f;
       l *= f;
-      if (t > t0) {
+      if (Kind::pair) keep *= f;
+      if ((t - t0) % C::ROUND != 0) {
 #pragma unroll 1
         for (int c = 32 * part; c < (C::SMALL ? 2 : 1) * DP; c += 32 * PARTS) {
           float o[32];
@@ -854,7 +913,8 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
     if ((bad = __syncthreads_or(bad))) break;
     if (mma()) {
       tc_fence_after();
-      products_weighted<Kind, KT, DP, C::SMALL>(tO, tS, sV + b * C::KV, p_pair, t > t0);
+      products_weighted<Kind, KT, DP, C::SMALL>(tO, tS, sV + b * C::KV, p_pair,
+                                                (t - t0) % C::ROUND != 0);
       if (t + 1 < t1) products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
       tc_commit(bar);
     }
@@ -880,21 +940,25 @@ __global__ void __launch_bounds__(FwdCfg<Kind, DP>::NT, FwdCfg<Kind, DP>::CTAS)
   using T = typename Kind::T;
   const float unscale = ldexpf(1.f, -ev);
   const bool in = row < nq;
-  // the row's columns: every PARTS-th 32, or what there is
-  constexpr int W = DP / PARTS < 32 ? 32 : DP / PARTS;
-  const int c0 = W * part, c1 = DP < c0 + W ? DP : c0 + W;
+  const float r = empty ? 0.f : 1.f / l;
+  const bool rounds = Kind::pair && t1 - t0 > C::ROUND;
+  if (rounds)
+    add_round<DP, C::SMALL>(tO + lane_off, unscale, keep, X.splits > 1 ? 1.f : r, in, empty, A.dim,
+                            dest(), c0, c1);
   if (X.splits > 1) {
-    float *po = X.part_o + ((split * A.num_q + i) * A.heads + h) * A.dim;
-    write_row<float, DP, C::SMALL>(tO + lane_off, unscale, in, empty, A.dim, po, nullptr, c0, c1);
+    if (!rounds)
+      write_row<float, DP, C::SMALL>(tO + lane_off, unscale, in, empty, A.dim, dest(), nullptr, c0,
+                                     c1);
     if (in && part == 0)
       X.part_s[((int64_t)split * A.heads + h) * A.num_q + i] =
           make_float2(empty ? -INFINITY : (m > -INFINITY ? m : 0.f) - kUp, empty ? 0.f : l);
   } else {
-    const float r = empty ? 0.f : 1.f / l;
     const int64_t at = (i * A.heads + h) * A.dim;
-    write_row<T, DP, C::SMALL>(tO + lane_off, unscale * r, in, empty, A.dim, (T *)A.out + at,
-                     A.out32 ? A.out32 + at : nullptr, c0, c1);
-    if (in && part == 0 && A.neg_m) A.put_stats(h, i, empty ? INFINITY : (m > -INFINITY ? m : 0.f) - kUp, r);
+    if (!rounds)
+      write_row<T, DP, C::SMALL>(tO + lane_off, unscale * r, in, empty, A.dim, (T *)A.out + at,
+                                 A.out32 ? A.out32 + at : nullptr, c0, c1);
+    if (in && part == 0 && A.neg_m)
+      A.put_stats(h, i, empty ? INFINITY : (m > -INFINITY ? m : 0.f) - kUp, r);
   }
   tc_fence_before();
   __syncthreads();
@@ -1120,6 +1184,7 @@ struct DqCfg {
   // two CTAs on an SM are worth more than a second buffer
   static constexpr int STAGES = 2 * Q + 4 * KV <= 100 * 1024 ? 2 : 1;
   static constexpr bool SMALL = Kind::pair;
+  static constexpr int ROUND = round_tiles<Kind, KT>(256);
   static constexpr int TMEM = tmem_round(2 * KT + (SMALL ? 2 : 1) * DP);
   static constexpr int NT = 128 * (KT / 32);
   static constexpr int pos = 2 * Q + 2 * STAGES * KV;  // TilePos<KT> [2]
@@ -1231,6 +1296,7 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
   B.dps = ldexpf(1.f, -ep);
   B.up = ldexpf(1.f, eu);
   B.p.set(live ? pos_of(A.q_pos, A.pos_dim, i) : AttnPos{0.f, 0.f, 0.f});
+  constexpr int W = DP / (NT / 128) < 32 ? 32 : DP / (NT / 128);  // columns of a thread's rounds
   DqSums S;
   const bool pos_grad = A.pos_q != nullptr;
   unsigned phase = 0;
@@ -1250,6 +1316,10 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
       if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
+    if (Kind::pair && t > 0 && t % C::ROUND == 0 && A.dq != nullptr)
+      add_round<DP, C::SMALL>(tD + lane_off, A.scale * ldexpf(1.f, -eu - ek), t > C::ROUND, 1.f,
+                              live, false, A.dim, (float *)A.dq + (i * A.heads + h) * A.dim,
+                              W * part, W * part + W);
     __syncwarp();
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
@@ -1288,7 +1358,8 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     if ((bad = __syncthreads_or(bad))) break;
     if (mma()) {
       tc_fence_after();
-      products_weighted<Kind, KT, DP, C::SMALL>(tD, tS, sK + b * C::KV, false, t > 0);
+      products_weighted<Kind, KT, DP, C::SMALL>(tD, tS, sK + b * C::KV, false,
+                                                t % C::ROUND != 0);
       if (C::STAGES > 1 && t + 1 < t1) {
         products_rows<Kind, KT, DP>(tS, sQ, sK + (b ^ 1) * C::KV);
         products_rows<Kind, KT, DP>(tP, sG, sV + (b ^ 1) * C::KV);
@@ -1319,9 +1390,15 @@ __global__ void __launch_bounds__(DqCfg<Kind, DP>::NT, DqCfg<Kind, DP>::CTAS)
     drain<NT>(full, *copied, 0, C::STAGES);
   }
   using T = typename Kind::T;
-  if (A.dq != nullptr && part == 0)
-    write_row<T, DP, C::SMALL>(tD + lane_off, A.scale * ldexpf(1.f, -eu - ek), in,
-                     !live || t1 == 0, A.dim, (T *)A.dq + (i * A.heads + h) * A.dim, nullptr);
+  if (A.dq != nullptr) {
+    const float f = A.scale * ldexpf(1.f, -eu - ek);
+    T *out = (T *)A.dq + (i * A.heads + h) * A.dim;
+    if (Kind::pair && t1 > C::ROUND)
+      add_round<DP, C::SMALL>(tD + lane_off, f, 1.f, 1.f, in, !live, A.dim, (float *)out, W * part,
+                              W * part + W);
+    else if (part == 0)
+      write_row<T, DP, C::SMALL>(tD + lane_off, f, in, !live || t1 == 0, A.dim, out, nullptr);
+  }
   // both halves of the columns; what the row's dS add up to is D's error
   float all[9] = {sum_of(S.ds)};
 #pragma unroll
@@ -1361,6 +1438,7 @@ struct DkvCfg {
   static constexpr int BR = QT < dq_rows<Kind, DP> ? QT : dq_rows<Kind, DP>;
   static constexpr int K = HALF * tile_bytes<128, DP>, QG = HALF * tile_bytes<QT, DP>;
   static constexpr bool SMALL = Kind::pair && DP <= 64;  // at 128 TMEM is full
+  static constexpr int ROUND = round_tiles<Kind, QT>(SMALL ? 512 : 128);
   static constexpr int TMEM = tmem_round(2 * QT + (SMALL ? 4 : 2) * DP);
   static constexpr int STAGES =
       2 * K + 4 * QG <= (TMEM == 512 ? 200 : 100) * 1024 ? 2 : 1;
@@ -1496,6 +1574,18 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     }
     g[0] = g[1] = g[2] = 0;
   };
+  const int64_t at = (j * A.kv_heads + hk) * A.dim;
+  constexpr int last = QT / 32 - 1;
+  auto f_dk = [&]() { return A.scale * ldexpf(1.f, -eu - eq); };
+  auto f_dv = [&]() { return ldexpf(1.f, -eg) / kUp; };
+  auto add_rounds = [&](float keep, bool on, bool zero) {
+    if (A.dk != nullptr && part == 0)
+      add_round<DP, C::SMALL>(tDk + lane_off, f_dk(), keep, 1.f, on, zero, A.dim,
+                              (float *)A.dk + at);
+    if (A.dv != nullptr && part == last)
+      add_round<DP, C::SMALL>(tDv + lane_off, f_dv(), keep, 1.f, on, zero, A.dim,
+                              (float *)A.dv + at);
+  };
   for (int t = 0; t < t1; ++t) {
     const int pb = t & 1, b = C::STAGES == 1 ? 0 : pb;
     const int h = hk * group + t / per;
@@ -1512,6 +1602,7 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
       if (C::STAGES > 1 && threadIdx.x == kTmaThread<NT> && !bad) issue(t + 1, 0);
       fetch(t + 1);
     }
+    if (Kind::pair && t > 0 && t % C::ROUND == 0) add_rounds(t > C::ROUND, live, false);
     __syncwarp();
     float v[32], dp[32];
     tmem_ld32(tS + lane_off + 32 * part, v);
@@ -1540,8 +1631,10 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     if ((bad = __syncthreads_or(bad))) break;
     if (mma()) {
       tc_fence_after();
-      products_weighted<Kind, QT, DP, C::SMALL>(tDv, tS, sG + b * C::QG, false, t > 0);
-      products_weighted<Kind, QT, DP, C::SMALL>(tDk, tP, sQ + b * C::QG, false, t > 0);
+      products_weighted<Kind, QT, DP, C::SMALL>(tDv, tS, sG + b * C::QG, false,
+                                                t % C::ROUND != 0);
+      products_weighted<Kind, QT, DP, C::SMALL>(tDk, tP, sQ + b * C::QG, false,
+                                                t % C::ROUND != 0);
       if (C::STAGES > 1 && t + 1 < t1) {
         products_rows<Kind, QT, DP>(tS, sK, sQ + (b ^ 1) * C::QG);
         products_rows<Kind, QT, DP>(tP, sV, sG + (b ^ 1) * C::QG);
@@ -1573,15 +1666,15 @@ __global__ void __launch_bounds__(DkvCfg<Kind, DP>::NT, DkvCfg<Kind, DP>::CTAS)
     drain<NT>(full, *copied, 0, C::STAGES);
   }
   using T = typename Kind::T;
-  const int64_t at = (j * A.kv_heads + hk) * A.dim;
   const bool zero = !live || t1 == 0;
-  constexpr int last = QT / 32 - 1;
-  if (A.dk != nullptr && part == 0)
-    write_row<T, DP, C::SMALL>(tDk + lane_off, A.scale * ldexpf(1.f, -eu - eq), in, zero,
-                     A.dim, (T *)A.dk + at, nullptr);
-  if (A.dv != nullptr && part == last)
-    write_row<T, DP, C::SMALL>(tDv + lane_off, ldexpf(1.f, -eg) / kUp, in, zero, A.dim,
-                     (T *)A.dv + at, nullptr);
+  if (Kind::pair && t1 > C::ROUND) {
+    add_rounds(1.f, in, zero);
+  } else {
+    if (A.dk != nullptr && part == 0)
+      write_row<T, DP, C::SMALL>(tDk + lane_off, f_dk(), in, zero, A.dim, (T *)A.dk + at, nullptr);
+    if (A.dv != nullptr && part == last)
+      write_row<T, DP, C::SMALL>(tDv + lane_off, f_dv(), in, zero, A.dim, (T *)A.dv + at, nullptr);
+  }
   if (pos_grad) {
     float4 *sum = reinterpret_cast<float4 *>(sm);  // [parts - 1][128]
     if (part > 0) sum[(part - 1) * 128 + row] = make_float4(px, py, pz, 0.f);
